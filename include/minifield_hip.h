@@ -366,6 +366,122 @@ mfh_status mfh_gated_short_convolution(mfh_ctx *ctx, mfh_buf *output,
 /* InferenceOps::swiglu (inference.rs:419-424). */
 mfh_status mfh_swiglu(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *gate, const mfh_buf *up);
 
+/* ---- paged caches and sampling (no counterpart in the reference) ------- */
+/*
+ * A server's decode step: one new token for each of many sequences, whose keys
+ * and values lie in pages that sequences can share.
+ *
+ * Page buffers.  [pages, kv_heads, page_size, head_dim], F32, or U8 of twice
+ * the last width holding binary16 values; key and value pages of a cache have
+ * one shape and format.  page_size is a power of two in [8, 4096].
+ * Tables.  `tables` is F32 [sequences, max_pages]: row s names the pages of
+ * sequence s in order, so that its token t lies in page tables[s][t /
+ * page_size] at row t % page_size.  Entries that a call has no need of are not
+ * read.  Several rows may name one page; whoever appends gives a sequence a
+ * page of its own first (mfh_copy_pages).
+ * Page ids, lengths, positions and sequence ids are whole numbers as exact f32
+ * values (below 2^24), like device token ids, and stay on the device: a call
+ * captured in a graph sees their new values on each replay.  The kernels check
+ * each; a bad one gives the answers stated at each call, never an access out of
+ * bounds.
+ */
+
+/* A zeroed page buffer of the Cache class, binary16 where `half` is 1. */
+mfh_status mfh_alloc_pages(mfh_ctx *ctx, uint64_t pages, uint32_t key_value_heads,
+                           uint32_t page_size, uint32_t head_dim, int half, mfh_buf **out);
+
+/* How rotation frequencies f_c = theta^(-2c / rotary_dim) are stretched. */
+typedef enum mfh_rope_scaling_kind {
+    MFH_ROPE_PLAIN = 0,
+    MFH_ROPE_LINEAR = 1,     /* f_c / factor */
+    MFH_ROPE_NTK = 2,        /* theta * factor^(r / (r - 2)) for theta, r = rotary_dim */
+    /* By turns n_c = original_positions * f_c / 2 pi: f_c where n_c >= high,
+     * f_c / factor where n_c <= low, linear in n_c between. */
+    MFH_ROPE_WAVELENGTH = 3,
+    /* Linear in c between the pairs that turn `high` and `low` times in
+     * original_positions (rounded outwards to whole c): f_c below, f_c / factor
+     * above (the YaRN rule). */
+    MFH_ROPE_YARN = 4
+} mfh_rope_scaling_kind;
+
+typedef struct mfh_rope_scaling {
+    uint32_t kind;            /* mfh_rope_scaling_kind */
+    float factor;             /* all but MFH_ROPE_PLAIN */
+    float original_positions; /* MFH_ROPE_WAVELENGTH, MFH_ROPE_YARN */
+    float low, high;          /* the same; 0 < low < high */
+    float magnitude;          /* every sine and cosine times this; 1 for none */
+} mfh_rope_scaling;
+
+/* Rotation coefficients by position: row p of `output` [positions, rotary_dim]
+ * holds the cosines of p * f_c, then the sines.  `scaling` null: plain.  Angles
+ * are formed in 64 bits, so far positions keep their precision (the reference's
+ * rotary operations round angles to f32). */
+mfh_status mfh_rotation_table(mfh_ctx *ctx, mfh_buf *output, float theta,
+                              const mfh_rope_scaling *scaling);
+
+/* Head norms and rotation of new tokens, and their keys and values into the
+ * caches.  Token t belongs to row sequences[t] of `tables` (null: row t) and
+ * has position positions[t].  Queries [tokens, query_heads * head_dim] and keys
+ * are RMS-normed per head (unless both weights are null), and the first
+ * rotary_dim columns of each head (the width of `rotation`, even, up to
+ * head_dim) turn by row `position` of `rotation`: pairs (c, rotary_dim / 2 + c),
+ * or (2c, 2c + 1) where `interleaved` is 1.  Queries go to `query_out`, keys
+ * and values to the token's row of its page; binary16 pages hold the nearest
+ * value, finite values past their range the largest.  A token whose position,
+ * sequence or page id is bad (a padded row: position -1) enters no cache and
+ * gets a NaN query row.  Two tokens of one call may not have one place (what
+ * lies there afterwards is a mix of both). */
+mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key_pages,
+                                  mfh_buf *value_pages, const mfh_buf *query, const mfh_buf *key,
+                                  const mfh_buf *value, const mfh_buf *query_weight,
+                                  const mfh_buf *key_weight, const mfh_buf *rotation,
+                                  const mfh_buf *tables, const mfh_buf *sequences,
+                                  const mfh_buf *positions, uint32_t query_heads,
+                                  uint32_t key_value_heads, uint32_t head_dim, int interleaved,
+                                  float epsilon);
+
+/* Attention of one token per sequence over its first lengths[s] cached tokens
+ * (the new one among them): softmax(q . k / sqrt(head_dim)) v, query heads
+ * grouped as in mfh_causal_gqa.  Length 0 gives zeros; a length that is no whole
+ * number or passes the table's row, and a bad page id among the pages that the
+ * length needs, give a NaN row.  What lies behind a sequence's length is not
+ * used, whatever it holds.  Keys and values of a binary16 cache are expected to
+ * be finite (one that is not makes its sequence's row NaN).  head_dim <= 1024.
+ * The workspace grows on a call outside of stream capture; under capture a call
+ * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT. */
+mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
+                         const mfh_buf *key_pages, const mfh_buf *value_pages,
+                         const mfh_buf *tables, const mfh_buf *lengths, uint32_t query_heads,
+                         uint32_t key_value_heads, uint32_t head_dim);
+
+/* Copy page from_pages[i] of sources[b] to page to_pages[i] of destinations[b],
+ * for every i < count and b < buffers (a model's key and value pages of all
+ * layers): what a fork of the page that two sequences would both write, a
+ * compaction, or a move to another cache needs.  A destination may be its own
+ * source.  Page shapes agree; formats may differ (f32 to binary16 rounds as
+ * appends do).  Every id is checked here; a page copied to twice, or in place
+ * copied from and to, is rejected, as is a destination that appears twice or as
+ * another pair's source. */
+mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
+                          const mfh_buf *const *sources, size_t buffers,
+                          const uint32_t *from_pages, const uint32_t *to_pages, size_t count);
+
+/* The next token of each row of `logits` [rows, width], as an exact f32 index,
+ * from uniforms[row] in [0, 1).  Row r of `params` (or its only row) holds
+ * temperature, top_k, top_p, min_p.  With w = exp((logit - maximum) /
+ * temperature): the first top_k tokens in descending order are kept (0: all;
+ * among equal logits the lower index comes first), of those the shortest run
+ * from the first whose weight reaches top_p (1: all) of theirs, at least one,
+ * of those the ones with w >= min_p; the token is the first, in index order, at
+ * which the sum of kept weights passes uniform * total.  Temperature 0 takes the
+ * first largest logit.  `mask`, when non-null, is U8 [rows or 1, ceil(width /
+ * 8)]: bit i % 8 of byte i / 8 admits token i.  Tokens not admitted, and logits
+ * of -infinity, are never chosen.  A row with an admitted NaN or +infinity,
+ * without a token, or with a uniform or parameter out of range gives NaN.
+ * Weights and sums are 64-bit. */
+mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
+                           const mfh_buf *uniforms, const mfh_buf *params, const mfh_buf *mask);
+
 /* ---- diagnostics (no counterpart in the reference) --------------------- */
 
 /* The HIP stream (hipStream_t) all work of `ctx` is ordered on, so a caller

@@ -43,6 +43,13 @@ class Report(ctypes.Structure):
                 ("pending_operations", ctypes.c_uint32)]
 
 
+class RopeScaling(ctypes.Structure):
+    """mfh_rope_scaling (include/minifield_hip.h)."""
+    _fields_ = [("kind", ctypes.c_uint32), ("factor", ctypes.c_float),
+                ("original_positions", ctypes.c_float), ("low", ctypes.c_float),
+                ("high", ctypes.c_float), ("magnitude", ctypes.c_float)]
+
+
 class MflConfig(ctypes.Structure):
     """mfl_config (include/minifield_lfm2.h)."""
     _fields_ = [("hidden", ctypes.c_uint32), ("intermediate", ctypes.c_uint32),
@@ -123,6 +130,15 @@ SIGNATURES = {
                            ctypes.c_uint32]),
     "mfh_gated_short_convolution": (S, [P, P, P, P, P, ctypes.c_uint32, ctypes.c_uint32]),
     "mfh_swiglu": (S, [P, P, P, P]),
+    # paged caches and sampling
+    "mfh_alloc_pages": (S, [P, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32,
+                            ctypes.c_uint32, ctypes.c_int, PP]),
+    "mfh_rotation_table": (S, [P, P, ctypes.c_float, ctypes.POINTER(RopeScaling)]),
+    "mfh_paged_qk_norm_rope": (S, [P] * 13 + [ctypes.c_uint32] * 3 + [ctypes.c_int,
+                                                                      ctypes.c_float]),
+    "mfh_paged_gqa": (S, [P] * 7 + [ctypes.c_uint32] * 3),
+    "mfh_copy_pages": (S, [P, PP, PP, SZ, c_u32_p, c_u32_p, SZ]),
+    "mfh_sample_rows": (S, [P] * 6),
     # LFM2 token pass (minifield_lfm2.h)
     "mfl_create": (S, [P, ctypes.POINTER(MflConfig), PP]),
     "mfl_destroy": (None, [P]),

@@ -433,6 +433,61 @@ class HipBackend:
     def swiglu(self, output: Buffer, gate: Buffer, up: Buffer) -> None:
         self._check(_ffi.lib().mfh_swiglu(self._ctx, output.handle, gate.handle, up.handle))
 
+    # ---- paged caches and sampling ------------------------------------------
+
+    def alloc_pages(self, pages: int, key_value_heads: int, page_size: int, head_dim: int,
+                    half: bool = False) -> Buffer:
+        """A zeroed page buffer: f32, or binary16 in a U8 buffer of twice the width."""
+        out = ctypes.c_void_p()
+        self._check(_ffi.lib().mfh_alloc_pages(self._ctx, pages, key_value_heads, page_size,
+                                               head_dim, int(half), ctypes.byref(out)))
+        return Buffer(out.value, self, U8 if half else F32,
+                      (pages, key_value_heads, page_size, head_dim * (2 if half else 1)))
+
+    def rotation_table(self, output: Buffer, theta: float,
+                       scaling: "RopeScaling | None" = None) -> None:
+        self._check(_ffi.lib().mfh_rotation_table(
+            self._ctx, output.handle, theta,
+            None if scaling is None else ctypes.byref(scaling.struct())))
+
+    def paged_qk_norm_rope(self, query_out: Buffer, key_pages: Buffer, value_pages: Buffer,
+                           query: Buffer, key: Buffer, value: Buffer,
+                           query_weight: Buffer | None, key_weight: Buffer | None,
+                           rotation: Buffer, tables: Buffer, sequences: Buffer | None,
+                           positions: Buffer, rope: "PagedRopeSpec", epsilon: float) -> None:
+        self._check(_ffi.lib().mfh_paged_qk_norm_rope(
+            self._ctx, query_out.handle, key_pages.handle, value_pages.handle, query.handle,
+            key.handle, value.handle, _h(query_weight), _h(key_weight), rotation.handle,
+            tables.handle, _h(sequences), positions.handle, rope.query_heads,
+            rope.key_value_heads, rope.head_dim, int(rope.interleaved), epsilon))
+
+    def paged_gqa(self, output: Buffer, query: Buffer, key_pages: Buffer, value_pages: Buffer,
+                  tables: Buffer, lengths: Buffer, spec: "GqaSpec") -> None:
+        self._check(_ffi.lib().mfh_paged_gqa(
+            self._ctx, output.handle, query.handle, key_pages.handle, value_pages.handle,
+            tables.handle, lengths.handle, spec.query_heads, spec.key_value_heads,
+            spec.head_dim))
+
+    def copy_pages(self, destinations: Sequence[Buffer], sources: Sequence[Buffer], from_pages,
+                   to_pages) -> None:
+        if len(destinations) != len(sources):
+            raise ValueError("one source for each destination")
+        source = np.ascontiguousarray(from_pages, dtype=np.uint32).reshape(-1)
+        target = np.ascontiguousarray(to_pages, dtype=np.uint32).reshape(-1)
+        if source.size != target.size:
+            raise ValueError("one target page for each source page")
+        handles = ctypes.c_void_p * max(1, len(sources))
+        self._check(_ffi.lib().mfh_copy_pages(
+            self._ctx, handles(*[b.handle for b in destinations]),
+            handles(*[b.handle for b in sources]), len(sources),
+            source.ctypes.data_as(_ffi.c_u32_p), target.ctypes.data_as(_ffi.c_u32_p),
+            source.size))
+
+    def sample_rows(self, output: Buffer, logits: Buffer, uniforms: Buffer, params: Buffer,
+                    mask: Buffer | None = None) -> None:
+        self._check(_ffi.lib().mfh_sample_rows(self._ctx, output.handle, logits.handle,
+                                               uniforms.handle, params.handle, _h(mask)))
+
 
 # ---- operation descriptors (engine-api/src/backend.rs:128-383) -------------
 # Plain carriers: the library validates them with the reference's rules and
@@ -471,6 +526,32 @@ class GqaSpec:
 class GatedShortConvSpec:
     hidden: int
     width: int
+
+
+@dataclass(frozen=True)
+class PagedRopeSpec:
+    query_heads: int
+    key_value_heads: int
+    head_dim: int
+    interleaved: bool = False
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """mfh_rope_scaling; `kind` is one of ROPE_SCALINGS."""
+    kind: str = "none"
+    factor: float = 1.0
+    original_positions: float = 0.0
+    low: float = 0.0
+    high: float = 0.0
+    magnitude: float = 1.0
+
+    def struct(self) -> _ffi.RopeScaling:
+        return _ffi.RopeScaling(ROPE_SCALINGS.index(self.kind), self.factor,
+                                self.original_positions, self.low, self.high, self.magnitude)
+
+
+ROPE_SCALINGS = ("none", "linear", "ntk", "wavelength", "yarn")
 
 
 @dataclass

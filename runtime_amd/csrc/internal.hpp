@@ -94,6 +94,11 @@ struct mfh_ctx {
     size_t work_scratch_capacity = 0;
     void *digits_scratch = nullptr;
     size_t digits_scratch_capacity = 0;
+    // Paged attention's records.  A block that a captured graph writes is kept
+    // until the context ends, also where a later call needs a larger one.
+    void *paged_scratch = nullptr;
+    size_t paged_scratch_capacity = 0;
+    bool paged_scratch_captured = false;
     // This device's address of the allocation-free entry point's fixed
     // scratch array (noalloc.hip), looked up at mfh_create; null if the
     // lookup failed.
@@ -236,10 +241,18 @@ void *optional_block(mfh_ctx *ctx, size_t bytes, size_t *capacity);
 void *ids_scratch(mfh_ctx *ctx, size_t bytes);
 void *work_scratch(mfh_ctx *ctx, size_t bytes);
 void *digits_scratch(mfh_ctx *ctx, size_t bytes);
+// Like the others, but safe to record in a graph: under stream capture nothing is
+// asked of the driver (null where the block is too small and no idle one serves;
+// the reason is recorded), and what a graph holds is never another buffer's.
+void *paged_scratch(mfh_ctx *ctx, size_t bytes);
 // Whether digits_scratch(ctx, bytes) is within the limit as things stand (after a
 // refusal: with every idle block returned).  Allocates nothing.
 bool digits_scratch_fits(const mfh_ctx *ctx, size_t bytes);
 inline mfh_status allocation_failed(mfh_ctx *) { return MFH_RESOURCE_LIMIT; }
+
+// A zeroed U8 buffer.
+mfh_status alloc_zeroed_u8(mfh_ctx *ctx, const uint64_t *dims, uint32_t rank, mfh_alloc_class cls,
+                           mfh_buf **out);
 
 // An F32 rank-2 buffer of binary16 file values: the 2-byte values are
 // uploaded into the buffer's binary16 shadow and decoded to f32 on the

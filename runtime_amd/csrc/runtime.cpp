@@ -287,6 +287,38 @@ void *digits_scratch(mfh_ctx *ctx, size_t bytes)
     return grow(ctx, &ctx->digits_scratch, &ctx->digits_scratch_capacity, bytes);
 }
 
+void *paged_scratch(mfh_ctx *ctx, size_t bytes)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &capture) != hipSuccess) {
+        (void)hipGetLastError();
+        capture = hipStreamCaptureStatusNone;
+    }
+    const bool capturing = capture != hipStreamCaptureStatusNone;
+    if (bytes > ctx->paged_scratch_capacity) {
+        const size_t want = scratch_size(bytes);
+        void *p = nullptr;
+        size_t got = 0;
+        if (capturing) {
+            p = ctx->pool->take(want, &got);
+            if (!p) {
+                (void)fail(ctx, MFH_RESOURCE_LIMIT,
+                           "under stream capture the workspace must be there from an earlier call");
+                return nullptr;
+            }
+        } else if (acquire(ctx, want, &p, &got)) {
+            return nullptr;
+        }
+        if (!ctx->paged_scratch_captured)
+            release_block(ctx, nullptr, ctx->paged_scratch, ctx->paged_scratch_capacity);
+        ctx->paged_scratch = p;
+        ctx->paged_scratch_capacity = got;
+        ctx->paged_scratch_captured = false;
+    }
+    ctx->paged_scratch_captured = ctx->paged_scratch_captured || capturing;
+    return ctx->paged_scratch;
+}
+
 bool digits_scratch_fits(const mfh_ctx *ctx, size_t bytes)
 {
     return bytes <= ctx->digits_scratch_capacity || fits(ctx, scratch_size(bytes));
@@ -679,6 +711,20 @@ mfh_status mfh_upload_u8(mfh_ctx *ctx, const uint64_t *dims, uint32_t rank, cons
 }  // extern "C"
 
 namespace mfh {
+
+mfh_status alloc_zeroed_u8(mfh_ctx *ctx, const uint64_t *dims, uint32_t rank, mfh_alloc_class cls,
+                           mfh_buf **out)
+{
+    DeviceGuard guard(ctx->device);
+    mfh_status s = make_buffer(ctx, dims, rank, MFH_DTYPE_U8, cls, out);
+    if (s)
+        return s;
+    // Pool blocks are whole multiples of 256 bytes.
+    if ((*out)->bytes)
+        launch_fill_f32(ctx->stream, static_cast<float *>((*out)->dev), ((*out)->bytes + 3) / 4,
+                        0.0f);
+    return MFH_OK;
+}
 
 mfh_status upload_scales_f16(mfh_ctx *ctx, const uint64_t *dims, const uint16_t *bits,
                              size_t count, mfh_alloc_class cls, mfh_buf **out)

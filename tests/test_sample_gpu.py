@@ -1,0 +1,198 @@
+"""Sampling on the GPU against a plain implementation in 64 bits.
+
+Sums differ from the plain ones in their order only: by about 2^-53 of the
+weights' sum a term, so a choice differs where a uniform value lies that near a
+token's border, which no case here does (a border is hit with probability about
+2^-36 in the largest).
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from runtime_amd.backend import ExecutorError, HipBackend
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*words):
+    print(*words, flush=True)
+
+
+def token(logits, u, temperature, top_k, top_p, min_p, admitted=None):
+    x = logits.astype(np.float64)
+    if admitted is not None:
+        x = np.where(admitted, x, -np.inf)
+    if np.any(np.isnan(x)) or np.any(x == np.inf) or np.all(x == -np.inf):
+        return np.nan
+    if temperature == 0.0:
+        return float(np.argmax(x))
+    with np.errstate(over="ignore"):
+        weight = np.exp((x - x.max()) / temperature)
+    order = np.argsort(-x, kind="stable")
+    if top_k:
+        order = order[:int(top_k)]
+    reached = np.cumsum(weight[order])
+    order = order[:1 + np.searchsorted(reached[:-1], top_p * reached[-1], side="left")]
+    order = np.sort(order[weight[order] >= min_p])
+    reached = np.cumsum(weight[order])
+    return float(order[np.searchsorted(reached, u * reached[-1], side="right")])
+
+
+def run(backend, logits, uniforms, params, mask=None):
+    logits = np.asarray(logits, np.float32)
+    out = backend.allocate_f32((len(logits),))
+    backend.sample_rows(out, backend.upload_f32(logits.shape, logits),
+                        backend.upload_f32((len(logits),), uniforms),
+                        backend.upload_f32(np.shape(params), params),
+                        None if mask is None else
+                        backend.upload_u8_classified(mask.shape, mask))
+    return backend.read(out)
+
+
+def check(backend, logits, uniforms, params, admitted=None):
+    logits = np.asarray(logits, np.float32)
+    uniforms = np.asarray(uniforms, np.float32)
+    params = np.asarray(params, np.float32)
+    mask = None
+    if admitted is not None:
+        mask = np.packbits(admitted, axis=1, bitorder="little")
+    got = run(backend, logits, uniforms, params, mask)
+    rows = len(logits)
+    each = np.broadcast_to(params.astype(np.float64), (rows, 4))
+    allowed = [None] * rows if admitted is None else np.broadcast_to(admitted, logits.shape)
+    want = [token(l, float(u), *p, a) for l, u, p, a in zip(logits, uniforms, each, allowed)]
+    assert np.array_equal(got, np.array(want, np.float32), equal_nan=True), (
+        [(i, g, w) for i, (g, w) in enumerate(zip(got, want)) if not (g == w)][:5])
+
+
+SETTINGS = {"all": (1.0, 0, 1.0, 0.0), "greedy": (0.0, 5, 0.5, 0.1), "hot": (1.7, 0, 1.0, 0.0),
+            "k1": (0.8, 1, 1.0, 0.0), "k50": (0.8, 50, 1.0, 0.0), "k900": (1.2, 900, 1.0, 0.0),
+            "p": (0.9, 0, 0.9, 0.0), "p0": (0.9, 0, 0.0, 0.0), "p-low": (1.3, 0, 0.05, 0.0),
+            "p-high": (2.0, 0, 0.999, 0.0), "min": (1.1, 0, 1.0, 0.05),
+            "min1": (1.1, 0, 1.0, 1.0), "kp": (0.7, 64, 0.95, 0.0),
+            "everything": (0.9, 300, 0.97, 0.002), "cold": (0.01, 40, 0.9, 0.0),
+            "k-wide": (1.0, 10 ** 6, 0.8, 0.0), "k5000": (3.0, 5000, 0.9, 0.0)}
+
+
+@pytest.mark.parametrize("rounded", [False, True], ids=["", "ties"])
+@pytest.mark.parametrize("width", [1, 2, 63, 64, 65, 1000, 4096, 65536, 65537, 130003])
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_settings(backend, name, width, rounded):
+    say("sample", name, width, rounded)
+    rng = np.random.default_rng(width + 7 * len(name))
+    rows = 6 if width < 5000 else 3
+    logits = 2.5 * rng.standard_normal((rows, width))
+    logits[:, ::max(1, width // 20)] += 5
+    if rounded:
+        logits = np.round(logits * 4) / 4
+    uniforms = rng.random(rows).astype(np.float32)
+    uniforms[0] = 0.0
+    uniforms[-1] = np.float32(1 - 2.0 ** -24)
+    check(backend, logits, uniforms, [SETTINGS[name]])
+
+
+def test_rows_have_their_own_settings(backend):
+    rng = np.random.default_rng(1)
+    params = np.array(list(SETTINGS.values()) * 9, np.float32)
+    check(backend, 3 * rng.standard_normal((len(params), 2047)), rng.random(len(params)), params)
+
+
+@pytest.mark.parametrize("name", list(SETTINGS))
+@pytest.mark.parametrize("value", [0.0, -3.4028235e38, 3.4028235e38, -0.0, 1e-40])
+def test_equal_logits(backend, value, name):
+    """Every token ties: the first ones by index are kept."""
+    rng = np.random.default_rng(2)
+    logits = np.full((4, 3001), value, np.float32)
+    check(backend, logits, rng.random(4), [SETTINGS[name]])
+
+
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_zeros_of_both_signs_tie(backend, name):
+    rng = np.random.default_rng(3)
+    logits = np.where(rng.random((8, 777)) < 0.5, 0.0, -0.0)
+    check(backend, logits, rng.random(8), [SETTINGS[name]])
+
+
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_masked_tokens(backend, name):
+    """Logits of -infinity and of the lowest value, and a mask; what the mask
+    leaves out may hold anything."""
+    say("masked", name)
+    rng = np.random.default_rng(4)
+    logits = 2 * rng.standard_normal((6, 1501))
+    logits[rng.random(logits.shape) < 0.3] = -np.inf
+    logits[rng.random(logits.shape) < 0.3] = -3.4028235e38
+    uniforms = rng.random(6)
+    check(backend, logits, uniforms, [SETTINGS[name]])
+    for rows in (1, 6):
+        admitted = rng.random((rows, 1501)) < 0.2
+        admitted[:, 3] = True
+        wild = logits.copy()
+        wild[:, 3] = 1.0
+        wild[:, ~admitted.any(axis=0)] = np.nan
+        check(backend, wild, uniforms, [SETTINGS[name]], admitted)
+    only = np.zeros((1, 1501), bool)
+    only[0, 1500] = True
+    logits[:, 1500] = -3.0
+    check(backend, logits, uniforms, [SETTINGS[name]], only)
+
+
+def test_logits_far_apart(backend):
+    logits = np.full((3, 300), -3.4028235e38, np.float32)
+    logits[0, 7], logits[1, 9], logits[2, 11] = 3.4028235e38, 1e-38, -3.4e38
+    for name in ("all", "p", "kp", "cold", "hot"):
+        check(backend, logits, [0.0, 0.5, 0.999], [SETTINGS[name]])
+
+
+def test_bad_rows_give_nan(backend):
+    rng = np.random.default_rng(5)
+    logits = rng.standard_normal((14, 100)).astype(np.float32)
+    logits[0, 50], logits[1, 99], logits[2] = np.nan, np.inf, -np.inf
+    uniforms = np.full(14, 0.5, np.float32)
+    uniforms[3], uniforms[4], uniforms[5] = 1.0, -0.1, np.nan
+    params = np.tile(np.array([1.0, 10, 0.9, 0.1], np.float32), (14, 1))
+    params[6, 0], params[7, 0], params[8, 1], params[9, 1] = -1, np.inf, 1.5, -1
+    params[10, 2], params[11, 3], params[12, 1] = 1.5, np.nan, np.nan
+    got = run(backend, logits, uniforms, params)
+    assert np.all(np.isnan(got[:13])) and got[13] == token(logits[13], 0.5, 1.0, 10,
+                                                           float(np.float32(0.9)),
+                                                           float(np.float32(0.1)))
+    nothing = np.zeros((1, 13), np.uint8)
+    assert np.all(np.isnan(run(backend, logits, uniforms, params, nothing)))
+
+
+def test_the_whole_range_of_uniforms(backend):
+    """Every token is chosen by the uniforms of its weight."""
+    logits = np.log(np.array([[1, 2, 3, 4, 0.5, 5.5]], np.float64)).repeat(256, axis=0)
+    uniforms = (np.arange(256) + 0.5) / 256
+    check(backend, logits, uniforms, [(1.0, 0, 1.0, 0.0)])
+    check(backend, logits, uniforms, [(1.0, 4, 0.9, 0.0)])
+
+
+def test_no_rows(backend):
+    assert run(backend, np.zeros((0, 5)), np.zeros(0), np.ones((1, 4))).shape == (0,)
+
+
+def test_refusals(backend):
+    f = backend.allocate_f32
+
+    def refused(variant, out, logits, uniforms, params, mask=None):
+        with pytest.raises(ExecutorError) as error:
+            backend.sample_rows(out, logits, uniforms, params, mask)
+        assert error.value.variant == variant, error.value
+
+    ok = f((3,)), f((3, 10)), f((3,)), f((1, 4))
+    refused("InvalidShape", f((2,)), *ok[1:])
+    refused("InvalidShape", ok[0], f((30,)), *ok[2:])
+    refused("Unsupported", ok[0], f((3, 0)), *ok[2:])
+    refused("InvalidShape", *ok[:2], f((1,)), ok[3])
+    refused("InvalidShape", *ok[:3], f((2, 4)))
+    refused("InvalidShape", *ok[:3], f((3, 3)))
+    refused("InvalidShape", *ok, backend.upload_u8_classified((1, 3), [1, 2, 3]))
+    refused("InvalidShape", *ok, backend.upload_u8_classified((2,), [1, 2]))
+    refused("InvalidDType", *ok, f((1, 2)))
+    refused("InvalidArgument", ok[2], *ok[1:])
+    other = HipBackend(0, owner=9)
+    refused("WrongBackend", *ok[:3], other.allocate_f32((1, 4)))
+    other.close()
