@@ -13,6 +13,8 @@
 // that a second launch joins in block order, so results do not depend on timing.
 // A run touches at most two shared items, its first and its last: two records a
 // block.
+#include <type_traits>
+
 #include "kernels.hpp"
 #include "paged.hpp"
 
@@ -262,8 +264,8 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
                 const float most = fmaxf(before, wave_max(s));
                 // Where every score so far is -infinity, nothing is added.
                 const float base_line = most == -__builtin_inff() ? 0.0f : most;
-                const float e = lane < count ? expf(s - base_line) : 0.0f;
-                const float rescale = expf(before - base_line);
+                const float e = lane < count ? exp2f(s - base_line) : 0.0f;
+                const float rescale = exp2f(before - base_line);
                 prob[r * kGeneralKeys + lane] = e;
                 const float sum = wave_sum(e);
                 if (lane == 0) {
@@ -300,10 +302,437 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
     }
 }
 
+// ---- head widths that are multiples of 16, on matrix cores ------------------------
+//
+// A wave takes every fourth tile of a part: TILE = 16 NB keys.  Per tile,
+// S^T = K Q^T leaves query row j in lane column j (lane 16 q + j holds the
+// scores of keys 16 c + 4 q + r in register r of block c), the softmax follows
+// online in the row's four lanes, and O^T += V^T P^T takes those registers as
+// its second operand as they are.  Both first operands come straight from the
+// cache to registers: a lane's piece of a key row is the operand of S^T, and
+// its piece of a value row (the columns s j .. s j + s - 1 of a chunk of s
+// 16-column tiles) is, column by column, an operand row of s tiles of O^T, whose
+// rows are then columns s i + t.  No LDS and no barrier until the part ends.
+//
+// f32 caches run on v_mfma_f32_16x16x4_f32: exact products, f32 sums.
+// Binary16 caches run on v_mfma_f32_16x16x32_f16: keys and values are operands
+// as they are, queries and probabilities are the sum of two binary16 parts
+// (each part the nearest to what is left, so the two are within 2^-24 of the
+// value, f32's own rounding).  A query row is first scaled by a power of two to
+// below 2^15, so what is cut off is below 2^-39 of its largest element;
+// probabilities carry 2^15, so what is cut off is below 2^-40 of the largest.
+//
+// Loads of the next tile's keys are issued as soon as the products have read
+// this tile's, its values' likewise: each is in flight behind the other's
+// arithmetic, in the same registers.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = kBlock / 64;
+constexpr uint32_t kRowsMost = 16;
+constexpr float kProbabilityShift = 15.0f;
+
+template <bool HALF>
+constexpr int key_blocks(int)
+{
+    return HALF ? 2 : 1;
+}
+
+// Chunks of a value row: as many 16-column tiles as one load holds (16 bytes,
+// then 8, 4, 2).
+template <bool HALF>
+__host__ __device__ constexpr int chunk_tiles(int left)
+{
+    const int most = HALF ? 8 : 4;
+    int s = most;
+    while (s > left)
+        s /= 2;
+    return s;
+}
+
+// f(first tile, tiles) for each chunk of N tiles, both as constants.
+template <int N, bool HALF, int T = 0, typename F>
+__device__ __forceinline__ void for_chunks(F f)
+{
+    if constexpr (T < N) {
+        constexpr int S = chunk_tiles<HALF>(N - T);
+        f(std::integral_constant<int, T>{}, std::integral_constant<int, S>{});
+        for_chunks<N, HALF, T + S>(f);
+    }
+}
+
+// Maximum over a row's four lanes.
+__device__ __forceinline__ float lanes_max(float v)
+{
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// a and b as two binary16 parts each.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const v2h h = {_Float16(a), _Float16(b)};
+    const v2h l = {_Float16(a - float(h[0])), _Float16(b - float(h[1]))};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// D: head width.  SMALL: pages of 8 keys (else a page holds whole 16-key blocks).
+template <int D, bool HALF, bool SMALL>
+__global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel(PagedAttention p)
+{
+    static_assert(D % 16 == 0 && D <= 256, "head width of the matrix-core path");
+    using T = typename std::conditional<HALF, _Float16, float>::type;
+    constexpr int NB = key_blocks<HALF>(D);
+    constexpr uint32_t TILE = 16 * NB;
+    constexpr int U = HALF ? (D + 31) / 32 : D / 16;  // 16-byte pieces of a key row per lane
+    constexpr int N = D / 16;                         // 16-column tiles
+    constexpr int W = HALF ? (N + 1) / 2 : N;         // dwords of a value row per lane
+    extern __shared__ float lds[];
+    const uint32_t rows = p.rows;
+    float *part_out = lds;                               // [kWaves][rows][D]
+    float *part_stat = lds + kWaves * rows * D;          // [kWaves][16][2]
+    __shared__ int bad_any;
+
+    const uint32_t lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t shift = p.shape.page_shift, inside = p.shape.page_size() - 1;
+    const T *keys = static_cast<const T *>(p.key_pages);
+    const T *values = static_cast<const T *>(p.value_pages);
+    Run run;
+    if (!find_run(p, run))
+        return;
+    Part part;
+    while (next_part(p, run, part)) {
+        const uint32_t head0 = part.kv_head * p.group + part.row_tile * rows;
+        const uint32_t left = p.group - part.row_tile * rows;
+        const uint32_t mine = left < rows ? left : rows;
+        const float *table = p.tables + uint64_t(part.sequence) * p.max_pages;
+        const uint32_t last_key = part.length - 1;
+        const uint64_t head_offset = (uint64_t(part.kv_head) << shift) * D;
+        int bad = 0;
+
+        // Page ids of a tile's 16-key blocks: the one of all its keys, or with
+        // small pages those of the lane's key row and of its value rows.
+        struct Ids {
+            float key[NB], value[SMALL ? NB : 1];
+        };
+        const auto load_ids = [&](uint32_t k0) {
+            Ids ids;
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                if (SMALL) {
+                    const uint32_t a = k0 + 16 * c + j, b = k0 + 16 * c + 4 * q;
+                    ids.key[c] = table[(a < last_key ? a : last_key) >> shift];
+                    ids.value[c] = table[(b < last_key ? b : last_key) >> shift];
+                } else {
+                    const uint32_t a = k0 + 16 * c;
+                    ids.key[c] = reinterpret_cast<const __attribute__((address_space(4))) float *>(
+                        reinterpret_cast<uint64_t>(table))[(a < last_key ? a : last_key) >> shift];
+                }
+            }
+            return ids;
+        };
+        const auto page_base = [&](float id) {
+            const bool ok = valid_index(id, p.shape.pages);
+            bad |= !ok;
+            return uint64_t(ok ? uint32_t(id) : 0) * p.shape.stride() + head_offset;
+        };
+
+        uint32_t kr[NB][U][4];
+        uint32_t vr[4 * NB][W];
+        const auto load_keys = [&](const Ids &ids, uint32_t k0) {
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                const uint32_t a = k0 + 16 * c + j;
+                const uint32_t slot = (a < last_key ? a : last_key) & inside;
+                const T *row = keys + page_base(ids.key[c]) + slot * uint32_t(D);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    // Past the head's end (its width an odd number of 16s) a
+                    // lane reads columns that its query's zeros drop.
+                    uint32_t column = HALF ? 32 * u + 8 * q : 16 * u + 4 * q;
+                    if (D % 32 != 0 && HALF && u == U - 1 && q >= 2)
+                        column -= 16;
+                    const v4u piece = *reinterpret_cast<const v4u *>(row + column);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        kr[c][u][e] = piece[e];
+                }
+            }
+        };
+        const auto load_values = [&](const Ids &ids, uint32_t k0) {
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                const uint64_t base = page_base(SMALL ? ids.value[c] : ids.key[c]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t a = k0 + 16 * c + 4 * q + r;
+                    const uint32_t slot = (a < last_key ? a : last_key) & inside;
+                    const T *row = values + base + slot * uint32_t(D);
+                    uint32_t *to = vr[4 * c + r];
+                    for_chunks<N, HALF>([&](auto first_tile, auto tiles) {
+                        constexpr int t = first_tile, n = tiles;
+                        constexpr int bytes = n * int(sizeof(T)), w = HALF ? t / 2 : t;
+                        const T *at = row + 16 * t + n * j;
+                        if constexpr (bytes == 16) {
+                            const v4u piece = *reinterpret_cast<const v4u *>(at);
+                            to[w] = piece[0], to[w + 1] = piece[1];
+                            to[w + 2] = piece[2], to[w + 3] = piece[3];
+                        } else if constexpr (bytes == 8) {
+                            const v2u piece = *reinterpret_cast<const v2u *>(at);
+                            to[w] = piece[0], to[w + 1] = piece[1];
+                        } else if constexpr (bytes == 4) {
+                            to[w] = *reinterpret_cast<const uint32_t *>(at);
+                        } else {
+                            to[w] = *reinterpret_cast<const uint16_t *>(at);
+                        }
+                    });
+                }
+            }
+        };
+
+        const uint32_t first = part.begin + wave * TILE;
+        Ids ids = load_ids(first < part.end ? first : part.begin);
+        // The lane's row of queries; rows past the group are zero.
+        const float *query = p.query + (uint64_t(part.sequence) * p.query_heads + head0 + j) * D;
+        float qf[U][HALF ? 8 : 4];
+        float most = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < (HALF ? 8 : 4); e += 4) {
+                const uint32_t column = HALF ? 32 * u + 8 * q + e : 16 * u + 4 * q + e;
+                const bool there = j < mine && column < uint32_t(D);
+                const v4f piece =
+                    there ? *reinterpret_cast<const v4f *>(query + column) : v4f{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    qf[u][e + i] = piece[i];
+                    most = fmaxf(most, fabsf(piece[i]));
+                }
+            }
+        if (first < part.end) {
+            load_keys(ids, first);
+            load_values(ids, first);
+        }
+        float factor = p.scale;
+        uint32_t qh[HALF ? U : 1][4], ql[HALF ? U : 1][4];
+        if (HALF) {
+            most = lanes_max(most);
+            // 2^14 <= most 2^exponent < 2^15 (0 and infinities as they are).
+            int exponent = 0;
+            if (most > 0.0f && most < __builtin_inff())
+                exponent = 15 - (ilogbf(most) + 1);
+            factor = ldexpf(p.scale, -exponent);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    split_pair(ldexpf(qf[u][2 * e], exponent), ldexpf(qf[u][2 * e + 1], exponent),
+                               qh[u][e], ql[u][e]);
+        }
+
+        v4f o[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+            o[t] = v4f{0, 0, 0, 0};
+        float m = -__builtin_inff(), l = 0.0f;
+        for (uint32_t k0 = first; k0 < part.end; k0 += kWaves * TILE) {
+            const uint32_t next = k0 + kWaves * TILE;
+            const bool more = next < part.end;
+            ids = load_ids(more ? next : k0);
+            v4f s[NB];
+#pragma unroll
+            for (int c = 0; c < NB; ++c)
+                s[c] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    const v4u piece = {kr[c][u][0], kr[c][u][1], kr[c][u][2], kr[c][u][3]};
+                    if constexpr (HALF) {
+                        const v4u hi = {qh[u][0], qh[u][1], qh[u][2], qh[u][3]};
+                        const v4u lo = {ql[u][0], ql[u][1], ql[u][2], ql[u][3]};
+                        const v8h k = __builtin_bit_cast(v8h, piece);
+                        s[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            k, __builtin_bit_cast(v8h, lo), s[c], 0, 0, 0);
+                        s[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            k, __builtin_bit_cast(v8h, hi), s[c], 0, 0, 0);
+                    } else {
+                        const v4f k = __builtin_bit_cast(v4f, piece);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[u][e], s[c], 0, 0,
+                                                                        0);
+                    }
+                }
+            if (more)
+                load_keys(ids, next);
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int c = 0; c < NB; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = s[c][r] * factor;
+                    if (k0 + 16 * c + 4 * q + r >= part.end)
+                        v = -__builtin_inff();
+                    s[c][r] = v;
+                    top = fmaxf(top, v);
+                }
+            top = fmaxf(m, lanes_max(top));
+            // While every score is -infinity, nothing is added.
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            if (__any(top > m)) {
+                const float rescale = __builtin_amdgcn_exp2f(m - base);
+                l *= rescale;
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+                    o[t] *= rescale;
+                m = top;
+            }
+#pragma unroll
+            for (int c = 0; c < NB; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[c][r] =
+                        __builtin_amdgcn_exp2f(s[c][r] - (HALF ? base - kProbabilityShift : base));
+                    l += s[c][r];
+                }
+            if (k0 + TILE > part.end) {
+                // Rows past the end repeat the last key's: they may hold
+                // what a zero weight does not drop.
+#pragma unroll
+                for (int i = 0; i < 4 * NB; ++i)
+                    if (k0 + 16 * (i / 4) + 4 * q + i % 4 >= part.end)
+#pragma unroll
+                        for (int w = 0; w < W; ++w)
+                            vr[i][w] = 0;
+            }
+            if constexpr (HALF) {
+                v4u hi, lo;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t a, b;
+                    split_pair(s[h / 2][2 * (h % 2)], s[h / 2][2 * (h % 2) + 1], a, b);
+                    hi[h] = a, lo[h] = b;
+                }
+#pragma unroll
+                for (int t = 0; t < N; ++t) {
+                    v4u column;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        column[h] =
+                            __builtin_amdgcn_perm(vr[2 * h + 1][t / 2], vr[2 * h][t / 2],
+                                                  t % 2 ? 0x07060302u : 0x05040100u);
+                    const v8h v = __builtin_bit_cast(v8h, column);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(v8h, lo),
+                                                                  o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(v8h, hi),
+                                                                  o[t], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int t = 0; t < N; ++t)
+                            o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(vr[4 * c + r][t]), s[c][r], o[t], 0, 0, 0);
+            }
+            if (more)
+                load_values(ids, next);
+        }
+
+        // The waves' shares of the part, joined in their order.
+        l = lanes_sum(l);
+        __syncthreads();  // an earlier part's shares have been read
+        if (threadIdx.x == 0)
+            bad_any = 0;
+        if (j < mine) {
+            float *row = part_out + (wave * rows + j) * D;
+            for_chunks<N, HALF>([&](auto first_tile, auto tiles) {
+                constexpr int t0 = first_tile, n = tiles;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int t = 0; t < n; ++t)
+                        row[16 * t0 + n * (4 * q + r) + t] = o[t0 + t][r];
+            });
+        }
+        if (q == 0) {
+            part_stat[(wave * 16 + j) * 2] = m;
+            part_stat[(wave * 16 + j) * 2 + 1] = l;
+        }
+        __syncthreads();
+        if (bad)
+            bad_any = 1;
+        __syncthreads();
+        const float poison = bad_any ? __builtin_nanf("") : 0.0f;
+        float *out = part.whole
+                         ? p.out + (uint64_t(part.sequence) * p.query_heads + head0) * D
+                         : p.records + uint64_t(part.record) * rows * D;
+        for (uint32_t i = threadIdx.x; i < mine * D; i += kBlock) {
+            const uint32_t r = i / D;
+            float top = part_stat[r * 2];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w)
+                top = fmaxf(top, part_stat[(w * 16 + r) * 2]);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            float a = 0.0f, sum = poison;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float weight = __builtin_amdgcn_exp2f(part_stat[(w * 16 + r) * 2] - base);
+                a += weight * part_out[w * rows * D + i];
+                sum += weight * part_stat[(w * 16 + r) * 2 + 1];
+            }
+            out[i] = part.whole ? a / sum : a;
+            if (!part.whole && i % D == 0) {
+                float *stats = record_stats(p) + (uint64_t(part.record) * rows + r) * 2;
+                stats[0] = top;
+                stats[1] = sum;
+            }
+        }
+    }
+}
+
+// The kernel of a head width, or null.
+using Kernel = void (*)(PagedAttention);
+template <int D>
+Kernel mfma_kernel_of(bool half, bool small)
+{
+    return half ? (small ? paged_gqa_mfma_kernel<D, true, true> : paged_gqa_mfma_kernel<D, true, false>)
+                : (small ? paged_gqa_mfma_kernel<D, false, true>
+                         : paged_gqa_mfma_kernel<D, false, false>);
+}
+Kernel mfma_kernel(const PageShape &shape)
+{
+    const bool half = shape.half, small = shape.page_shift < 4;
+    switch (shape.head_dim) {
+    case 32: return mfma_kernel_of<32>(half, small);
+    case 64: return mfma_kernel_of<64>(half, small);
+    case 80: return mfma_kernel_of<80>(half, small);
+    case 96: return mfma_kernel_of<96>(half, small);
+    case 128: return mfma_kernel_of<128>(half, small);
+    case 256: return mfma_kernel_of<256>(half, small);
+    default: return nullptr;
+    }
+}
+
 // ---- the join --------------------------------------------------------------------
 
-// One block per (item, row).  Shared items: out = sum_i a_i e^(m_i - M) / sum_i l_i
-// e^(m_i - M) over the records, in block order.  Sequences without a key give
+// One block per (item, row).  Shared items: out = sum_i a_i 2^(m_i - M) / sum_i l_i
+// 2^(m_i - M) over the records, in block order.  Sequences without a key give
 // zeros, those whose length is invalid NaN.
 __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p)
 {
@@ -336,7 +765,7 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
     const float base_line = most == -__builtin_inff() ? 0.0f : most;
     float sum = 0.0f;
     for (uint32_t i = threadIdx.x & 63; i < share.count; i += 64)
-        sum += stats[2 * record(i) + 1] * expf(stats[2 * record(i)] - base_line);
+        sum += stats[2 * record(i) + 1] * exp2f(stats[2 * record(i)] - base_line);
     sum = wave_sum(sum);
     // Threads: `parts` interleaved shares of the records by up to kBlock columns.
     const uint32_t width = d < kBlock ? d : kBlock, parts = kBlock / width;
@@ -346,7 +775,7 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
         float a = 0.0f;
         if (mine < parts && c < d)
             for (uint32_t i = mine; i < share.count; i += parts)
-                a += p.records[record(i) * d + c] * expf(stats[2 * record(i)] - base_line);
+                a += p.records[record(i) * d + c] * exp2f(stats[2 * record(i)] - base_line);
         __syncthreads();
         if (mine < parts)
             part[threadIdx.x] = a;
@@ -364,10 +793,11 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
 bool paged_gqa_plan(PagedAttention &p, int cu_count)
 {
     const uint32_t d = p.shape.head_dim;
-    const uint32_t most_rows = kGeneralLds / d < 16 ? kGeneralLds / d : 16;
+    const bool mfma = mfma_kernel(p.shape) != nullptr;
+    const uint32_t most_rows = mfma || kGeneralLds / d >= kRowsMost ? kRowsMost : kGeneralLds / d;
     p.rows = p.group < most_rows ? p.group : most_rows;
     p.row_tiles = (p.group + p.rows - 1) / p.rows;
-    p.unit_keys = kGeneralKeys;
+    p.unit_keys = !mfma ? kGeneralKeys : p.shape.half ? 128 : 64;
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     const uint64_t longest = uint64_t(p.max_pages) << p.shape.page_shift;
     const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys;
@@ -392,7 +822,11 @@ void launch_paged_gqa(hipStream_t stream, const PagedAttention &p)
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     if (!items)
         return;
-    if (p.blocks) {
+    if (const Kernel kernel = p.blocks ? mfma_kernel(p.shape) : nullptr) {
+        const size_t bytes =
+            (size_t(kWaves) * p.rows * p.shape.head_dim + kWaves * 16 * 2) * sizeof(float);
+        kernel<<<p.blocks, kBlock, bytes, stream>>>(p);
+    } else if (p.blocks) {
         const size_t bytes =
             (2 * size_t(p.rows) * p.shape.head_dim + size_t(p.rows) * (kGeneralKeys + 3)) *
             sizeof(float);

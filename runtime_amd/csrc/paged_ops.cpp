@@ -342,7 +342,8 @@ mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
     p.max_pages = uint32_t(tables->dims[1]);
     p.query_heads = query_heads;
     p.group = query_heads / key_value_heads;
-    p.scale = 1.0f / std::sqrt(float(head_dim));
+    // Scores are formed times log2 e: the kernels take powers of two.
+    p.scale = float(1.4426950408889634 / std::sqrt(double(head_dim)));
     if (!paged_gqa_plan(p, ctx->cu_count))
         return fail(ctx, MFH_OVERFLOW, "paged attention extent exceeds the kernel index range");
     DeviceGuard guard(ctx->device);
