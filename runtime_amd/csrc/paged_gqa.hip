@@ -66,40 +66,79 @@ __device__ __forceinline__ uint32_t length_of(const PagedAttention &p, uint32_t 
     return uint64_t(v) <= (uint64_t(p.max_pages) << p.shape.page_shift) ? uint32_t(v) : UINT32_MAX;
 }
 
+// An item's place on the line: `item_units` for what every item costs, then its
+// units of keys.
 __device__ __forceinline__ uint32_t units_of(const PagedAttention &p, uint32_t length)
 {
-    return length == UINT32_MAX ? 0 : (length + p.unit_keys - 1) / p.unit_keys;
+    return length == UINT32_MAX || length == 0
+               ? 0
+               : (length + p.unit_keys - 1) / p.unit_keys + p.item_units;
 }
 
 // A block's place on the line of units.
 struct Run {
     uint32_t sequence, head;  // the item of the next unit
+    uint32_t length;          // of the sequence
     uint32_t unit;            // of that item
-    uint32_t at, end;         // on the line
-    uint32_t per;             // units of a block
+    uint32_t start, at, end;  // on the line
+    uint32_t total, blocks;   // units of the line, blocks that share them
 };
 
-// Adds up the sequences' units (every thread a run of sequences, then a scan
-// over threads) and finds the block's first unit.  False: nothing to do.
+// A block's units out of `total`, even to one, and whether it has any.
+__device__ __forceinline__ bool take_units(const PagedAttention &p, uint32_t total, Run &run)
+{
+    const uint32_t most = (total + p.least_units - 1) / p.least_units;
+    run.blocks = most < p.blocks ? most : p.blocks;
+    run.total = total;
+    if (blockIdx.x >= run.blocks)
+        return false;
+    run.start = run.at = uint32_t(uint64_t(blockIdx.x) * total / run.blocks);
+    run.end = uint32_t((uint64_t(blockIdx.x) + 1) * total / run.blocks);
+    return true;
+}
+
+// Adds up the sequences' units and finds the block's first one.  Up to 64
+// sequences are a scan over the lanes of each wave, without a barrier; more are a
+// run of sequences for every thread, then a scan over the block.  False, for
+// every thread: nothing to do.
 __device__ bool find_run(const PagedAttention &p, Run &run)
 {
-    __shared__ uint32_t sums[kBlock / 64];
-    __shared__ uint32_t found[3];
     const uint32_t heads = p.shape.kv_heads * p.row_tiles;
+    const uint32_t lane = threadIdx.x & 63;
+    const auto scan = [&](uint32_t v) {
+#pragma unroll
+        for (int offset = 1; offset < 64; offset <<= 1) {
+            const uint32_t other = __shfl_up(v, offset, 64);
+            if (int(lane) >= offset)
+                v += other;
+        }
+        return v;
+    };
+    if (p.sequences <= 64) {
+        const uint32_t length = lane < p.sequences ? length_of(p, lane) : 0;
+        const uint32_t units = units_of(p, length), upto = scan(units);
+        if (!take_units(p, __builtin_amdgcn_readlane(upto, 63) * heads, run))
+            return false;
+        const uint64_t past = __ballot(run.at < upto * heads);
+        const uint32_t s = __builtin_ctzll(past);
+        const uint32_t mine = __builtin_amdgcn_readlane(units, s);
+        const uint32_t inside = run.at - (__builtin_amdgcn_readlane(upto, s) - mine) * heads;
+        run.sequence = s;
+        run.length = __builtin_amdgcn_readlane(length, s);
+        run.head = inside / mine;
+        run.unit = inside % mine;
+        return true;
+    }
+    __shared__ uint32_t sums[kBlock / 64];
+    __shared__ uint32_t found[4];
     const uint32_t each = (p.sequences + kBlock - 1) / kBlock;
     const uint32_t first = threadIdx.x * each;
     const uint32_t last = first + each < p.sequences ? first + each : p.sequences;
     uint32_t mine = 0;
     for (uint32_t s = first; s < last; ++s)
         mine += units_of(p, length_of(p, s));
-    uint32_t upto = mine;  // inclusive scan over the wave
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) {
-        const uint32_t v = __shfl_up(upto, offset, 64);
-        if (int(threadIdx.x & 63) >= offset)
-            upto += v;
-    }
-    if ((threadIdx.x & 63) == 63)
+    uint32_t upto = scan(mine);
+    if (lane == 63)
         sums[threadIdx.x >> 6] = upto;
     __syncthreads();
     uint32_t total = 0;
@@ -109,30 +148,28 @@ __device__ bool find_run(const PagedAttention &p, Run &run)
             upto += sums[w];
         total += sums[w];
     }
-    total *= heads;
-    run.per = (total + p.blocks - 1) / p.blocks;
-    run.at = blockIdx.x * run.per;
-    if (run.at >= total)
-        return false;  // the same for every thread
-    run.end = run.at + run.per < total ? run.at + run.per : total;
+    if (!take_units(p, total * heads, run))
+        return false;
     uint32_t before = upto - mine;
     if (run.at >= before * heads && run.at < upto * heads) {
         for (uint32_t s = first; s < last; ++s) {
-            const uint32_t units = units_of(p, length_of(p, s));
+            const uint32_t length = length_of(p, s), units = units_of(p, length);
             if (run.at < (before + units) * heads) {
                 const uint32_t inside = run.at - before * heads;
                 found[0] = s;
-                found[1] = inside / units;
-                found[2] = inside % units;
+                found[1] = length;
+                found[2] = inside / units;
+                found[3] = inside % units;
                 break;
             }
             before += units;
         }
     }
     __syncthreads();
-    run.sequence = found[0];
-    run.head = found[1];
-    run.unit = found[2];
+    run.sequence = __builtin_amdgcn_readfirstlane(found[0]);
+    run.length = __builtin_amdgcn_readfirstlane(found[1]);
+    run.head = __builtin_amdgcn_readfirstlane(found[2]);
+    run.unit = __builtin_amdgcn_readfirstlane(found[3]);
     return true;
 }
 
@@ -145,34 +182,38 @@ struct Part {
     uint32_t record;       // where it is not
 };
 
-// The next part of a run, false at its end.  The block that holds an item's
-// first unit says how the item is shared.
+// The next part of a run, false at its end; it may have no keys (begin == end).  The
+// block that holds an item's first keys says how the item is shared.
 __device__ bool next_part(const PagedAttention &p, Run &run, Part &part)
 {
     if (run.at >= run.end)
         return false;
     const uint32_t heads = p.shape.kv_heads * p.row_tiles;
-    uint32_t length = length_of(p, run.sequence);
-    uint32_t units = units_of(p, length);
+    uint32_t units = units_of(p, run.length);
     while (!units) {  // at < end: another unit follows
-        ++run.sequence;
-        length = length_of(p, run.sequence);
-        units = units_of(p, length);
+        run.length = length_of(p, ++run.sequence);
+        units = units_of(p, run.length);
     }
+    const uint32_t length = run.length;
     const uint32_t left = units - run.unit;
     const uint32_t take = left < run.end - run.at ? left : run.end - run.at;
+    // Units of keys, past the item's own.
+    const uint32_t own = p.item_units;
+    const uint32_t begin = run.unit > own ? run.unit - own : 0;
+    const uint32_t end = run.unit + take > own ? run.unit + take - own : 0;
     part.sequence = run.sequence;
     part.kv_head = run.head / p.row_tiles;
     part.row_tile = run.head % p.row_tiles;
     part.item = run.sequence * heads + run.head;
     part.length = length;
-    part.begin = run.unit * p.unit_keys;
-    const uint32_t end = (run.unit + take) * p.unit_keys;
-    part.end = end < length ? end : length;
-    part.whole = take == units;
-    part.record = 2 * blockIdx.x + (run.at == blockIdx.x * run.per ? 0 : 1);
-    if (run.unit == 0 && threadIdx.x == 0) {
-        const uint32_t last = (run.at + units - 1) / run.per;
+    part.begin = begin * p.unit_keys;
+    part.end = end * p.unit_keys < length ? end * p.unit_keys : length;
+    part.whole = begin == 0 && end == units - own;
+    part.record = 2 * blockIdx.x + (run.at == run.start ? 0 : 1);
+    if (begin == 0 && end > 0 && threadIdx.x == 0) {
+        // The block that holds the item's last unit.
+        const uint64_t past = uint64_t(run.at - run.unit) + units;
+        const uint32_t last = uint32_t((past * run.blocks - 1) / run.total);
         item_shares(p)[part.item] = {part.record, part.whole ? 0 : last - blockIdx.x + 1};
     }
     run.at += take;
@@ -182,6 +223,7 @@ __device__ bool next_part(const PagedAttention &p, Run &run, Part &part)
         if (++run.head == heads) {
             run.head = 0;
             ++run.sequence;
+            run.length = run.at < run.end ? length_of(p, run.sequence) : 0;
         }
     }
     return true;
@@ -215,6 +257,8 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
         return;
     Part part;
     while (next_part(p, run, part)) {
+        if (part.begin == part.end)
+            continue;
         __syncthreads();
         const uint32_t head0 = part.kv_head * p.group + part.row_tile * rows;
         const uint32_t left = p.group - part.row_tile * rows;
@@ -386,9 +430,15 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// Blocks of the kernel that a CU holds, by its registers.
+constexpr int resident_blocks(int d, bool half)
+{
+    return d > 128 ? 1 : d > 96 && half ? 2 : d > 64 || half ? 3 : 4;
+}
+
 // D: head width.  SMALL: pages of 8 keys (else a page holds whole 16-key blocks).
 template <int D, bool HALF, bool SMALL>
-__global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel(PagedAttention p)
+__global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mfma_kernel(PagedAttention p)
 {
     static_assert(D % 16 == 0 && D <= 256, "head width of the matrix-core path");
     using T = typename std::conditional<HALF, _Float16, float>::type;
@@ -413,6 +463,8 @@ __global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel
         return;
     Part part;
     while (next_part(p, run, part)) {
+        if (part.begin == part.end)
+            continue;
         const uint32_t head0 = part.kv_head * p.group + part.row_tile * rows;
         const uint32_t left = p.group - part.row_tile * rows;
         const uint32_t mine = left < rows ? left : rows;
@@ -463,7 +515,7 @@ __global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel
                     uint32_t column = HALF ? 32 * u + 8 * q : 16 * u + 4 * q;
                     if (D % 32 != 0 && HALF && u == U - 1 && q >= 2)
                         column -= 16;
-                    const v4u piece = *reinterpret_cast<const v4u *>(row + column);
+                    const v4u piece = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(row + column));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         kr[c][u][e] = piece[e];
@@ -485,11 +537,11 @@ __global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel
                         constexpr int bytes = n * int(sizeof(T)), w = HALF ? t / 2 : t;
                         const T *at = row + 16 * t + n * j;
                         if constexpr (bytes == 16) {
-                            const v4u piece = *reinterpret_cast<const v4u *>(at);
+                            const v4u piece = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(at));
                             to[w] = piece[0], to[w + 1] = piece[1];
                             to[w + 2] = piece[2], to[w + 3] = piece[3];
                         } else if constexpr (bytes == 8) {
-                            const v2u piece = *reinterpret_cast<const v2u *>(at);
+                            const v2u piece = __builtin_nontemporal_load(reinterpret_cast<const v2u *>(at));
                             to[w] = piece[0], to[w + 1] = piece[1];
                         } else if constexpr (bytes == 4) {
                             to[w] = *reinterpret_cast<const uint32_t *>(at);
@@ -706,16 +758,21 @@ __global__ __launch_bounds__(kBlock, D > 128 ? 1 : 2) void paged_gqa_mfma_kernel
     }
 }
 
-// The kernel of a head width, or null.
-using Kernel = void (*)(PagedAttention);
+// The kernel of a page shape (null: none) and the blocks of it that a CU holds.
+struct MfmaKernel {
+    void (*run)(PagedAttention) = nullptr;
+    int resident = 0;
+};
 template <int D>
-Kernel mfma_kernel_of(bool half, bool small)
+MfmaKernel mfma_kernel_of(bool half, bool small)
 {
-    return half ? (small ? paged_gqa_mfma_kernel<D, true, true> : paged_gqa_mfma_kernel<D, true, false>)
-                : (small ? paged_gqa_mfma_kernel<D, false, true>
-                         : paged_gqa_mfma_kernel<D, false, false>);
+    if (half)
+        return {small ? paged_gqa_mfma_kernel<D, true, true> : paged_gqa_mfma_kernel<D, true, false>,
+                resident_blocks(D, true)};
+    return {small ? paged_gqa_mfma_kernel<D, false, true> : paged_gqa_mfma_kernel<D, false, false>,
+            resident_blocks(D, false)};
 }
-Kernel mfma_kernel(const PageShape &shape)
+MfmaKernel mfma_kernel(const PageShape &shape)
 {
     const bool half = shape.half, small = shape.page_shift < 4;
     switch (shape.head_dim) {
@@ -725,24 +782,33 @@ Kernel mfma_kernel(const PageShape &shape)
     case 96: return mfma_kernel_of<96>(half, small);
     case 128: return mfma_kernel_of<128>(half, small);
     case 256: return mfma_kernel_of<256>(half, small);
-    default: return nullptr;
+    default: return {};
     }
 }
 
 // ---- the join --------------------------------------------------------------------
 
 // One block per (item, row).  Shared items: out = sum_i a_i 2^(m_i - M) / sum_i l_i
-// 2^(m_i - M) over the records, in block order.  Sequences without a key give
-// zeros, those whose length is invalid NaN.
+// 2^(m_i - M) over the records.  Sequences without a key give zeros, those whose
+// length is invalid NaN.  The records' weights are formed once; then the threads
+// are as many shares of the records as rows of V-column pieces fit the block
+// (V = 4 where the head width allows), each summed in record order, and the
+// shares in order.  Bound by three dependent reads, of what other XCDs' blocks
+// wrote, of which the last fetches all records at once.
+template <int V>
 __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p)
 {
-    extern __shared__ float part[];  // [parts][width]
+    typedef float piece __attribute__((ext_vector_type(V)));
+    __shared__ float weight[kBlock];
+    __shared__ float scratch[2 * kBlock / 64];
+    __shared__ piece sums[kBlock];
     const uint32_t heads = p.shape.kv_heads * p.row_tiles, d = p.shape.head_dim;
     const uint32_t item = blockIdx.x / p.rows, row = blockIdx.x % p.rows;
     const uint32_t sequence = item / heads, head = item % heads;
     const uint32_t in_group = head % p.row_tiles * p.rows + row;
     if (in_group >= p.group)
         return;
+    const ItemShare share = item_shares(p)[item];  // unset where there is no key
     float *out = p.out + (uint64_t(sequence) * p.query_heads +
                           head / p.row_tiles * p.group + in_group) * d;
     const uint32_t length = length_of(p, sequence);
@@ -751,39 +817,65 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
             out[c] = length ? __builtin_nanf("") : 0.0f;
         return;
     }
-    const ItemShare share = item_shares(p)[item];
     if (!share.count)
         return;
     const auto record = [&](uint32_t i) {
         return uint64_t(i ? share.first / 2 * 2 + 2 * i : share.first) * p.rows + row;
     };
-    const float *stats = record_stats(p);
-    float most = -__builtin_inff();
-    for (uint32_t i = threadIdx.x & 63; i < share.count; i += 64)
-        most = fmaxf(most, stats[2 * record(i)]);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
+    v2f own = {-__builtin_inff(), 0.0f};  // the thread's record of the first kBlock
+    if (threadIdx.x < share.count)
+        own = stats[record(threadIdx.x)];
+    float most = own[0];
+    for (uint32_t i = threadIdx.x + kBlock; i < share.count; i += kBlock)
+        most = fmaxf(most, stats[record(i)][0]);
     most = wave_max(most);
-    const float base_line = most == -__builtin_inff() ? 0.0f : most;
-    float sum = 0.0f;
-    for (uint32_t i = threadIdx.x & 63; i < share.count; i += 64)
-        sum += stats[2 * record(i) + 1] * exp2f(stats[2 * record(i)] - base_line);
-    sum = wave_sum(sum);
-    // Threads: `parts` interleaved shares of the records by up to kBlock columns.
-    const uint32_t width = d < kBlock ? d : kBlock, parts = kBlock / width;
+    if (lane == 0)
+        scratch[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kBlock / 64; ++w)
+        most = fmaxf(most, scratch[w]);
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    const uint32_t columns = d / V;
+    const uint32_t width = columns < kBlock ? columns : kBlock, shares = kBlock / width;
     const uint32_t mine = threadIdx.x / width;
-    for (uint32_t c0 = 0; c0 < d; c0 += width) {
+    float sum = 0.0f;
+    for (uint32_t c0 = 0; c0 < columns; c0 += width) {
         const uint32_t c = c0 + threadIdx.x % width;
-        float a = 0.0f;
-        if (mine < parts && c < d)
-            for (uint32_t i = mine; i < share.count; i += parts)
-                a += p.records[record(i) * d + c] * exp2f(stats[2 * record(i)] - base_line);
+        piece a = {};
+        for (uint32_t i0 = 0; i0 < share.count; i0 += kBlock) {
+            const uint32_t count = share.count - i0 < kBlock ? share.count - i0 : kBlock;
+            __syncthreads();
+            if (threadIdx.x < count) {
+                const v2f stat = i0 ? stats[record(i0 + threadIdx.x)] : own;
+                weight[threadIdx.x] = __builtin_amdgcn_exp2f(stat[0] - base);
+                if (c0 == 0)
+                    sum += stat[1] * weight[threadIdx.x];
+            }
+            __syncthreads();
+            if (mine < shares && c < columns)
+#pragma unroll 8
+                for (uint32_t i = mine; i < count; i += shares)
+                    a += weight[i] *
+                         *reinterpret_cast<const piece *>(p.records + record(i0 + i) * d + c * V);
+        }
+        sums[threadIdx.x] = a;
+        if (c0 == 0) {
+            sum = wave_sum(sum);
+            if (lane == 0)
+                scratch[kBlock / 64 + wave] = sum;
+        }
         __syncthreads();
-        if (mine < parts)
-            part[threadIdx.x] = a;
-        __syncthreads();
-        if (threadIdx.x < width && c < d) {
-            for (uint32_t i = 1; i < parts; ++i)
-                a += part[i * width + threadIdx.x];
-            out[c] = a / sum;
+        if (threadIdx.x < width && c < columns) {
+            for (uint32_t i = 1; i < shares; ++i)
+                a += sums[i * width + threadIdx.x];
+            float total = scratch[kBlock / 64];
+#pragma unroll
+            for (uint32_t w = 1; w < kBlock / 64; ++w)
+                total += scratch[kBlock / 64 + w];
+            *reinterpret_cast<piece *>(out + c * V) = a / total;
         }
     }
 }
@@ -793,20 +885,26 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
 bool paged_gqa_plan(PagedAttention &p, int cu_count)
 {
     const uint32_t d = p.shape.head_dim;
-    const bool mfma = mfma_kernel(p.shape) != nullptr;
-    const uint32_t most_rows = mfma || kGeneralLds / d >= kRowsMost ? kRowsMost : kGeneralLds / d;
+    const MfmaKernel mfma = mfma_kernel(p.shape);
+    const uint32_t most_rows =
+        mfma.run || kGeneralLds / d >= kRowsMost ? kRowsMost : kGeneralLds / d;
     p.rows = p.group < most_rows ? p.group : most_rows;
     p.row_tiles = (p.group + p.rows - 1) / p.rows;
-    p.unit_keys = !mfma ? kGeneralKeys : p.shape.half ? 128 : 64;
+    // A unit is a wave's tile, and a block has one for each wave at least; all
+    // blocks are resident at once.
+    p.unit_keys = !mfma.run ? kGeneralKeys : p.shape.half ? 32 : 16;
+    p.least_units = mfma.run ? kWaves : 1;
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     const uint64_t longest = uint64_t(p.max_pages) << p.shape.page_shift;
-    const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys;
-    const uint64_t limit = uint64_t(1) << 31;
-    if (items * p.rows > limit || per_item > limit || (per_item && items > limit / per_item))
+    p.item_units = mfma.run ? 3 : 0;
+    const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys + p.item_units;
+    // Units stay in 32 bits; the join's launch has 256 threads for each row.
+    if (items * p.rows > (uint64_t(1) << 23) ||
+        (per_item && items > (uint64_t(1) << 31) / per_item))
         return false;
-    // What the block's end and the last block's start reach stays in 32 bits.
-    const uint64_t most_blocks = uint64_t(cu_count) * 4, units = items * per_item;
-    p.blocks = uint32_t(units < most_blocks ? units : most_blocks);
+    const uint64_t most_blocks = uint64_t(cu_count) * (mfma.run ? mfma.resident : 4);
+    const uint64_t wanted = (items * per_item + p.least_units - 1) / p.least_units;
+    p.blocks = uint32_t(wanted < most_blocks ? wanted : most_blocks);
     return true;
 }
 
@@ -822,10 +920,11 @@ void launch_paged_gqa(hipStream_t stream, const PagedAttention &p)
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     if (!items)
         return;
-    if (const Kernel kernel = p.blocks ? mfma_kernel(p.shape) : nullptr) {
+    const MfmaKernel mfma = mfma_kernel(p.shape);
+    if (p.blocks && mfma.run) {
         const size_t bytes =
             (size_t(kWaves) * p.rows * p.shape.head_dim + kWaves * 16 * 2) * sizeof(float);
-        kernel<<<p.blocks, kBlock, bytes, stream>>>(p);
+        mfma.run<<<p.blocks, kBlock, bytes, stream>>>(p);
     } else if (p.blocks) {
         const size_t bytes =
             (2 * size_t(p.rows) * p.shape.head_dim + size_t(p.rows) * (kGeneralKeys + 3)) *
@@ -835,7 +934,11 @@ void launch_paged_gqa(hipStream_t stream, const PagedAttention &p)
         else
             paged_gqa_general_kernel<float><<<p.blocks, kBlock, bytes, stream>>>(p);
     }
-    paged_gqa_join_kernel<<<unsigned(items * p.rows), kBlock, kBlock * sizeof(float), stream>>>(p);
+    const unsigned blocks = unsigned(items * p.rows);
+    if (p.shape.head_dim % 4 == 0)
+        paged_gqa_join_kernel<4><<<blocks, kBlock, 0, stream>>>(p);
+    else
+        paged_gqa_join_kernel<1><<<blocks, kBlock, 0, stream>>>(p);
 }
 
 }  // namespace mfh
