@@ -137,7 +137,7 @@ SIGNATURES = {
     "mfh_paged_qk_norm_rope": (S, [P] * 13 + [ctypes.c_uint32] * 3 + [ctypes.c_int,
                                                                       ctypes.c_float]),
     "mfh_paged_gqa": (S, [P] * 7 + [ctypes.c_uint32] * 3),
-    "mfh_copy_pages": (S, [P, PP, PP, SZ, c_u32_p, c_u32_p, SZ]),
+    "mfh_copy_pages": (S, [P, PP, PP, SZ, P, P, SZ]),
     "mfh_sample_rows": (S, [P] * 6),
     # LFM2 token pass (minifield_lfm2.h)
     "mfl_create": (S, [P, ctypes.POINTER(MflConfig), PP]),

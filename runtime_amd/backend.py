@@ -477,11 +477,11 @@ class HipBackend:
         if source.size != target.size:
             raise ValueError("one target page for each source page")
         handles = ctypes.c_void_p * max(1, len(sources))
+        to = handles(*[b.handle for b in destinations])
+        of = to if sources is destinations else handles(*[b.handle for b in sources])
         self._check(_ffi.lib().mfh_copy_pages(
-            self._ctx, handles(*[b.handle for b in destinations]),
-            handles(*[b.handle for b in sources]), len(sources),
-            source.ctypes.data_as(_ffi.c_u32_p), target.ctypes.data_as(_ffi.c_u32_p),
-            source.size))
+            self._ctx, to, of, len(sources), source.__array_interface__["data"][0],
+            target.__array_interface__["data"][0], source.size))
 
     def sample_rows(self, output: Buffer, logits: Buffer, uniforms: Buffer, params: Buffer,
                     mask: Buffer | None = None) -> None:
