@@ -433,7 +433,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
 // Blocks of the kernel that a CU holds, by its registers.
 constexpr int resident_blocks(int d, bool half)
 {
-    return d > 128 ? 1 : d > 96 && half ? 2 : d > 64 || half ? 3 : 4;
+    return d > 128 ? 1 : d <= 64 ? 4 : half ? 2 : 3;
 }
 
 // D: head width.  SMALL: pages of 8 keys (else a page holds whole 16-key blocks).
@@ -553,8 +553,10 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
             }
         };
 
+        // The wave's tiles; one without any takes the part's first without a key.
         const uint32_t first = part.begin + wave * TILE;
-        Ids ids = load_ids(first < part.end ? first : part.begin);
+        const bool any = first < part.end;
+        Ids ids = load_ids(any ? first : part.begin);
         // The lane's row of queries; rows past the group are zero.
         const float *query = p.query + (uint64_t(part.sequence) * p.query_heads + head0 + j) * D;
         float qf[U][HALF ? 8 : 4];
@@ -573,10 +575,6 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
                     most = fmaxf(most, fabsf(piece[i]));
                 }
             }
-        if (first < part.end) {
-            load_keys(ids, first);
-            load_values(ids, first);
-        }
         float factor = p.scale;
         uint32_t qh[HALF ? U : 1][4], ql[HALF ? U : 1][4];
         if (HALF) {
@@ -599,10 +597,11 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
         for (int t = 0; t < N; ++t)
             o[t] = v4f{0, 0, 0, 0};
         float m = -__builtin_inff(), l = 0.0f;
-        for (uint32_t k0 = first; k0 < part.end; k0 += kWaves * TILE) {
+        const auto tile = [&](uint32_t k0, auto last) {
+            constexpr bool LAST = last;
             const uint32_t next = k0 + kWaves * TILE;
-            const bool more = next < part.end;
-            ids = load_ids(more ? next : k0);
+            if constexpr (!LAST)
+                ids = load_ids(next);
             v4f s[NB];
 #pragma unroll
             for (int c = 0; c < NB; ++c)
@@ -628,7 +627,7 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
                                                                         0);
                     }
                 }
-            if (more)
+            if constexpr (!LAST)
                 load_keys(ids, next);
             float top = -__builtin_inff();
 #pragma unroll
@@ -636,7 +635,7 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float v = s[c][r] * factor;
-                    if (k0 + 16 * c + 4 * q + r >= part.end)
+                    if (LAST && k0 + 16 * c + 4 * q + r >= part.end)
                         v = -__builtin_inff();
                     s[c][r] = v;
                     top = fmaxf(top, v);
@@ -660,7 +659,7 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
                         __builtin_amdgcn_exp2f(s[c][r] - (HALF ? base - kProbabilityShift : base));
                     l += s[c][r];
                 }
-            if (k0 + TILE > part.end) {
+            if (LAST && k0 + TILE > part.end) {
                 // Rows past the end repeat the last key's: they may hold
                 // what a zero weight does not drop.
 #pragma unroll
@@ -702,8 +701,20 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
                             o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                                 __uint_as_float(vr[4 * c + r][t]), s[c][r], o[t], 0, 0, 0);
             }
-            if (more)
+            if constexpr (!LAST)
                 load_values(ids, next);
+        };
+        // The last tile apart: it alone has keys past the end, and without a
+        // condition on the others' loads the compiler knows how many are in flight
+        // and waits for no more than it needs.
+        if (any) {
+            load_keys(ids, first);
+            load_values(ids, first);
+            uint32_t k0 = first;
+#pragma unroll 1
+            for (; k0 + kWaves * TILE < part.end; k0 += kWaves * TILE)
+                tile(k0, std::false_type{});
+            tile(k0, std::true_type{});
         }
 
         // The waves' shares of the part, joined in their order.
@@ -788,21 +799,21 @@ MfmaKernel mfma_kernel(const PageShape &shape)
 
 // ---- the join --------------------------------------------------------------------
 
-// One block per (item, row).  Shared items: out = sum_i a_i 2^(m_i - M) / sum_i l_i
+// One wave per (item, row).  Shared items: out = sum_i a_i 2^(m_i - M) / sum_i l_i
 // 2^(m_i - M) over the records.  Sequences without a key give zeros, those whose
-// length is invalid NaN.  The records' weights are formed once; then the threads
-// are as many shares of the records as rows of V-column pieces fit the block
-// (V = 4 where the head width allows), each summed in record order, and the
-// shares in order.  Bound by three dependent reads, of what other XCDs' blocks
-// wrote, of which the last fetches all records at once.
+// length is invalid NaN.  Lanes are as many shares of the records as rows of
+// V-column pieces fit the wave (V = 4 where the head width allows), each summed in
+// record order, and the shares in order; lane i forms the weight of record i of
+// 64.  Bound by three dependent reads, of what other XCDs' blocks wrote, and by
+// the code's own fetch: a block of 256 threads with barriers took 5.1 to 6.1 us
+// where this takes 3.9 to 5.0, and holding the first records while the weights are
+// formed, one read less, 5.8 to 10.7.
 template <int V>
-__global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p)
+__global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
 {
     typedef float piece __attribute__((ext_vector_type(V)));
-    __shared__ float weight[kBlock];
-    __shared__ float scratch[2 * kBlock / 64];
-    __shared__ piece sums[kBlock];
     const uint32_t heads = p.shape.kv_heads * p.row_tiles, d = p.shape.head_dim;
+    const uint32_t lane = threadIdx.x;
     const uint32_t item = blockIdx.x / p.rows, row = blockIdx.x % p.rows;
     const uint32_t sequence = item / heads, head = item % heads;
     const uint32_t in_group = head % p.row_tiles * p.rows + row;
@@ -813,7 +824,7 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
                           head / p.row_tiles * p.group + in_group) * d;
     const uint32_t length = length_of(p, sequence);
     if (length == 0 || length == UINT32_MAX) {
-        for (uint32_t c = threadIdx.x; c < d; c += kBlock)
+        for (uint32_t c = lane; c < d; c += 64)
             out[c] = length ? __builtin_nanf("") : 0.0f;
         return;
     }
@@ -822,61 +833,64 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_join_kernel(PagedAttention p
     const auto record = [&](uint32_t i) {
         return uint64_t(i ? share.first / 2 * 2 + 2 * i : share.first) * p.rows + row;
     };
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
-    v2f own = {-__builtin_inff(), 0.0f};  // the thread's record of the first kBlock
-    if (threadIdx.x < share.count)
-        own = stats[record(threadIdx.x)];
+    v2f own = {-__builtin_inff(), 0.0f};  // the lane's of the first 64
+    if (lane < share.count)
+        own = stats[record(lane)];
     float most = own[0];
-    for (uint32_t i = threadIdx.x + kBlock; i < share.count; i += kBlock)
+    for (uint32_t i = lane + 64; i < share.count; i += 64)
         most = fmaxf(most, stats[record(i)][0]);
     most = wave_max(most);
-    if (lane == 0)
-        scratch[wave] = most;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kBlock / 64; ++w)
-        most = fmaxf(most, scratch[w]);
     const float base = most == -__builtin_inff() ? 0.0f : most;
     const uint32_t columns = d / V;
-    const uint32_t width = columns < kBlock ? columns : kBlock, shares = kBlock / width;
-    const uint32_t mine = threadIdx.x / width;
-    float sum = 0.0f;
+    const uint32_t width = columns < 64 ? columns : 64, shares = 64 / width;
+    const uint32_t mine = lane / width;  // lanes past the last share add to none
+    float total = 0.0f;
+#pragma unroll 1
     for (uint32_t c0 = 0; c0 < columns; c0 += width) {
-        const uint32_t c = c0 + threadIdx.x % width;
+        const uint32_t c = c0 + lane % width;
         piece a = {};
-        for (uint32_t i0 = 0; i0 < share.count; i0 += kBlock) {
-            const uint32_t count = share.count - i0 < kBlock ? share.count - i0 : kBlock;
-            __syncthreads();
-            if (threadIdx.x < count) {
-                const v2f stat = i0 ? stats[record(i0 + threadIdx.x)] : own;
-                weight[threadIdx.x] = __builtin_amdgcn_exp2f(stat[0] - base);
-                if (c0 == 0)
-                    sum += stat[1] * weight[threadIdx.x];
-            }
-            __syncthreads();
-            if (mine < shares && c < columns)
-#pragma unroll 8
-                for (uint32_t i = mine; i < count; i += shares)
-                    a += weight[i] *
-                         *reinterpret_cast<const piece *>(p.records + record(i0 + i) * d + c * V);
-        }
-        sums[threadIdx.x] = a;
-        if (c0 == 0) {
-            sum = wave_sum(sum);
-            if (lane == 0)
-                scratch[kBlock / 64 + wave] = sum;
-        }
-        __syncthreads();
-        if (threadIdx.x < width && c < columns) {
-            for (uint32_t i = 1; i < shares; ++i)
-                a += sums[i * width + threadIdx.x];
-            float total = scratch[kBlock / 64];
+#pragma unroll 1
+        for (uint32_t i0 = 0; i0 < share.count; i0 += 64) {
+            const uint32_t count = share.count - i0 < 64 ? share.count - i0 : 64;
+            v2f stat = own;
+            if (i0)
+                stat = lane < count ? stats[record(i0 + lane)] : v2f{-__builtin_inff(), 0.0f};
+            const float weight = __builtin_amdgcn_exp2f(stat[0] - base);
+            if (c0 == 0)
+                total += lane < count ? stat[1] * weight : 0.0f;
+            // kHeld records a lane in flight: loads without a condition, under
+            // which the compiler waits for each.
+            constexpr uint32_t kHeld = 8;
+#pragma unroll 1
+            for (uint32_t n = 0; n < count; n += kHeld * shares) {
+                piece held[kHeld];
 #pragma unroll
-            for (uint32_t w = 1; w < kBlock / 64; ++w)
-                total += scratch[kBlock / 64 + w];
-            *reinterpret_cast<piece *>(out + c * V) = a / total;
+                for (uint32_t u = 0; u < kHeld; ++u) {
+                    const uint32_t i = n + u * shares + mine;
+                    held[u] = *reinterpret_cast<const piece *>(
+                        p.records + record(i0 + (i < count ? i : count - 1)) * d +
+                        (c < columns ? c : 0) * V);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kHeld; ++u) {
+                    const uint32_t i = n + u * shares + mine;
+                    const float w = __shfl(weight, int(i & 63), 64);
+                    if (i < count)
+                        a += w * held[u];
+                }
+            }
         }
+        if (c0 == 0)
+            total = wave_sum(total);
+        piece sum = a;
+#pragma unroll 1
+        for (uint32_t s = 1; s < shares; ++s)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                sum[e] += __shfl(a[e], int((lane + s * width) & 63), 64);
+        if (mine == 0 && c < columns)
+            *reinterpret_cast<piece *>(out + c * V) = sum / total;
     }
 }
 
@@ -898,8 +912,8 @@ bool paged_gqa_plan(PagedAttention &p, int cu_count)
     const uint64_t longest = uint64_t(p.max_pages) << p.shape.page_shift;
     p.item_units = mfma.run ? 3 : 0;
     const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys + p.item_units;
-    // Units stay in 32 bits; the join's launch has 256 threads for each row.
-    if (items * p.rows > (uint64_t(1) << 23) ||
+    // Units stay in 32 bits, and so do the join's threads, 64 for each row.
+    if (items * p.rows > (uint64_t(1) << 25) ||
         (per_item && items > (uint64_t(1) << 31) / per_item))
         return false;
     const uint64_t most_blocks = uint64_t(cu_count) * (mfma.run ? mfma.resident : 4);
@@ -936,9 +950,9 @@ void launch_paged_gqa(hipStream_t stream, const PagedAttention &p)
     }
     const unsigned blocks = unsigned(items * p.rows);
     if (p.shape.head_dim % 4 == 0)
-        paged_gqa_join_kernel<4><<<blocks, kBlock, 0, stream>>>(p);
+        paged_gqa_join_kernel<4><<<blocks, 64, 0, stream>>>(p);
     else
-        paged_gqa_join_kernel<1><<<blocks, kBlock, 0, stream>>>(p);
+        paged_gqa_join_kernel<1><<<blocks, 64, 0, stream>>>(p);
 }
 
 }  // namespace mfh
