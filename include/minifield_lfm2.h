@@ -104,6 +104,18 @@ mfh_status mfl_sample(mfl_model *model);
  * buffer of `steps` elements; nothing is read back to the host. */
 mfh_status mfl_generate(mfl_model *model, uint32_t steps, mfh_buf *ids_out);
 
+/* As mfl_sample, from a uniform value: mfh_sample_rows over the current logits
+ * with `uniform` F32 [1], `params` F32 [1, 4] (temperature, top_k, top_p, min_p)
+ * and `mask` (may be null) U8 [1, ceil(vocab / 8)]. */
+mfh_status mfl_sample_with(mfl_model *model, const mfh_buf *uniform, const mfh_buf *params,
+                           const mfh_buf *mask);
+
+/* As mfl_generate, from uniform values: step i samples with uniforms[i] (F32
+ * [steps]) and the same params and mask.  A row that mfh_sample_rows answers with
+ * NaN gives NaN ids from there on. */
+mfh_status mfl_generate_sampled(mfl_model *model, uint32_t steps, const mfh_buf *uniforms,
+                                const mfh_buf *params, const mfh_buf *mask, mfh_buf *ids_out);
+
 /* The model-owned logits [1, vocab] and sampled-id [1] buffers (valid until
  * mfl_destroy; readable with mfh_read_f32_async). */
 const mfh_buf *mfl_logits(const mfl_model *model);

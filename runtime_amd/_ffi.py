@@ -148,6 +148,8 @@ SIGNATURES = {
     "mfl_append": (S, [P, c_u32_p, SZ, P, ctypes.c_int]),
     "mfl_sample": (S, [P]),
     "mfl_generate": (S, [P, ctypes.c_uint32, P]),
+    "mfl_sample_with": (S, [P, P, P, P]),
+    "mfl_generate_sampled": (S, [P, ctypes.c_uint32, P, P, P, P]),
     "mfl_logits": (P, [P]),
     "mfl_sampled": (P, [P]),
     "mfl_snapshot": (S, [P, PP]),

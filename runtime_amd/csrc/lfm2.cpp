@@ -18,6 +18,7 @@
 #include "../../include/minifield_loader.h"
 #include "internal.hpp"
 #include "kernels.hpp"
+#include "paged.hpp"
 
 namespace mfh {
 namespace {
@@ -829,6 +830,47 @@ mfh_status mfl_generate(mfl_model *m, uint32_t steps, mfh_buf *ids_out)
         }
         if ((s = append(m, nullptr, 0, m->sampled.buf, true)))
             return s;
+    }
+    return MFH_OK;
+}
+
+mfh_status mfl_sample_with(mfl_model *m, const mfh_buf *uniform, const mfh_buf *params,
+                           const mfh_buf *mask)
+{
+    if (!m)
+        return MFH_INVALID_ARGUMENT;
+    return mfh_sample_rows(m->ctx, m->sampled.buf, m->logits.buf, uniform, params, mask);
+}
+
+mfh_status mfl_generate_sampled(mfl_model *m, uint32_t steps, const mfh_buf *uniforms,
+                                const mfh_buf *params, const mfh_buf *mask, mfh_buf *ids_out)
+{
+    if (!m)
+        return MFH_INVALID_ARGUMENT;
+    mfh_ctx *c = m->ctx;
+    Sampling call;
+    const uint64_t dims[1] = {steps};
+    mfh_status s = admit_sample_rows(c, m->sampled.buf, m->logits.buf, uniforms, steps, params,
+                                     mask, &call);
+    if (!s)
+        s = check_output(c, ids_out, dims, 1);
+    if (s)
+        return s;
+    if (aliases(ids_out, {uniforms, params, mask, m->logits.buf, m->sampled.buf}))
+        return fail(c, MFH_INVALID_ARGUMENT, "output aliases an input");
+    if (m->length + steps > m->config.max_tokens)
+        return fail(c, MFH_OUT_OF_BOUNDS, "append exceeds configured logical prefix capacity");
+    mark_written(ids_out);
+    call.copy = static_cast<float *>(ids_out->dev);
+    for (uint32_t i = 0; i < steps; ++i) {
+        {
+            DeviceGuard guard(c->device);
+            launch_sample_rows(c->stream, call);
+        }
+        if ((s = append(m, nullptr, 0, m->sampled.buf, true)))
+            return s;
+        ++call.uniforms;
+        ++call.copy;
     }
     return MFH_OK;
 }

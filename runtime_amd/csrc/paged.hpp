@@ -114,9 +114,10 @@ struct Sampling {
     bool one_params = false, one_mask = false;
 };
 void launch_sample_rows(hipStream_t stream, const Sampling &s);
-// mfh_sample_rows' admission: fills `call`, enqueues nothing.
+// mfh_sample_rows' admission, for `uniform_count` values in `uniforms` (a row's, or
+// those of several calls): fills `call`, enqueues nothing.
 mfh_status admit_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
-                             const mfh_buf *uniforms, const mfh_buf *params, const mfh_buf *mask,
-                             Sampling *call);
+                             const mfh_buf *uniforms, uint64_t uniform_count,
+                             const mfh_buf *params, const mfh_buf *mask, Sampling *call);
 
 }  // namespace mfh

@@ -454,7 +454,9 @@ mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
     if (!ctx)
         return MFH_INVALID_ARGUMENT;
     Sampling call;
-    mfh_status s = admit_sample_rows(ctx, output, logits, uniforms, params, mask, &call);
+    mfh_status s = check_f32(ctx, logits);
+    if (!s)
+        s = admit_sample_rows(ctx, output, logits, uniforms, logits->dims[0], params, mask, &call);
     if (s)
         return s;
     DeviceGuard guard(ctx->device);
@@ -468,8 +470,8 @@ mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
 namespace mfh {
 
 mfh_status admit_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
-                             const mfh_buf *uniforms, const mfh_buf *params, const mfh_buf *mask,
-                             Sampling *call)
+                             const mfh_buf *uniforms, uint64_t uniform_count,
+                             const mfh_buf *params, const mfh_buf *mask, Sampling *call)
 {
     mfh_status s = check_operation(ctx, MFH_OP_ARGMAX);
     if (!s)
@@ -482,7 +484,8 @@ mfh_status admit_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logit
     if (width == 0 || width > kIndexLimit)
         return fail(ctx, MFH_UNSUPPORTED,
                     "sampling width must be in [1, 2^24] for exact f32 indices");
-    if ((s = check_vector(ctx, uniforms, rows, "uniform values must be one per row")) ||
+    if ((s = check_vector(ctx, uniforms, uniform_count,
+                          "uniform values must be one per row and step")) ||
         (s = check_f32(ctx, params)))
         return s;
     if (params->rank != 2 || params->dims[1] != 4 || (params->dims[0] != rows && params->dims[0] != 1))

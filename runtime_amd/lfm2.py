@@ -168,6 +168,11 @@ class Lfm2Model:
     def sample(self) -> None:
         self.backend._check(_ffi.lib().mfl_sample(self._model))
 
+    def sample_with(self, uniform: Buffer, params: Buffer, mask: Buffer | None = None) -> None:
+        """Sample from the current logits (HipBackend.sample_rows' parameters)."""
+        self.backend._check(_ffi.lib().mfl_sample_with(
+            self._model, uniform.handle, params.handle, mask.handle if mask else None))
+
     def snapshot(self) -> "Lfm2Prefix":
         """An immutable copy of the current prefix state (mfl_snapshot)."""
         out = ctypes.c_void_p()
@@ -182,6 +187,16 @@ class Lfm2Model:
         """Greedy decode: returns the f32 device buffer of the `steps` ids."""
         ids = ids if ids is not None else self.backend.allocate_f32((steps,))
         self.backend._check(_ffi.lib().mfl_generate(self._model, steps, ids.handle))
+        return ids
+
+    def generate_sampled(self, steps: int, uniforms: Buffer, params: Buffer,
+                         mask: Buffer | None = None, ids: Buffer | None = None) -> Buffer:
+        """Sampled decode, one uniform value a step: returns the f32 device buffer
+        of the `steps` ids."""
+        ids = ids if ids is not None else self.backend.allocate_f32((steps,))
+        self.backend._check(_ffi.lib().mfl_generate_sampled(
+            self._model, steps, uniforms.handle, params.handle, mask.handle if mask else None,
+            ids.handle))
         return ids
 
 

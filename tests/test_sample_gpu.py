@@ -196,3 +196,56 @@ def test_refusals(backend):
     other = HipBackend(0, owner=9)
     refused("WrongBackend", *ok[:3], other.allocate_f32((1, 4)))
     other.close()
+
+
+def test_a_model_generates_sampled_tokens(backend):
+    """The device loop against its steps one by one, each token checked against
+    the logits it was drawn from."""
+    from runtime_amd.lfm2 import ATTENTION, CONV, Lfm2Config, Lfm2Model, synthetic_weights
+
+    cfg = Lfm2Config(hidden=256, intermediate=512, attention_heads=4, key_value_heads=2,
+                     vocab=1000, layers=[CONV, ATTENTION], max_tokens=64,
+                     formats={"embedding": "int8", "conv": "nf4", "attention": "nf4",
+                              "ffn": "ternary"})
+    model = Lfm2Model(backend, cfg)
+    synthetic_weights(model)
+    model.append([1, 2, 3, 4, 5])
+    prefix = model.snapshot()
+    rng = np.random.default_rng(12)
+    steps, settings = 9, (0.9, 40, 0.95, 0.01)
+    uniforms = rng.random(steps).astype(np.float32)
+    params = backend.upload_f32((1, 4), settings)
+    for admitted in (None, rng.random(1000) < 0.5):
+        mask = None
+        if admitted is not None:
+            bits = np.packbits(admitted[None], axis=1, bitorder="little")
+            mask = backend.upload_u8_classified(bits.shape, bits)
+        model.restore(prefix)
+        ids = backend.read(model.generate_sampled(steps, backend.upload_f32((steps,), uniforms),
+                                                  params, mask))
+        assert model.length == 5 + steps
+        model.restore(prefix)
+        for i in range(steps):
+            logits = backend.read(model.logits)[0]
+            model.sample_with(backend.upload_f32((1,), uniforms[i:i + 1]), params, mask)
+            want = token(logits, float(uniforms[i]), *(float(np.float32(p)) for p in settings),
+                         admitted)
+            assert backend.read(model.sampled)[0] == ids[i] == want
+            model.append(model.sampled)
+    model.restore(prefix)
+    bad = backend.upload_f32((1, 4), (-1.0, 40, 0.95, 0.01))
+    halves = backend.upload_f32((3,), [0.5] * 3)
+    assert np.isnan(backend.read(model.generate_sampled(3, halves, bad))).all()
+    one = backend.upload_f32((1,), [0.5])
+    for variant, call in [
+            ("InvalidShape", lambda: model.generate_sampled(3, one, params)),
+            ("InvalidShape", lambda: model.generate_sampled(1, one, one)),
+            ("InvalidShape", lambda: model.generate_sampled(1, one, params, ids=params)),
+            ("InvalidArgument", lambda: model.generate_sampled(1, one, params, ids=one)),
+            ("InvalidShape", lambda: model.sample_with(params, params)),
+            ("OutOfBounds", lambda: model.generate_sampled(
+                60, backend.allocate_f32((60,)), params))]:
+        with pytest.raises(ExecutorError) as error:
+            call()
+        assert error.value.variant == variant, error.value
+    model.close()
