@@ -21,8 +21,8 @@
 // bin in which the row's weight reaches the share is found from a histogram of
 // weights (whole numbers of 2^-46 or so, so that the order of additions does not
 // matter), its tokens are listed, and the cut is found among them.  The choice is
-// made from a list of the kept tokens, or, where they are more than it holds,
-// from sums of 256 tokens each.  Rows with more tokens about a cut than the list
+// made from a list of the tokens down to there, or, where they are more than it
+// holds, of all.  Rows with more tokens about a cut than the list
 // holds (many equal values, or a temperature far above the logits' spread) are
 // searched digit by digit of the values' order-preserving keys.
 //
@@ -40,11 +40,10 @@ namespace {
 constexpr int kBlock = 1024;
 constexpr int kWaves = kBlock / 64;
 constexpr uint32_t kChunk = 4 * kBlock;   // tokens of one float4 a thread
-constexpr uint32_t kSegmentChunks = 64;   // chunks whose sums LDS holds
+constexpr uint32_t kSegmentChunks = 32;   // chunks whose codes LDS holds
 // Bins of a histogram (44 temperatures: what lies below weighs less than 2^-63 of
 // the largest), tokens listed about a cut, tokens kept in a list.
 constexpr uint32_t kBins = 2048, kList = 2048, kMany = 16384;
-constexpr uint32_t kGroups = kSegmentChunks * kWaves;  // of 256 tokens, of a segment
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));  // rows of any width
@@ -125,18 +124,17 @@ struct Shared {
     union {
         uint64_t weight[kBins];
         uint32_t count[kBins];
-        uint64_t votes[kSegmentChunks * kChunk / 64];
+        uint64_t codes[kSegmentChunks * kBlock / 8];  // a byte for four tokens
     } bins;
     uint32_t index[kMany];
+    uint32_t pick[kList];
     float value[kList];
     double weight[kList];
     uint32_t sub[kList];
-    double group[kGroups];
-    double segment[(1u << 24) / (kSegmentChunks * kChunk)];
     uint64_t scratch[kWaves];
     float floats[kWaves];
     uint32_t flags[kWaves];
-    uint32_t found, below;
+    uint32_t found;
     uint64_t before;
     uint32_t reached;
 };
@@ -160,14 +158,13 @@ __device__ __forceinline__ Row row_of(Lds *sh)
     return row;
 }
 
-// The thread's four tokens of a chunk, -infinity where there is none or the mask
-// leaves it out.
-__device__ __forceinline__ v4f load_chunk(const Row &row, uint32_t c)
+// Tokens i .. i + 3, -infinity where there is none or the mask leaves it out;
+// `whole`: they are all there, for every thread.
+__device__ __forceinline__ v4f load_four(const Row &row, uint32_t i, bool whole)
 {
-    const uint32_t i = c * kChunk + 4 * threadIdx.x;
     constexpr float kNone = -__builtin_inff();
     v4f v;
-    if ((c + 1) * kChunk <= row.width) {
+    if (whole) {
         v = *(Global<v4f_any>)(row.logits + i);
     } else {
 #pragma unroll
@@ -185,6 +182,10 @@ __device__ __forceinline__ v4f load_chunk(const Row &row, uint32_t c)
             v[e] = bits >> e & 1 ? v[e] : kNone;
     }
     return v;
+}
+__device__ __forceinline__ v4f load_chunk(const Row &row, uint32_t c)
+{
+    return load_four(row, c * kChunk + 4 * threadIdx.x, (c + 1) * kChunk <= row.width);
 }
 
 // f(chunk, values) over chunks [begin, end), AHEAD chunks' loads in flight before
@@ -218,40 +219,41 @@ __device__ __forceinline__ void each_next(const Row &row, uint32_t begin, uint32
     }
 }
 
-// (v - from) / temperature in steps of ln 2 / 32, -65536 at the least; and raised by
-// 1.5 * 2^52, which leaves the nearest whole number in the low bits.
-constexpr double kRaise = 6755399441055744.0;
+// (v - from) / temperature in steps of ln 2 / 32, and its whole part (towards zero;
+// what an int does not hold, -infinity too, is its least or largest).
 __device__ __forceinline__ double steps_of(const Row &row, float v, double from)
 {
-    return __builtin_fmax((double(v) - from) * row.per_step, -65536.0);
+    return (double(v) - from) * row.per_step;
 }
-__device__ __forceinline__ int whole_of(double raised)
+__device__ __forceinline__ int whole_of(double steps)
 {
-    return int(uint32_t(__builtin_bit_cast(uint64_t, raised)));
+    int whole;
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(whole) : "v"(steps));
+    return whole;
 }
-// The bin of a value: whole steps below `from` (0 for what is above, kBins past the
+// The bin of that: whole steps below `from` (0 for what is above, kBins past the
 // range).  Monotone in v.
 __device__ __forceinline__ uint32_t bin_of(const Row &row, float v, double from)
 {
-    const int b = -whole_of(steps_of(row, v, from) + kRaise);
-    return b < 0 ? 0 : b < int(kBins) ? uint32_t(b) : kBins;
+    const int n = whole_of(steps_of(row, v, from));
+    const uint32_t b = 0u - uint32_t(n);
+    return n > 0 ? 0 : b < kBins ? b : kBins;
 }
 
-// exp((v - largest) / temperature) as 2^(n / 32) 2^(f / 32), |f| <= 1/2, the latter by
-// its series to the fifth power: within 2^-47 (the argument's own rounding, where
-// a weight matters, and 2^-48 of what the series leaves).  `steps`: -n.
+// exp((v - largest) / temperature) as 2^(n / 32) 2^(-f / 32), 0 <= f < 1, the latter
+// by the polynomial of fourth degree, 1 at 0, that is nearest to it (2^-43.3; the
+// argument's own rounding is less where a weight matters).  `steps`: n.  Of no
+// meaning for -infinity.
 __device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v, int *steps)
 {
-    constexpr double k = 0.021660849392498290;  // ln 2 / 32
-    const double t = steps_of(row, v, row.largest);
-    const double raised = t + kRaise, f = t - (raised - kRaise), f2 = f * f;
-    const double low = __builtin_fma(f, k, 1.0);
-    const double middle = __builtin_fma(f, k * k * k / 6, k * k / 2);
-    const double high = __builtin_fma(f, k * k * k * k * k / 120, k * k * k * k / 24);
-    const double e = __builtin_fma(__builtin_fma(high, f2, middle), f2, low);
-    const int whole = whole_of(raised);
-    *steps = -whole;
-    return __builtin_ldexp(sh->table[whole & 31] * e, whole >> 5);
+    const double t = steps_of(row, v, row.largest), f = __builtin_amdgcn_fract(-t);
+    const int n = whole_of(t);
+    double e = __builtin_fma(f, 9.076184072276023e-09, -1.6937700541791561e-06);
+    e = __builtin_fma(e, f, 0.0002345961713900732);
+    e = __builtin_fma(e, f, -0.021660849389733828);
+    e = __builtin_fma(e, f, 1.0);
+    *steps = n;
+    return __builtin_ldexp(sh->table[n & 31] * e, n >> 5);
 }
 __device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v)
 {
@@ -341,7 +343,11 @@ struct Units {
     }
     __device__ unsigned long long raised(double w) const
     {
-        return __builtin_bit_cast(uint64_t, w) - __builtin_bit_cast(uint64_t, shift);
+        // shift's low word is zero.
+        const uint64_t bits = __builtin_bit_cast(uint64_t, w);
+        const uint32_t high = uint32_t(bits >> 32);
+        return uint64_t(high - uint32_t(__builtin_bit_cast(uint64_t, shift) >> 32)) << 32 |
+               uint32_t(bits);
     }
 };
 
@@ -389,8 +395,8 @@ __device__ __attribute__((noinline)) void histogram(Lds *sh, uint32_t chunks, do
             asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (bin[e] < int(kBins))
-                    add_to_bin(sh, uint32_t(bin[e]), units.raised(w[e]));
+                if (bin[e] > -int(kBins))
+                    add_to_bin(sh, 0u - uint32_t(bin[e]), units.raised(w[e]));
         });
     __syncthreads();
 }
@@ -434,7 +440,7 @@ __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double
 __device__ __attribute__((noinline)) float edge_of(Lds *sh, uint32_t b, double from)
 {
     const Row row = row_of(sh);
-    const double reach = (double(b) + 0.5) / row.per_step, near = from - reach;
+    const double reach = (double(b) + 1.0) / row.per_step, near = from - reach;
     const double room = 1.5e-7 * __builtin_fabs(near) + 1e-12 * (__builtin_fabs(from) + reach);
     constexpr double kMost = 3.4028234663852886e38;
     uint32_t low = key_of(float(near - room > -kMost ? near - room : -kMost));
@@ -468,87 +474,90 @@ struct Cut {
     }
 };
 
-// The votes of a chunk's tokens for low <= v < high, to LDS: tokens are taken a
-// wave's 64 neighbours at a time, so that the words and their bits are in the
-// tokens' order.  f(value) is called for each.
+// Codes of chunks to LDS, a byte for a thread's four tokens: bit e for low <= v, and
+// bit 4 + e where also v < high.  f(values) is called for each.
+constexpr uint64_t kListed = 0x0f0f0f0f0f0f0f0full;
 template <typename F>
-__device__ __forceinline__ void vote_chunks(Lds *sh, const Row &row, uint32_t begin, uint32_t end,
+__device__ __forceinline__ void code_chunks(Lds *sh, const Row &row, uint32_t begin, uint32_t end,
                                             float low, float high, F f)
 {
-    constexpr uint32_t kRuns = kChunk / kBlock;  // of kBlock tokens, of a chunk
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool first_lane = (threadIdx.x & 63) == 0;
-#pragma unroll 1
-    for (uint32_t c = begin; c < end; c += 2) {
-        float v[2 * kRuns];
+    const auto codes = reinterpret_cast<__attribute__((address_space(3))) uint8_t *>(
+        &sh->bins.codes[0]);
+    each<4>(row, begin, end, [&](uint32_t c, v4f v) {
+        f(v);
+        uint32_t code = 0;
 #pragma unroll
-        for (uint32_t e = 0; e < 2 * kRuns; ++e) {
-            const uint32_t i = c * kChunk + e * kBlock + threadIdx.x;
-            v[e] = row.logits[i < row.width ? i : row.width - 1];
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t both = v[e] < high ? 0x11u << e : 1u << e;
+            code |= v[e] >= low ? both : 0;
         }
-#pragma unroll
-        for (uint32_t e = 0; e < 2 * kRuns; ++e) {
-            const uint32_t i = c * kChunk + e * kBlock + threadIdx.x;
-            v[e] = i < row.width ? v[e] : -__builtin_inff();
-        }
-        if (row.mask)
-#pragma unroll
-            for (uint32_t e = 0; e < 2 * kRuns; ++e) {
-                const uint32_t i = c * kChunk + e * kBlock + threadIdx.x;
-                const uint32_t at = i < row.width ? i : 0;
-                v[e] = row.mask[at >> 3] >> (at & 7) & 1 ? v[e] : -__builtin_inff();
-            }
-        uint64_t votes[2 * kRuns];
-#pragma unroll
-        for (uint32_t e = 0; e < 2 * kRuns; ++e)
-            votes[e] = __ballot(v[e] >= low && v[e] < high);
-        f(v4f{v[0], v[1], v[2], v[3]});
-        f(v4f{v[4], v[5], v[6], v[7]});
-        // A chunk past the end, of an odd count, has no votes and a place.
-        if (first_lane)
-#pragma unroll
-            for (uint32_t e = 0; e < 2 * kRuns; ++e)
-                sh->bins.votes[((c - begin) * kRuns + e) * kWaves + wave] = votes[e];
+        codes[(c - begin) * kBlock + threadIdx.x] = uint8_t(code);
+    });
+}
+// A thread's run of a segment's code words (eight bytes, 32 tokens).
+struct Words {
+    uint32_t first, last;
+    __device__ __forceinline__ explicit Words(uint32_t chunks)
+    {
+        const uint32_t words = chunks * (kBlock / 8), each_has = (words + kBlock - 1) / kBlock;
+        first = threadIdx.x * each_has < words ? threadIdx.x * each_has : words;
+        last = first + each_has < words ? first + each_has : words;
     }
+};
+// The token of a word's lowest bit, of those in kListed.
+__device__ __forceinline__ uint32_t token_of(uint32_t begin, uint32_t word, uint64_t bits)
+{
+    const uint32_t bit = __builtin_ctzll(bits);
+    return begin * kChunk + 32 * word + 4 * (bit >> 3) + (bit & 7);
 }
 
 struct Listed {
-    uint32_t count;
+    uint32_t count, picked;
     float most;  // the row's largest, or NaN (join_extremes)
 };
-// Lists the indices of the tokens with low <= v < high, but -infinity, in their
-// order: as many as are there, or kMany + 1, and no list, where they are more.
+// Lists the tokens with low <= v, but -infinity, in sh->index and those with also
+// v < high in sh->pick, in their order; what passes the lists' ends is counted.
 __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, float high)
 {
     const Row row = row_of(sh);
     low = fmaxf(low, -3.4028235e38f);
     Extremes extremes;
-    uint32_t listed = 0;
+    uint64_t listed = 0;  // and, in the high word, picked
 #pragma unroll 1
     for (uint32_t begin = 0; begin < row.chunks; begin += kSegmentChunks) {
         const uint32_t end =
             row.chunks - begin < kSegmentChunks ? row.chunks : begin + kSegmentChunks;
         __syncthreads();
-        vote_chunks(sh, row, begin, end, low, high, [&](v4f v) { extremes.take(v); });
+        code_chunks(sh, row, begin, end, low, high, [&](v4f v) { extremes.take(v); });
         __syncthreads();
-        // A thread lists the tokens of a run of words.
-        const uint32_t words = (end - begin) * (kChunk / 64);
-        const uint32_t each_has = (words + kBlock - 1) / kBlock;
-        const uint32_t first = threadIdx.x * each_has < words ? threadIdx.x * each_has : words;
-        const uint32_t last = first + each_has < words ? first + each_has : words;
+        const Words words(end - begin);
         uint64_t mine = 0;
-        for (uint32_t w = first; w < last; ++w)
-            mine += __popcll(sh->bins.votes[w]);
-        const Scan<uint64_t> scan = block_scan(sh, mine);
-        if (listed + scan.total <= kMany && mine) {
-            uint32_t at = listed + uint32_t(scan.upto - mine);
-            for (uint32_t w = first; w < last; ++w)
-                for (uint64_t votes = sh->bins.votes[w]; votes; votes &= votes - 1)
-                    sh->index[at++] = begin * kChunk + 64 * w + __builtin_ctzll(votes);
+        for (uint32_t w = words.first; w < words.last; ++w) {
+            const uint64_t word = sh->bins.codes[w];
+            mine += __popcll(word & kListed) | uint64_t(__popcll(word >> 4 & kListed)) << 32;
         }
-        listed = listed + scan.total < kMany + 1 ? uint32_t(listed + scan.total) : kMany + 1;
+        const Scan<uint64_t> scan = block_scan(sh, mine);
+        uint32_t at = uint32_t(listed + scan.upto - mine);
+        uint32_t pick = uint32_t((listed + scan.upto - mine) >> 32);
+#pragma unroll 1
+        for (uint32_t w = words.first; w < words.last; ++w) {
+            const uint64_t word = sh->bins.codes[w];
+#pragma unroll 1
+            for (uint64_t bits = word & kListed; bits; bits &= bits - 1, ++at) {
+                const uint32_t token = token_of(begin, w, bits);
+                if (at < kMany)
+                    sh->index[at] = token;
+                if (word >> 4 & bits & -bits) {
+                    if (pick < kList)
+                        sh->pick[pick] = token;
+                    ++pick;
+                }
+            }
+        }
+        listed += scan.total;
     }
-    return {listed, join_extremes(sh, extremes.most, extremes.nan)};
+    return {uint32_t(listed), uint32_t(listed >> 32),
+            join_extremes(sh, extremes.most, extremes.nan)};
 }
 
 // How many equal tokens of weight `each` fit above `above` short of `goal`: those
@@ -559,15 +568,17 @@ __device__ __forceinline__ uint32_t ties_within(double goal, double above, doubl
     return fit < 1.0 ? 1 : fit < 1e9 ? uint32_t(fit) : 1000000000u;
 }
 
-// Where `goal` (or a share of all) is reached among the n listed tokens that
+// Where `goal` (or a share of all) is reached among the n tokens of `list` that
 // `first` keeps: the smallest value with less than it (counts, or weights) above,
 // `over` among that, and the index of the last equal token whose predecessors stay
 // below it.  Bins are (steps below `from` - offset) * zoom; their tokens are few
 // (unless they are equal): one wave tries the values of up to 64 at once, or
 // halves the range of more.
-__device__ __attribute__((noinline)) Cut list_cut(Lds *sh, uint32_t n, bool counts, double goal,
-                                                  double share, double over, Cut first,
-                                                  double from, double offset, double zoom)
+typedef const __attribute__((address_space(3))) uint32_t *LdsList;
+__device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_t n, bool counts,
+                                                  double goal, double share, double over,
+                                                  Cut first, double from, double offset,
+                                                  double zoom)
 {
     const Row row = row_of(sh);
     const Units units(row.width);
@@ -579,18 +590,18 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, uint32_t n, bool coun
     clear_bins(sh);
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
-        const float v = row.logits[sh->index[i]];
+        const float v = row.logits[list[i]];
         const double w = counts ? 1.0 : weight_of(sh, row, v);
         sh->value[i] = v;
         sh->weight[i] = w;
-        if (first.keeps(v, sh->index[i]))
+        if (first.keeps(v, list[i]))
             add_to_bin(sh, bin(v), counts ? 1ull : units.of(w));
     }
     __syncthreads();
     const Found found = find_bin(sh, goal, share, over, counts ? 1.0 : units.scale);
     // The bin's tokens in their order: a thread looks at neighbours.
     const auto in = [&](uint32_t i) {
-        return i < n && first.keeps(sh->value[i], sh->index[i]) && bin(sh->value[i]) == found.bin;
+        return i < n && first.keeps(sh->value[i], list[i]) && bin(sh->value[i]) == found.bin;
     };
     static_assert(kList == 2 * kBlock, "neighbours of a thread");
     const bool a = in(2 * threadIdx.x), b = in(2 * threadIdx.x + 1);
@@ -669,11 +680,11 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, uint32_t n, bool coun
             if (here >= ties) {
                 for (; ties > 1; --ties)
                     equal &= equal - 1;
-                index = sh->index[sh->sub[base + __builtin_ctzll(equal)]];
+                index = list[sh->sub[base + __builtin_ctzll(equal)]];
                 break;
             }
             ties -= here;
-            index = sh->index[sh->sub[base + 63 - __builtin_clzll(equal)]];
+            index = list[sh->sub[base + 63 - __builtin_clzll(equal)]];
         }
         if (lane == 0) {
             sh->floats[0] = value;
@@ -722,7 +733,7 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
     }
     const float value = value_of(prefix);
     uint32_t ties = ties_within(goal, over, counts ? 1.0 : weight_of(sh, row, value));
-    // The index of the last of that many equal tokens, by the waves' votes.
+    // The index of the last of that many equal tokens, by their codes.
     uint32_t last = 0;
 #pragma unroll 1
     for (uint32_t begin = 0; begin < row.chunks; begin += kSegmentChunks) {
@@ -730,22 +741,20 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
             row.chunks - begin < kSegmentChunks ? row.chunks : begin + kSegmentChunks;
         __syncthreads();
         // [value, value] as a range: up to the next value above.
-        vote_chunks(sh, row, begin, end, value, value_of(key_of(value) + 1), [](v4f) {});
+        code_chunks(sh, row, begin, end, value, value_of(key_of(value) + 1), [](v4f) {});
         __syncthreads();
-        const uint32_t words = (end - begin) * (kChunk / 64);
-        const uint32_t each_has = (words + kBlock - 1) / kBlock;
-        const uint32_t from = threadIdx.x * each_has < words ? threadIdx.x * each_has : words;
-        const uint32_t to = from + each_has < words ? from + each_has : words;
+        const Words words(end - begin);
         uint64_t mine = 0;
-        for (uint32_t w = from; w < to; ++w)
-            mine += __popcll(sh->bins.votes[w]);
+        for (uint32_t w = words.first; w < words.last; ++w)
+            mine += __popcll(sh->bins.codes[w] >> 4 & kListed);
         const Scan<uint64_t> scan = block_scan(sh, mine);
         const uint64_t wanted = ties < scan.total ? ties : scan.total;  // the last one here, else
         if (scan.total && scan.upto >= wanted && scan.upto - mine < wanted) {
             uint64_t left = wanted - (scan.upto - mine);
-            for (uint32_t w = from; w < to && left; ++w)
-                for (uint64_t votes = sh->bins.votes[w]; votes && left; votes &= votes - 1, --left)
-                    sh->found = begin * kChunk + 64 * w + __builtin_ctzll(votes);
+            for (uint32_t w = words.first; w < words.last && left; ++w)
+                for (uint64_t bits = sh->bins.codes[w] >> 4 & kListed; bits && left;
+                     bits &= bits - 1, --left)
+                    sh->found = token_of(begin, w, bits);
         }
         __syncthreads();
         if (scan.total)
@@ -758,9 +767,10 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
     return {value, last};
 }
 
-// The weights of four tokens that a cut and min_p leave, formed side by side.
-__device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, uint32_t i, Cut cut,
-                                         double min_p, double (&w)[4])
+// The weights of four tokens that a cut (not of -infinity) and min_p leave, formed
+// side by side.
+__device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, const uint32_t (&i)[4],
+                                         Cut cut, double min_p, double (&w)[4])
 {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -768,36 +778,104 @@ __device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, uint32_
     asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        w[e] = bool(cut.keeps(v[e], i + e) & (w[e] >= min_p)) ? w[e] : 0.0;
+        w[e] = bool(cut.keeps(v[e], i[e]) & (w[e] >= min_p)) ? w[e] : 0.0;
 }
 
-// Sums of the kept weights of each 256 tokens (a wave's float4s) of a segment, in
-// sh->group: returns the thread's own and the scan of all.
-struct Groups {
-    double own, upto, total;
-};
-__device__ __attribute__((noinline)) Groups group_sums(Lds *sh, uint32_t begin, Cut cut,
-                                                       double min_p)
+// Of some lanes with sums, the one that holds the target: the first that passes it,
+// or else the last with any.
+__device__ __forceinline__ uint32_t holder(double own, double upto, double target)
+{
+    const uint64_t some = __ballot(own > 0.0), past = __ballot(own > 0.0 && upto > target);
+    return past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : 0;
+}
+// The first kept token, in the vocabulary's order, at which the sum of kept weights
+// passes u * total (the last kept one where rounding leaves none): of all tokens,
+// or of `listed` in sh->index.  Each wave sums a run of tiles of 256, a lane four
+// neighbours of each; the run that holds the target is shared out again, until it
+// is one tile a wave.
+__device__ __attribute__((noinline)) void choose(Lds *sh, uint32_t listed, Cut cut, double min_p,
+                                                 double u, float *out, float *copy)
 {
     const Row row = row_of(sh);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    const uint32_t end =
-        row.chunks - begin < kSegmentChunks ? row.chunks : begin + kSegmentChunks;
-    __syncthreads();
-    each_next(row, begin, end, [&](uint32_t c, v4f v) {
-        double sum = 0.0;
-        if (__any(max3(max3(v[0], v[1], v[2]), v[3], v[3]) >= cut.value)) {
-            double w[4];
-            terms_of(sh, row, v, c * kChunk + 4 * threadIdx.x, cut, min_p, w);
-            sum = wave_scan((w[0] + w[1]) + (w[2] + w[3]));
+    listed = __builtin_amdgcn_readfirstlane(listed);
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t begin = 0, tiles = ((listed ? listed : row.width) + 255) / 256;
+    double passed = 0.0, target = -1.0;
+#pragma unroll 1
+    for (;;) {
+        const uint32_t each_has = (tiles + kWaves - 1) / kWaves;
+        const uint32_t first = wave * each_has < tiles ? wave * each_has : tiles;
+        const uint32_t last = first + each_has < tiles ? first + each_has : tiles;
+        double w[4] = {0.0, 0.0, 0.0, 0.0}, own = 0.0;
+        v4f v = {0, 0, 0, 0}, next = v;
+        uint32_t i[4] = {0, 0, 0, 0}, next_i[4] = {0, 0, 0, 0};
+        // The next tile's loads are in flight behind this one's weights.
+#pragma unroll 1
+        for (uint32_t t = first; t <= last; ++t) {
+            if (t < last) {
+                const uint32_t at = (begin + t) * 256 + 4 * lane;
+                if (listed) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        next_i[e] = sh->index[at + e < listed ? at + e : listed - 1];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        next[e] = row.logits[next_i[e]];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        next[e] = at + e < listed ? next[e] : -__builtin_inff();
+                } else {
+                    next = load_four(row, at, (begin + t + 1) * 256 <= row.width);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        next_i[e] = at + e;
+                }
+            }
+            if (t > first) {
+                terms_of(sh, row, v, i, cut, min_p, w);
+                own += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+            v = next;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                i[e] = next_i[e];
         }
-        if ((threadIdx.x & 63) == 63)
-            sh->group[(c - begin) * kWaves + (threadIdx.x >> 6)] = sum;
-    });
-    __syncthreads();
-    const double own = threadIdx.x < (end - begin) * kWaves ? sh->group[threadIdx.x] : 0.0;
-    const Scan<double> scan = block_scan(sh, own);
-    return {own, scan.upto, scan.total};
+        const double upto = wave_scan(own);
+        __syncthreads();
+        if (lane == 63)
+            sh->scratch[wave] = __builtin_bit_cast(uint64_t, upto);
+        __syncthreads();
+        const double run = lane < kWaves ? __builtin_bit_cast(double, sh->scratch[lane]) : 0.0;
+        const double runs = wave_scan(run);
+        if (target < 0.0)
+            target = u * lane_value(runs, kWaves - 1);
+        const uint32_t chosen =
+            __builtin_amdgcn_readfirstlane(holder(run, passed + runs, target));
+        if (chosen)
+            passed += lane_value(runs, int(chosen) - 1);
+        if (each_has > 1) {
+            begin += chosen * each_has;
+            tiles = tiles - chosen * each_has < each_has ? tiles - chosen * each_has : each_has;
+            continue;
+        }
+        if (wave == chosen && lane == holder(own, passed + upto, target)) {
+            double at = passed + (upto - own);
+            uint32_t token = 0;
+            bool done = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (w[e] > 0.0 && !done) {
+                    at += w[e];
+                    token = i[e];
+                    done = at > target;
+                }
+            *out = float(token);
+            if (copy)
+                *copy = float(token);
+        }
+        return;
+    }
 }
 
 // ---- the kernel -------------------------------------------------------------------
@@ -877,10 +955,9 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
 
     const uint32_t k = top_k > 0.0f && top_k < float(s.width) ? uint32_t(top_k) : 0;
     const double share = top_p < 1.0f ? double(top_p) : -1.0;
-    Cut cut = {-__builtin_inff(), UINT32_MAX};
-    bool bounded = k || top_p < 1.0f;  // tokens below cut.value are not kept
-    uint32_t listed = 0;               // tokens of the list, where it holds every kept one
-    Listed list = {0, 0.0f};
+    Cut cut = {-3.4028235e38f, UINT32_MAX};
+    uint32_t listed = 0;  // tokens of the list, where it holds every kept one
+    Listed list = {0, 0, 0.0f};
     if (k) {
         // A value that the k-th largest of the row does not lie below: of the
         // first tokens, enough for about 1024 listed ones.
@@ -912,9 +989,10 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     if (k && list.count <= kList) {
         listed = list.count;
         if (listed > k)
-            cut = list_cut(sh, listed, true, double(k), -1.0, 0.0, cut, from, -0.5, 1.0);
+            cut = list_cut(sh, &sh->index[0], listed, true, double(k), -1.0, 0.0, cut, from, 0.0,
+                           1.0);
         if (share >= 0.0)
-            cut = list_cut(sh, listed, false, 0.0, share, 0.0, cut, from, -0.5, 1.0);
+            cut = list_cut(sh, &sh->index[0], listed, false, 0.0, share, 0.0, cut, from, 0.0, 1.0);
     } else if (k) {
         cut = digit_cut(sh, true, double(k), -1.0, cut);
         if (share >= 0.0)
@@ -924,11 +1002,13 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale);
         const float low = edge_of(sh, found.bin, from);
         const float high = found.bin ? edge_of(sh, found.bin - 1, from) : __builtin_inff();
-        const uint32_t n = list_tokens(sh, low, high).count;
+        list = list_tokens(sh, low, high);
         // Within the bin: its own equal steps.
-        cut = n <= kList ? list_cut(sh, n, false, found.goal, -1.0, found.over, cut, from,
-                                    double(found.bin) - 0.5, double(kBins))
-                         : digit_cut(sh, false, found.goal, -1.0, cut);
+        cut = list.picked <= kList
+                  ? list_cut(sh, &sh->pick[0], list.picked, false, found.goal, -1.0, found.over,
+                             cut, from, double(found.bin), double(kBins))
+                  : digit_cut(sh, false, found.goal, -1.0, cut);
+        listed = list.count <= kMany ? list.count : 0;
     }
     if (min_p > 0.0f) {
         // A value whose weight is surely below min_p: a bound, with room for
@@ -937,139 +1017,13 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
             list.most + temperature * (logf(min_p) - 0.01f) - 1e-5f * fabsf(list.most);
         if (bound > cut.value)
             cut = {bound, UINT32_MAX};
-        bounded = true;
     }
-    const auto term = [&](float v, uint32_t i) {
-        const double w = weight_of(sh, row, v);
-        return bool(cut.keeps(v, i) & (w >= double(min_p))) ? w : 0.0;
-    };
-    if (bounded && !listed) {
+    // A list of what a cut has left, where there is none yet.
+    if (!listed && ((k && list.count > kList) || (!k && share < 0.0 && min_p > 0.0f))) {
         const uint32_t n = list_tokens(sh, cut.value, __builtin_inff()).count;
         listed = n <= kMany ? n : 0;
     }
-
-    // The choice: the first kept token at which their sum passes the target (the
-    // last kept one where rounding leaves none).
-    if (threadIdx.x == 0) {
-        sh->found = UINT32_MAX;
-        sh->below = 0;
-    }
-    if (listed) {
-        // A thread has neighbours of the list.
-        const uint32_t each_has = (listed + kBlock - 1) / kBlock;
-        const uint32_t first = threadIdx.x * each_has < listed ? threadIdx.x * each_has : listed;
-        const uint32_t last = first + each_has < listed ? first + each_has : listed;
-        double mine = 0.0, at = 0.0, target = __builtin_inf();
-        uint32_t token = 0;
-        // Sums, then a walk by the thread that holds the target.
-#pragma unroll 1
-        for (int walk = 0; walk < 2; ++walk) {
-            double sum = 0.0;
-#pragma unroll 1
-            for (uint32_t i = first; i < last; ++i) {
-                const double t = term(row.logits[sh->index[i]], sh->index[i]);
-                sum += t;
-                if (walk && t > 0.0) {
-                    token = sh->index[i];
-                    if (at + sum > target)
-                        break;
-                }
-            }
-            if (walk) {
-                answer(float(token));
-                return;
-            }
-            mine = sum;
-            const Scan<double> scan = block_scan(sh, mine);
-            target = double(u) * scan.total;
-            at = scan.upto - mine;
-            if (mine > 0.0) {
-                if (scan.upto > target)
-                    atomicMin(&shared.found, threadIdx.x);
-                atomicMax(&shared.below, threadIdx.x);
-            }
-            __syncthreads();
-            if (threadIdx.x != (sh->found != UINT32_MAX ? sh->found : sh->below))
-                return;
-        }
-    }
-    // Too many for the list: sums of 256 tokens (a wave's float4s), of the segment
-    // that holds the target, then that wave's lanes.
-    const uint32_t segments = (row.chunks + kSegmentChunks - 1) / kSegmentChunks;
-    double total = 0.0, passed = 0.0, target = 0.0;
-    uint32_t begin = 0;
-    Groups groups = {0.0, 0.0, 0.0};
-    // Every segment's sum; then, of several, the one that holds the target again.
-#pragma unroll 1
-    for (uint32_t g = 0; g <= segments; ++g) {
-        if (g == segments) {
-            target = double(u) * total;
-            if (segments == 1)
-                break;
-            // The first that passes the target (the last with a token where
-            // rounding leaves none).
-            __syncthreads();
-            uint32_t chosen = 0;
-            double at = 0.0;
-            for (uint32_t i = 0; i < segments; ++i) {
-                const double sum = sh->segment[i];
-                if (sum > 0.0) {
-                    chosen = i;
-                    passed = at;
-                }
-                at += sum;
-                if (sum > 0.0 && at > target)
-                    break;
-            }
-            begin = chosen * kSegmentChunks;
-        } else {
-            begin = g * kSegmentChunks;
-        }
-        groups = group_sums(sh, begin, cut, double(min_p));
-        if (g < segments) {
-            if (threadIdx.x == 0)
-                sh->segment[g] = groups.total;
-            total += groups.total;
-        }
-    }
-    // The first group that passes it, likewise.
-    if (groups.own > 0.0) {
-        if (passed + groups.upto > target)
-            atomicMin(&shared.found, threadIdx.x);
-        atomicMax(&shared.below, threadIdx.x);
-    }
-    __syncthreads();
-    const uint32_t group = sh->found != UINT32_MAX ? sh->found : sh->below;
-    if (threadIdx.x == group)
-        sh->segment[0] = passed + (groups.upto - groups.own);
-    __syncthreads();
-    if (wave != group % kWaves)
-        return;
-    const double start = sh->segment[0];
-    const uint32_t chunk = begin + group / kWaves;
-    const v4f v = load_chunk(row, chunk);
-    const uint32_t i = chunk * kChunk + 4 * threadIdx.x;
-    double w[4];
-    terms_of(sh, row, v, i, cut, double(min_p), w);
-    const double own = (w[0] + w[1]) + (w[2] + w[3]);
-    const double upto = wave_scan(own);
-    const uint64_t some = __ballot(own > 0.0);
-    const uint64_t past = __ballot(own > 0.0 && start + upto > target);
-    if (!some)
-        return;  // not reached: the group's sum is positive
-    if (lane == (past ? uint32_t(__builtin_ctzll(past)) : 63 - uint32_t(__builtin_clzll(some)))) {
-        double at = start + (upto - own);
-        uint32_t token = i;
-        bool passed_it = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (w[e] > 0.0 && !passed_it) {
-                at += w[e];
-                token = i + e;
-                passed_it = at > target;
-            }
-        answer(float(token));
-    }
+    choose(sh, listed, cut, double(min_p), double(u), s.out + r, s.copy ? s.copy + r : nullptr);
 }
 
 }  // namespace
