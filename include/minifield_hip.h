@@ -448,7 +448,9 @@ mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key
  * used, whatever it holds.  Keys and values of a binary16 cache are expected to
  * be finite (one that is not makes its sequence's row NaN).  head_dim <= 1024.
  * The workspace grows on a call outside of stream capture; under capture a call
- * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT. */
+ * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT.  A
+ * context's calls and the graphs captured from it share one workspace: replay
+ * such graphs on the context's stream, or in an order with it. */
 mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                          const mfh_buf *key_pages, const mfh_buf *value_pages,
                          const mfh_buf *tables, const mfh_buf *lengths, uint32_t query_heads,

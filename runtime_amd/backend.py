@@ -472,8 +472,7 @@ class HipBackend:
                    to_pages) -> None:
         if len(destinations) != len(sources):
             raise ValueError("one source for each destination")
-        source = np.ascontiguousarray(from_pages, dtype=np.uint32).reshape(-1)
-        target = np.ascontiguousarray(to_pages, dtype=np.uint32).reshape(-1)
+        source, target = _page_ids(from_pages), _page_ids(to_pages)
         if source.size != target.size:
             raise ValueError("one target page for each source page")
         handles = ctypes.c_void_p * max(1, len(sources))
@@ -487,6 +486,16 @@ class HipBackend:
                     mask: Buffer | None = None) -> None:
         self._check(_ffi.lib().mfh_sample_rows(self._ctx, output.handle, logits.handle,
                                                uniforms.handle, params.handle, _h(mask)))
+
+
+def _page_ids(ids) -> np.ndarray:
+    """Host page ids as the library takes them, none of them changed by the conversion."""
+    given = np.asarray(ids).reshape(-1)
+    if given.dtype == np.uint32 or given.size == 0:
+        return np.ascontiguousarray(given, dtype=np.uint32)
+    if given.dtype.kind not in "iu" or given.min() < 0 or given.max() >= 1 << 32:
+        raise ValueError("page ids must be whole numbers in [0, 2^32)")
+    return given.astype(np.uint32)
 
 
 # ---- operation descriptors (engine-api/src/backend.rs:128-383) -------------

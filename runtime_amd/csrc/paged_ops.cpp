@@ -394,14 +394,13 @@ mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
         least_to = to.pages < least_to ? to.pages : least_to;
         least_from = from.pages < least_from ? from.pages : least_from;
         in_place = in_place || destinations[i]->dev == sources[i]->dev;
+    }
+    for (size_t i = 0; i < buffers; ++i)
         for (size_t j = 0; j < buffers; ++j)
-            if (j != i && check_buffer(ctx, sources[j]) == MFH_OK &&
-                check_buffer(ctx, destinations[j]) == MFH_OK &&
-                (destinations[i]->dev == sources[j]->dev ||
-                 destinations[i]->dev == destinations[j]->dev))
+            if (j != i && (destinations[i]->dev == sources[j]->dev ||
+                           destinations[i]->dev == destinations[j]->dev))
                 return fail(ctx, MFH_INVALID_ARGUMENT,
                             "a destination is another pair's source or destination");
-    }
     for (size_t i = 0; buffers && i < count; ++i)
         if (from_pages[i] >= least_from || to_pages[i] >= least_to)
             return fail(ctx, MFH_OUT_OF_BOUNDS, "page id exceeds the page count");

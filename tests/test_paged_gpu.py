@@ -617,6 +617,161 @@ def test_a_captured_workspace_is_kept():
     backend.close()
 
 
+def captured(backend, call):
+    """The call as a graph: (replay, end)."""
+    hip, stream = hiptime.hip(), ctypes.c_void_p(backend.stream())
+    graph, program = ctypes.c_void_p(), ctypes.c_void_p()
+    hiptime.check(hip.hipStreamBeginCapture(stream, 0), "begin capture")
+    try:
+        call()
+    finally:
+        hiptime.check(hip.hipStreamEndCapture(stream, ctypes.byref(graph)), "end capture")
+    hiptime.check(hip.hipGraphInstantiate(ctypes.byref(program), graph, None, None,
+                                          ctypes.c_size_t(0)), "instantiate")
+
+    def replay():
+        hiptime.check(hip.hipGraphLaunch(program, stream), "launch")
+
+    def end():
+        hiptime.check(hip.hipGraphExecDestroy(program), "destroy")
+        hiptime.check(hip.hipGraphDestroy(graph), "destroy")
+
+    return replay, end
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,size", [
+    (16, 1, 256, 16), (17, 1, 256, 8), (66, 2, 64, 32), (20, 1, 80, 4096), (40, 2, 128, 64),
+    (9, 1, 1000, 16)])
+def test_wide_groups(backend, heads, kv_heads, dim, size, half):
+    """Groups of query heads that fill a row tile, and pass it by one or more."""
+    say("groups", heads, kv_heads, dim, size, half)
+    rng = np.random.default_rng(heads + dim)
+    lengths = [4097, 1, 0, 130]
+    pages, table = tables_for(rng, lengths, size)
+    keys, values = (random_pages(rng, pages, kv_heads, size, dim, half) for _ in range(2))
+    query = rng.standard_normal((len(lengths), heads * dim)).astype(np.float32)
+    got = run_attention(backend, query, keys, values, table, lengths, heads, kv_heads, dim)
+    want, bound = attend(query, keys, values, table, lengths, heads)
+    assert np.all(np.abs(got - want) <= bound), np.nanmax(np.abs(got - want) / (bound + 1e-30))
+
+
+def test_a_padded_batch(backend):
+    """Rows with position -1 and length 0 around two sequences: nothing enters the
+    caches for them and their attention is zeros; a table may name a page twice."""
+    rng = np.random.default_rng(23)
+    heads, kv_heads, dim, size = 4, 2, 64, 16
+    keys, values = (random_pages(rng, 9, kv_heads, size, dim, False) for _ in range(2))
+    k, v = upload(backend, keys), upload(backend, values)
+    table = np.array([[-1, -1, -1], [4, 7, 4], [0, 2, -1], [np.nan, 1e9, -1]], np.float32)
+    positions = np.array([-1, 31, 16, -1], np.float32)
+    lengths = np.array([0, 32, 17, 0], np.float32)
+    rows = [rng.standard_normal((4, h * dim)).astype(np.float32) for h in (heads, kv_heads, kv_heads)]
+    turn = backend.allocate_f32((64, 0))
+    query, out = (backend.allocate_f32((4, heads * dim)) for _ in range(2))
+    backend.paged_qk_norm_rope(query, k, v, *(upload(backend, a) for a in rows), None, None, turn,
+                               upload(backend, table), None, upload(backend, positions),
+                               PagedRopeSpec(heads, kv_heads, dim), EPSILON)
+    for pages, new in ((keys, rows[1]), (values, rows[2])):
+        pages[7, :, 15] = new[1].reshape(kv_heads, dim)
+        pages[2, :, 0] = new[2].reshape(kv_heads, dim)
+    assert np.array_equal(backend.read(k), keys) and np.array_equal(backend.read(v), values)
+    got_query = backend.read(query)
+    assert np.array_equal(got_query[1:3], rows[0][1:3]) and np.isnan(got_query[[0, 3]]).all()
+    tables = upload(backend, table)
+    backend.paged_gqa(out, query, k, v, tables, upload(backend, lengths),
+                      GqaSpec(heads, kv_heads, dim))
+    alone = backend.allocate_f32((1, heads * dim))
+    got = backend.read(out)
+    assert np.all(got[[0, 3]] == 0.0)
+    for s in (1, 2):
+        # As the sequence alone.  Scores are the same products; their distance from
+        # the maximum, the exponent and sums of up to 32 terms, on both sides, are
+        # under 64 roundings of a mean of values below 5.
+        backend.paged_gqa(alone, upload(backend, got_query[s:s + 1]), k, v,
+                          upload(backend, table[s:s + 1]), upload(backend, lengths[s:s + 1]),
+                          GqaSpec(heads, kv_heads, dim))
+        assert np.max(np.abs(backend.read(alone)[0] - got[s])) <= 64 * 5 * F32
+
+
+def test_a_captured_step_of_everything(backend):
+    """Append, attention, a page copy and sampling in one graph; replays with other
+    inputs and eager calls between them equal eager calls."""
+    rng = np.random.default_rng(29)
+    heads, kv_heads, dim, size, rows = 8, 2, 64, 16, 3
+    spec, rope = GqaSpec(heads, kv_heads, dim), PagedRopeSpec(heads, kv_heads, dim)
+    first = [random_pages(rng, 24, kv_heads, size, dim, True) for _ in range(2)]
+    table = rng.permutation(24)[:21].reshape(3, 7).astype(np.float32)
+    spare = sorted(set(range(24)) - set(table.astype(int).reshape(-1)))[0]
+    turn = backend.allocate_f32((112, dim))
+    backend.rotation_table(turn, 1.0e4)
+    tables = upload(backend, table)
+    params = backend.upload_f32((1, 4), (0.8, 40, 0.9, 0.0))
+
+    def world():
+        return {"k": upload(backend, first[0]), "v": upload(backend, first[1]),
+                "in": [backend.allocate_f32((rows, h * dim)) for h in (heads, kv_heads, kv_heads)],
+                "position": backend.allocate_f32((rows,)), "length": backend.allocate_f32((rows,)),
+                "u": backend.allocate_f32((rows,)), "ids": backend.allocate_f32((rows,)),
+                "q": backend.allocate_f32((rows, heads * dim)),
+                "out": backend.allocate_f32((rows, heads * dim))}
+
+    def step(w):
+        backend.paged_qk_norm_rope(w["q"], w["k"], w["v"], *w["in"], None, None, turn, tables,
+                                   None, w["position"], rope, EPSILON)
+        backend.paged_gqa(w["out"], w["q"], w["k"], w["v"], tables, w["length"], spec)
+        backend.copy_pages([w["k"], w["v"]], [w["k"], w["v"]], [int(table[1, 2])], [spare])
+        backend.sample_rows(w["ids"], w["out"], w["u"], params)
+
+    eager, graphed = world(), world()
+    step(graphed)  # the workspace
+    for name, pages in zip("kv", first):
+        graphed[name] = upload(backend, pages)
+    replay, end = captured(backend, lambda: step(graphed))
+    for i in range(5):
+        new = [rng.standard_normal((rows, h * dim)).astype(np.float32)
+               for h in (heads, kv_heads, kv_heads)]
+        position = np.array([3 + i, 37 + i, 100 + i], np.float32)
+        u = rng.random(rows).astype(np.float32)
+        for w in (eager, graphed):
+            for to, a in zip((*w["in"], w["position"], w["length"], w["u"]),
+                             (*new, position, position + 1, u)):
+                backend.copy(to, upload(backend, a))
+        step(eager)
+        replay()
+        for name in ("out", "ids", "q"):
+            assert np.array_equal(backend.read(eager[name]), backend.read(graphed[name])), (i, name)
+    end()
+    for name in "kv":
+        wide = [backend.alloc_pages(24, kv_heads, size, dim) for _ in range(2)]
+        backend.copy_pages(wide, [eager[name], graphed[name]], range(24), range(24))
+        assert np.array_equal(backend.read(wide[0]), backend.read(wide[1])), name
+
+
+def test_two_contexts_at_once():
+    """Calls of two contexts, queued without waiting, equal each one's alone."""
+    rng = np.random.default_rng(31)
+    spec = GqaSpec(8, 2, 64)
+    keys, values = (random_pages(rng, 300, 2, 16, 64, False) for _ in range(2))
+    worlds = []
+    for n in (4800, 3333):
+        backend = HipBackend(0)
+        query = rng.standard_normal((1, 512)).astype(np.float32)
+        args = (upload(backend, query), upload(backend, keys), upload(backend, values),
+                upload(backend, rng.permutation(300).astype(np.float32)[None]),
+                upload(backend, np.array([n], np.float32)))
+        alone = backend.allocate_f32((1, 512))
+        backend.paged_gqa(alone, *args, spec)
+        worlds.append((backend, args, backend.read(alone),
+                       [backend.allocate_f32((1, 512)) for _ in range(20)]))
+    for i in range(20):
+        for backend, args, _, outs in worlds:
+            backend.paged_gqa(outs[i], *args, spec)
+    for backend, _, want, outs in worlds:
+        assert all(np.array_equal(backend.read(out), want) for out in outs)
+        backend.close()
+
+
 # ---- refusals ---------------------------------------------------------------------------------
 
 def refused(variant, call, *args):
@@ -723,6 +878,17 @@ def test_attention_refusals(backend):
                 GqaSpec(4, 2, 16))
     finally:
         backend.clear_cancel()
+
+
+def test_host_page_ids_are_not_converted(backend):
+    a, b = (backend.alloc_pages(5, 2, 8, 32) for _ in range(2))
+    for ids in ([-1], [2 ** 32 + 3], [1.5], np.array([-2]), np.array([2 ** 32], np.uint64)):
+        with pytest.raises((ValueError, OverflowError)):
+            backend.copy_pages([a], [b], ids, [2])
+        with pytest.raises((ValueError, OverflowError)):
+            backend.copy_pages([a], [b], [2], ids)
+    backend.copy_pages([a], [b], np.array([1], np.int8), (2,))
+    backend.copy_pages([a], [b], [], [])
 
 
 def test_copy_refusals(backend):

@@ -1,9 +1,9 @@
 """Sampling on the GPU against a plain implementation in 64 bits.
 
-Sums differ from the plain ones in their order only: by about 2^-53 of the
-weights' sum a term, so a choice differs where a uniform value lies that near a
-token's border, which no case here does (a border is hit with probability about
-2^-36 in the largest).
+Weights differ from the plain ones by 2^-43 of each and sums in their order: a
+choice differs where a uniform value lies that near a token's border, which no
+case here does (a border is hit with probability about 2^-25 at 300001 tokens and
+2^-19 at 2^24).
 """
 from __future__ import annotations
 
@@ -90,6 +90,30 @@ def test_settings(backend, name, width, rounded):
     uniforms[0] = 0.0
     uniforms[-1] = np.float32(1 - 2.0 ** -24)
     check(backend, logits, uniforms, [SETTINGS[name]])
+
+
+@pytest.mark.parametrize("rounded", [False, True], ids=["", "ties"])
+@pytest.mark.parametrize("width", [131072, 131073, 300001])
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_wide_rows(backend, name, width, rounded):
+    """Rows that are coded in several pieces; with half of the tokens admitted too."""
+    say("wide", name, width, rounded)
+    rng = np.random.default_rng(width + 5 * len(name))
+    logits = 2.5 * rng.standard_normal((2, width))
+    logits[:, ::width // 20] += 5
+    if rounded:
+        logits = np.round(logits * 4) / 4
+    uniforms = rng.random(2).astype(np.float32)
+    check(backend, logits, uniforms, [SETTINGS[name]])
+    check(backend, logits, uniforms, [SETTINGS[name]], rng.random((2, width)) < 0.5)
+
+
+@pytest.mark.parametrize("name", ["all", "greedy", "k50", "p", "min"])
+def test_the_widest_row(backend, name):
+    say("widest", name)
+    rng = np.random.default_rng(41)
+    logits = rng.standard_normal((1, 1 << 24), dtype=np.float32) * 2
+    check(backend, logits, [0.73], [SETTINGS[name]])
 
 
 def test_rows_have_their_own_settings(backend):
