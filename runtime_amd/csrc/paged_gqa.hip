@@ -234,8 +234,8 @@ __device__ bool next_part(const PagedAttention &p, Run &run, Part &part)
 // A block walks its part 64 keys at a time: each wave forms the scores of every
 // fourth key by dot products over its lanes, the rows' maxima and sums follow
 // online, and the block's threads add the keys' values to outputs in LDS.
-// Bound by the dots' shuffles; head widths that are multiples of 16 have
-// kernels of their own.
+// Bound by the dots' shuffles: 32 sequences of 2048 keys of 4 heads of 144 take 607
+// us, of 160, which has a kernel of its own, 61.
 constexpr uint32_t kGeneralKeys = 64;
 constexpr uint32_t kGeneralLds = 4096;  // most rows * head_dim of an item
 
@@ -430,10 +430,11 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// Blocks of the kernel that a CU holds, by its registers.
+// Blocks of the kernel that a CU holds, by its registers (an odd number of 16s in
+// binary16 takes more: half a register of each row is idle).
 constexpr int resident_blocks(int d, bool half)
 {
-    return d > 128 ? 1 : d <= 64 ? 4 : half ? 2 : 3;
+    return d > 128 ? 1 : d > 64 ? (half ? 2 : 3) : d == 48 && half ? 3 : 4;
 }
 
 // D: head width.  SMALL: pages of 8 keys (else a page holds whole 16-key blocks).
@@ -787,11 +788,16 @@ MfmaKernel mfma_kernel(const PageShape &shape)
 {
     const bool half = shape.half, small = shape.page_shift < 4;
     switch (shape.head_dim) {
+    case 16: return mfma_kernel_of<16>(half, small);
     case 32: return mfma_kernel_of<32>(half, small);
+    case 48: return mfma_kernel_of<48>(half, small);
     case 64: return mfma_kernel_of<64>(half, small);
     case 80: return mfma_kernel_of<80>(half, small);
     case 96: return mfma_kernel_of<96>(half, small);
+    case 112: return mfma_kernel_of<112>(half, small);
     case 128: return mfma_kernel_of<128>(half, small);
+    case 160: return mfma_kernel_of<160>(half, small);
+    case 192: return mfma_kernel_of<192>(half, small);
     case 256: return mfma_kernel_of<256>(half, small);
     default: return {};
     }

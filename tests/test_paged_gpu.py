@@ -642,7 +642,8 @@ def captured(backend, call):
 @pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
 @pytest.mark.parametrize("heads,kv_heads,dim,size", [
     (16, 1, 256, 16), (17, 1, 256, 8), (66, 2, 64, 32), (20, 1, 80, 4096), (40, 2, 128, 64),
-    (9, 1, 1000, 16)])
+    (9, 1, 1000, 16), (8, 2, 48, 16), (6, 2, 112, 8), (8, 2, 160, 16), (12, 2, 192, 8),
+    (12, 2, 192, 64), (18, 1, 16, 8)])
 def test_wide_groups(backend, heads, kv_heads, dim, size, half):
     """Groups of query heads that fill a row tile, and pass it by one or more."""
     say("groups", heads, kv_heads, dim, size, half)
