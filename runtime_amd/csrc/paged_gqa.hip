@@ -13,6 +13,12 @@
 // that a second launch joins in block order, so results do not depend on timing.
 // A run touches at most two shared items, its first and its last: two records a
 // block.
+//
+// Bound by the reads of the cache.  Both launches, in us (and the cache's TB/s): 96
+// sequences of 33 to 2048 keys, 8 key heads of 64, f32 40.6 (4.8); 48 of 17 to 8191,
+// 8 of 128, binary16 61 (4.5); one of 131071, 8 of 64, binary16 53.5 (5.0), f32 90.7
+// (5.9).  About 9 us of each are the two launches and their dependent reads, which
+// is all that a short call takes: one sequence of 2047 keys 10.8.
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -67,7 +73,8 @@ __device__ __forceinline__ uint32_t length_of(const PagedAttention &p, uint32_t 
 }
 
 // An item's place on the line: `item_units` for what every item costs, then its
-// units of keys.
+// units of keys.  Three, for the waits of an item's start and end (without them a
+// block could be given many short items: 48 sequences of 17 to 8191 keys 166 us).
 __device__ __forceinline__ uint32_t units_of(const PagedAttention &p, uint32_t length)
 {
     return length == UINT32_MAX || length == 0
@@ -368,7 +375,12 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
 //
 // Loads of the next tile's keys are issued as soon as the products have read
 // this tile's, its values' likewise: each is in flight behind the other's
-// arithmetic, in the same registers.
+// arithmetic, in the same registers.  They are read once, and said to be
+// (nontemporal): 42.5 / 55.5 / 53.3 us for the first three calls above with that
+// said of both, 47.5 / 64.2 / 58.3 without, in between with one.
+//
+// A tile is 32 keys in binary16 (a product's depth) and 16 in f32: of twice that
+// the registers hold fewer blocks.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -430,7 +442,8 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// Blocks of the kernel that a CU holds, by its registers (an odd number of 16s in
+// Blocks of the kernel that a CU holds, by its registers: a grid is as many for
+// every CU, so that all run at once (an odd number of 16s in
 // binary16 takes more: half a register of each row is idle).
 constexpr int resident_blocks(int d, bool half)
 {
@@ -812,8 +825,8 @@ MfmaKernel mfma_kernel(const PageShape &shape)
 // record order, and the shares in order; lane i forms the weight of record i of
 // 64.  Bound by three dependent reads, of what other XCDs' blocks wrote, and by
 // the code's own fetch: a block of 256 threads with barriers took 5.1 to 6.1 us
-// where this takes 3.9 to 5.0, and holding the first records while the weights are
-// formed, one read less, 5.8 to 10.7.
+// where this takes 4.7 to 5.1 (7.0 with 128 records an item), and holding the first
+// records while the weights are formed, one read less, 5.8 to 10.7.
 template <int V>
 __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
 {
