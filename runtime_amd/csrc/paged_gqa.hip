@@ -823,10 +823,10 @@ MfmaKernel mfma_kernel(const PageShape &shape)
 // length is invalid NaN.  Lanes are as many shares of the records as rows of
 // V-column pieces fit the wave (V = 4 where the head width allows), each summed in
 // record order, and the shares in order; lane i forms the weight of record i of
-// 64.  Bound by three dependent reads, of what other XCDs' blocks wrote, and by
-// the code's own fetch: a block of 256 threads with barriers took 5.1 to 6.1 us
-// where this takes 4.7 to 5.1 (7.0 with 128 records an item), and holding the first
-// records while the weights are formed, one read less, 5.8 to 10.7.
+// 64.  Bound by two dependent reads, of what other XCDs' blocks wrote, and by the
+// code's own fetch: 4.5 to 4.7 us, 6.0 with 128 records an item (4.7 to 5.1 and 7.0
+// with the records read once the weights are formed, up to 12.8 with a condition on
+// the loads, 5.1 to 6.1 for a block of 256 threads with barriers).
 template <int V>
 __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
 {
@@ -853,54 +853,73 @@ __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
         return uint64_t(i ? share.first / 2 * 2 + 2 * i : share.first) * p.rows + row;
     };
     const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
-    v2f own = {-__builtin_inff(), 0.0f};  // the lane's of the first 64
-    if (lane < share.count)
-        own = stats[record(lane)];
-    float most = own[0];
+    const uint32_t columns = d / V;
+    const uint32_t width = columns < 64 ? columns : 64, shares = 64 / width;
+    const uint32_t mine = lane / width;  // lanes past the last share add to none
+    // kHeld records a lane in flight, the next ones behind the arithmetic: loads
+    // without a condition, under which the compiler waits for each.
+    constexpr uint32_t kHeld = 8;
+    struct At {
+        uint32_t column, group, n;  // of 64 records
+    } at = {0, 0, 0};
+    piece next[kHeld];
+    const auto load = [&] {
+        const uint32_t c = at.column + lane % width;
+#pragma unroll
+        for (uint32_t u = 0; u < kHeld; ++u) {
+            const uint32_t i = at.group + at.n + u * shares + mine;
+            next[u] = *reinterpret_cast<const piece *>(
+                p.records + record(i < share.count ? i : share.count - 1) * d +
+                (c < columns ? c : 0) * V);
+        }
+    };
+    load();
+    v2f stat = stats[record(lane < share.count ? lane : 0)];
+    float most = stat[0];
+#pragma unroll 1
     for (uint32_t i = lane + 64; i < share.count; i += 64)
         most = fmaxf(most, stats[record(i)][0]);
     most = wave_max(most);
     const float base = most == -__builtin_inff() ? 0.0f : most;
-    const uint32_t columns = d / V;
-    const uint32_t width = columns < 64 ? columns : 64, shares = 64 / width;
-    const uint32_t mine = lane / width;  // lanes past the last share add to none
-    float total = 0.0f;
+    float total = 0.0f, weight = 0.0f;
+    piece a = {};
 #pragma unroll 1
-    for (uint32_t c0 = 0; c0 < columns; c0 += width) {
-        const uint32_t c = c0 + lane % width;
-        piece a = {};
-#pragma unroll 1
-        for (uint32_t i0 = 0; i0 < share.count; i0 += 64) {
-            const uint32_t count = share.count - i0 < 64 ? share.count - i0 : 64;
-            v2f stat = own;
-            if (i0)
-                stat = lane < count ? stats[record(i0 + lane)] : v2f{-__builtin_inff(), 0.0f};
-            const float weight = __builtin_amdgcn_exp2f(stat[0] - base);
-            if (c0 == 0)
+    while (at.column < columns) {
+        const At now = at;
+        const uint32_t c = now.column + lane % width;
+        const uint32_t left = share.count - now.group, count = left < 64 ? left : 64;
+        if (now.n == 0) {
+            if (now.group || now.column)
+                stat = stats[record(now.group + (lane < count ? lane : 0))];
+            weight = __builtin_amdgcn_exp2f(stat[0] - base);
+            if (now.column == 0)
                 total += lane < count ? stat[1] * weight : 0.0f;
-            // kHeld records a lane in flight: loads without a condition, under
-            // which the compiler waits for each.
-            constexpr uint32_t kHeld = 8;
-#pragma unroll 1
-            for (uint32_t n = 0; n < count; n += kHeld * shares) {
-                piece held[kHeld];
+        }
+        piece held[kHeld];
 #pragma unroll
-                for (uint32_t u = 0; u < kHeld; ++u) {
-                    const uint32_t i = n + u * shares + mine;
-                    held[u] = *reinterpret_cast<const piece *>(
-                        p.records + record(i0 + (i < count ? i : count - 1)) * d +
-                        (c < columns ? c : 0) * V);
-                }
-#pragma unroll
-                for (uint32_t u = 0; u < kHeld; ++u) {
-                    const uint32_t i = n + u * shares + mine;
-                    const float w = __shfl(weight, int(i & 63), 64);
-                    if (i < count)
-                        a += w * held[u];
-                }
+        for (uint32_t u = 0; u < kHeld; ++u)
+            held[u] = next[u];
+        at.n += kHeld * shares;
+        if (at.n >= count) {
+            at.n = 0;
+            at.group += 64;
+            if (at.group >= share.count) {
+                at.group = 0;
+                at.column += width;
             }
         }
-        if (c0 == 0)
+        if (at.column < columns)
+            load();
+#pragma unroll
+        for (uint32_t u = 0; u < kHeld; ++u) {
+            const uint32_t i = now.n + u * shares + mine;
+            const float w = __shfl(weight, int(i & 63), 64);
+            if (i < count)
+                a += w * held[u];
+        }
+        if (at.column == now.column)
+            continue;
+        if (now.column == 0)
             total = wave_sum(total);
         piece sum = a;
 #pragma unroll 1
@@ -910,6 +929,7 @@ __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
                 sum[e] += __shfl(a[e], int((lane + s * width) & 63), 64);
         if (mine == 0 && c < columns)
             *reinterpret_cast<piece *>(out + c * V) = sum / total;
+        a = piece{};
     }
 }
 
