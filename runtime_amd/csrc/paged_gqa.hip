@@ -16,7 +16,7 @@
 //
 // Bound by the reads of the cache.  Both launches, in us (and the cache's TB/s): 96
 // sequences of 33 to 2048 keys, 8 key heads of 64, f32 40.6 (4.8); 48 of 17 to 8191,
-// 8 of 128, binary16 61 (4.5); one of 131071, 8 of 64, binary16 53.5 (5.0), f32 90.7
+// 8 of 128, binary16 53.8 (5.1); one of 131071, 8 of 64, binary16 53.5 (5.0), f32 90.7
 // (5.9).  About 9 us of each are the two launches and their dependent reads, which
 // is all that a short call takes: one sequence of 2047 keys 10.8.
 #include <type_traits>
@@ -73,8 +73,10 @@ __device__ __forceinline__ uint32_t length_of(const PagedAttention &p, uint32_t 
 }
 
 // An item's place on the line: `item_units` for what every item costs, then its
-// units of keys.  Three, for the waits of an item's start and end (without them a
-// block could be given many short items: 48 sequences of 17 to 8191 keys 166 us).
+// units of keys.  Five, for the waits of an item's start and end, in the time of a
+// unit: a block can be given many short items.  48 sequences of 17 to 8191 keys in
+// any order take 69 to 75 us with two, 63 with three, 55.7, 53.6, 53.6 and 54 with
+// four, five, six and eight (166 without).
 __device__ __forceinline__ uint32_t units_of(const PagedAttention &p, uint32_t length)
 {
     return length == UINT32_MAX || length == 0
@@ -376,8 +378,8 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
 // Loads of the next tile's keys are issued as soon as the products have read
 // this tile's, its values' likewise: each is in flight behind the other's
 // arithmetic, in the same registers.  They are read once, and said to be
-// (nontemporal): 42.5 / 55.5 / 53.3 us for the first three calls above with that
-// said of both, 47.5 / 64.2 / 58.3 without, in between with one.
+// (nontemporal): with that said of both, of neither, or of one, the first three calls
+// above took 42.5 / 55.5 / 53.3, 47.5 / 64.2 / 58.3, and a time in between.
 //
 // A tile is 32 keys in binary16 (a product's depth) and 16 in f32: of twice that
 // the registers hold fewer blocks.
@@ -389,6 +391,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = kBlock / 64;
+constexpr uint32_t kItemUnits = 5;
 constexpr uint32_t kRowsMost = 16;
 constexpr float kProbabilityShift = 15.0f;
 
@@ -949,7 +952,7 @@ bool paged_gqa_plan(PagedAttention &p, int cu_count)
     p.least_units = mfma.run ? kWaves : 1;
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     const uint64_t longest = uint64_t(p.max_pages) << p.shape.page_shift;
-    p.item_units = mfma.run ? 3 : 0;
+    p.item_units = mfma.run ? kItemUnits : 0;
     const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys + p.item_units;
     // Units stay in 32 bits, and so do the join's threads, 64 for each row.
     if (items * p.rows > (uint64_t(1) << 25) ||
