@@ -90,10 +90,12 @@ struct PagedAttention {
     uint32_t sequences = 0, max_pages = 0, query_heads = 0, group = 0;
     float scale = 0.0f;
     // Filled by paged_gqa_plan: query rows of a key/value head that one item
-    // holds, items per key/value head, keys of a unit, units that an item costs
-    // besides, units that a block takes at least, blocks.
-    uint32_t rows = 0, row_tiles = 0, unit_keys = 0, item_units = 0, least_units = 0;
+    // holds, items per key/value head, keys of a unit and units that a block takes at
+    // least (their logarithms), units that an item costs besides, blocks, the longest
+    // length.
+    uint32_t rows = 0, row_tiles = 0, unit_shift = 0, least_shift = 0, item_units = 0;
     uint32_t blocks = 0;
+    float longest = 0.0f;
     float *records = nullptr;  // paged_gqa_scratch_bytes
 };
 // Widest head that the kernels serve.

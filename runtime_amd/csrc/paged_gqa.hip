@@ -4,7 +4,7 @@
 // p_j = exp(s_j - max s) and s_j = q . k_j / sqrt(head_dim); query heads
 // kv_head * group .. of a key/value head share its keys.
 //
-// The work is a line of units: `unit_keys` keys of one item, an item being
+// The work is a line of units: a few keys (a power of two) of one item, an item being
 // (sequence, key/value head, tile of `rows` of its query heads), items in order.
 // Lengths live on the device, so every block adds up the units of the sequences
 // itself and takes an equal run of them, which balances a batch of any mix of
@@ -62,14 +62,15 @@ __host__ __device__ inline ItemShare *item_shares(const PagedAttention &p)
     return reinterpret_cast<ItemShare *>(record_stats(p) + 4 * uint64_t(p.blocks) * p.rows);
 }
 
-// Keys of sequence s, or UINT32_MAX where its length is not a whole number
-// that its table row has room for.
+// A length, or UINT32_MAX where it is not a whole number that a table row has room
+// for.
+__device__ __forceinline__ uint32_t checked_length(const PagedAttention &p, float v)
+{
+    return v >= 0.0f && v <= p.longest && truncf(v) == v ? uint32_t(v) : UINT32_MAX;
+}
 __device__ __forceinline__ uint32_t length_of(const PagedAttention &p, uint32_t s)
 {
-    const float v = p.lengths[s];
-    if (!(v >= 0.0f && v <= 16777216.0f && truncf(v) == v))
-        return UINT32_MAX;
-    return uint64_t(v) <= (uint64_t(p.max_pages) << p.shape.page_shift) ? uint32_t(v) : UINT32_MAX;
+    return checked_length(p, p.lengths[s]);
 }
 
 // An item's place on the line: `item_units` for what every item costs, then its
@@ -79,63 +80,117 @@ __device__ __forceinline__ uint32_t length_of(const PagedAttention &p, uint32_t 
 // four, five, six and eight (166 without).
 __device__ __forceinline__ uint32_t units_of(const PagedAttention &p, uint32_t length)
 {
-    return length == UINT32_MAX || length == 0
-               ? 0
-               : (length + p.unit_keys - 1) / p.unit_keys + p.item_units;
+    const uint32_t units = (length + (1u << p.unit_shift) - 1) >> p.unit_shift;
+    return length == UINT32_MAX || length == 0 ? 0 : units + p.item_units;
 }
 
-// A block's place on the line of units.
+// A block's place on the line of units: block b of n starts at floor(b total / n), so
+// that items of one length start where blocks do wherever they can.
 struct Run {
-    uint32_t sequence, head;  // the item of the next unit
-    uint32_t length;          // of the sequence
-    uint32_t unit;            // of that item
-    uint32_t start, at, end;  // on the line
-    uint32_t total, blocks;   // units of the line, blocks that share them
+    uint32_t sequence, kv_head, row_tile;  // the item of the next unit
+    uint32_t length;                       // of the sequence
+    uint32_t unit;                         // of that item
+    uint32_t start, at, end;               // on the line
+    uint32_t total, blocks;                // of the line
 };
 
 // A block's units out of `total`, even to one, and whether it has any.
 __device__ __forceinline__ bool take_units(const PagedAttention &p, uint32_t total, Run &run)
 {
-    const uint32_t most = (total + p.least_units - 1) / p.least_units;
-    run.blocks = most < p.blocks ? most : p.blocks;
-    run.total = total;
-    if (blockIdx.x >= run.blocks)
+    const uint32_t most = (total + (1u << p.least_shift) - 1) >> p.least_shift;
+    const uint32_t blocks = most < p.blocks ? most : p.blocks, b = blockIdx.x;
+    if (b >= blocks)
         return false;
-    run.start = run.at = uint32_t(uint64_t(blockIdx.x) * total / run.blocks);
-    run.end = uint32_t((uint64_t(blockIdx.x) + 1) * total / run.blocks);
+    run.total = total;
+    run.blocks = blocks;
+    // The products stay in 32 bits: blocks are at most a few for every CU.
+    const uint32_t quotient = total / blocks, odd = total - quotient * blocks;
+    run.start = run.at = b * quotient + b * odd / blocks;
+    run.end = (b + 1) * quotient + (b + 1) * odd / blocks;
     return true;
 }
+// The block that has a unit: the quotient of whole numbers below 2^53, so the
+// rounded one is below the next whole number where the exact one is.
+__device__ __forceinline__ uint32_t block_of(const Run &run, uint32_t unit)
+{
+    const double after = (double(unit) + 1.0) * double(run.blocks) - 1.0;
+    return uint32_t(after / double(run.total));
+}
 
-// Adds up the sequences' units and finds the block's first one.  Up to 64
-// sequences are a scan over the lanes of each wave, without a barrier; more are a
+// Inclusive scan over the wave's lanes by DPP moves; lane 63 ends with the sum.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v)
+{
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t lanes_scan(uint32_t v)
+{
+    v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // row 0's and 2's last lane to the next row
+    v += moved<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+
+// The item that a block's first unit is in, `inside` the units of a sequence whose
+// items have `units` each.
+__device__ __forceinline__ void start_run(const PagedAttention &p, Run &run, uint32_t sequence,
+                                          uint32_t length, uint32_t units, uint32_t inside)
+{
+    const auto scalar = [](uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(v)); };
+    const uint32_t head = scalar(inside) / scalar(units);
+    run.sequence = scalar(sequence);
+    run.length = scalar(length);
+    run.unit = scalar(inside) - head * scalar(units);
+    run.kv_head = head;
+    run.row_tile = 0;
+    if (p.row_tiles > 1) {
+        run.kv_head = head / p.row_tiles;
+        run.row_tile = head - run.kv_head * p.row_tiles;
+    }
+}
+
+// Adds up the sequences' units and finds the block's first one.  Up to 256
+// sequences are four for every lane of each wave, without a barrier; more are a
 // run of sequences for every thread, then a scan over the block.  False, for
-// every thread: nothing to do.
-__device__ bool find_run(const PagedAttention &p, Run &run)
+// every thread: nothing to do.  A call's first reads wait for this code, which runs
+// once and is fetched as it runs: divisions are few and of 32 bits, scans are moves
+// between lanes, and the first tile's reads go out before anything that can wait (with
+// 64-bit divisions and shuffles before them calls took 0.3 to 3.6 us longer, 128
+// sequences of 128 keys 22.1 for 19.5).
+__device__ __forceinline__ bool find_run(const PagedAttention &p, Run &run)
 {
     const uint32_t heads = p.shape.kv_heads * p.row_tiles;
     const uint32_t lane = threadIdx.x & 63;
-    const auto scan = [&](uint32_t v) {
+    if (p.sequences <= 256) {
+        float value[4];
 #pragma unroll
-        for (int offset = 1; offset < 64; offset <<= 1) {
-            const uint32_t other = __shfl_up(v, offset, 64);
-            if (int(lane) >= offset)
-                v += other;
+        for (uint32_t e = 0; e < 4; ++e)
+            value[e] = p.lengths[4 * lane + e < p.sequences ? 4 * lane + e : p.sequences - 1];
+        uint32_t length[4], upto[4], sum = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            length[e] = 4 * lane + e < p.sequences ? checked_length(p, value[e]) : 0;
+            upto[e] = sum += units_of(p, length[e]);
         }
-        return v;
-    };
-    if (p.sequences <= 64) {
-        const uint32_t length = lane < p.sequences ? length_of(p, lane) : 0;
-        const uint32_t units = units_of(p, length), upto = scan(units);
-        if (!take_units(p, __builtin_amdgcn_readlane(upto, 63) * heads, run))
+        const uint32_t scan = lanes_scan(sum);
+        if (!take_units(p, __builtin_amdgcn_readlane(scan, 63) * heads, run))
             return false;
-        const uint64_t past = __ballot(run.at < upto * heads);
-        const uint32_t s = __builtin_ctzll(past);
-        const uint32_t mine = __builtin_amdgcn_readlane(units, s);
-        const uint32_t inside = run.at - (__builtin_amdgcn_readlane(upto, s) - mine) * heads;
-        run.sequence = s;
-        run.length = __builtin_amdgcn_readlane(length, s);
-        run.head = inside / mine;
-        run.unit = inside % mine;
+        const uint32_t from = __builtin_ctzll(__ballot(run.at < scan * heads));
+        const auto of = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(v, from)); };
+        const uint32_t before = of(scan) - of(sum);
+        uint32_t e = 0, last = 0, next = of(upto[0]), keys = of(length[0]);
+#pragma unroll
+        for (uint32_t n = 1; n < 4; ++n)
+            if (run.at >= (before + next) * heads) {
+                e = n;
+                last = next;
+                next = of(upto[n]);
+                keys = of(length[n]);
+            }
+        start_run(p, run, 4 * from + e, keys, next - last, run.at - (before + last) * heads);
         return true;
     }
     __shared__ uint32_t sums[kBlock / 64];
@@ -146,7 +201,7 @@ __device__ bool find_run(const PagedAttention &p, Run &run)
     uint32_t mine = 0;
     for (uint32_t s = first; s < last; ++s)
         mine += units_of(p, length_of(p, s));
-    uint32_t upto = scan(mine);
+    uint32_t upto = lanes_scan(mine);
     if (lane == 63)
         sums[threadIdx.x >> 6] = upto;
     __syncthreads();
@@ -157,47 +212,43 @@ __device__ bool find_run(const PagedAttention &p, Run &run)
             upto += sums[w];
         total += sums[w];
     }
-    if (!take_units(p, total * heads, run))
+    if (!take_units(p, __builtin_amdgcn_readfirstlane(total) * heads, run))
         return false;
     uint32_t before = upto - mine;
     if (run.at >= before * heads && run.at < upto * heads) {
         for (uint32_t s = first; s < last; ++s) {
             const uint32_t length = length_of(p, s), units = units_of(p, length);
             if (run.at < (before + units) * heads) {
-                const uint32_t inside = run.at - before * heads;
                 found[0] = s;
                 found[1] = length;
-                found[2] = inside / units;
-                found[3] = inside % units;
+                found[2] = units;
+                found[3] = run.at - before * heads;
                 break;
             }
             before += units;
         }
     }
     __syncthreads();
-    run.sequence = __builtin_amdgcn_readfirstlane(found[0]);
-    run.length = __builtin_amdgcn_readfirstlane(found[1]);
-    run.head = __builtin_amdgcn_readfirstlane(found[2]);
-    run.unit = __builtin_amdgcn_readfirstlane(found[3]);
+    start_run(p, run, found[0], found[1], found[2], found[3]);
     return true;
 }
 
 // The part of an item that a block holds.
 struct Part {
-    uint32_t sequence, kv_head, row_tile, item;
+    uint32_t sequence, kv_head, row_tile;
     uint32_t length;       // keys of the sequence
     uint32_t begin, end;   // its keys
     bool whole;            // all of the item
     uint32_t record;       // where it is not
+    uint32_t last_unit;    // on the line, of the item; UINT32_MAX but for its first keys
 };
 
 // The next part of a run, false at its end; it may have no keys (begin == end).  The
 // block that holds an item's first keys says how the item is shared.
-__device__ bool next_part(const PagedAttention &p, Run &run, Part &part)
+__device__ __forceinline__ bool next_part(const PagedAttention &p, Run &run, Part &part)
 {
     if (run.at >= run.end)
         return false;
-    const uint32_t heads = p.shape.kv_heads * p.row_tiles;
     uint32_t units = units_of(p, run.length);
     while (!units) {  // at < end: another unit follows
         run.length = length_of(p, ++run.sequence);
@@ -211,31 +262,41 @@ __device__ bool next_part(const PagedAttention &p, Run &run, Part &part)
     const uint32_t begin = run.unit > own ? run.unit - own : 0;
     const uint32_t end = run.unit + take > own ? run.unit + take - own : 0;
     part.sequence = run.sequence;
-    part.kv_head = run.head / p.row_tiles;
-    part.row_tile = run.head % p.row_tiles;
-    part.item = run.sequence * heads + run.head;
+    part.kv_head = run.kv_head;
+    part.row_tile = run.row_tile;
     part.length = length;
-    part.begin = begin * p.unit_keys;
-    part.end = end * p.unit_keys < length ? end * p.unit_keys : length;
+    part.begin = begin << p.unit_shift;
+    part.end = end << p.unit_shift < length ? end << p.unit_shift : length;
     part.whole = begin == 0 && end == units - own;
     part.record = 2 * blockIdx.x + (run.at == run.start ? 0 : 1);
-    if (begin == 0 && end > 0 && threadIdx.x == 0) {
-        // The block that holds the item's last unit.
-        const uint64_t past = uint64_t(run.at - run.unit) + units;
-        const uint32_t last = uint32_t((past * run.blocks - 1) / run.total);
-        item_shares(p)[part.item] = {part.record, part.whole ? 0 : last - blockIdx.x + 1};
-    }
+    part.last_unit = begin == 0 && end > 0 ? run.at - run.unit + units - 1 : UINT32_MAX;
     run.at += take;
     run.unit += take;
     if (run.unit == units) {
         run.unit = 0;
-        if (++run.head == heads) {
-            run.head = 0;
-            ++run.sequence;
-            run.length = run.at < run.end ? length_of(p, run.sequence) : 0;
+        if (++run.row_tile == p.row_tiles) {
+            run.row_tile = 0;
+            if (++run.kv_head == p.shape.kv_heads) {
+                run.kv_head = 0;
+                ++run.sequence;
+                run.length = run.at < run.end ? length_of(p, run.sequence) : 0;
+            }
         }
     }
     return true;
+}
+
+// Said once the part's reads are on their way.
+__device__ __forceinline__ void say_share(const PagedAttention &p, const Run &run,
+                                          const Part &part)
+{
+    if (part.last_unit == UINT32_MAX)
+        return;
+    const uint32_t count = part.whole ? 0 : block_of(run, part.last_unit) - blockIdx.x + 1;
+    const uint32_t item =
+        (part.sequence * p.shape.kv_heads + part.kv_head) * p.row_tiles + part.row_tile;
+    if (threadIdx.x == 0)
+        item_shares(p)[item] = {part.record, count};
 }
 
 // ---- any head width -----------------------------------------------------------
@@ -268,6 +329,7 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
     while (next_part(p, run, part)) {
         if (part.begin == part.end)
             continue;
+        say_share(p, run, part);
         __syncthreads();
         const uint32_t head0 = part.kv_head * p.group + part.row_tile * rows;
         const uint32_t left = p.group - part.row_tile * rows;
@@ -445,17 +507,22 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// Blocks of the kernel that a CU holds, by its registers: a grid is as many for
-// every CU, so that all run at once (an odd number of 16s in
-// binary16 takes more: half a register of each row is idle).
-constexpr int resident_blocks(int d, bool half)
+// Blocks of the kernel for every CU; all run at once.  Two keep 64 KB or more of
+// reads in flight, which is enough, and make fewer starts, ends and records than
+// what the registers hold: 32 sequences of 2048 keys, one of 65536, 64 of 20 to
+// 4000, 128 of 256, with 4 to 8 key heads of 64, f32: 28.4 / 48.0 / 41.4 / 26.0 us
+// with two, 29.2 / 50.2 / 41.3 / 26.1 with four; of 96 39.7 / 70.7 / 59.2 / 38.9 and
+// with three 39.7 / 73.2 / 58.8 / 43.9.  Narrow heads, whose tiles are small, take
+// four (width 32, binary16: 14.3 / 18.9 / 18.8 / 11.7, two 14.0 / 18.0 / 20.9 /
+// 13.1), wide ones the one that their registers allow.
+constexpr int resident_blocks(int d)
 {
-    return d > 128 ? 1 : d > 64 ? (half ? 2 : 3) : d == 48 && half ? 3 : 4;
+    return d > 128 ? 1 : d > 32 ? 2 : 4;
 }
 
 // D: head width.  SMALL: pages of 8 keys (else a page holds whole 16-key blocks).
 template <int D, bool HALF, bool SMALL>
-__global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mfma_kernel(PagedAttention p)
+__global__ __launch_bounds__(kBlock, resident_blocks(D)) void paged_gqa_mfma_kernel(PagedAttention p)
 {
     static_assert(D % 16 == 0 && D <= 256, "head width of the matrix-core path");
     using T = typename std::conditional<HALF, _Float16, float>::type;
@@ -574,23 +641,35 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
         const uint32_t first = part.begin + wave * TILE;
         const bool any = first < part.end;
         Ids ids = load_ids(any ? first : part.begin);
-        // The lane's row of queries; rows past the group are zero.
-        const float *query = p.query + (uint64_t(part.sequence) * p.query_heads + head0 + j) * D;
+        // The lane's row of queries; rows past the group, and columns past the head's
+        // end, are zero.
+        const float *query =
+            p.query + (uint64_t(part.sequence) * p.query_heads + head0 + (j < mine ? j : 0)) * D;
         float qf[U][HALF ? 8 : 4];
-        float most = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < (HALF ? 8 : 4); e += 4) {
                 const uint32_t column = HALF ? 32 * u + 8 * q + e : 16 * u + 4 * q + e;
-                const bool there = j < mine && column < uint32_t(D);
                 const v4f piece =
-                    there ? *reinterpret_cast<const v4f *>(query + column) : v4f{0, 0, 0, 0};
+                    *reinterpret_cast<const v4f *>(query + (column < uint32_t(D) ? column : 0));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4; ++i)
                     qf[u][e + i] = piece[i];
-                    most = fmaxf(most, fabsf(piece[i]));
-                }
+            }
+        if (any) {
+            load_keys(ids, first);
+            load_values(ids, first);
+        }
+        say_share(p, run, part);
+        float most = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < (HALF ? 8 : 4); ++i) {
+                const uint32_t column = HALF ? 32 * u + 8 * q + i : 16 * u + 4 * q + i;
+                qf[u][i] = j < mine && column < uint32_t(D) ? qf[u][i] : 0.0f;
+                most = fmaxf(most, fabsf(qf[u][i]));
             }
         float factor = p.scale;
         uint32_t qh[HALF ? U : 1][4], ql[HALF ? U : 1][4];
@@ -725,8 +804,6 @@ __global__ __launch_bounds__(kBlock, resident_blocks(D, HALF)) void paged_gqa_mf
         // condition on the others' loads the compiler knows how many are in flight
         // and waits for no more than it needs.
         if (any) {
-            load_keys(ids, first);
-            load_values(ids, first);
             uint32_t k0 = first;
 #pragma unroll 1
             for (; k0 + kWaves * TILE < part.end; k0 += kWaves * TILE)
@@ -796,9 +873,9 @@ MfmaKernel mfma_kernel_of(bool half, bool small)
 {
     if (half)
         return {small ? paged_gqa_mfma_kernel<D, true, true> : paged_gqa_mfma_kernel<D, true, false>,
-                resident_blocks(D, true)};
+                resident_blocks(D)};
     return {small ? paged_gqa_mfma_kernel<D, false, true> : paged_gqa_mfma_kernel<D, false, false>,
-            resident_blocks(D, false)};
+            resident_blocks(D)};
 }
 MfmaKernel mfma_kernel(const PageShape &shape)
 {
@@ -836,14 +913,18 @@ __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
     typedef float piece __attribute__((ext_vector_type(V)));
     const uint32_t heads = p.shape.kv_heads * p.row_tiles, d = p.shape.head_dim;
     const uint32_t lane = threadIdx.x;
-    const uint32_t item = blockIdx.x / p.rows, row = blockIdx.x % p.rows;
-    const uint32_t sequence = item / heads, head = item % heads;
-    const uint32_t in_group = head % p.row_tiles * p.rows + row;
+    const uint32_t item = blockIdx.x, row = blockIdx.y;
+    const ItemShare share = item_shares(p)[item];  // unset where there is no key
+    const uint32_t sequence = item / heads, head = item - sequence * heads;
+    uint32_t kv_head = head, row_tile = 0;
+    if (p.row_tiles > 1) {
+        kv_head = head / p.row_tiles;
+        row_tile = head - kv_head * p.row_tiles;
+    }
+    const uint32_t in_group = row_tile * p.rows + row;
     if (in_group >= p.group)
         return;
-    const ItemShare share = item_shares(p)[item];  // unset where there is no key
-    float *out = p.out + (uint64_t(sequence) * p.query_heads +
-                          head / p.row_tiles * p.group + in_group) * d;
+    float *out = p.out + (uint64_t(sequence) * p.query_heads + kv_head * p.group + in_group) * d;
     const uint32_t length = length_of(p, sequence);
     if (length == 0 || length == UINT32_MAX) {
         for (uint32_t c = lane; c < d; c += 64)
@@ -948,18 +1029,19 @@ bool paged_gqa_plan(PagedAttention &p, int cu_count)
     p.row_tiles = (p.group + p.rows - 1) / p.rows;
     // A unit is a wave's tile, and a block has one for each wave at least; all
     // blocks are resident at once.
-    p.unit_keys = !mfma.run ? kGeneralKeys : p.shape.half ? 32 : 16;
-    p.least_units = mfma.run ? kWaves : 1;
+    p.unit_shift = !mfma.run ? 6 : p.shape.half ? 5 : 4;
+    p.least_shift = mfma.run ? 2 : 0;
+    static_assert(kGeneralKeys == 1 << 6 && kWaves == 1 << 2, "shifts of a unit");
     const uint64_t items = uint64_t(p.sequences) * p.shape.kv_heads * p.row_tiles;
     const uint64_t longest = uint64_t(p.max_pages) << p.shape.page_shift;
     p.item_units = mfma.run ? kItemUnits : 0;
-    const uint64_t per_item = (longest + p.unit_keys - 1) / p.unit_keys + p.item_units;
+    p.longest = float(longest < (1u << 24) ? longest : 1u << 24);
+    const uint64_t per_item = (longest >> p.unit_shift) + 1 + p.item_units;
     // Units stay in 32 bits, and so do the join's threads, 64 for each row.
-    if (items * p.rows > (uint64_t(1) << 25) ||
-        (per_item && items > (uint64_t(1) << 31) / per_item))
+    if (items * p.rows > (uint64_t(1) << 25) || items > (uint64_t(1) << 31) / per_item)
         return false;
     const uint64_t most_blocks = uint64_t(cu_count) * (mfma.run ? mfma.resident : 4);
-    const uint64_t wanted = (items * per_item + p.least_units - 1) / p.least_units;
+    const uint64_t wanted = (items * per_item + (1u << p.least_shift) - 1) >> p.least_shift;
     p.blocks = uint32_t(wanted < most_blocks ? wanted : most_blocks);
     return true;
 }
@@ -990,7 +1072,7 @@ void launch_paged_gqa(hipStream_t stream, const PagedAttention &p)
         else
             paged_gqa_general_kernel<float><<<p.blocks, kBlock, bytes, stream>>>(p);
     }
-    const unsigned blocks = unsigned(items * p.rows);
+    const dim3 blocks(unsigned(items), p.rows);
     if (p.shape.head_dim % 4 == 0)
         paged_gqa_join_kernel<4><<<blocks, 64, 0, stream>>>(p);
     else
