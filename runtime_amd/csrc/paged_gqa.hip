@@ -15,10 +15,10 @@
 // block.
 //
 // Bound by the reads of the cache.  Both launches, in us (and the cache's TB/s): 96
-// sequences of 33 to 2048 keys, 8 key heads of 64, f32 40.6 (4.8); 48 of 17 to 8191,
-// 8 of 128, binary16 53.8 (5.1); one of 131071, 8 of 64, binary16 53.5 (5.0), f32 90.7
-// (5.9).  About 9 us of each are the two launches and their dependent reads, which
-// is all that a short call takes: one sequence of 2047 keys 10.8.
+// sequences of 33 to 2048 keys, 8 key heads of 64, f32 39.8 (4.9); 48 of 17 to 8191,
+// 8 of 128, binary16 52.5 (5.2); one of 131071, 8 of 64, binary16 48.7 (5.5), f32 88.1
+// (6.1).  About 9 us of each are the two launches and their dependent reads, which
+// is all that a short call takes: one sequence of 2047 keys 10.4.
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -440,8 +440,8 @@ __global__ __launch_bounds__(kBlock) void paged_gqa_general_kernel(PagedAttentio
 // Loads of the next tile's keys are issued as soon as the products have read
 // this tile's, its values' likewise: each is in flight behind the other's
 // arithmetic, in the same registers.  They are read once, and said to be
-// (nontemporal): with that said of both, of neither, or of one, the first three calls
-// above took 42.5 / 55.5 / 53.3, 47.5 / 64.2 / 58.3, and a time in between.
+// (nontemporal): with that said of neither the first three calls above took 12, 16 and
+// 9 % longer, of one a time in between.
 //
 // A tile is 32 keys in binary16 (a product's depth) and 16 in f32: of twice that
 // the registers hold fewer blocks.
@@ -904,9 +904,9 @@ MfmaKernel mfma_kernel(const PageShape &shape)
 // V-column pieces fit the wave (V = 4 where the head width allows), each summed in
 // record order, and the shares in order; lane i forms the weight of record i of
 // 64.  Bound by two dependent reads, of what other XCDs' blocks wrote, and by the
-// code's own fetch: 4.5 to 4.7 us, 6.0 with 128 records an item (4.7 to 5.1 and 7.0
-// with the records read once the weights are formed, up to 12.8 with a condition on
-// the loads, 5.1 to 6.1 for a block of 256 threads with barriers).
+// code's own fetch: 4.5 to 4.7 us (0.2 to 1 more with the records read once the
+// weights are formed, up to 12.8 with a condition on the loads, 5.1 to 6.1 for a
+// block of 256 threads with barriers).
 template <int V>
 __global__ __launch_bounds__(64) void paged_gqa_join_kernel(PagedAttention p)
 {

@@ -326,6 +326,29 @@ def test_many_ragged_sequences(backend, dim, half):
     assert np.all(np.abs(got - want) <= bound)
 
 
+@pytest.mark.parametrize("dim", [64, 20])
+@pytest.mark.parametrize("count", [3, 64, 65, 203, 255, 256, 257])
+def test_any_count_of_sequences(backend, count, dim):
+    """Some without a key, some with an invalid length, the last and first long."""
+    say("count", count, dim)
+    rng = np.random.default_rng(count + dim)
+    lengths = rng.integers(0, 40, count)
+    lengths[[0, -1]] = 333, 555
+    lengths[rng.random(count) < 0.3] = 0
+    pages, table = tables_for(rng, lengths, 16)
+    keys, values = (random_pages(rng, pages, 2, 16, dim, True) for _ in range(2))
+    query = rng.standard_normal((count, 6 * dim)).astype(np.float32)
+    want, bound = attend(query, keys, values, table, lengths, 6)
+    given = lengths.astype(np.float32)
+    bad = np.arange(1, count, 7)
+    given[bad] = np.resize(np.array([-1, 0.5, np.nan, np.inf, 16 * table.shape[1] + 1, 2e7],
+                                    np.float32), len(bad))
+    got = run_attention(backend, query, keys, values, table, given, 6, 2, dim)
+    good = np.setdiff1d(np.arange(count), bad)
+    assert np.isnan(got[bad]).all()
+    assert np.all(np.abs(got - want)[good] <= bound[good])
+
+
 @pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
 @pytest.mark.parametrize("dim", [64, 128, 36])
 def test_small_weights_keep_their_precision(backend, dim, half):
