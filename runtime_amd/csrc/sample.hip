@@ -103,6 +103,38 @@ __device__ __forceinline__ T wave_total(T v)
     return lane_value(wave_scan(v), 63);
 }
 
+// f over a wave's values, or the first row's 16 lanes, by the same moves.
+template <int CTRL, int ROWS, typename F>
+__device__ __forceinline__ uint32_t joined(uint32_t v, F f)
+{
+    return f(v, uint32_t(__builtin_amdgcn_update_dpp(int(v), int(v), CTRL, ROWS, 0xf, false)));
+}
+template <bool ROW, typename F>
+__device__ __forceinline__ uint32_t wave_join(uint32_t v, F f)
+{
+    v = joined<0x111, 0xf>(v, f);
+    v = joined<0x112, 0xf>(v, f);
+    v = joined<0x114, 0xf>(v, f);
+    v = joined<0x118, 0xf>(v, f);
+    if constexpr (!ROW) {
+        v = joined<0x142, 0xa>(v, f);
+        v = joined<0x143, 0xc>(v, f);
+    }
+    return __builtin_amdgcn_readlane(int(v), ROW ? 15 : 63);
+}
+template <bool ROW = false>
+__device__ __forceinline__ float wave_largest(float v)
+{
+    return __uint_as_float(wave_join<ROW>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+template <bool ROW = false>
+__device__ __forceinline__ uint32_t wave_least(uint32_t v)
+{
+    return wave_join<ROW>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
 // A kernel's LDS, as functions take it.
 struct Shared;
 typedef __attribute__((address_space(3))) Shared Lds;
@@ -305,19 +337,13 @@ struct Extremes {
 // The largest of the block's, NaN where one is NaN or +infinity.
 __device__ __attribute__((noinline)) float join_extremes(Lds *sh, float most, bool nan)
 {
-#pragma unroll
-    for (int offset = 32; offset > 0; offset >>= 1)
-        most = fmaxf(most, __shfl_xor(most, offset, 64));
+    most = wave_largest(most);
     const bool any = __any(nan);
     __syncthreads();
     if ((threadIdx.x & 63) == 0)
         sh->floats[threadIdx.x >> 6] = any ? __builtin_inff() : most;
     __syncthreads();
-    most = sh->floats[threadIdx.x % kWaves];
-#pragma unroll
-    for (int offset = kWaves / 2; offset > 0; offset >>= 1)
-        most = fmaxf(most, __shfl_xor(most, offset, 64));
-    most = __uint_as_float(__builtin_amdgcn_readfirstlane(int(__float_as_uint(most))));
+    most = wave_largest<true>(sh->floats[threadIdx.x % kWaves]);
     return most < __builtin_inff() ? most : __builtin_nanf("");
 }
 
@@ -638,13 +664,7 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
                 above += other > value ? lane_value(weight, int(i)) : 0.0;
             }
             // The largest always qualifies.
-            high = above < found.goal ? key_of(value) : UINT32_MAX;
-#pragma unroll
-            for (int step = 32; step > 0; step >>= 1) {
-                const uint32_t other = __shfl_xor(high, step, 64);
-                high = other < high ? other : high;
-            }
-            high = __builtin_amdgcn_readfirstlane(high);
+            high = wave_least(above < found.goal ? key_of(value) : UINT32_MAX);
         } else {
             uint32_t least = UINT32_MAX, most = 0;
             for (uint32_t i = lane; i < m; i += 64) {
@@ -652,14 +672,8 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
                 least = k < least ? k : least;
                 most = k > most ? k : most;
             }
-#pragma unroll
-            for (int step = 32; step > 0; step >>= 1) {
-                const uint32_t c = __shfl_xor(least, step, 64), d = __shfl_xor(most, step, 64);
-                least = c < least ? c : least;
-                most = d > most ? d : most;
-            }
-            uint32_t low = __builtin_amdgcn_readfirstlane(least) - 1;
-            high = __builtin_amdgcn_readfirstlane(most);
+            uint32_t low = wave_least(least) - 1;
+            high = ~wave_least(~most);
 #pragma unroll 1
             while (high - low > 1) {
                 const uint32_t middle = low + (high - low) / 2;
@@ -939,19 +953,13 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         });
         const float most = join_extremes(sh, extremes.most, extremes.nan);
         first = best == most ? first : UINT32_MAX;
-#pragma unroll
-        for (int offset = 32; offset > 0; offset >>= 1) {
-            const uint32_t other = __shfl_xor(first, offset, 64);
-            first = other < first ? other : first;
-        }
+        first = wave_least(first);
         if (lane == 0)
             sh->flags[wave] = first;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kWaves; ++w)
-                first = sh->flags[w] < first ? sh->flags[w] : first;
+        first = wave_least<true>(sh->flags[threadIdx.x % kWaves]);
+        if (threadIdx.x == 0)
             answer(most > -__builtin_inff() ? float(first) : __builtin_nanf(""));
-        }
         return;
     }
     __syncthreads();
