@@ -233,7 +233,8 @@ __device__ __forceinline__ void each(const Row &row, uint32_t begin, uint32_t en
         v4f v[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-            v[a] = load_chunk(row, c + a < end ? c + a : end - 1);
+            if (c + a < end)
+                v[a] = load_chunk(row, c + a);
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
             if (c + a < end)
