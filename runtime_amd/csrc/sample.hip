@@ -371,21 +371,23 @@ struct Units {
     {
         return raised(w + shift);
     }
+    // What lies behind the exponent, which is shift's.
     __device__ unsigned long long raised(double w) const
     {
-        // shift's low word is zero.
-        const uint64_t bits = __builtin_bit_cast(uint64_t, w);
-        const uint32_t high = uint32_t(bits >> 32);
-        return uint64_t(high - uint32_t(__builtin_bit_cast(uint64_t, shift) >> 32)) << 32 |
-               uint32_t(bits);
+        return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
     }
 };
 
-__device__ __forceinline__ void add_to_bin(Lds *sh, uint32_t b, unsigned long long v)
+// Bins stand in reverse: bin b in slot kBins - 1 - b.
+__device__ __forceinline__ void add_to_slot(Lds *sh, int slot, unsigned long long v)
 {
     (void)__hip_atomic_fetch_add(reinterpret_cast<__attribute__((address_space(3))) uint64_t *>(
-                                     &sh->bins.weight[b]),
+                                     &sh->bins.weight[slot]),
                                  uint64_t(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ void add_to_bin(Lds *sh, uint32_t b, unsigned long long v)
+{
+    add_to_slot(sh, int(kBins - 1 - b), v);
 }
 
 __device__ __attribute__((noinline)) void clear_bins(Lds *sh)
@@ -426,7 +428,7 @@ __device__ __attribute__((noinline)) void histogram(Lds *sh, uint32_t chunks, do
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (bin[e] > -int(kBins))
-                    add_to_bin(sh, 0u - uint32_t(bin[e]), units.raised(w[e]));
+                    add_to_slot(sh, int(kBins - 1) + bin[e], units.raised(w[e]));
         });
     __syncthreads();
 }
@@ -445,7 +447,8 @@ __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double
 {
     constexpr uint32_t kEach = kBins / kBlock;
     static_assert(kEach == 2, "neighbours of a thread");
-    const uint64_t a = sh->bins.weight[2 * threadIdx.x], b = sh->bins.weight[2 * threadIdx.x + 1];
+    const uint32_t last = kBins - 1 - 2 * threadIdx.x;
+    const uint64_t a = sh->bins.weight[last], b = sh->bins.weight[last - 1];
     const Scan<uint64_t> scan = block_scan(sh, a + b);
     const double total = double(scan.total) * unit;
     if (share >= 0.0)
