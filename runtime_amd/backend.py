@@ -493,9 +493,10 @@ def _page_ids(ids) -> np.ndarray:
     given = np.asarray(ids).reshape(-1)
     if given.dtype == np.uint32 or given.size == 0:
         return np.ascontiguousarray(given, dtype=np.uint32)
-    if given.dtype.kind not in "iu" or given.min() < 0 or given.max() >= 1 << 32:
+    converted = given.astype(np.uint32) if given.dtype.kind in "iu" else None
+    if converted is None or not (converted == given).all():
         raise ValueError("page ids must be whole numbers in [0, 2^32)")
-    return given.astype(np.uint32)
+    return converted
 
 
 # ---- operation descriptors (engine-api/src/backend.rs:128-383) -------------

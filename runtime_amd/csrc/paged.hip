@@ -314,8 +314,8 @@ __global__ __launch_bounds__(kBlock) void paged_rope_vector_kernel(PagedRope p, 
 // thread's in flight at once.  The host has checked that no page is written
 // twice, and none written that is read.  Page sizes are multiples of 8 rows, so a
 // page is whole 8-element pieces.  Bound by the bytes: 599 pages of 16 KB in 12
-// buffers (236 MB read and written) take 52 us, 4.5 TB/s, in three launches of 256
-// pages at most (an element a thread took 124); one page of 12 buffers 3.4 us, a
+// buffers (236 MB read and written) take 50 us, 4.7 TB/s, in two launches (an element a
+// thread took 124); one page of 12 buffers 3.4 us, a
 // launch.
 constexpr uint32_t kCopyPieces = 4;  // of 8 elements, of a thread
 constexpr uint64_t kCopyPart = 8 * kCopyPieces * kBlock;
@@ -361,7 +361,8 @@ __device__ __forceinline__ void copy_part(const void *from, void *to, uint64_t e
     }
 }
 
-__global__ __launch_bounds__(kBlock) void copy_pages_kernel(PageCopy c)
+template <uint32_t PAIRS>
+__global__ __launch_bounds__(kBlock) void copy_pages_kernel(PageCopy<PAIRS> c)
 {
     const uint32_t pair = blockIdx.y, buffer = blockIdx.z;
     const bool from_half = c.from_half[buffer], to_half = c.to_half[buffer];
@@ -424,10 +425,13 @@ void launch_paged_qk_norm_rope(hipStream_t stream, const PagedRope &p)
     paged_rope_kernel<<<grid_for(segments, kBlock / 64), kBlock, 0, stream>>>(p);
 }
 
-void launch_copy_pages(hipStream_t stream, const PageCopy &c)
+template <uint32_t PAIRS>
+void launch_copy_pages(hipStream_t stream, const PageCopy<PAIRS> &c)
 {
     const uint64_t parts = (c.elements + kCopyPart - 1) / kCopyPart;
-    copy_pages_kernel<<<dim3(unsigned(parts), c.pairs, c.buffers), kBlock, 0, stream>>>(c);
+    copy_pages_kernel<PAIRS><<<dim3(unsigned(parts), c.pairs, c.buffers), kBlock, 0, stream>>>(c);
 }
+template void launch_copy_pages(hipStream_t, const PageCopy<kCopyPairs> &);
+template void launch_copy_pages(hipStream_t, const PageCopy<kCopyFewPairs> &);
 
 }  // namespace mfh

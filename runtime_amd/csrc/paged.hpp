@@ -67,17 +67,21 @@ struct PagedRope {
 };
 void launch_paged_qk_norm_rope(hipStream_t stream, const PagedRope &p);
 
-// One launch of a page copy: `pairs` (from, to) pages in each of `buffers`.
-constexpr uint32_t kCopyPairs = 256, kCopyBuffers = 32;
+// One launch of a page copy: `pairs` (from, to) pages in each of `buffers`.  It is the
+// kernel's argument, of 4 KB at most, which the host writes for every launch: a short
+// form serves the few pages of a fork.
+constexpr uint32_t kCopyBuffers = 32, kCopyPairs = 416, kCopyFewPairs = 8;
+template <uint32_t PAIRS>
 struct PageCopy {
     uint32_t pairs = 0, buffers = 0;
     uint64_t elements = 0;  // of one page
-    void *to[kCopyBuffers] = {};
-    const void *from[kCopyBuffers] = {};
-    uint8_t to_half[kCopyBuffers] = {}, from_half[kCopyBuffers] = {};
-    uint32_t from_page[kCopyPairs] = {}, to_page[kCopyPairs] = {};
+    void *to[kCopyBuffers];
+    const void *from[kCopyBuffers];
+    uint8_t to_half[kCopyBuffers], from_half[kCopyBuffers];
+    uint32_t from_page[PAIRS], to_page[PAIRS];
 };
-void launch_copy_pages(hipStream_t stream, const PageCopy &c);
+template <uint32_t PAIRS>
+void launch_copy_pages(hipStream_t stream, const PageCopy<PAIRS> &c);
 
 // One new token per sequence over paged caches.
 struct PagedAttention {

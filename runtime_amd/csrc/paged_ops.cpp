@@ -127,6 +127,33 @@ mfh_status aliased(mfh_ctx *ctx)
     return fail(ctx, MFH_INVALID_ARGUMENT, "output aliases an input");
 }
 
+// The launches of a page copy, PAIRS pages and kCopyBuffers buffers at most in each.
+template <uint32_t PAIRS>
+void copy_pairs(hipStream_t stream, uint64_t elements, mfh_buf *const *destinations,
+                const mfh_buf *const *sources, size_t buffers, const uint32_t *from_pages,
+                const uint32_t *to_pages, size_t count)
+{
+    PageCopy<PAIRS> c;
+    c.elements = elements;
+    for (size_t b = 0; count && b < buffers; b += c.buffers) {
+        c.buffers = uint32_t(buffers - b < kCopyBuffers ? buffers - b : kCopyBuffers);
+        for (uint32_t i = 0; i < c.buffers; ++i) {
+            c.to[i] = destinations[b + i]->dev;
+            c.from[i] = sources[b + i]->dev;
+            c.to_half[i] = destinations[b + i]->dtype == MFH_DTYPE_U8;
+            c.from_half[i] = sources[b + i]->dtype == MFH_DTYPE_U8;
+        }
+        for (size_t n = 0; n < count; n += c.pairs) {
+            c.pairs = uint32_t(count - n < PAIRS ? count - n : PAIRS);
+            for (uint32_t i = 0; i < c.pairs; ++i) {
+                c.from_page[i] = from_pages[n + i];
+                c.to_page[i] = to_pages[n + i];
+            }
+            launch_copy_pages(stream, c);
+        }
+    }
+}
+
 bool positive(float v) { return std::isfinite(v) && v > 0.0f; }
 
 }  // namespace
@@ -425,25 +452,12 @@ mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
     DeviceGuard guard(ctx->device);
     for (size_t i = 0; i < buffers; ++i)
         mark_written(destinations[i]);
-    PageCopy c;
-    c.elements = first.stride();
-    for (size_t b = 0; count && b < buffers; b += c.buffers) {
-        c.buffers = uint32_t(buffers - b < kCopyBuffers ? buffers - b : kCopyBuffers);
-        for (uint32_t i = 0; i < c.buffers; ++i) {
-            c.to[i] = destinations[b + i]->dev;
-            c.from[i] = sources[b + i]->dev;
-            c.to_half[i] = destinations[b + i]->dtype == MFH_DTYPE_U8;
-            c.from_half[i] = sources[b + i]->dtype == MFH_DTYPE_U8;
-        }
-        for (size_t n = 0; n < count; n += c.pairs) {
-            c.pairs = uint32_t(count - n < kCopyPairs ? count - n : kCopyPairs);
-            for (uint32_t i = 0; i < c.pairs; ++i) {
-                c.from_page[i] = from_pages[n + i];
-                c.to_page[i] = to_pages[n + i];
-            }
-            launch_copy_pages(ctx->stream, c);
-        }
-    }
+    if (count <= kCopyFewPairs)
+        copy_pairs<kCopyFewPairs>(ctx->stream, first.stride(), destinations, sources, buffers,
+                                  from_pages, to_pages, count);
+    else
+        copy_pairs<kCopyPairs>(ctx->stream, first.stride(), destinations, sources, buffers,
+                               from_pages, to_pages, count);
     return launched(ctx);
 }
 

@@ -31,9 +31,9 @@
 // without work takes 9000 cycles), and by the fetch of code that runs once: a pass is
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
-// times as long).  One row of 65536 takes, in us: greedy 6.6, min-p 14, all tokens
-// 21, top-k 50 20.7 and with top-p 25.4, top-p 0.9 at temperatures 0.6 / 1 / 1.5
-// 34 / 40 / 54; 192 rows 11, 23, 28, 26 and 31, 44 / 53 / 66.
+// times as long).  One row of 65536 takes, in us: greedy 6.0, min-p 13.6, all
+// tokens 21, top-k 50 19.9 and with top-p 24.3, top-p 0.9 at temperatures 0.6 / 1 /
+// 1.5 32.6 / 38.5 / 52.5; 192 rows 11, 22, 28, 25 and 30, 43 / 52 / 65.
 #include "kernels.hpp"
 #include "paged.hpp"
 
