@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 
 from runtime_amd import hiptime
-from runtime_amd.backend import (CACHE, ExecutorError, CacheLength, GqaSpec, HipBackend,
+from runtime_amd.backend import (CACHE, ExecutorError, CacheLength, GqaSpec, HipBackend, Limits,
                                  PackedHeadSpec, PagedRopeSpec, RopeScaling, RotarySpec)
 
 pytestmark = pytest.mark.gpu
@@ -638,6 +638,27 @@ def test_a_captured_workspace_is_kept():
     hiptime.check(hip.hipGraphExecDestroy(program), "destroy")
     hiptime.check(hip.hipGraphDestroy(graph), "destroy")
     backend.close()
+
+
+def test_a_workspace_past_the_limit_is_refused():
+    """Nothing is written then, and with room the same call works."""
+    for limit, variant in ((6 << 20, "ResourceLimit"), (64 << 20, None)):
+        backend = HipBackend(0, limits=Limits(max_total_bytes=limit))
+        k, v = (backend.alloc_pages(1, 1, 16, 256, half=True) for _ in range(2))
+        query = backend.allocate_f32((64, 16 * 256))
+        out = upload(backend, np.full((64, 16 * 256), 7.0, np.float32))
+        # 64 items of 53 units each: 256 blocks of two records of 16 rows of 256.
+        args = (out, query, k, v, backend.allocate_f32((64, 100)),
+                upload(backend, np.full(64, 5.0, np.float32)), GqaSpec(16, 1, 256))
+        if variant:
+            with pytest.raises(ExecutorError) as error:
+                backend.paged_gqa(*args)
+            assert error.value.variant == variant
+            assert np.all(backend.read(out) == 7.0)
+        else:
+            backend.paged_gqa(*args)
+            assert np.all(backend.read(out) == 0.0)
+        backend.close()
 
 
 def captured(backend, call):
