@@ -572,14 +572,16 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
         const Scan<uint64_t> scan = block_scan(sh, mine);
         uint32_t at = uint32_t(listed + scan.upto - mine);
         uint32_t pick = uint32_t((listed + scan.upto - mine) >> 32);
+        // Of more than the list holds nothing is listed but what is picked.
+        const bool fits = uint32_t(listed + scan.total) <= kMany;
 #pragma unroll 1
         for (uint32_t w = words.first; w < words.last; ++w) {
             const uint64_t word = sh->bins.codes[w];
 #pragma unroll 1
-            for (uint64_t bits = word & kListed; bits; bits &= bits - 1, ++at) {
+            for (uint64_t bits = (fits ? word : word >> 4) & kListed; bits; bits &= bits - 1) {
                 const uint32_t token = token_of(begin, w, bits);
-                if (at < kMany)
-                    sh->index[at] = token;
+                if (fits)
+                    sh->index[at++] = token;
                 if (word >> 4 & bits & -bits) {
                     if (pick < kList)
                         sh->pick[pick] = token;
