@@ -31,9 +31,9 @@
 // without work takes 9000 cycles), and by the fetch of code that runs once: a pass is
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
-// times as long).  One row of 65536 takes, in us: greedy 6.0, min-p 13.6, all
+// times as long).  One row of 65536 takes, in us: greedy 6.0, min-p 12.9, all
 // tokens 21, top-k 50 19.9 and with top-p 24.3, top-p 0.9 at temperatures 0.6 / 1 /
-// 1.5 32.6 / 38.5 / 52.5; 192 rows 11, 22, 28, 25 and 30, 43 / 52 / 65.
+// 1.5 31.9 / 37.6 / 46.3; 192 rows 11, 22, 28, 25 and 30, 42 / 52 / 59.
 #include "kernels.hpp"
 #include "paged.hpp"
 
@@ -546,11 +546,12 @@ __device__ __forceinline__ uint32_t token_of(uint32_t begin, uint32_t word, uint
 
 struct Listed {
     uint32_t count, picked;
-    float most;  // the row's largest, or NaN (join_extremes)
+    float most;  // the row's largest, or NaN (join_extremes), where asked for
 };
 // Lists the tokens with low <= v, but -infinity, in sh->index and those with also
 // v < high in sh->pick, in their order; what passes the lists' ends is counted.
-__device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, float high)
+__device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, float high,
+                                                        bool want_most)
 {
     const Row row = row_of(sh);
     low = fmaxf(low, -3.4028235e38f);
@@ -561,7 +562,10 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
         const uint32_t end =
             row.chunks - begin < kSegmentChunks ? row.chunks : begin + kSegmentChunks;
         __syncthreads();
-        code_chunks(sh, row, begin, end, low, high, [&](v4f v) { extremes.take(v); });
+        code_chunks(sh, row, begin, end, low, high, [&](v4f v) {
+            if (want_most)
+                extremes.take(v);
+        });
         __syncthreads();
         const Words words(end - begin);
         uint64_t mine = 0;
@@ -591,8 +595,12 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
         }
         listed += scan.total;
     }
-    return {uint32_t(listed), uint32_t(listed >> 32),
-            join_extremes(sh, extremes.most, extremes.nan)};
+    float most = 0.0f;
+    if (want_most)
+        most = join_extremes(sh, extremes.most, extremes.nan);
+    else
+        __syncthreads();  // the lists are there (as behind join_extremes' first wait)
+    return {uint32_t(listed), uint32_t(listed >> 32), most};
 }
 
 // How many equal tokens of weight `each` fit above `above` short of `goal`: those
@@ -990,7 +998,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
                 floor = edge_of(sh, found.reached ? found.bin : kBins - 1, double(from));
             }
         }
-        list = list_tokens(sh, floor, __builtin_inff());
+        list = list_tokens(sh, floor, __builtin_inff(), true);
     } else {
         list.most = row_extremes(sh, row.chunks);
     }
@@ -1019,7 +1027,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale);
         const float low = edge_of(sh, found.bin, from);
         const float high = found.bin ? edge_of(sh, found.bin - 1, from) : __builtin_inff();
-        list = list_tokens(sh, low, high);
+        list = list_tokens(sh, low, high, false);
         // Within the bin: its own equal steps.
         cut = list.picked <= kList
                   ? list_cut(sh, &sh->pick[0], list.picked, false, found.goal, -1.0, found.over,
@@ -1037,7 +1045,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     }
     // A list of what a cut has left, where there is none yet.
     if (!listed && ((k && list.count > kList) || (!k && share < 0.0 && min_p > 0.0f))) {
-        const uint32_t n = list_tokens(sh, cut.value, __builtin_inff()).count;
+        const uint32_t n = list_tokens(sh, cut.value, __builtin_inff(), false).count;
         listed = n <= kMany ? n : 0;
     }
     choose(sh, listed, cut, double(min_p), double(u), s.out + r, s.copy ? s.copy + r : nullptr);
