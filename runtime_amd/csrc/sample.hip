@@ -31,9 +31,9 @@
 // without work takes 9000 cycles), and by the fetch of code that runs once: a pass is
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
-// times as long).  One row of 65536 takes, in us: greedy 6.0, min-p 12.9, all
-// tokens 21, top-k 50 19.9 and with top-p 24.3, top-p 0.9 at temperatures 0.6 / 1 /
-// 1.5 31.9 / 37.6 / 46.3; 192 rows 11, 22, 28, 25 and 30, 42 / 52 / 59.
+// times as long).  One row of 65536 takes, in us: greedy 6.1, min-p 12.7, all
+// tokens 20, top-k 50 19.9 and with top-p 24.3, top-p 0.9 at temperatures 0.6 / 1 /
+// 1.5 31.6 / 36.7 / 45.6; 192 rows 11, 22, 27, 25 and 30, 42 / 51 / 58.
 #include "kernels.hpp"
 #include "paged.hpp"
 
@@ -799,17 +799,20 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
 }
 
 // The weights of four tokens that a cut (not of -infinity) and min_p leave, formed
-// side by side.
-__device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, const uint32_t (&i)[4],
-                                         Cut cut, double min_p, double (&w)[4])
+// side by side; `tied(e)`: whether token e is kept where its value is the cut's.
+template <typename F>
+__device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, Cut cut, double min_p,
+                                         double (&w)[4], F tied)
 {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         w[e] = weight_of(sh, row, v[e]);
     asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        w[e] = bool(cut.keeps(v[e], i[e]) & (w[e] >= min_p)) ? w[e] : 0.0;
+    for (int e = 0; e < 4; ++e) {
+        const bool kept = (v[e] > cut.value) | ((v[e] == cut.value) & tied(e));
+        w[e] = kept & (w[e] >= min_p) ? w[e] : 0.0;
+    }
 }
 
 // Of some lanes with sums, the one that holds the target: the first that passes it,
@@ -839,38 +842,41 @@ __device__ __attribute__((noinline)) void choose(Lds *sh, uint32_t listed, Cut c
         const uint32_t first = wave * each_has < tiles ? wave * each_has : tiles;
         const uint32_t last = first + each_has < tiles ? first + each_has : tiles;
         double w[4] = {0.0, 0.0, 0.0, 0.0}, own = 0.0;
-        v4f v = {0, 0, 0, 0}, next = v;
-        uint32_t i[4] = {0, 0, 0, 0}, next_i[4] = {0, 0, 0, 0};
-        // The next tile's loads are in flight behind this one's weights.
+        if (listed) {
 #pragma unroll 1
-        for (uint32_t t = first; t <= last; ++t) {
-            if (t < last) {
-                const uint32_t at = (begin + t) * 256 + 4 * lane;
-                if (listed) {
+            for (uint32_t t = begin + first; t < begin + last; ++t) {
+                const uint32_t at = t * 256 + 4 * lane;
+                uint32_t i[4];
+                v4f v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        next_i[e] = sh->index[at + e < listed ? at + e : listed - 1];
+                for (int e = 0; e < 4; ++e)
+                    i[e] = sh->index[at + e < listed ? at + e : listed - 1];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        next[e] = row.logits[next_i[e]];
+                for (int e = 0; e < 4; ++e)
+                    v[e] = row.logits[i[e]];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        next[e] = at + e < listed ? next[e] : -__builtin_inff();
-                } else {
-                    next = load_four(row, at, (begin + t + 1) * 256 <= row.width);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        next_i[e] = at + e;
-                }
-            }
-            if (t > first) {
-                terms_of(sh, row, v, i, cut, min_p, w);
+                for (int e = 0; e < 4; ++e)
+                    v[e] = at + e < listed ? v[e] : -__builtin_inff();
+                terms_of(sh, row, v, cut, min_p, w, [&](int e) { return i[e] <= cut.index; });
                 own += (w[0] + w[1]) + (w[2] + w[3]);
             }
-            v = next;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                i[e] = next_i[e];
+        } else if (first < last) {
+            // The next tile's loads are in flight behind this one's weights.
+            const auto load = [&](uint32_t t) {
+                return load_four(row, t * 256 + 4 * lane, (t + 1) * 256 <= row.width);
+            };
+            v4f next = load(begin + first);
+#pragma unroll 1
+            for (uint32_t t = begin + first; t < begin + last; ++t) {
+                const v4f v = next;
+                if (t + 1 < begin + last)
+                    next = load(t + 1);
+                const int room = int(cut.index < 0x7fffffffu ? cut.index : 0x7fffffffu) -
+                                 int(t * 256);
+                terms_of(sh, row, v, cut, min_p, w,
+                         [&](int e) { return int(4 * lane) + e <= room; });
+                own += (w[0] + w[1]) + (w[2] + w[3]);
+            }
         }
         const double upto = wave_scan(own);
         __syncthreads();
@@ -898,9 +904,11 @@ __device__ __attribute__((noinline)) void choose(Lds *sh, uint32_t listed, Cut c
             for (int e = 0; e < 4; ++e)
                 if (w[e] > 0.0 && !done) {
                     at += w[e];
-                    token = i[e];
+                    token = (begin + first) * 256 + 4 * lane + e;
                     done = at > target;
                 }
+            if (listed)
+                token = sh->index[token];
             *out = float(token);
             if (copy)
                 *copy = float(token);
