@@ -88,6 +88,17 @@ __device__ __forceinline__ T wave_scan(T v)
     v = plus(v, moved<0x143, 0xc>(bits(v)));  // lane 31 to rows 2 and 3
     return v;
 }
+__device__ __forceinline__ uint32_t lanes_scan(uint32_t v)  // of a row of 16
+{
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false));
+    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane)
+{
+    return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
+}
 template <typename T>
 __device__ __forceinline__ T lane_value(T v, int lane)
 {
@@ -170,8 +181,8 @@ struct Shared {
     float floats[kWaves];
     uint32_t flags[kWaves];
     uint32_t found;
-    uint64_t before;
     uint32_t reached;
+    double over;
 };
 
 // The row in scalar registers.
@@ -295,6 +306,14 @@ __device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v)
 {
     int steps;
     return weight_of(sh, row, v, &steps);
+}
+
+// Of lanes with `some` of what is summed, the one that holds a target: the first that
+// reaches it (`past`), or else the last.
+__device__ __forceinline__ uint32_t holder(bool some, bool past)
+{
+    const uint64_t with = __ballot(some), over = __ballot(some && past);
+    return over ? __builtin_ctzll(over) : with ? 63 - __builtin_clzll(with) : 0;
 }
 
 template <typename T>
@@ -447,25 +466,34 @@ __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double
 {
     constexpr uint32_t kEach = kBins / kBlock;
     static_assert(kEach == 2, "neighbours of a thread");
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t last = kBins - 1 - 2 * threadIdx.x;
     const uint64_t a = sh->bins.weight[last], b = sh->bins.weight[last - 1];
-    const Scan<uint64_t> scan = block_scan(sh, a + b);
-    const double total = double(scan.total) * unit;
+    const uint64_t scan = wave_scan(a + b);
+    if (lane == 63)
+        sh->scratch[wave] = scan;
+    __syncthreads();
+    // Every wave finds the one that holds the goal; that one alone goes on.
+    const uint64_t own = sh->scratch[lane % kWaves], upto = wave_scan(own);  // a row's
     if (share >= 0.0)
-        goal = share > 0.0 ? share * total : 0x1p-60;
-    const auto look = [&](uint32_t bin, uint64_t before, uint64_t own) {
-        const bool reached = over + double(before + own) * unit >= goal;
-        if (own && over + double(before) * unit < goal &&
-            (reached || before + own == scan.total)) {
-            sh->found = bin;
-            sh->before = before;
+        goal = share > 0.0 ? share * (double(lane_value(upto, kWaves - 1)) * unit) : 0x1p-60;
+    const uint32_t here = holder(lane < kWaves && own, over + double(upto) * unit >= goal);
+    if (wave == here) {
+        const uint64_t end = lane_value(upto, int(here)) - lane_value(own, int(here)) + scan;
+        // Boundaries of the thread's bins, as doubles that neighbours share.
+        const double from = over + double(end - a - b) * unit, middle = over + double(end - b) * unit;
+        const double to = over + double(end) * unit;
+        const bool reached = to >= goal;
+        if (lane == holder(a + b, reached)) {
+            const bool first = a && (!b || middle >= goal);
+            sh->found = 2 * threadIdx.x + (first ? 0 : 1);
+            sh->over = first ? from : middle;
             sh->reached = reached;
         }
-    };
-    look(2 * threadIdx.x, scan.upto - a - b, a);
-    look(2 * threadIdx.x + 1, scan.upto - b, b);
+    }
     __syncthreads();
-    return {goal, over + double(sh->before) * unit, sh->found, sh->reached != 0};
+    return {goal, sh->over, sh->found, sh->reached != 0};
 }
 
 // The smallest value of a bin up to `b`, -infinity where all finite ones are: by
@@ -648,14 +676,20 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
     };
     static_assert(kList == 2 * kBlock, "neighbours of a thread");
     const bool a = in(2 * threadIdx.x), b = in(2 * threadIdx.x + 1);
-    const Scan<uint64_t> scan = block_scan(sh, uint64_t(a) + b);
+    const uint64_t some_a = __ballot(a), some_b = __ballot(b), below = (1ull << lane) - 1;
+    if (lane == 0)
+        sh->flags[threadIdx.x >> 6] = __popcll(some_a) + __popcll(some_b);
+    __syncthreads();
+    const uint32_t in_wave = sh->flags[lane % kWaves], waves = lanes_scan(in_wave);
+    uint32_t at = __popcll(some_a & below) + __popcll(some_b & below);
+    at += lane_value(waves - in_wave, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
     if (a)
-        sh->sub[scan.upto - a - b] = 2 * threadIdx.x;
+        sh->sub[at] = 2 * threadIdx.x;
     if (b)
-        sh->sub[scan.upto - b] = 2 * threadIdx.x + 1;
+        sh->sub[at + a] = 2 * threadIdx.x + 1;
     __syncthreads();
     if (threadIdx.x < 64) {
-        const uint32_t m = __builtin_amdgcn_readfirstlane(uint32_t(scan.total));
+        const uint32_t m = lane_value(waves, kWaves - 1);
         const auto above_of = [&](uint32_t key) {
             double above = 0.0;
             for (uint32_t i = lane; i < m; i += 64) {
@@ -815,13 +849,6 @@ __device__ __forceinline__ void terms_of(Lds *sh, const Row &row, v4f v, Cut cut
     }
 }
 
-// Of some lanes with sums, the one that holds the target: the first that passes it,
-// or else the last with any.
-__device__ __forceinline__ uint32_t holder(double own, double upto, double target)
-{
-    const uint64_t some = __ballot(own > 0.0), past = __ballot(own > 0.0 && upto > target);
-    return past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : 0;
-}
 // The first kept token, in the vocabulary's order, at which the sum of kept weights
 // passes u * total (the last kept one where rounding leaves none): of all tokens,
 // or of `listed` in sh->index.  Each wave sums a run of tiles of 256, a lane four
@@ -888,7 +915,7 @@ __device__ __attribute__((noinline)) void choose(Lds *sh, uint32_t listed, Cut c
         if (target < 0.0)
             target = u * lane_value(runs, kWaves - 1);
         const uint32_t chosen =
-            __builtin_amdgcn_readfirstlane(holder(run, passed + runs, target));
+            __builtin_amdgcn_readfirstlane(holder(run > 0.0, passed + runs > target));
         if (chosen)
             passed += lane_value(runs, int(chosen) - 1);
         if (each_has > 1) {
@@ -896,7 +923,7 @@ __device__ __attribute__((noinline)) void choose(Lds *sh, uint32_t listed, Cut c
             tiles = tiles - chosen * each_has < each_has ? tiles - chosen * each_has : each_has;
             continue;
         }
-        if (wave == chosen && lane == holder(own, passed + upto, target)) {
+        if (wave == chosen && lane == holder(own > 0.0, passed + upto > target)) {
             double at = passed + (upto - own);
             uint32_t token = 0;
             bool done = false;
