@@ -88,12 +88,18 @@ __device__ __forceinline__ T wave_scan(T v)
     v = plus(v, moved<0x143, 0xc>(bits(v)));  // lane 31 to rows 2 and 3
     return v;
 }
-__device__ __forceinline__ uint32_t lanes_scan(uint32_t v)  // of a row of 16
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_scan(uint32_t v)  // of a row's 16 lanes, or all
 {
     v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false));
     v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false));
     v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false));
-    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
+    if constexpr (LANES == 64) {
+        v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xa, 0xf, false));
+        v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xc, 0xf, false));
+    }
+    return v;
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane)
 {
@@ -354,6 +360,10 @@ struct Extremes {
         nan = nan || __builtin_isunordered(v[0], v[1]) || __builtin_isunordered(v[2], v[3]);
     }
 };
+__device__ __forceinline__ float extremes_of(float most)
+{
+    return most < __builtin_inff() ? most : __builtin_nanf("");
+}
 // The largest of the block's, NaN where one is NaN or +infinity.
 __device__ __attribute__((noinline)) float join_extremes(Lds *sh, float most, bool nan)
 {
@@ -363,8 +373,7 @@ __device__ __attribute__((noinline)) float join_extremes(Lds *sh, float most, bo
     if ((threadIdx.x & 63) == 0)
         sh->floats[threadIdx.x >> 6] = any ? __builtin_inff() : most;
     __syncthreads();
-    most = wave_largest<true>(sh->floats[threadIdx.x % kWaves]);
-    return most < __builtin_inff() ? most : __builtin_nanf("");
+    return extremes_of(wave_largest<true>(sh->floats[threadIdx.x % kWaves]));
 }
 
 __device__ __attribute__((noinline)) float row_extremes(Lds *sh, uint32_t chunks)
@@ -498,9 +507,8 @@ __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double
 
 // The smallest value of a bin up to `b`, -infinity where all finite ones are: by
 // halving, from a few neighbours where the steps' rounding allows.
-__device__ __attribute__((noinline)) float edge_of(Lds *sh, uint32_t b, double from)
+__device__ __forceinline__ float edge_of(const Row &row, uint32_t b, double from)
 {
-    const Row row = row_of(sh);
     const double reach = (double(b) + 1.0) / row.per_step, near = from - reach;
     const double room = 1.5e-7 * __builtin_fabs(near) + 1e-12 * (__builtin_fabs(from) + reach);
     constexpr double kMost = 3.4028234663852886e38;
@@ -523,6 +531,24 @@ __device__ __attribute__((noinline)) float edge_of(Lds *sh, uint32_t b, double f
             low = middle;
     }
     return value_of(high);
+}
+
+// The smallest values of bins up to `b` and, for all but bin 0, up to b - 1: by a wave
+// each.
+struct Edges {
+    float low, high;
+};
+__device__ __attribute__((noinline)) Edges edges_of(Lds *sh, uint32_t b, double from)
+{
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave < 2) {
+        const Row row = row_of(sh);
+        const float edge = wave > b ? __builtin_inff() : edge_of(row, b - wave, from);
+        if ((threadIdx.x & 63) == 0)
+            sh->floats[wave] = edge;
+    }
+    __syncthreads();
+    return {sh->floats[0], sh->floats[1]};
 }
 
 // The kept tokens: values above `value`, and equal ones up to `index`.
@@ -583,8 +609,10 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
 {
     const Row row = row_of(sh);
     low = fmaxf(low, -3.4028235e38f);
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Extremes extremes;
-    uint64_t listed = 0;  // and, in the high word, picked
+    uint32_t listed = 0, picked = 0;
 #pragma unroll 1
     for (uint32_t begin = 0; begin < row.chunks; begin += kSegmentChunks) {
         const uint32_t end =
@@ -596,16 +624,30 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
         });
         __syncthreads();
         const Words words(end - begin);
-        uint64_t mine = 0;
+        // Listed and picked, in two halves of a word: a wave has 8192 tokens at most.
+        static_assert(kSegmentChunks * kChunk / kWaves < 65536, "a wave's tokens of a segment");
+        uint32_t mine = 0;
         for (uint32_t w = words.first; w < words.last; ++w) {
             const uint64_t word = sh->bins.codes[w];
-            mine += __popcll(word & kListed) | uint64_t(__popcll(word >> 4 & kListed)) << 32;
+            mine += __popcll(word & kListed) + (__popcll(word >> 4 & kListed) << 16);
         }
-        const Scan<uint64_t> scan = block_scan(sh, mine);
-        uint32_t at = uint32_t(listed + scan.upto - mine);
-        uint32_t pick = uint32_t((listed + scan.upto - mine) >> 32);
+        const uint32_t scan = lanes_scan<64>(mine), before = scan - mine;
+        const float most = wave_largest(extremes.most);
+        const bool bad = __any(extremes.nan);
+        if (lane == 63) {
+            sh->flags[wave] = scan;
+            sh->floats[wave] = bad ? __builtin_inff() : most;
+        }
+        __syncthreads();
+        const uint32_t in_wave = sh->flags[lane % kWaves];
+        const uint32_t here = in_wave & 0xffff, picks = in_wave >> 16;
+        const uint32_t here_upto = lanes_scan<16>(here), picks_upto = lanes_scan<16>(picks);
+        uint32_t at = listed + lane_value(here_upto - here, wave) + (before & 0xffff);
+        uint32_t pick = picked + lane_value(picks_upto - picks, wave) + (before >> 16);
+        listed += lane_value(here_upto, kWaves - 1);
+        picked += lane_value(picks_upto, kWaves - 1);
         // Of more than the list holds nothing is listed but what is picked.
-        const bool fits = uint32_t(listed + scan.total) <= kMany;
+        const bool fits = listed <= kMany;
 #pragma unroll 1
         for (uint32_t w = words.first; w < words.last; ++w) {
             const uint64_t word = sh->bins.codes[w];
@@ -621,14 +663,9 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
                 }
             }
         }
-        listed += scan.total;
     }
-    float most = 0.0f;
-    if (want_most)
-        most = join_extremes(sh, extremes.most, extremes.nan);
-    else
-        __syncthreads();  // the lists are there (as behind join_extremes' first wait)
-    return {uint32_t(listed), uint32_t(listed >> 32), most};
+    __syncthreads();  // the lists are there
+    return {listed, picked, extremes_of(wave_largest<true>(sh->floats[lane % kWaves]))};
 }
 
 // How many equal tokens of weight `each` fit above `above` short of `goal`: those
@@ -680,7 +717,7 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
     if (lane == 0)
         sh->flags[threadIdx.x >> 6] = __popcll(some_a) + __popcll(some_b);
     __syncthreads();
-    const uint32_t in_wave = sh->flags[lane % kWaves], waves = lanes_scan(in_wave);
+    const uint32_t in_wave = sh->flags[lane % kWaves], waves = lanes_scan<16>(in_wave);
     uint32_t at = __popcll(some_a & below) + __popcll(some_b & below);
     at += lane_value(waves - in_wave, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
     if (a)
@@ -1030,7 +1067,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
                 histogram(sh, chunks, double(from), true);
                 const Found found = find_bin(sh, double(k), -1.0, 0.0, 1.0);
                 // Tokens past the bins' range weigh nothing: its end bounds too.
-                floor = edge_of(sh, found.reached ? found.bin : kBins - 1, double(from));
+                floor = edges_of(sh, found.reached ? found.bin : kBins - 1, double(from)).low;
             }
         }
         list = list_tokens(sh, floor, __builtin_inff(), true);
@@ -1060,9 +1097,8 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     } else if (share >= 0.0) {
         histogram(sh, row.chunks, from, false);
         const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale);
-        const float low = edge_of(sh, found.bin, from);
-        const float high = found.bin ? edge_of(sh, found.bin - 1, from) : __builtin_inff();
-        list = list_tokens(sh, low, high, false);
+        const Edges edges = edges_of(sh, found.bin, from);
+        list = list_tokens(sh, edges.low, edges.high, false);
         // Within the bin: its own equal steps.
         cut = list.picked <= kList
                   ? list_cut(sh, &sh->pick[0], list.picked, false, found.goal, -1.0, found.over,
