@@ -727,16 +727,6 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
     __syncthreads();
     if (threadIdx.x < 64) {
         const uint32_t m = lane_value(waves, kWaves - 1);
-        const auto above_of = [&](uint32_t key) {
-            double above = 0.0;
-            for (uint32_t i = lane; i < m; i += 64) {
-                const uint32_t t = sh->sub[i];
-                if (key_of(sh->value[t]) > key)
-                    above += sh->weight[t];
-            }
-            return found.over + wave_total(above);
-        };
-        uint32_t high;
         if (m <= 64) {
             const uint32_t t = sh->sub[lane < m ? lane : 0];
             const float value = sh->value[t];
@@ -749,16 +739,35 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
                 above += other > value ? lane_value(weight, int(i)) : 0.0;
             }
             // The largest always qualifies.
-            high = wave_least(above < found.goal ? key_of(value) : UINT32_MAX);
+            const uint32_t high =
+                wave_least(lane < m && above < found.goal ? key_of(value) : UINT32_MAX);
+            uint64_t equal = __ballot(lane < m && key_of(value) == high);
+            const int one = __builtin_ctzll(equal);
+            const uint32_t count = __popcll(equal);
+            uint32_t ties = ties_within(found.goal, lane_value(above, one), lane_value(weight, one));
+            for (ties = ties < count ? ties : count; ties > 1; --ties)
+                equal &= equal - 1;
+            if (lane == uint32_t(__builtin_ctzll(equal))) {
+                sh->floats[0] = value;
+                sh->flags[0] = list[t];
+            }
         } else {
+            const auto above_of = [&](uint32_t key) {
+                double above = 0.0;
+                for (uint32_t i = lane; i < m; i += 64) {
+                    const uint32_t t = sh->sub[i];
+                    if (key_of(sh->value[t]) > key)
+                        above += sh->weight[t];
+                }
+                return found.over + wave_total(above);
+            };
             uint32_t least = UINT32_MAX, most = 0;
             for (uint32_t i = lane; i < m; i += 64) {
                 const uint32_t k = key_of(sh->value[sh->sub[i]]);
                 least = k < least ? k : least;
                 most = k > most ? k : most;
             }
-            uint32_t low = wave_least(least) - 1;
-            high = ~wave_least(~most);
+            uint32_t low = wave_least(least) - 1, high = ~wave_least(~most);
 #pragma unroll 1
             while (high - low > 1) {
                 const uint32_t middle = low + (high - low) / 2;
@@ -767,30 +776,30 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
                 else
                     low = middle;
             }
-        }
-        const float value = value_of(high);
-        uint32_t ties = ties_within(found.goal, above_of(high),
-                                    counts ? 1.0 : weight_of(sh, row, value));
-        uint32_t index = 0;
+            const float value = value_of(high);
+            uint32_t ties = ties_within(found.goal, above_of(high),
+                                        counts ? 1.0 : weight_of(sh, row, value));
+            uint32_t index = 0;
 #pragma unroll 1
-        for (uint32_t base = 0; base < m; base += 64) {
-            const uint32_t i = base + lane;
-            uint64_t equal = __ballot(i < m && sh->value[sh->sub[i < m ? i : 0]] == value);
-            const uint32_t here = __popcll(equal);
-            if (!here)
-                continue;
-            if (here >= ties) {
-                for (; ties > 1; --ties)
-                    equal &= equal - 1;
-                index = list[sh->sub[base + __builtin_ctzll(equal)]];
-                break;
+            for (uint32_t base = 0; base < m; base += 64) {
+                const uint32_t i = base + lane;
+                uint64_t equal = __ballot(i < m && sh->value[sh->sub[i < m ? i : 0]] == value);
+                const uint32_t here = __popcll(equal);
+                if (!here)
+                    continue;
+                if (here >= ties) {
+                    for (; ties > 1; --ties)
+                        equal &= equal - 1;
+                    index = list[sh->sub[base + __builtin_ctzll(equal)]];
+                    break;
+                }
+                ties -= here;
+                index = list[sh->sub[base + 63 - __builtin_clzll(equal)]];
             }
-            ties -= here;
-            index = list[sh->sub[base + 63 - __builtin_clzll(equal)]];
-        }
-        if (lane == 0) {
-            sh->floats[0] = value;
-            sh->flags[0] = index;
+            if (lane == 0) {
+                sh->floats[0] = value;
+                sh->flags[0] = index;
+            }
         }
     }
     __syncthreads();
