@@ -31,9 +31,9 @@
 // without work takes 9000 cycles), and by the fetch of code that runs once: a pass is
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
-// times as long).  One row of 65536 takes, in us: greedy 6.1, min-p 12.7, all
-// tokens 20, top-k 50 19.9 and with top-p 24.3, top-p 0.9 at temperatures 0.6 / 1 /
-// 1.5 31.6 / 36.7 / 45.6; 192 rows 11, 22, 27, 25 and 30, 42 / 51 / 58.
+// times as long).  One row of 65536 takes, in us: greedy 6.1, min-p 12, all
+// tokens 20, top-k 50 17.5 and with top-p 20.7, top-p 0.9 at temperatures 0.6 / 1 /
+// 1.5 28.6 / 33.5 / 42.3; 192 rows 11, 21, 27, 23 and 26, 39 / 48 / 55.
 #include "kernels.hpp"
 #include "paged.hpp"
 
@@ -604,8 +604,8 @@ struct Listed {
 };
 // Lists the tokens with low <= v, but -infinity, in sh->index and those with also
 // v < high in sh->pick, in their order; what passes the lists' ends is counted.
-__device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, float high,
-                                                        bool want_most)
+template <bool MOST>
+__device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, float high)
 {
     const Row row = row_of(sh);
     low = fmaxf(low, -3.4028235e38f);
@@ -619,7 +619,7 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
             row.chunks - begin < kSegmentChunks ? row.chunks : begin + kSegmentChunks;
         __syncthreads();
         code_chunks(sh, row, begin, end, low, high, [&](v4f v) {
-            if (want_most)
+            if constexpr (MOST)
                 extremes.take(v);
         });
         __syncthreads();
@@ -632,11 +632,13 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
             mine += __popcll(word & kListed) + (__popcll(word >> 4 & kListed) << 16);
         }
         const uint32_t scan = lanes_scan<64>(mine), before = scan - mine;
-        const float most = wave_largest(extremes.most);
-        const bool bad = __any(extremes.nan);
-        if (lane == 63) {
+        if (lane == 63)
             sh->flags[wave] = scan;
-            sh->floats[wave] = bad ? __builtin_inff() : most;
+        if constexpr (MOST) {
+            const float most = wave_largest(extremes.most);
+            const bool bad = __any(extremes.nan);
+            if (lane == 63)
+                sh->floats[wave] = bad ? __builtin_inff() : most;
         }
         __syncthreads();
         const uint32_t in_wave = sh->flags[lane % kWaves];
@@ -665,7 +667,8 @@ __device__ __attribute__((noinline)) Listed list_tokens(Lds *sh, float low, floa
         }
     }
     __syncthreads();  // the lists are there
-    return {listed, picked, extremes_of(wave_largest<true>(sh->floats[lane % kWaves]))};
+    return {listed, picked,
+            MOST ? extremes_of(wave_largest<true>(sh->floats[lane % kWaves])) : 0.0f};
 }
 
 // How many equal tokens of weight `each` fit above `above` short of `goal`: those
@@ -681,12 +684,12 @@ __device__ __forceinline__ uint32_t ties_within(double goal, double above, doubl
 // `over` among that, and the index of the last equal token whose predecessors stay
 // below it.  Bins are (steps below `from` - offset) * zoom; their tokens are few
 // (unless they are equal): one wave tries the values of up to 64 at once, or
-// halves the range of more.
+// halves the range of more.  `again`: the list is that of the call before.
 typedef const __attribute__((address_space(3))) uint32_t *LdsList;
 __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_t n, bool counts,
                                                   double goal, double share, double over,
                                                   Cut first, double from, double offset,
-                                                  double zoom)
+                                                  double zoom, bool again)
 {
     const Row row = row_of(sh);
     const Units units(row.width);
@@ -698,9 +701,12 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
     clear_bins(sh);
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
-        const float v = row.logits[list[i]];
+        float v;
+        if (again)
+            v = sh->value[i];
+        else
+            sh->value[i] = v = row.logits[list[i]];
         const double w = counts ? 1.0 : weight_of(sh, row, v);
-        sh->value[i] = v;
         sh->weight[i] = w;
         if (first.keeps(v, list[i]))
             add_to_bin(sh, bin(v), counts ? 1ull : units.of(w));
@@ -1079,7 +1085,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
                 floor = edges_of(sh, found.reached ? found.bin : kBins - 1, double(from)).low;
             }
         }
-        list = list_tokens(sh, floor, __builtin_inff(), true);
+        list = list_tokens<true>(sh, floor, __builtin_inff());
     } else {
         list.most = row_extremes(sh, row.chunks);
     }
@@ -1096,9 +1102,10 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         listed = list.count;
         if (listed > k)
             cut = list_cut(sh, &sh->index[0], listed, true, double(k), -1.0, 0.0, cut, from, 0.0,
-                           1.0);
+                           1.0, false);
         if (share >= 0.0)
-            cut = list_cut(sh, &sh->index[0], listed, false, 0.0, share, 0.0, cut, from, 0.0, 1.0);
+            cut = list_cut(sh, &sh->index[0], listed, false, 0.0, share, 0.0, cut, from, 0.0, 1.0,
+                           listed > k);
     } else if (k) {
         cut = digit_cut(sh, true, double(k), -1.0, cut);
         if (share >= 0.0)
@@ -1107,11 +1114,11 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         histogram(sh, row.chunks, from, false);
         const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale);
         const Edges edges = edges_of(sh, found.bin, from);
-        list = list_tokens(sh, edges.low, edges.high, false);
+        list = list_tokens<false>(sh, edges.low, edges.high);
         // Within the bin: its own equal steps.
         cut = list.picked <= kList
                   ? list_cut(sh, &sh->pick[0], list.picked, false, found.goal, -1.0, found.over,
-                             cut, from, double(found.bin), double(kBins))
+                             cut, from, double(found.bin), double(kBins), false)
                   : digit_cut(sh, false, found.goal, -1.0, cut);
         listed = list.count <= kMany ? list.count : 0;
     }
@@ -1125,7 +1132,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     }
     // A list of what a cut has left, where there is none yet.
     if (!listed && ((k && list.count > kList) || (!k && share < 0.0 && min_p > 0.0f))) {
-        const uint32_t n = list_tokens(sh, cut.value, __builtin_inff(), false).count;
+        const uint32_t n = list_tokens<false>(sh, cut.value, __builtin_inff()).count;
         listed = n <= kMany ? n : 0;
     }
     choose(sh, listed, cut, double(min_p), double(u), s.out + r, s.copy ? s.copy + r : nullptr);
