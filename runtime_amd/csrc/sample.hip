@@ -360,11 +360,13 @@ struct Extremes {
         nan = nan || __builtin_isunordered(v[0], v[1]) || __builtin_isunordered(v[2], v[3]);
     }
 };
+// The largest of some values, NaN where one is NaN or +infinity (which a wave with a
+// NaN says it has).
 __device__ __forceinline__ float extremes_of(float most)
 {
     return most < __builtin_inff() ? most : __builtin_nanf("");
 }
-// The largest of the block's, NaN where one is NaN or +infinity.
+// The largest of the block's, or NaN (extremes_of).
 __device__ __attribute__((noinline)) float join_extremes(Lds *sh, float most, bool nan)
 {
     most = wave_largest(most);
@@ -600,7 +602,7 @@ __device__ __forceinline__ uint32_t token_of(uint32_t begin, uint32_t word, uint
 
 struct Listed {
     uint32_t count, picked;
-    float most;  // the row's largest, or NaN (join_extremes), where asked for
+    float most;  // the row's largest, or NaN (extremes_of), where asked for
 };
 // Lists the tokens with low <= v, but -infinity, in sh->index and those with also
 // v < high in sh->pick, in their order; what passes the lists' ends is counted.
