@@ -446,7 +446,9 @@ mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key
  * number or passes the table's row, and a bad page id among the pages that the
  * length needs, give a NaN row.  What lies behind a sequence's length is not
  * used, whatever it holds.  Keys and values of a binary16 cache are expected to
- * be finite (one that is not makes its sequence's row NaN).  head_dim <= 1024.
+ * be finite (one that is not makes its sequence's row NaN).  head_dim <= 1024; 16,
+ * 32, 48, 64, 80, 96, 112, 128, 160, 192 and 256 run on matrix cores, others about
+ * ten times slower.
  * The workspace grows on a call outside of stream capture; under capture a call
  * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT.  A
  * context's calls and the graphs captured from it share one workspace: replay
@@ -480,7 +482,7 @@ mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
  * 8)]: bit i % 8 of byte i / 8 admits token i.  Tokens not admitted, and logits
  * of -infinity, are never chosen.  A row with an admitted NaN or +infinity,
  * without a token, or with a uniform or parameter out of range gives NaN.
- * Weights and sums are 64-bit. */
+ * Weights (to within 2^-43 of each) and their sums are 64-bit. */
 mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
                            const mfh_buf *uniforms, const mfh_buf *params, const mfh_buf *mask);
 
