@@ -482,7 +482,8 @@ mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
  * 8)]: bit i % 8 of byte i / 8 admits token i.  Tokens not admitted, and logits
  * of -infinity, are never chosen.  A row with an admitted NaN or +infinity,
  * without a token, or with a uniform or parameter out of range gives NaN.
- * Weights (to within 2^-43 of each) and their sums are 64-bit. */
+ * Weights (to within 2^-43 of each) and their sums are 64-bit; where a run reaches top_p
+ * is found to within 2^-41 of the sum, 2^-38 in rows wider than 2^20. */
 mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
                            const mfh_buf *uniforms, const mfh_buf *params, const mfh_buf *mask);
 

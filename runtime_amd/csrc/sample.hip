@@ -19,8 +19,8 @@
 // in the row's first tokens gives a value that the cut cannot lie below; one pass
 // lists all tokens from there up in LDS, where the cut is found.  top-p: the
 // bin in which the row's weight reaches the share is found from a histogram of
-// weights (whole numbers of 2^-46 or so, so that the order of additions does not
-// matter), its tokens are listed, and the cut is found among them.  The choice is
+// weights (whole numbers, of units that follow the bins, so that the order of additions
+// does not matter), its tokens are listed, and the cut is found among them.  The choice is
 // made from a list of the tokens down to there, or, where they are more than it
 // holds, of all.  Rows with more tokens about a cut than the list
 // holds (many equal values, or a temperature far above the logits' spread) are
@@ -31,9 +31,9 @@
 // without work takes 9000 cycles), and by the fetch of code that runs once: a pass is
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
-// times as long).  One row of 65536 takes, in us: greedy 6.1, min-p 12, all
-// tokens 20, top-k 50 17.5 and with top-p 20.7, top-p 0.9 at temperatures 0.6 / 1 /
-// 1.5 28.6 / 33.5 / 42.3; 192 rows 11, 21, 27, 23 and 26, 39 / 48 / 55.
+// times as long).  One row of 65536 takes, in us: greedy 6.2, min-p 12, all
+// tokens 20, top-k 50 17.8 and with top-p 21.0, top-p 0.9 at temperatures 0.6 / 1 /
+// 1.5 27.4 / 32.3 / 41.1; 192 rows 11, 21, 27, 23 and 26, 38 / 47 / 54.
 #include "kernels.hpp"
 #include "paged.hpp"
 
@@ -174,7 +174,7 @@ struct Shared {
     double table[32];  // 2^(j / 32)
     Row row;
     union {
-        uint64_t weight[kBins];
+        uint64_t weight[2 * kBins];  // the second half for Bins::two
         uint32_t count[kBins];
         uint64_t codes[kSegmentChunks * kBlock / 8];  // a byte for four tokens
     } bins;
@@ -295,9 +295,10 @@ __device__ __forceinline__ uint32_t bin_of(const Row &row, float v, double from)
 
 // exp((v - largest) / temperature) as 2^(n / 32) 2^(-f / 32), 0 <= f < 1, the latter
 // by the polynomial of fourth degree, 1 at 0, that is nearest to it (2^-43.3; the
-// argument's own rounding is less where a weight matters).  `steps`: n.  Of no
-// meaning for -infinity.
-__device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v, int *steps)
+// argument's own rounding is less where a weight matters).  Of no meaning for
+// -infinity.  graded_of: without the power of two's whole part, so in (0.97, 1.96), and
+// `steps`: n.
+__device__ __forceinline__ double graded_of(Lds *sh, const Row &row, float v, int *steps)
 {
     const double t = steps_of(row, v, row.largest), f = __builtin_amdgcn_fract(-t);
     const int n = whole_of(t);
@@ -306,12 +307,13 @@ __device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v, in
     e = __builtin_fma(e, f, -0.021660849389733828);
     e = __builtin_fma(e, f, 1.0);
     *steps = n;
-    return __builtin_ldexp(sh->table[n & 31] * e, n >> 5);
+    return sh->table[n & 31] * e;
 }
 __device__ __forceinline__ double weight_of(Lds *sh, const Row &row, float v)
 {
     int steps;
-    return weight_of(sh, row, v, &steps);
+    const double graded = graded_of(sh, row, v, &steps);
+    return __builtin_ldexp(graded, steps >> 5);
 }
 
 // Of lanes with `some` of what is summed, the one that holds a target: the first that
@@ -386,14 +388,13 @@ __device__ __attribute__((noinline)) float row_extremes(Lds *sh, uint32_t chunks
     return join_extremes(sh, extremes.most, extremes.nan);
 }
 
-// Weights as whole numbers of 2^-unit: adding 2^(52 - unit) leaves them in the
-// low bits.
+// Values below 1.96 as whole numbers of 2^-unit, of which `count` add up below 2^64:
+// adding 2^(52 - unit) leaves them in the low bits.
 struct Units {
     double scale, shift;
-    __device__ explicit Units(uint32_t width)
+    __device__ explicit Units(uint32_t count)
     {
-        // Their sum over the row stays below 2^63.
-        const int most = 62 - (32 - __builtin_clz(width)), unit = most < 46 ? most : 46;
+        const int most = 63 - (32 - __clz(int(count - 1))), unit = most < 51 ? most : 51;
         scale = __builtin_ldexp(1.0, -unit);
         shift = __builtin_ldexp(1.0, 52 - unit);
     }
@@ -408,6 +409,18 @@ struct Units {
     }
 };
 
+// What a bin's whole number stands for.  A row's weights span 2^64, so in units that are
+// fine enough for one of them another is lost: bins of steps hold graded weights, each
+// bin's in units of its own power of two, and every weight keeps 38 bits or more in rows
+// of 2^24 (46 at 65536).  Where a bin's weights have no power in common there are two
+// words, the second of what the first's units leave.
+enum class Bins { plain, steps, two };
+// The power of two that weights `steps` whole steps below the largest are graded by.
+__device__ __forceinline__ int grade_of(uint32_t steps)
+{
+    return -int(steps) >> 5;
+}
+
 // Bins stand in reverse: bin b in slot kBins - 1 - b.
 __device__ __forceinline__ void add_to_slot(Lds *sh, int slot, unsigned long long v)
 {
@@ -420,22 +433,22 @@ __device__ __forceinline__ void add_to_bin(Lds *sh, uint32_t b, unsigned long lo
     add_to_slot(sh, int(kBins - 1 - b), v);
 }
 
-__device__ __attribute__((noinline)) void clear_bins(Lds *sh)
+__device__ __attribute__((noinline)) void clear_bins(Lds *sh, Bins kind)
 {
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kBlock)
+    for (uint32_t i = threadIdx.x; i < (kind == Bins::two ? 2 : 1) * kBins; i += kBlock)
         sh->bins.weight[i] = 0;
     __syncthreads();
 }
 
 // The bins of the first chunks' tokens below `from`: how many, or (`from` being the
-// largest) their weight.
+// largest) their graded weights.
 __device__ __attribute__((noinline)) void histogram(Lds *sh, uint32_t chunks, double from,
                                                     bool counts)
 {
     const Row row = row_of(sh);
     const Units units(row.width);
-    clear_bins(sh);
+    clear_bins(sh, Bins::plain);
     if (counts)
         each_next(row, 0, chunks, [&](uint32_t, v4f v) {
 #pragma unroll
@@ -453,7 +466,7 @@ __device__ __attribute__((noinline)) void histogram(Lds *sh, uint32_t chunks, do
             int bin[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                w[e] = weight_of(sh, row, v[e], &bin[e]) + units.shift;
+                w[e] = graded_of(sh, row, v[e], &bin[e]) + units.shift;
             asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -463,41 +476,51 @@ __device__ __attribute__((noinline)) void histogram(Lds *sh, uint32_t chunks, do
     __syncthreads();
 }
 
-// The first bin with which `goal` is reached, over + the bins before it times
-// `unit` being below it (the last bin that holds any where none reaches it), and
-// what is over with those before it.  A share of the bins' total takes goal's place
-// where `share` is not negative.
+// The first bin with which `goal` is reached, over + the bins before it being below it
+// (the last bin that holds any where none reaches it), and what is over with those
+// before it.  A whole number of a bin stands for `unit`, by `kind`.  A share of the
+// bins' total takes goal's place where `share` is not negative.
 struct Found {
     double goal, over;
     uint32_t bin;
     bool reached;
 };
 __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double share,
-                                                    double over, double unit)
+                                                    double over, double unit, Bins kind)
 {
     constexpr uint32_t kEach = kBins / kBlock;
     static_assert(kEach == 2, "neighbours of a thread");
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t last = kBins - 1 - 2 * threadIdx.x;
-    const uint64_t a = sh->bins.weight[last], b = sh->bins.weight[last - 1];
-    const uint64_t scan = wave_scan(a + b);
+    const auto held = [&](uint32_t bin) {
+        const uint32_t slot = kBins - 1 - bin;
+        double v = double(sh->bins.weight[slot]) * unit;
+        if (kind == Bins::steps)
+            v = __builtin_ldexp(v, grade_of(bin));
+        if (kind == Bins::two)
+            v += double(sh->bins.weight[kBins + slot]) * (unit * unit);
+        return v;
+    };
+    const double a = held(2 * threadIdx.x), b = held(2 * threadIdx.x + 1);
+    const double scan = wave_scan(a + b);
     if (lane == 63)
-        sh->scratch[wave] = scan;
+        sh->scratch[wave] = __builtin_bit_cast(uint64_t, scan);
     __syncthreads();
     // Every wave finds the one that holds the goal; that one alone goes on.
-    const uint64_t own = sh->scratch[lane % kWaves], upto = wave_scan(own);  // a row's
+    const double own = __builtin_bit_cast(double, sh->scratch[lane % kWaves]);
+    const double upto = wave_scan(own);  // a row's
     if (share >= 0.0)
-        goal = share > 0.0 ? share * (double(lane_value(upto, kWaves - 1)) * unit) : 0x1p-60;
-    const uint32_t here = holder(lane < kWaves && own, over + double(upto) * unit >= goal);
+        goal = share > 0.0 ? share * lane_value(upto, kWaves - 1) : 0x1p-60;
+    const uint32_t here = holder(lane < kWaves && own > 0.0, over + upto >= goal);
     if (wave == here) {
-        const uint64_t end = lane_value(upto, int(here)) - lane_value(own, int(here)) + scan;
-        // Boundaries of the thread's bins, as doubles that neighbours share.
-        const double from = over + double(end - a - b) * unit, middle = over + double(end - b) * unit;
-        const double to = over + double(end) * unit;
+        // Boundaries of the thread's bins: sums that neighbours share.
+        const double base = here ? lane_value(upto, int(here) - 1) : 0.0;
+        const double before = __shfl_up(scan, 1, 64);
+        const double from = over + (lane ? base + before : base), to = over + (base + scan);
+        const double middle = from + a;
         const bool reached = to >= goal;
-        if (lane == holder(a + b, reached)) {
-            const bool first = a && (!b || middle >= goal);
+        if (lane == holder(a + b > 0.0, reached)) {
+            const bool first = a > 0.0 && (!(b > 0.0) || middle >= goal);
             sh->found = 2 * threadIdx.x + (first ? 0 : 1);
             sh->over = first ? from : middle;
             sh->reached = reached;
@@ -684,8 +707,8 @@ __device__ __forceinline__ uint32_t ties_within(double goal, double above, doubl
 // Where `goal` (or a share of all) is reached among the n tokens of `list` that
 // `first` keeps: the smallest value with less than it (counts, or weights) above,
 // `over` among that, and the index of the last equal token whose predecessors stay
-// below it.  Bins are (steps below `from` - offset) * zoom; their tokens are few
-// (unless they are equal): one wave tries the values of up to 64 at once, or
+// below it.  Bins are (steps below `from` - offset) * zoom, the zoom being 1 or that of
+// one such step's bins; their tokens are few (unless they are equal): one wave tries the values of up to 64 at once, or
 // halves the range of more.  `again`: the list is that of the call before.
 typedef const __attribute__((address_space(3))) uint32_t *LdsList;
 __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_t n, bool counts,
@@ -694,13 +717,15 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
                                                   double zoom, bool again)
 {
     const Row row = row_of(sh);
-    const Units units(row.width);
+    const Units units(n);
     const uint32_t lane = threadIdx.x & 63;
+    const Bins kind = !counts && zoom == 1.0 ? Bins::steps : Bins::plain;
+    const auto grade = [&](uint32_t b) { return grade_of(zoom == 1.0 ? b : uint32_t(offset)); };
     const auto bin = [&](float v) {
         const double x = (-steps_of(row, v, from) - offset) * zoom;
         return x < 0.0 ? 0u : x < double(kBins - 1) ? uint32_t(x) : kBins - 1;
     };
-    clear_bins(sh);
+    clear_bins(sh, kind);
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
         float v;
@@ -710,11 +735,15 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
             sh->value[i] = v = row.logits[list[i]];
         const double w = counts ? 1.0 : weight_of(sh, row, v);
         sh->weight[i] = w;
-        if (first.keeps(v, list[i]))
-            add_to_bin(sh, bin(v), counts ? 1ull : units.of(w));
+        if (first.keeps(v, list[i])) {
+            const uint32_t b = bin(v);
+            add_to_bin(sh, b, counts ? 1ull : units.of(__builtin_ldexp(w, -grade(b))));
+        }
     }
     __syncthreads();
-    const Found found = find_bin(sh, goal, share, over, counts ? 1.0 : units.scale);
+    const double unit = kind == Bins::steps ? units.scale
+                                            : __builtin_ldexp(units.scale, grade(0));
+    const Found found = find_bin(sh, goal, share, over, counts ? 1.0 : unit, kind);
     // The bin's tokens in their order: a thread looks at neighbours.
     const auto in = [&](uint32_t i) {
         return i < n && first.keeps(sh->value[i], list[i]) && bin(sh->value[i]) == found.bin;
@@ -817,13 +846,14 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
 }
 
 // The same over the whole row, 11 bits of the values' keys at a time: for rows with
-// too many tokens about the cut to list.
+// too many tokens about the cut to list.  A bin's weights are of any size.
 __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double goal, double share,
                                                    Cut first)
 {
     const Row row = row_of(sh);
     const Units units(row.width);
-    const double unit = counts ? 1.0 : units.scale;
+    const double unit = counts ? 1.0 : units.scale, finer = 1.0 / unit;
+    const Bins kind = counts ? Bins::plain : Bins::two;
     double over = 0.0;
     uint32_t prefix = 0;  // the digits found, in place
     constexpr uint32_t kDigit = kBins - 1;
@@ -832,19 +862,26 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
         // Digits of bits 31 .. 21, 20 .. 10 and 9 .. 0.
         const uint32_t shift = low > 0 ? low : 0, above = low > 0 ? low + 11 : 10;
         const uint32_t digit = (1u << (above - shift)) - 1;
-        clear_bins(sh);
+        clear_bins(sh, kind);
         each_next(row, 0, row.chunks, [&](uint32_t c, v4f v) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t key = key_of(v[e]);
                 if (v[e] > -__builtin_inff() && (above > 31 || key >> above == prefix >> above) &&
-                    first.keeps(v[e], c * kChunk + 4 * threadIdx.x + e))
-                    add_to_bin(sh, kDigit - (key >> shift & digit),
-                               counts ? 1ull : units.of(weight_of(sh, row, v[e])));
+                    first.keeps(v[e], c * kChunk + 4 * threadIdx.x + e)) {
+                    const uint32_t b = kDigit - (key >> shift & digit);
+                    if (counts) {
+                        add_to_bin(sh, b, 1);
+                        continue;
+                    }
+                    const double w = weight_of(sh, row, v[e]) * finer, high = __builtin_floor(w);
+                    add_to_bin(sh, b, uint64_t(high));
+                    add_to_slot(sh, int(2 * kBins - 1 - b), uint64_t((w - high) * finer));
+                }
             }
         });
         __syncthreads();
-        const Found found = find_bin(sh, goal, share, over, unit);
+        const Found found = find_bin(sh, goal, share, over, unit, kind);
         goal = found.goal;
         over = found.over;
         share = -1.0;
@@ -1082,7 +1119,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
             const float from = row_extremes(sh, chunks);
             if (from > -__builtin_inff()) {
                 histogram(sh, chunks, double(from), true);
-                const Found found = find_bin(sh, double(k), -1.0, 0.0, 1.0);
+                const Found found = find_bin(sh, double(k), -1.0, 0.0, 1.0, Bins::plain);
                 // Tokens past the bins' range weigh nothing: its end bounds too.
                 floor = edges_of(sh, found.reached ? found.bin : kBins - 1, double(from)).low;
             }
@@ -1114,7 +1151,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
             cut = digit_cut(sh, false, 0.0, share, cut);
     } else if (share >= 0.0) {
         histogram(sh, row.chunks, from, false);
-        const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale);
+        const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale, Bins::steps);
         const Edges edges = edges_of(sh, found.bin, from);
         list = list_tokens<false>(sh, edges.low, edges.high);
         // Within the bin: its own equal steps.

@@ -7,6 +7,9 @@ case here does (a border is hit with probability about 2^-25 at 300001 tokens an
 """
 from __future__ import annotations
 
+import math
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -273,3 +276,34 @@ def test_a_model_generates_sampled_tokens(backend):
             call()
         assert error.value.variant == variant, error.value
     model.close()
+
+
+@pytest.mark.parametrize("k", [0, 10 ** 7], ids=["", "k"])
+@pytest.mark.parametrize("exponent,kept", [(-0.6, 0.6), (0.5, 0.75)])
+@pytest.mark.parametrize("width", [1 << 20, 1 << 22, 1 << 24])
+def test_flat_tails(backend, width, exponent, kept, k):
+    """One token and a wide flat tail of tokens of 2^-41 to 2^-37 of its weight, of which
+    top-p keeps a part: none is lost for being small.
+
+    The share is found to within e = 2^-41 (2^-38 past 2^20) of the sum, so the tail's
+    kept part, a number of equal weights w, to within e / w tokens; the last uniform
+    value below one chooses near its end, 2^-24 of the sum before.  A token each for
+    the rounding of that number, of the choice and of its sums.
+    """
+    say("flat", width, exponent, k)
+    logits = np.full((1, width), (exponent - 61 + math.log2(width)) * math.log(2), np.float32)
+    logits[0, 5] = 0.0
+    w = Fraction(math.exp(float(logits[0, 0])))  # within 2^-52 of itself
+    tail = (min(width, k) if k else width) - 1
+    total = 1 + tail * w
+    p = np.float32(float((1 + Fraction(kept) * tail * w) / total))
+    u = np.float32(1 - 2.0 ** -24)
+    assert p < 1
+    goal = Fraction(float(p)) * total
+    ties = min(tail, math.ceil((goal - 1) / w))
+    want = math.floor((Fraction(float(u)) * (1 + ties * w) - 1) / w) + 1
+    assert 1000 < want < ties < tail
+    got = run(backend, logits, [u], [(1.0, k, p, 0.0)])[0]
+    error = 2.0 ** (-41 if width <= 1 << 20 else -38)
+    say("want", want, "got", got)
+    assert abs(got - want) <= error / float(w) + 3
