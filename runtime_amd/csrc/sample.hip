@@ -15,8 +15,8 @@
 // Nothing is sorted: every cut is a value and an index (kept: values above, and
 // equal ones up to the index).
 //
-// top-k: the count's bin among equal steps of the logit (ln 2 / 32 temperatures)
-// in the row's first tokens gives a value that the cut cannot lie below; one pass
+// top-k: the count's bin among equal steps of the logit (ln 2 / 32 temperatures, or 64
+// times that) in the row's first tokens gives a value that the cut cannot lie below; one pass
 // lists all tokens from there up in LDS, where the cut is found.  top-p: the
 // bin in which the row's weight reaches the share is found from a histogram of
 // weights (whole numbers, of units that follow the bins, so that the order of additions
@@ -32,7 +32,7 @@
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
 // times as long).  One row of 65536 takes, in us: greedy 6.2, min-p 12, all
-// tokens 20, top-k 50 17.8 and with top-p 21.0, top-p 0.9 at temperatures 0.6 / 1 /
+// tokens 20, top-k 50 18.0 and with top-p 21.2, top-p 0.9 at temperatures 0.6 / 1 /
 // 1.5 27.4 / 32.3 / 41.1; 192 rows 11, 21, 27, 23 and 26, 38 / 47 / 54.
 #include "kernels.hpp"
 #include "paged.hpp"
@@ -1118,10 +1118,28 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
             chunks = chunks < row.chunks ? chunks : row.chunks;
             const float from = row_extremes(sh, chunks);
             if (from > -__builtin_inff()) {
-                histogram(sh, chunks, double(from), true);
-                const Found found = find_bin(sh, double(k), -1.0, 0.0, 1.0, Bins::plain);
-                // Tokens past the bins' range weigh nothing: its end bounds too.
-                floor = edges_of(sh, found.reached ? found.bin : kBins - 1, double(from)).low;
+                // Where fewer than k lie in the bins (a low temperature, few tokens
+                // admitted) bins 64 times as wide are tried, then all tokens are
+                // listed: k are kept however little they weigh.
+                bool reached = false;
+#pragma unroll 1
+                for (int wider = 0; wider < 2 && !reached; ++wider) {
+                    if (wider) {
+                        if (threadIdx.x == 0)
+                            sh->row.per_step = row.per_step / 64.0;
+                        __syncthreads();
+                    }
+                    histogram(sh, chunks, double(from), true);
+                    const Found found = find_bin(sh, double(k), -1.0, 0.0, 1.0, Bins::plain);
+                    reached = found.reached;
+                    if (reached)
+                        floor = edges_of(sh, found.bin, double(from)).low;
+                    if (wider) {
+                        if (threadIdx.x == 0)
+                            sh->row.per_step = row.per_step;
+                        __syncthreads();
+                    }
+                }
             }
         }
         list = list_tokens<true>(sh, floor, __builtin_inff());

@@ -307,3 +307,33 @@ def test_flat_tails(backend, width, exponent, kept, k):
     error = 2.0 ** (-41 if width <= 1 << 20 else -38)
     say("want", want, "got", got)
     assert abs(got - want) <= error / float(w) + 3
+
+
+@pytest.mark.parametrize("k", [2, 50, 3000])
+@pytest.mark.parametrize("temperature", [0.1, 0.05, 0.01, 1e-4, 1e-30])
+@pytest.mark.parametrize("width", [2048, 2049, 4097, 65536, 130003])
+def test_top_k_keeps_what_weighs_little(backend, width, temperature, k):
+    """A uniform value of zero takes the first token of the k, however small its weight:
+    what is too small for 64 bits is zero.  (token() would lose tokens that add nothing
+    to a sum at top_p = 1, where all are kept.)"""
+    say("cold", width, temperature, k)
+    rng = np.random.default_rng(width + k)
+    logits = 2.5 * rng.standard_normal((6, width))
+    logits[1:3] = np.round(logits[1:3] * 4) / 4
+    logits[2:4, 100] = 13.0
+    logits[3, 37] = 11.9  # e^-11 to e^-110 of the largest at the first three temperatures
+    logits[4] = -logits[4] ** 2
+    logits = logits.astype(np.float32)
+    uniforms = np.float32([0, 0, 0, 0, 0, 1e-30])
+    t = float(np.float32(temperature))
+    for share in (None, 0.5, 30 / width):
+        admitted = np.ones((6, width), bool) if share is None else rng.random((6, width)) < share
+        want = []
+        for row, u, allowed in zip(logits, uniforms, admitted):
+            x = np.where(allowed, row.astype(np.float64), -np.inf)
+            kept = np.sort(np.argsort(-x, kind="stable")[:k])
+            reached = np.cumsum(np.exp((x[kept] - x.max()) / t))
+            want.append(kept[np.searchsorted(reached, float(u) * reached[-1], side="right")])
+        got = run(backend, logits, uniforms, [(temperature, k, 1.0, 0.0)],
+                  None if share is None else np.packbits(admitted, axis=1, bitorder="little"))
+        assert np.array_equal(got, np.float32(want)), (share, got, want)
