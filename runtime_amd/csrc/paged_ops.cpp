@@ -30,6 +30,26 @@ constexpr uint64_t kIndexLimit = uint64_t(1) << 24;
 
 // The geometry of a page buffer: [pages, kv_heads, page_size, head_dim] F32, or
 // U8 with twice the width.
+mfh_status page_shape_of(mfh_ctx *ctx, const uint64_t (&dims)[4], bool half, PageShape *out)
+{
+    out->half = half;
+    if (half && dims[3] % 2 != 0)
+        return fail(ctx, MFH_INVALID_SHAPE, "binary16 page rows must hold an even byte count");
+    const uint64_t d = half ? dims[3] / 2 : dims[3], size = dims[2];
+    if (dims[0] == 0 || dims[1] == 0 || d == 0)
+        return fail(ctx, MFH_INVALID_SHAPE, "page buffers must have a page, a head and a column");
+    if (size < 8 || size > 4096 || (size & (size - 1)))
+        return fail(ctx, MFH_INVALID_SHAPE, "page size must be a power of two in [8, 4096]");
+    if (dims[0] > kIndexLimit)
+        return fail(ctx, MFH_UNSUPPORTED, "page count exceeds the exact f32 index range");
+    if (dims[1] > UINT16_MAX || d > UINT16_MAX)
+        return fail(ctx, MFH_OVERFLOW, "page extent exceeds the kernel index range");
+    out->pages = uint32_t(dims[0]);
+    out->kv_heads = uint32_t(dims[1]);
+    out->page_shift = uint32_t(__builtin_ctzll(size));
+    out->head_dim = uint32_t(d);
+    return MFH_OK;
+}
 mfh_status page_shape(mfh_ctx *ctx, const mfh_buf *buf, PageShape *out)
 {
     mfh_status s = check_buffer(ctx, buf);
@@ -38,23 +58,7 @@ mfh_status page_shape(mfh_ctx *ctx, const mfh_buf *buf, PageShape *out)
     if (buf->rank != 4)
         return fail(ctx, MFH_INVALID_SHAPE,
                     "page buffers must be [pages, kv_heads, page_size, head_dim]");
-    out->half = buf->dtype == MFH_DTYPE_U8;
-    if (out->half && buf->dims[3] % 2 != 0)
-        return fail(ctx, MFH_INVALID_SHAPE, "binary16 page rows must hold an even byte count");
-    const uint64_t d = out->half ? buf->dims[3] / 2 : buf->dims[3], size = buf->dims[2];
-    if (buf->dims[0] == 0 || buf->dims[1] == 0 || d == 0)
-        return fail(ctx, MFH_INVALID_SHAPE, "page buffers must have a page, a head and a column");
-    if (size < 8 || size > 4096 || (size & (size - 1)))
-        return fail(ctx, MFH_INVALID_SHAPE, "page size must be a power of two in [8, 4096]");
-    if (buf->dims[0] > kIndexLimit)
-        return fail(ctx, MFH_UNSUPPORTED, "page count exceeds the exact f32 index range");
-    if (buf->dims[1] > UINT16_MAX || d > UINT16_MAX)
-        return fail(ctx, MFH_OVERFLOW, "page extent exceeds the kernel index range");
-    out->pages = uint32_t(buf->dims[0]);
-    out->kv_heads = uint32_t(buf->dims[1]);
-    out->page_shift = uint32_t(__builtin_ctzll(size));
-    out->head_dim = uint32_t(d);
-    return MFH_OK;
+    return page_shape_of(ctx, buf->dims, buf->dtype == MFH_DTYPE_U8, out);
 }
 
 // Key and value pages of one cache.
@@ -173,18 +177,11 @@ mfh_status mfh_alloc_pages(mfh_ctx *ctx, uint64_t pages, uint32_t key_value_head
     *out = nullptr;
     const uint64_t dims[4] = {pages, key_value_heads, page_size,
                               half ? 2 * uint64_t(head_dim) : head_dim};
-    mfh_buf *buf = nullptr;
-    mfh_status s = half ? alloc_zeroed_u8(ctx, dims, 4, MFH_CLASS_CACHE, &buf)
-                        : mfh_alloc_f32(ctx, dims, 4, MFH_CLASS_CACHE, 1, &buf);
     PageShape shape;
-    if (!s && (s = page_shape(ctx, buf, &shape))) {
-        mfh_release(buf);
-        buf = nullptr;
-    }
-    if (s)
+    if (mfh_status s = page_shape_of(ctx, dims, half != 0, &shape))
         return s;
-    *out = buf;
-    return MFH_OK;
+    return half ? alloc_zeroed_u8(ctx, dims, 4, MFH_CLASS_CACHE, out)
+                : mfh_alloc_f32(ctx, dims, 4, MFH_CLASS_CACHE, 1, out);
 }
 
 mfh_status mfh_rotation_table(mfh_ctx *ctx, mfh_buf *output, float theta,

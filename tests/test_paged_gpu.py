@@ -950,3 +950,18 @@ def test_copy_refusals(backend):
     refused("InvalidShape", copy, [a], [backend.allocate_f32((5, 256))], [1], [2])
     copy([], [], [1, 1], [2, 2])
     copy([a], [b], [6, 6], [1, 2])
+
+
+def test_page_shapes_are_checked_before_room():
+    """A bad shape is one at any size, and costs no memory."""
+    backend = HipBackend(0, limits=Limits(max_total_bytes=1 << 20))
+    big = 1 << 24
+    for half in (False, True):
+        refused("InvalidShape", backend.alloc_pages, big, 64, 12, 256, half)
+        refused("InvalidShape", backend.alloc_pages, big, 64, 8192, 256, half)
+        refused("InvalidShape", backend.alloc_pages, big, 0, 8192, 256, half)
+        refused("Unsupported", backend.alloc_pages, big + 1, 1, 16, 8, half)
+        refused("Overflow", backend.alloc_pages, 1, 1 << 16, 8, 8, half)
+        refused("Overflow", backend.alloc_pages, 1, 1, 8, 1 << 16, half)
+        refused("ResourceLimit", backend.alloc_pages, big, 64, 16, 256, half)
+    backend.close()
