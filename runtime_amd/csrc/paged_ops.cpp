@@ -158,6 +158,52 @@ void copy_pairs(hipStream_t stream, uint64_t elements, mfh_buf *const *destinati
     }
 }
 
+// Page ids, by open addressing in a table of twice their number or more: the work
+// follows the ids, whatever the cache's page count.  The few ids of a fork need no
+// allocation.
+class PageSet {
+  public:
+    explicit PageSet(size_t count)
+    {
+        while (size_t(1) << bits_ < 2 * count)
+            ++bits_;
+        if (size_t(1) << bits_ > kFew) {
+            heap_.reset(new (std::nothrow) uint32_t[size_t(1) << bits_]);
+            slots_ = heap_.get();
+        }
+        for (size_t i = 0; slots_ && i < size_t(1) << bits_; ++i)
+            slots_[i] = kNone;
+    }
+    bool allocated() const { return slots_ != nullptr; }
+    // The id's slot, or the free one that it would have.
+    uint32_t &slot(uint32_t id)
+    {
+        // The upper bits of a product with 2^32 over the golden ratio.
+        size_t at = uint32_t(id * 2654435769u) >> (32 - bits_);
+        while (slots_[at] != kNone && slots_[at] != id)
+            at = (at + 1) & ((size_t(1) << bits_) - 1);
+        return slots_[at];
+    }
+    bool has(uint32_t id) { return slot(id) == id; }
+    // False where it was there.
+    bool add(uint32_t id)
+    {
+        uint32_t &to = slot(id);
+        if (to == id)
+            return false;
+        to = id;
+        return true;
+    }
+
+  private:
+    static constexpr uint32_t kNone = UINT32_MAX;  // no page: ids are below 2^24
+    static constexpr size_t kFew = 32;
+    unsigned bits_ = 1;
+    uint32_t few_[kFew];
+    std::unique_ptr<uint32_t[]> heap_;
+    uint32_t *slots_ = few_;
+};
+
 bool positive(float v) { return std::isfinite(v) && v > 0.0f; }
 
 }  // namespace
@@ -432,16 +478,17 @@ mfh_status mfh_copy_pages(mfh_ctx *ctx, mfh_buf *const *destinations,
     // copies run in no order.
     if (buffers && count > 1) {
         const char *message = "a page is copied to twice, or copied from and to";
-        std::unique_ptr<uint8_t[]> seen(new (std::nothrow) uint8_t[least_to]());
-        if (!seen)
+        // More than every page once is a page twice; the table stays small.
+        if (count > least_to)
+            return fail(ctx, MFH_INVALID_ARGUMENT, message);
+        PageSet targets(count);
+        if (!targets.allocated())
             return fail(ctx, MFH_RESOURCE_LIMIT, "host allocation failed");
-        for (size_t i = 0; i < count; ++i) {
-            if (seen[to_pages[i]])
+        for (size_t i = 0; i < count; ++i)
+            if (!targets.add(to_pages[i]))
                 return fail(ctx, MFH_INVALID_ARGUMENT, message);
-            seen[to_pages[i]] = 1;
-        }
         for (size_t i = 0; in_place && i < count; ++i)
-            if (from_pages[i] < least_to && seen[from_pages[i]])
+            if (targets.has(from_pages[i]))
                 return fail(ctx, MFH_INVALID_ARGUMENT, message);
     } else if (buffers && count == 1 && in_place && from_pages[0] == to_pages[0]) {
         return fail(ctx, MFH_INVALID_ARGUMENT, "a page is copied to twice, or copied from and to");

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import time
 
 import numpy as np
 import pytest
@@ -965,3 +966,48 @@ def test_page_shapes_are_checked_before_room():
         refused("Overflow", backend.alloc_pages, 1, 1, 8, 1 << 16, half)
         refused("ResourceLimit", backend.alloc_pages, big, 64, 16, 256, half)
     backend.close()
+
+
+@pytest.mark.parametrize("count", [2, 16, 17, 300, 4999])
+def test_copied_pages_are_compared_wherever_they_stand(backend, count):
+    """A target named twice, or copied from as well, anywhere in lists of any length."""
+    rng = np.random.default_rng(count)
+    pages = 10000
+    a, b = (backend.alloc_pages(pages, 1, 8, 2) for _ in range(2))
+    order = rng.permutation(pages)
+    source, target = order[:count], order[count:2 * count]
+    whole = upload(backend, rng.standard_normal((pages, 16)).astype(np.float32))
+    ramp = backend.read(whole)
+    cache = backend.upload_f32((pages, 1, 8, 2), ramp.reshape(pages, 1, 8, 2))
+    backend.copy_pages([cache], [cache], source, target)
+    want = ramp.copy()
+    want[target] = ramp[source]
+    assert np.array_equal(backend.read(cache).reshape(pages, 16), want)
+    for _ in range(4):
+        i, j = rng.choice(count, 2, replace=False)
+        twice = target.copy()
+        twice[i] = twice[j]
+        refused("InvalidArgument", backend.copy_pages, [a], [b], source, twice)
+        both = target.copy()
+        both[i] = source[j]
+        refused("InvalidArgument", backend.copy_pages, [a], [a], source, both)
+        backend.copy_pages([a], [b], source, both)
+    refused("InvalidArgument", backend.copy_pages, [a], [b], np.zeros(pages + 1, np.uint32),
+            np.arange(pages + 1) % pages)
+
+
+def test_a_few_pages_cost_the_same_in_any_cache(backend):
+    """The host's part of a two-page copy, in a cache of 8 pages and in one of 2^24, which
+    took 13 times as long when the call went over all of its pages."""
+    times = []
+    for pages in (8, 1 << 24):
+        cache = backend.alloc_pages(pages, 1, 8, 2, half=True)
+        each = []
+        for _ in range(31):
+            backend.synchronize()
+            begin = time.perf_counter()
+            backend.copy_pages([cache], [cache], [0, 1], [pages - 1, pages - 2])
+            each.append(time.perf_counter() - begin)
+        times.append(sorted(each)[15])
+    say("us a call", [1e6 * t for t in times])
+    assert times[1] < 5 * times[0]
