@@ -863,11 +863,8 @@ mfh_status mfl_generate_sampled(mfl_model *m, uint32_t steps, const mfh_buf *uni
     mark_written(ids_out);
     call.copy = static_cast<float *>(ids_out->dev);
     for (uint32_t i = 0; i < steps; ++i) {
-        {
-            DeviceGuard guard(c->device);
-            launch_sample_rows(c->stream, call);
-        }
-        if ((s = append(m, nullptr, 0, m->sampled.buf, true)))
+        if ((s = run_sample_rows(c, call)) ||
+            (s = append(m, nullptr, 0, m->sampled.buf, true)))
             return s;
         ++call.uniforms;
         ++call.copy;

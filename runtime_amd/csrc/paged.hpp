@@ -125,5 +125,7 @@ void launch_sample_rows(hipStream_t stream, const Sampling &s);
 mfh_status admit_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
                              const mfh_buf *uniforms, uint64_t uniform_count,
                              const mfh_buf *params, const mfh_buf *mask, Sampling *call);
+// Enqueues an admitted call.
+mfh_status run_sample_rows(mfh_ctx *ctx, const Sampling &call);
 
 }  // namespace mfh

@@ -516,10 +516,8 @@ mfh_status mfh_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logits,
         s = admit_sample_rows(ctx, output, logits, uniforms, logits->dims[0], params, mask, &call);
     if (s)
         return s;
-    DeviceGuard guard(ctx->device);
     mark_written(output);
-    launch_sample_rows(ctx->stream, call);
-    return launched(ctx);
+    return run_sample_rows(ctx, call);
 }
 
 }  // extern "C"
@@ -570,6 +568,15 @@ mfh_status admit_sample_rows(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *logit
     call->width = uint32_t(width);
     call->one_params = params->dims[0] == 1;
     call->one_mask = mask && mask->dims[0] == 1;
+    return MFH_OK;
+}
+
+mfh_status run_sample_rows(mfh_ctx *ctx, const Sampling &call)
+{
+    DeviceGuard guard(ctx->device);
+    launch_sample_rows(ctx->stream, call);
+    if (hipGetLastError() != hipSuccess)
+        return fail(ctx, MFH_BACKEND_FAILURE, "sampling launch failed");
     return MFH_OK;
 }
 

@@ -13,6 +13,7 @@ from fractions import Fraction
 import numpy as np
 import pytest
 
+from runtime_amd import hiptime
 from runtime_amd.backend import ExecutorError, HipBackend
 
 pytestmark = pytest.mark.gpu
@@ -337,3 +338,31 @@ def test_top_k_keeps_what_weighs_little(backend, width, temperature, k):
         got = run(backend, logits, uniforms, [(temperature, k, 1.0, 0.0)],
                   None if share is None else np.packbits(admitted, axis=1, bitorder="little"))
         assert np.array_equal(got, np.float32(want)), (share, got, want)
+
+
+def test_a_failed_draw_ends_the_loop_before_the_step(backend):
+    """An error of a draw's launch (here one that an earlier HIP call of the thread left)
+    is the draw's: no step is queued behind it, and the model is where it was."""
+    from runtime_amd.lfm2 import ATTENTION, CONV, Lfm2Config, Lfm2Model, synthetic_weights
+
+    cfg = Lfm2Config(hidden=256, intermediate=512, attention_heads=4, key_value_heads=2,
+                     vocab=1000, layers=[CONV, ATTENTION], max_tokens=64,
+                     formats={"embedding": "int8", "conv": "nf4", "attention": "nf4",
+                              "ffn": "ternary"})
+    model = Lfm2Model(backend, cfg)
+    synthetic_weights(model)
+    model.append([1, 2, 3, 4, 5])
+    prefix = model.snapshot()
+    uniforms = backend.upload_f32((9,), np.random.default_rng(13).random(9).astype(np.float32))
+    params = backend.upload_f32((1, 4), (0.9, 40, 0.95, 0.01))
+    want = backend.read(model.generate_sampled(9, uniforms, params))
+    model.restore(prefix)
+    logits = backend.read(model.logits)
+    assert hiptime.hip().hipSetDevice(9999) != 0
+    with pytest.raises(ExecutorError) as error:
+        model.generate_sampled(9, uniforms, params)
+    assert error.value.variant == "BackendFailure" and "sampling" in str(error.value)
+    assert model.length == 5
+    assert np.array_equal(backend.read(model.logits), logits)
+    assert np.array_equal(backend.read(model.generate_sampled(9, uniforms, params)), want)
+    model.close()
