@@ -452,7 +452,11 @@ mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key
  * The workspace grows on a call outside of stream capture; under capture a call
  * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT.  A
  * context's calls and the graphs captured from it share one workspace: replay
- * such graphs on the context's stream, or in an order with it. */
+ * such graphs on the context's stream, or in an order with it.  A workspace that a
+ * captured call uses is kept until the context ends, also once a larger call has
+ * replaced it and the graph is gone; what replaces it outside of capture is at least
+ * twice as large where the limits have room, so what is kept so does not add up to more
+ * than the one in use. */
 mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                          const mfh_buf *key_pages, const mfh_buf *value_pages,
                          const mfh_buf *tables, const mfh_buf *lengths, uint32_t query_heads,

@@ -297,16 +297,25 @@ void *paged_scratch(mfh_ctx *ctx, size_t bytes)
     const bool capturing = capture != hipStreamCaptureStatusNone;
     if (bytes > ctx->paged_scratch_capacity) {
         const size_t want = scratch_size(bytes);
+        // What a graph holds stays held: the next block is at least twice as large where
+        // there is room, so that a graph for each of many sizes leaves blocks that
+        // together are no larger than the last.
+        size_t more = want;
+        if (ctx->paged_scratch_captured && 2 * ctx->paged_scratch_capacity > want)
+            more = 2 * ctx->paged_scratch_capacity;
         void *p = nullptr;
         size_t got = 0;
         if (capturing) {
-            p = ctx->pool->take(want, &got);
+            p = ctx->pool->take(more, &got);
+            if (!p)
+                p = ctx->pool->take(want, &got);
             if (!p) {
                 (void)fail(ctx, MFH_RESOURCE_LIMIT,
                            "under stream capture the workspace must be there from an earlier call");
                 return nullptr;
             }
-        } else if (acquire(ctx, want, &p, &got)) {
+        } else if (acquire(ctx, fits(ctx, more) ? more : want, &p, &got) &&
+                   (more == want || acquire(ctx, want, &p, &got))) {
             return nullptr;
         }
         if (!ctx->paged_scratch_captured)

@@ -1011,3 +1011,39 @@ def test_a_few_pages_cost_the_same_in_any_cache(backend):
         times.append(sorted(each)[15])
     say("us a call", [1e6 * t for t in times])
     assert times[1] < 5 * times[0]
+
+
+def test_a_graph_for_each_batch_size():
+    """Every size's workspace is larger than the last one's; the ones that the graphs hold
+    stay theirs, and together are no larger than the last."""
+    backend = HipBackend(0)
+    rng = np.random.default_rng(31)
+    keys, values = (random_pages(rng, 7, 1, 16, 256, False) for _ in range(2))
+    k, v = upload(backend, keys), upload(backend, values)
+    spec, graphs = GqaSpec(16, 1, 256), []
+    held = 0
+    for count in range(24, 172, 8):
+        query = rng.standard_normal((count, 16 * 256)).astype(np.float32)
+        table = rng.integers(0, 7, (count, 1)).astype(np.float32)
+        lengths = rng.integers(1, 17, count).astype(np.float32)
+        args = (backend.allocate_f32((count, 16 * 256)), upload(backend, query), k, v,
+                upload(backend, table), upload(backend, lengths), spec)
+        before = backend.resource_report().scratch_bytes
+        backend.paged_gqa(*args)  # outside of capture, so that there is room
+        held += backend.resource_report().scratch_bytes - before
+        graphs.append((args, backend.read(args[0]), *captured(backend,
+                                                              lambda: backend.paged_gqa(*args))))
+    # 256 blocks of two records of 16 rows of 256 and two statistics: the last one's.
+    largest = 2 * 256 * 16 * 258 * 4 + 172 * 8
+    say("held", held, "largest", largest)
+    # Twice, for the last one's room, twice, for the ones replaced, an eighth for the pool's
+    # steps.
+    assert held <= 4 * largest * 9 / 8
+    for _ in range(3):
+        for args, want, replay, _end in graphs:
+            backend.paged_gqa(*graphs[-1][0])
+            replay()
+            assert np.array_equal(backend.read(args[0]), want)
+    for *_rest, end in graphs:
+        end()
+    backend.close()
