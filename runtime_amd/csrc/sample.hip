@@ -175,7 +175,6 @@ struct Shared {
     Row row;
     union {
         uint64_t weight[2 * kBins];  // the second half for Bins::two
-        uint32_t count[kBins];
         uint64_t codes[kSegmentChunks * kBlock / 8];  // a byte for four tokens
     } bins;
     uint32_t index[kMany];
