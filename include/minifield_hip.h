@@ -447,8 +447,8 @@ mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key
  * length needs, give a NaN row.  What lies behind a sequence's length is not
  * used, whatever it holds.  Keys and values of a binary16 cache are expected to
  * be finite (one that is not makes its sequence's row NaN).  head_dim <= 1024; 16,
- * 32, 48, 64, 80, 96, 112, 128, 160, 192 and 256 run on matrix cores, others about
- * ten times slower.
+ * 32, 48, 64, 80, 96, 112, 128, 160, 192 and 256 run on matrix cores, others ten to
+ * sixteen times slower.
  * The workspace grows on a call outside of stream capture; under capture a call
  * that needs a larger one than there is fails with MFH_RESOURCE_LIMIT.  A
  * context's calls and the graphs captured from it share one workspace: replay

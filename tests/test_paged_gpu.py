@@ -1047,3 +1047,29 @@ def test_a_graph_for_each_batch_size():
     for *_rest, end in graphs:
         end()
     backend.close()
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("dim", [64, 7, 300])
+def test_prepared_keys_enter_as_they_are(backend, dim, interleaved, half):
+    """Without weights and with no rotated column nothing is changed but by the pages'
+    format: the keys of a prompt that ran over contiguous caches."""
+    rng = np.random.default_rng(dim)
+    tokens, heads, kv_heads, size = 21, 6, 3, 8
+    q, k, v = (rng.standard_normal((tokens, h * dim)).astype(np.float32)
+               for h in (heads, kv_heads, kv_heads))
+    keys, values = (backend.alloc_pages(4, kv_heads, size, dim, half) for _ in range(2))
+    table = np.array([[2, 0, 3]], np.float32)
+    out = backend.allocate_f32((tokens, heads * dim))
+    backend.paged_qk_norm_rope(out, keys, values, *(upload(backend, a) for a in (q, k, v)), None,
+                               None, backend.allocate_f32((tokens, 0)), upload(backend, table),
+                               upload(backend, np.zeros(tokens, np.float32)),
+                               upload(backend, np.arange(tokens, dtype=np.float32)),
+                               PagedRopeSpec(heads, kv_heads, dim, interleaved), EPSILON)
+    assert np.array_equal(backend.read(out), q)
+    for pages, rows in ((keys, k), (values, v)):
+        got = read_pages(backend, pages)[[2, 0, 3]].transpose(0, 2, 1, 3).reshape(-1, kv_heads, dim)
+        want = rows.reshape(tokens, kv_heads, dim).astype(np.float16 if half else np.float32)
+        assert np.array_equal(got[:tokens], want)
+        assert not got[tokens:].any()
