@@ -575,6 +575,9 @@ __device__ __attribute__((noinline)) Edges edges_of(Lds *sh, uint32_t b, double 
     return {sh->floats[0], sh->floats[1]};
 }
 
+// Bins of counts where a temperature's are too narrow: 64 times as wide.
+constexpr double kWider = 1.0 / 64.0;
+
 // The kept tokens: values above `value`, and equal ones up to `index`.
 struct Cut {
     float value;
@@ -706,8 +709,8 @@ __device__ __forceinline__ uint32_t ties_within(double goal, double above, doubl
 // Where `goal` (or a share of all) is reached among the n tokens of `list` that
 // `first` keeps: the smallest value with less than it (counts, or weights) above,
 // `over` among that, and the index of the last equal token whose predecessors stay
-// below it.  Bins are (steps below `from` - offset) * zoom, the zoom being 1 or that of
-// one such step's bins; their tokens are few (unless they are equal): one wave tries the values of up to 64 at once, or
+// below it.  Bins are (steps below `from` - offset) * zoom, the zoom being 1, that of one
+// such step's bins, or for counts kWider; their tokens are few (unless they are equal): one wave tries the values of up to 64 at once, or
 // halves the range of more.  `again`: the list is that of the call before.
 typedef const __attribute__((address_space(3))) uint32_t *LdsList;
 __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_t n, bool counts,
@@ -844,16 +847,20 @@ __device__ __attribute__((noinline)) Cut list_cut(Lds *sh, LdsList list, uint32_
     return cut;
 }
 
-// The same over the whole row, 11 bits of the values' keys at a time: for rows with
-// too many tokens about the cut to list.  A bin's weights are of any size.
+// The same over the row's tokens in `range`, 11 bits of the values' keys at a time: for
+// rows with too many tokens about the cut to list.  `grade` is that of the range's
+// weights, or kAnyGrade where they are of any size.
+constexpr int kAnyGrade = 1;
 __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double goal, double share,
-                                                   Cut first)
+                                                   double over, Cut first, Edges range, int grade)
 {
     const Row row = row_of(sh);
     const Units units(row.width);
-    const double unit = counts ? 1.0 : units.scale, finer = 1.0 / unit;
-    const Bins kind = counts ? Bins::plain : Bins::two;
-    double over = 0.0;
+    const Bins kind = !counts && grade == kAnyGrade ? Bins::two : Bins::plain;
+    const double unit = counts               ? 1.0
+                        : kind == Bins::two ? units.scale
+                                            : __builtin_ldexp(units.scale, grade);
+    const double finer = 1.0 / unit;
     uint32_t prefix = 0;  // the digits found, in place
     constexpr uint32_t kDigit = kBins - 1;
 #pragma unroll 1
@@ -866,16 +873,22 @@ __device__ __attribute__((noinline)) Cut digit_cut(Lds *sh, bool counts, double 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t key = key_of(v[e]);
-                if (v[e] > -__builtin_inff() && (above > 31 || key >> above == prefix >> above) &&
+                if (v[e] > -__builtin_inff() && v[e] >= range.low && v[e] < range.high &&
+                    (above > 31 || key >> above == prefix >> above) &&
                     first.keeps(v[e], c * kChunk + 4 * threadIdx.x + e)) {
                     const uint32_t b = kDigit - (key >> shift & digit);
                     if (counts) {
                         add_to_bin(sh, b, 1);
                         continue;
                     }
-                    const double w = weight_of(sh, row, v[e]) * finer, high = __builtin_floor(w);
+                    const double w = weight_of(sh, row, v[e]);
+                    if (kind == Bins::plain) {
+                        add_to_bin(sh, b, units.of(__builtin_ldexp(w, -grade)));
+                        continue;
+                    }
+                    const double high = __builtin_floor(w * finer);
                     add_to_bin(sh, b, uint64_t(high));
-                    add_to_slot(sh, int(2 * kBins - 1 - b), uint64_t((w - high) * finer));
+                    add_to_slot(sh, int(2 * kBins - 1 - b), uint64_t((w * finer - high) * finer));
                 }
             }
         });
@@ -1108,10 +1121,10 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     Cut cut = {-3.4028235e38f, UINT32_MAX};
     uint32_t listed = 0;  // tokens of the list, where it holds every kept one
     Listed list = {0, 0, 0.0f};
+    float floor = -__builtin_inff();
     if (k) {
         // A value that the k-th largest of the row does not lie below: of the
         // first tokens, enough for about 1024 listed ones.
-        float floor = -__builtin_inff();
         if (s.width > kList) {
             uint32_t chunks = uint32_t((uint64_t(row.chunks) * k + 1023) / 1024);
             chunks = chunks < row.chunks ? chunks : row.chunks;
@@ -1125,7 +1138,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
                 for (int wider = 0; wider < 2 && !reached; ++wider) {
                     if (wider) {
                         if (threadIdx.x == 0)
-                            sh->row.per_step = row.per_step / 64.0;
+                            sh->row.per_step = row.per_step * kWider;
                         __syncthreads();
                     }
                     histogram(sh, chunks, double(from), true);
@@ -1156,16 +1169,22 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
     __syncthreads();
     if (k && list.count <= kList) {
         listed = list.count;
-        if (listed > k)
+        if (listed > k) {
+            // The bins reach down to the list's floor, or nearly all of it would lie in
+            // the last one (T = 0.05, one row of 65536: 76 us, with this 24).
+            const bool near = !(floor > -__builtin_inff()) ||
+                              (from - double(floor)) * row.per_step < double(kBins);
             cut = list_cut(sh, &sh->index[0], listed, true, double(k), -1.0, 0.0, cut, from, 0.0,
-                           1.0, false);
+                           near ? 1.0 : kWider, false);
+        }
         if (share >= 0.0)
             cut = list_cut(sh, &sh->index[0], listed, false, 0.0, share, 0.0, cut, from, 0.0, 1.0,
                            listed > k);
     } else if (k) {
-        cut = digit_cut(sh, true, double(k), -1.0, cut);
+        const Edges all = {-__builtin_inff(), __builtin_inff()};
+        cut = digit_cut(sh, true, double(k), -1.0, 0.0, cut, all, kAnyGrade);
         if (share >= 0.0)
-            cut = digit_cut(sh, false, 0.0, share, cut);
+            cut = digit_cut(sh, false, 0.0, share, 0.0, cut, all, kAnyGrade);
     } else if (share >= 0.0) {
         histogram(sh, row.chunks, from, false);
         const Found found = find_bin(sh, 0.0, share, 0.0, Units(s.width).scale, Bins::steps);
@@ -1175,7 +1194,8 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(Sampling s)
         cut = list.picked <= kList
                   ? list_cut(sh, &sh->pick[0], list.picked, false, found.goal, -1.0, found.over,
                              cut, from, double(found.bin), double(kBins), false)
-                  : digit_cut(sh, false, found.goal, -1.0, cut);
+                  : digit_cut(sh, false, found.goal, -1.0, found.over, cut, edges,
+                              grade_of(found.bin));
         listed = list.count <= kMany ? list.count : 0;
     }
     if (min_p > 0.0f) {
