@@ -514,8 +514,9 @@ __device__ __attribute__((noinline)) Found find_bin(Lds *sh, double goal, double
     if (wave == here) {
         // Boundaries of the thread's bins: sums that neighbours share.
         const double base = here ? lane_value(upto, int(here) - 1) : 0.0;
-        const double before = __shfl_up(scan, 1, 64);
-        const double from = over + (lane ? base + before : base), to = over + (base + scan);
+        const double before =  // the lane's before, zero for the first
+            __builtin_bit_cast(double, moved<0x138, 0xf>(__builtin_bit_cast(uint64_t, scan)));
+        const double from = over + (base + before), to = over + (base + scan);
         const double middle = from + a;
         const bool reached = to >= goal;
         if (lane == holder(a + b > 0.0, reached)) {
