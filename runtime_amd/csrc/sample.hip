@@ -32,8 +32,8 @@
 // a small loop of its own, and what several steps need is a function that is called,
 // not inlined (inlined, with loops unrolled by 4 to 8, one row of 65536 took 1.5 to 2
 // times as long).  One row of 65536 takes, in us: greedy 6.2, min-p 12, all
-// tokens 20, top-k 50 18.0 and with top-p 21.2, top-p 0.9 at temperatures 0.6 / 1 /
-// 1.5 27.4 / 32.3 / 41.1; 192 rows 11, 21, 27, 23 and 27, 38 / 47 / 54.
+// tokens 20, top-k 50 18.1 and with top-p 21.3, top-p 0.9 at temperatures 0.6 / 1 /
+// 1.5 27.6 / 32.5 / 41.3; 192 rows 11, 21, 27, 23 and 27, 38 / 47 / 54.
 #include "kernels.hpp"
 #include "paged.hpp"
 
