@@ -212,6 +212,8 @@ void mfh_fence_free(mfh_fence *fence);
 
 /* InferenceOps::read_f32_async (inference.rs:111). */
 mfh_status mfh_read_f32_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out);
+/* The same for a U8 buffer: each byte comes out as its value, 0 to 255. */
+mfh_status mfh_read_u8_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out);
 /* Poll a readback. When ready, copies min(capacity, n) values into `dst`,
  * stores n in *count, and the completion is consumed: a second ready poll
  * returns MFH_COMPLETION_CONSUMED. */
@@ -461,6 +463,118 @@ mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                          const mfh_buf *key_pages, const mfh_buf *value_pages,
                          const mfh_buf *tables, const mfh_buf *lengths, uint32_t query_heads,
                          uint32_t key_value_heads, uint32_t head_dim);
+
+/* mfh_paged_qk_norm_rope with a place of its own for each token: token t turns by
+ * positions[t] and is stored at places[t] of its sequence.  Tokens of a drafted tree
+ * that could follow the same token have one position and different places.  A bad
+ * place counts as a bad position does. */
+mfh_status mfh_paged_qk_norm_rope_at(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key_pages,
+                                     mfh_buf *value_pages, const mfh_buf *query,
+                                     const mfh_buf *key, const mfh_buf *value,
+                                     const mfh_buf *query_weight, const mfh_buf *key_weight,
+                                     const mfh_buf *rotation, const mfh_buf *tables,
+                                     const mfh_buf *sequences, const mfh_buf *positions,
+                                     const mfh_buf *places, uint32_t query_heads,
+                                     uint32_t key_value_heads, uint32_t head_dim,
+                                     int interleaved, float epsilon);
+
+/*
+ * Runs: several new tokens of each sequence in one call.  The run of sequence s is
+ * tokens starts[s] .. starts[s + 1] - 1 of the batch (`starts` F32 [sequences + 1]),
+ * possibly none; its token i is cached at place lengths[s] + i, behind the
+ * lengths[s] tokens that the sequence holds without it.  The first entry of
+ * `starts` that is no whole number, falls below the one before it or passes the
+ * batch ends the list: sequences from there on have no run.  Rows of the batch
+ * that are in no run (behind the last one, or padding before the first) are
+ * left as they were by the attention calls.
+ * Trees: parents[t] (F32 [tokens]) is the token of the same run that token t follows, as
+ * its number in the run, below t's own; -1 for one that follows the cached tokens
+ * alone.  Null: every token follows the one before it.
+ * Masks: `mask` is U8 [tokens, bytes]: bit i % 8 of byte i / 8 of row t says that t
+ * attends token i of its run; tokens behind the row's last bit are not attended.
+ */
+
+/* Where a batch of runs stands, once for all layers of a step: each token's sequence,
+ * its position lengths[s] + (its ancestors' number), its place lengths[s] + i, and in
+ * `mask` (null: not wanted) the bits of itself and of its ancestors.  F32 [tokens] but
+ * for the mask.  A token in no run, with a bad parent or a bad ancestor, of a sequence
+ * whose length is no whole number or leaves places of 2^24 and more, or with a number
+ * past the mask's last bit has sequence, position and place -1 and no bit: the append
+ * calls then store nothing for it and give it a NaN query. */
+mfh_status mfh_draft_layout(mfh_ctx *ctx, mfh_buf *sequences, mfh_buf *positions,
+                            mfh_buf *places, mfh_buf *mask, const mfh_buf *starts,
+                            const mfh_buf *parents, const mfh_buf *lengths);
+
+/* Attention of runs over their sequences' cached tokens and over the run itself, whose
+ * keys and values are in the cache already: token t attends all lengths[s] cached
+ * tokens before the run and, of the run, those that its mask row names (`mask` null:
+ * itself and all before it, as in a prompt).  `starts` null: one token for each row
+ * of `tables`.  Queries [tokens, query_heads * head_dim], otherwise as
+ * mfh_paged_gqa, its workspace included.  A token that attends nothing gives zeros; one
+ * of a sequence whose length is no whole number, or that passes the table's row or
+ * 2^24 with its run, and one that attends a key whose page id is bad, give NaN
+ * rows.  What a token does not attend does not reach its row, whatever it holds (NaN
+ * included); what it attends is expected to be finite.  head_dim <= 1024; 32, 64, 80, 96,
+ * 112, 128, 160, 192 and 256 run on matrix cores, others many times slower. */
+mfh_status mfh_paged_tree_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
+                              const mfh_buf *key_pages, const mfh_buf *value_pages,
+                              const mfh_buf *tables, const mfh_buf *starts,
+                              const mfh_buf *lengths, const mfh_buf *mask, uint32_t query_heads,
+                              uint32_t key_value_heads, uint32_t head_dim);
+
+/*
+ * Latent caches: one row of rank + rope columns per token that all heads share, in
+ * page buffers of one head ([pages, 1, page_size, rank + rope]; mfh_alloc_pages).  Its
+ * first `rank` columns, the latent, are key and value, the last `rope`, rotated, are
+ * key alone.
+ */
+
+/* New tokens into a latent cache.  `latent` [tokens, rank] is RMS-normed by
+ * `latent_weight` (null: as it is), `key` [tokens, rope] turned by row positions[t] of
+ * `rotation` [positions, rope], and both stored at place places[t] (null:
+ * positions[t]) of sequence sequences[t] (null: t); `query` [tokens, query_heads *
+ * rope] turned likewise into `query_out`.  Pairs, padded rows, bad ids and binary16 pages as
+ * in mfh_paged_qk_norm_rope. */
+mfh_status mfh_paged_latent_append(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *pages,
+                                   const mfh_buf *query, const mfh_buf *latent,
+                                   const mfh_buf *key, const mfh_buf *latent_weight,
+                                   const mfh_buf *rotation, const mfh_buf *tables,
+                                   const mfh_buf *sequences, const mfh_buf *positions,
+                                   const mfh_buf *places, uint32_t query_heads, int interleaved,
+                                   float epsilon);
+
+/* Attention of runs over latent caches, in the absorbed form: head h of token t has the
+ * query (latent_query, rotary_query) of rank + rope columns (latent_query [tokens,
+ * query_heads * rank], the key up-projection folded in; rotary_query [tokens,
+ * query_heads * rope], rotated), scores are its products with the cached rows times
+ * `scale`, and its output [tokens, query_heads * rank] is their softmax times the cached
+ * latents.  Runs, masks, lengths, bad ids and the workspace as in mfh_paged_tree_gqa.
+ * rank + rope <= 1024; ranks 128, 256 and 512 with rope 32 or 64 run on matrix cores,
+ * others many times slower. */
+mfh_status mfh_paged_latent_attention(mfh_ctx *ctx, mfh_buf *output,
+                                      const mfh_buf *latent_query, const mfh_buf *rotary_query,
+                                      const mfh_buf *pages, const mfh_buf *tables,
+                                      const mfh_buf *starts, const mfh_buf *lengths,
+                                      const mfh_buf *mask, uint32_t query_heads, float scale);
+
+/* What the model accepts of each run, and the caches without the rest.  A run's first token
+ * is one that the sequence has chosen already; choices[t] is the model's choice of
+ * the token behind t (mfh_argmax, mfh_sample_rows) and tokens[t] what was drafted, F32
+ * [tokens] each.  The accepted path starts at the run's first token and goes on to the
+ * first child of its last one whose token is that one's choice, while there is one and
+ * the path is shorter than `emitted` [sequences, columns] is wide.  Row s of `emitted`
+ * holds the choices along the path, then -1; counts[s] is the path's length (0 without a
+ * run), by which the sequence's length grows; next[s] is the last choice, the first
+ * token of its next run (-1 without a run).  In each of the page buffers (of any heads,
+ * widths and formats, one page size; all layers' keys, values or latents) the path's rows are
+ * moved to places lengths[s], lengths[s] + 1, ...; what lies behind them is as before
+ * or a moved row.  A sequence whose length is bad, or whose path has a place without a
+ * page, is left as it is, with NaN for its three outputs.  columns <= 1024. */
+mfh_status mfh_settle_drafts(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mfh_buf *next,
+                             mfh_buf *const *pages, size_t buffers, const mfh_buf *tokens,
+                             const mfh_buf *choices, const mfh_buf *starts,
+                             const mfh_buf *parents, const mfh_buf *lengths,
+                             const mfh_buf *tables);
 
 /* Copy page from_pages[i] of sources[b] to page to_pages[i] of destinations[b],
  * for every i < count and b < buffers (a model's key and value pages of all

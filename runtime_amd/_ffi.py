@@ -94,6 +94,7 @@ SIGNATURES = {
     "mfh_fence_cancel": (S, [P]),
     "mfh_fence_free": (None, [P]),
     "mfh_read_f32_async": (S, [P, P, PP]),
+    "mfh_read_u8_async": (S, [P, P, PP]),
     "mfh_readback_poll": (S, [P, ctypes.POINTER(ctypes.c_int), c_float_p, SZ,
                               ctypes.POINTER(SZ)]),
     "mfh_readback_cancel": (S, [P]),
@@ -136,7 +137,14 @@ SIGNATURES = {
     "mfh_rotation_table": (S, [P, P, ctypes.c_float, ctypes.POINTER(RopeScaling)]),
     "mfh_paged_qk_norm_rope": (S, [P] * 13 + [ctypes.c_uint32] * 3 + [ctypes.c_int,
                                                                       ctypes.c_float]),
+    "mfh_paged_qk_norm_rope_at": (S, [P] * 14 + [ctypes.c_uint32] * 3 + [ctypes.c_int,
+                                                                         ctypes.c_float]),
     "mfh_paged_gqa": (S, [P] * 7 + [ctypes.c_uint32] * 3),
+    "mfh_draft_layout": (S, [P] * 8),
+    "mfh_paged_tree_gqa": (S, [P] * 9 + [ctypes.c_uint32] * 3),
+    "mfh_paged_latent_append": (S, [P] * 12 + [ctypes.c_uint32, ctypes.c_int, ctypes.c_float]),
+    "mfh_paged_latent_attention": (S, [P] * 9 + [ctypes.c_uint32, ctypes.c_float]),
+    "mfh_settle_drafts": (S, [P] * 4 + [PP, SZ] + [P] * 6),
     "mfh_copy_pages": (S, [P, PP, PP, SZ, P, P, SZ]),
     "mfh_sample_rows": (S, [P] * 6),
     # LFM2 token pass (minifield_lfm2.h)

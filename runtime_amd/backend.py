@@ -271,6 +271,21 @@ class HipBackend:
         count = int(np.prod(buf.shape)) if buf.shape else 1
         return Readback(out.value, self, count)
 
+    def read_u8_async(self, buf: Buffer) -> Readback:
+        """The bytes of a U8 buffer, as values."""
+        out = ctypes.c_void_p()
+        self._check(_ffi.lib().mfh_read_u8_async(self._ctx, buf.handle, ctypes.byref(out)))
+        count = int(np.prod(buf.shape)) if buf.shape else 1
+        return Readback(out.value, self, count)
+
+    def read_u8(self, buf: Buffer) -> np.ndarray:
+        """`read` of a U8 buffer."""
+        rb = self.read_u8_async(buf)
+        while True:
+            values = rb.poll_step()
+            if values is not None:
+                return values.reshape(buf.shape).astype(np.uint8)
+
     def read(self, buf: Buffer) -> np.ndarray:
         """Submit a readback and poll it to completion (test convenience)."""
         rb = self.read_f32_async(buf)
@@ -467,6 +482,60 @@ class HipBackend:
             self._ctx, output.handle, query.handle, key_pages.handle, value_pages.handle,
             tables.handle, lengths.handle, spec.query_heads, spec.key_value_heads,
             spec.head_dim))
+
+    def paged_qk_norm_rope_at(self, query_out: Buffer, key_pages: Buffer, value_pages: Buffer,
+                              query: Buffer, key: Buffer, value: Buffer,
+                              query_weight: Buffer | None, key_weight: Buffer | None,
+                              rotation: Buffer, tables: Buffer, sequences: Buffer | None,
+                              positions: Buffer, places: Buffer, rope: "PagedRopeSpec",
+                              epsilon: float) -> None:
+        self._check(_ffi.lib().mfh_paged_qk_norm_rope_at(
+            self._ctx, query_out.handle, key_pages.handle, value_pages.handle, query.handle,
+            key.handle, value.handle, _h(query_weight), _h(key_weight), rotation.handle,
+            tables.handle, _h(sequences), positions.handle, places.handle, rope.query_heads,
+            rope.key_value_heads, rope.head_dim, int(rope.interleaved), epsilon))
+
+    def draft_layout(self, sequences: Buffer, positions: Buffer, places: Buffer,
+                     mask: Buffer | None, starts: Buffer, parents: Buffer | None,
+                     lengths: Buffer) -> None:
+        self._check(_ffi.lib().mfh_draft_layout(
+            self._ctx, sequences.handle, positions.handle, places.handle, _h(mask),
+            starts.handle, _h(parents), lengths.handle))
+
+    def paged_tree_gqa(self, output: Buffer, query: Buffer, key_pages: Buffer,
+                       value_pages: Buffer, tables: Buffer, starts: Buffer | None,
+                       lengths: Buffer, mask: Buffer | None, spec: "GqaSpec") -> None:
+        self._check(_ffi.lib().mfh_paged_tree_gqa(
+            self._ctx, output.handle, query.handle, key_pages.handle, value_pages.handle,
+            tables.handle, _h(starts), lengths.handle, _h(mask), spec.query_heads,
+            spec.key_value_heads, spec.head_dim))
+
+    def paged_latent_append(self, query_out: Buffer, pages: Buffer, query: Buffer,
+                            latent: Buffer, key: Buffer, latent_weight: Buffer | None,
+                            rotation: Buffer, tables: Buffer, sequences: Buffer | None,
+                            positions: Buffer, places: Buffer | None, query_heads: int,
+                            interleaved: bool, epsilon: float) -> None:
+        self._check(_ffi.lib().mfh_paged_latent_append(
+            self._ctx, query_out.handle, pages.handle, query.handle, latent.handle, key.handle,
+            _h(latent_weight), rotation.handle, tables.handle, _h(sequences), positions.handle,
+            _h(places), query_heads, int(interleaved), epsilon))
+
+    def paged_latent_attention(self, output: Buffer, latent_query: Buffer,
+                               rotary_query: Buffer, pages: Buffer, tables: Buffer,
+                               starts: Buffer | None, lengths: Buffer, mask: Buffer | None,
+                               query_heads: int, scale: float) -> None:
+        self._check(_ffi.lib().mfh_paged_latent_attention(
+            self._ctx, output.handle, latent_query.handle, rotary_query.handle, pages.handle,
+            tables.handle, _h(starts), lengths.handle, _h(mask), query_heads, scale))
+
+    def settle_drafts(self, emitted: Buffer, counts: Buffer, next: Buffer,
+                      pages: Sequence[Buffer], tokens: Buffer, choices: Buffer, starts: Buffer,
+                      parents: Buffer | None, lengths: Buffer, tables: Buffer) -> None:
+        handles = (ctypes.c_void_p * max(1, len(pages)))(*[b.handle for b in pages])
+        self._check(_ffi.lib().mfh_settle_drafts(
+            self._ctx, emitted.handle, counts.handle, next.handle, handles, len(pages),
+            tokens.handle, choices.handle, starts.handle, _h(parents), lengths.handle,
+            tables.handle))
 
     def copy_pages(self, destinations: Sequence[Buffer], sources: Sequence[Buffer], from_pages,
                    to_pages) -> None:

@@ -153,8 +153,9 @@ struct mfh_fence {
 struct mfh_readback {
     mfh_ctx *ctx = nullptr;
     hipEvent_t event = nullptr;
-    float *host = nullptr;
-    size_t count = 0;
+    void *host = nullptr;  // `bytes` of staging
+    size_t count = 0, bytes = 0;
+    bool narrow = false;  // bytes, which a poll gives out as their values
     bool consumed = false;
     bool cancelled = false;
 };

@@ -107,14 +107,21 @@ __device__ __forceinline__ bool place_of(const PagedRope &p, uint64_t token, Pla
     if (!valid_index(position, p.rotation_rows) || !valid_index(sequence, p.sequence_count))
         return false;
     place.position = uint32_t(position);
-    const uint32_t column = place.position >> p.shape.page_shift;
+    uint32_t at = place.position;
+    if (p.places) {
+        const float given = p.places[token];
+        if (!valid_index(given, 1u << 24))
+            return false;
+        at = uint32_t(given);
+    }
+    const uint32_t column = at >> p.shape.page_shift;
     if (column >= p.max_pages)
         return false;
     const float page = p.tables[uint64_t(uint32_t(sequence)) * p.max_pages + column];
     if (!valid_index(page, p.shape.pages))
         return false;
     place.row = uint64_t(uint32_t(page)) * p.shape.stride() +
-                uint64_t(place.position & (p.shape.page_size() - 1)) * p.shape.head_dim;
+                uint64_t(at & (p.shape.page_size() - 1)) * p.shape.head_dim;
     return true;
 }
 

@@ -58,6 +58,7 @@ struct PagedRope {
     const float *tables = nullptr;     // [sequences, max_pages]
     const float *sequences = nullptr;  // [tokens], null: token t is sequence t
     const float *positions = nullptr;  // [tokens]
+    const float *places = nullptr;     // [tokens], null: the positions
     PageShape shape;
     uint64_t tokens = 0;
     uint32_t rotation_rows = 0, rotary_dim = 0, sequence_count = 0, max_pages = 0;

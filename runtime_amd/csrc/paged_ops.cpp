@@ -11,125 +11,10 @@
 #include "internal.hpp"
 #include "kernels.hpp"
 #include "paged.hpp"
+#include "paged_checks.hpp"
 
 namespace mfh {
 namespace {
-
-const float *dev_f32(const mfh_buf *b) { return static_cast<const float *>(b->dev); }
-float *dev_f32(mfh_buf *b) { return static_cast<float *>(b->dev); }
-
-mfh_status launched(mfh_ctx *ctx)
-{
-    if (hipGetLastError() != hipSuccess)
-        return fail(ctx, MFH_BACKEND_FAILURE, "paged kernel launch failed");
-    return MFH_OK;
-}
-
-// Exact f32 values reach 2^24.
-constexpr uint64_t kIndexLimit = uint64_t(1) << 24;
-
-// The geometry of a page buffer: [pages, kv_heads, page_size, head_dim] F32, or
-// U8 with twice the width.
-mfh_status page_shape_of(mfh_ctx *ctx, const uint64_t (&dims)[4], bool half, PageShape *out)
-{
-    out->half = half;
-    if (half && dims[3] % 2 != 0)
-        return fail(ctx, MFH_INVALID_SHAPE, "binary16 page rows must hold an even byte count");
-    const uint64_t d = half ? dims[3] / 2 : dims[3], size = dims[2];
-    if (dims[0] == 0 || dims[1] == 0 || d == 0)
-        return fail(ctx, MFH_INVALID_SHAPE, "page buffers must have a page, a head and a column");
-    if (size < 8 || size > 4096 || (size & (size - 1)))
-        return fail(ctx, MFH_INVALID_SHAPE, "page size must be a power of two in [8, 4096]");
-    if (dims[0] > kIndexLimit)
-        return fail(ctx, MFH_UNSUPPORTED, "page count exceeds the exact f32 index range");
-    if (dims[1] > UINT16_MAX || d > UINT16_MAX)
-        return fail(ctx, MFH_OVERFLOW, "page extent exceeds the kernel index range");
-    out->pages = uint32_t(dims[0]);
-    out->kv_heads = uint32_t(dims[1]);
-    out->page_shift = uint32_t(__builtin_ctzll(size));
-    out->head_dim = uint32_t(d);
-    return MFH_OK;
-}
-mfh_status page_shape(mfh_ctx *ctx, const mfh_buf *buf, PageShape *out)
-{
-    mfh_status s = check_buffer(ctx, buf);
-    if (s)
-        return s;
-    if (buf->rank != 4)
-        return fail(ctx, MFH_INVALID_SHAPE,
-                    "page buffers must be [pages, kv_heads, page_size, head_dim]");
-    return page_shape_of(ctx, buf->dims, buf->dtype == MFH_DTYPE_U8, out);
-}
-
-// Key and value pages of one cache.
-mfh_status cache_shape(mfh_ctx *ctx, const mfh_buf *key_pages, const mfh_buf *value_pages,
-                       uint32_t key_value_heads, uint32_t head_dim, PageShape *out)
-{
-    PageShape value;
-    mfh_status s = page_shape(ctx, key_pages, out);
-    if (!s)
-        s = page_shape(ctx, value_pages, &value);
-    if (s)
-        return s;
-    if (key_pages->dtype != value_pages->dtype || !same_shape(key_pages, value_pages))
-        return fail(ctx, MFH_INVALID_SHAPE, "key and value pages must have one shape and format");
-    if (key_pages->dev == value_pages->dev)
-        return fail(ctx, MFH_INVALID_ARGUMENT, "key and value caches must have distinct storage");
-    if (out->kv_heads != key_value_heads || out->head_dim != head_dim)
-        return fail(ctx, MFH_INVALID_SHAPE, "page buffer heads differ from descriptor");
-    return MFH_OK;
-}
-
-mfh_status check_heads(mfh_ctx *ctx, uint32_t query_heads, uint32_t key_value_heads,
-                       uint32_t head_dim)
-{
-    if (key_value_heads == 0 || query_heads == 0 || query_heads % key_value_heads != 0)
-        return fail(ctx, MFH_INVALID_SHAPE,
-                    "query heads must be a nonzero multiple of key/value heads");
-    if (head_dim == 0)
-        return fail(ctx, MFH_INVALID_ARGUMENT, "head count and head dimension must be nonzero");
-    return MFH_OK;
-}
-
-// A sequence table: [sequences, max_pages] page ids.
-mfh_status check_tables(mfh_ctx *ctx, const mfh_buf *tables)
-{
-    mfh_status s = check_f32(ctx, tables);
-    if (s)
-        return s;
-    if (tables->rank != 2)
-        return fail(ctx, MFH_INVALID_SHAPE, "page tables must be [sequences, max_pages]");
-    if (tables->dims[0] > kIndexLimit || tables->dims[1] > kIndexLimit)
-        return fail(ctx, MFH_UNSUPPORTED, "page table extent exceeds the exact f32 index range");
-    return MFH_OK;
-}
-
-// An F32 operand of shape [dims[0], ...].
-mfh_status check_dims(mfh_ctx *ctx, const mfh_buf *buf, uint64_t rows, uint64_t columns,
-                      const char *message)
-{
-    mfh_status s = check_f32(ctx, buf);
-    if (s)
-        return s;
-    if (buf->rank != 2 || buf->dims[0] != rows || buf->dims[1] != columns)
-        return fail(ctx, MFH_INVALID_SHAPE, message);
-    return MFH_OK;
-}
-
-mfh_status check_vector(mfh_ctx *ctx, const mfh_buf *buf, uint64_t count, const char *message)
-{
-    mfh_status s = check_f32(ctx, buf);
-    if (s)
-        return s;
-    if (buf->rank != 1 || buf->dims[0] != count)
-        return fail(ctx, MFH_INVALID_SHAPE, message);
-    return MFH_OK;
-}
-
-mfh_status aliased(mfh_ctx *ctx)
-{
-    return fail(ctx, MFH_INVALID_ARGUMENT, "output aliases an input");
-}
 
 // The launches of a page copy, PAIRS pages and kCopyBuffers buffers at most in each.
 template <uint32_t PAIRS>
@@ -204,7 +89,103 @@ class PageSet {
     uint32_t *slots_ = few_;
 };
 
-bool positive(float v) { return std::isfinite(v) && v > 0.0f; }
+// New tokens into key/value caches; `places` may be null.
+mfh_status enter(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key_pages, mfh_buf *value_pages,
+                 const mfh_buf *query, const mfh_buf *key, const mfh_buf *value,
+                 const mfh_buf *query_weight, const mfh_buf *key_weight, const mfh_buf *rotation,
+                 const mfh_buf *tables, const mfh_buf *sequences, const mfh_buf *positions,
+                 const mfh_buf *places, uint32_t query_heads, uint32_t key_value_heads,
+                 uint32_t head_dim, int interleaved, float epsilon)
+{
+    if (!ctx)
+        return MFH_INVALID_ARGUMENT;
+    mfh_status s = check_heads(ctx, query_heads, key_value_heads, head_dim);
+    if (!s)
+        s = check_operation(ctx, MFH_OP_QK_NORM_ROPE);
+    if (s)
+        return s;
+    if (!positive(epsilon))
+        return fail(ctx, MFH_INVALID_ARGUMENT, "RMS epsilon must be finite and positive");
+    PagedRope p;
+    if ((s = cache_shape(ctx, key_pages, value_pages, key_value_heads, head_dim, &p.shape)) ||
+        (s = check_f32(ctx, query)))
+        return s;
+    if (query->rank != 2 || query->dims[1] != uint64_t(query_heads) * head_dim)
+        return fail(ctx, MFH_INVALID_SHAPE, "packed head tensor width differs from descriptor");
+    const uint64_t tokens = query->dims[0], kv_width = uint64_t(key_value_heads) * head_dim;
+    if ((s = check_dims(ctx, key, tokens, kv_width, "keys must be [tokens, kv_heads * head_dim]")) ||
+        (s = check_dims(ctx, value, tokens, kv_width,
+                        "values must be [tokens, kv_heads * head_dim]")))
+        return s;
+    if (!query_weight != !key_weight)
+        return fail(ctx, MFH_INVALID_ARGUMENT,
+                    "query and key norm weights must be given together");
+    if (query_weight &&
+        ((s = check_vector(ctx, query_weight, head_dim,
+                           "head RMS weight must have head_dim entries")) ||
+         (s = check_vector(ctx, key_weight, head_dim,
+                           "head RMS weight must have head_dim entries"))))
+        return s;
+    if ((s = check_f32(ctx, rotation)))
+        return s;
+    if (rotation->rank != 2 || rotation->dims[1] % 2 != 0 || rotation->dims[1] > head_dim)
+        return fail(ctx, MFH_INVALID_SHAPE,
+                    "rotation table must be [positions, even width up to head_dim]");
+    if (rotation->dims[0] > kIndexLimit)
+        return fail(ctx, MFH_UNSUPPORTED, "rotation table exceeds the exact f32 index range");
+    if ((s = check_tables(ctx, tables)))
+        return s;
+    if (sequences) {
+        if ((s = check_vector(ctx, sequences, tokens, "sequence ids must be one per token")))
+            return s;
+    } else if (tables->dims[0] != tokens) {
+        return fail(ctx, MFH_INVALID_SHAPE,
+                    "without sequence ids the page tables must have a row per token");
+    }
+    if (places && (s = check_vector(ctx, places, tokens, "places must be one per token")))
+        return s;
+    if ((s = check_vector(ctx, positions, tokens, "positions must be one per token")) ||
+        (s = check_output(ctx, query_out, query->dims, 2)))
+        return s;
+    if (tokens > uint64_t(INT32_MAX) / 256 / (query_heads + 2 * uint64_t(key_value_heads)))
+        return fail(ctx, MFH_OVERFLOW, "token count exceeds the kernel index range");
+    if (aliases(query_out, {query, key, value, query_weight, key_weight, rotation, tables,
+                            sequences, positions, places, key_pages, value_pages}) ||
+        aliases(key_pages, {query, key, value, query_weight, key_weight, rotation, tables,
+                            sequences, positions, places}) ||
+        aliases(value_pages, {query, key, value, query_weight, key_weight, rotation, tables,
+                              sequences, positions, places}))
+        return aliased(ctx);
+    DeviceGuard guard(ctx->device);
+    mark_written(query_out);
+    mark_written(key_pages);
+    mark_written(value_pages);
+    if (!tokens)
+        return MFH_OK;
+    p.query_out = dev_f32(query_out);
+    p.key_pages = key_pages->dev;
+    p.value_pages = value_pages->dev;
+    p.query = dev_f32(query);
+    p.key = dev_f32(key);
+    p.value = dev_f32(value);
+    p.query_weight = query_weight ? dev_f32(query_weight) : nullptr;
+    p.key_weight = key_weight ? dev_f32(key_weight) : nullptr;
+    p.rotation = dev_f32(rotation);
+    p.tables = dev_f32(tables);
+    p.sequences = sequences ? dev_f32(sequences) : nullptr;
+    p.positions = dev_f32(positions);
+    p.places = places ? dev_f32(places) : nullptr;
+    p.tokens = tokens;
+    p.rotation_rows = uint32_t(rotation->dims[0]);
+    p.rotary_dim = uint32_t(rotation->dims[1]);
+    p.sequence_count = uint32_t(tables->dims[0]);
+    p.max_pages = uint32_t(tables->dims[1]);
+    p.query_heads = query_heads;
+    p.interleaved = interleaved != 0;
+    p.epsilon = epsilon;
+    launch_paged_qk_norm_rope(ctx->stream, p);
+    return launched(ctx);
+}
 
 }  // namespace
 }  // namespace mfh
@@ -292,91 +273,28 @@ mfh_status mfh_paged_qk_norm_rope(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key
                                   uint32_t key_value_heads, uint32_t head_dim, int interleaved,
                                   float epsilon)
 {
+    return enter(ctx, query_out, key_pages, value_pages, query, key, value, query_weight,
+                 key_weight, rotation, tables, sequences, positions, nullptr, query_heads,
+                 key_value_heads, head_dim, interleaved, epsilon);
+}
+
+mfh_status mfh_paged_qk_norm_rope_at(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *key_pages,
+                                     mfh_buf *value_pages, const mfh_buf *query,
+                                     const mfh_buf *key, const mfh_buf *value,
+                                     const mfh_buf *query_weight, const mfh_buf *key_weight,
+                                     const mfh_buf *rotation, const mfh_buf *tables,
+                                     const mfh_buf *sequences, const mfh_buf *positions,
+                                     const mfh_buf *places, uint32_t query_heads,
+                                     uint32_t key_value_heads, uint32_t head_dim,
+                                     int interleaved, float epsilon)
+{
     if (!ctx)
         return MFH_INVALID_ARGUMENT;
-    mfh_status s = check_heads(ctx, query_heads, key_value_heads, head_dim);
-    if (!s)
-        s = check_operation(ctx, MFH_OP_QK_NORM_ROPE);
-    if (s)
+    if (mfh_status s = check_f32(ctx, places))
         return s;
-    if (!positive(epsilon))
-        return fail(ctx, MFH_INVALID_ARGUMENT, "RMS epsilon must be finite and positive");
-    PagedRope p;
-    if ((s = cache_shape(ctx, key_pages, value_pages, key_value_heads, head_dim, &p.shape)) ||
-        (s = check_f32(ctx, query)))
-        return s;
-    if (query->rank != 2 || query->dims[1] != uint64_t(query_heads) * head_dim)
-        return fail(ctx, MFH_INVALID_SHAPE, "packed head tensor width differs from descriptor");
-    const uint64_t tokens = query->dims[0], kv_width = uint64_t(key_value_heads) * head_dim;
-    if ((s = check_dims(ctx, key, tokens, kv_width, "keys must be [tokens, kv_heads * head_dim]")) ||
-        (s = check_dims(ctx, value, tokens, kv_width,
-                        "values must be [tokens, kv_heads * head_dim]")))
-        return s;
-    if (!query_weight != !key_weight)
-        return fail(ctx, MFH_INVALID_ARGUMENT,
-                    "query and key norm weights must be given together");
-    if (query_weight &&
-        ((s = check_vector(ctx, query_weight, head_dim,
-                           "head RMS weight must have head_dim entries")) ||
-         (s = check_vector(ctx, key_weight, head_dim,
-                           "head RMS weight must have head_dim entries"))))
-        return s;
-    if ((s = check_f32(ctx, rotation)))
-        return s;
-    if (rotation->rank != 2 || rotation->dims[1] % 2 != 0 || rotation->dims[1] > head_dim)
-        return fail(ctx, MFH_INVALID_SHAPE,
-                    "rotation table must be [positions, even width up to head_dim]");
-    if (rotation->dims[0] > kIndexLimit)
-        return fail(ctx, MFH_UNSUPPORTED, "rotation table exceeds the exact f32 index range");
-    if ((s = check_tables(ctx, tables)))
-        return s;
-    if (sequences) {
-        if ((s = check_vector(ctx, sequences, tokens, "sequence ids must be one per token")))
-            return s;
-    } else if (tables->dims[0] != tokens) {
-        return fail(ctx, MFH_INVALID_SHAPE,
-                    "without sequence ids the page tables must have a row per token");
-    }
-    if ((s = check_vector(ctx, positions, tokens, "positions must be one per token")) ||
-        (s = check_output(ctx, query_out, query->dims, 2)))
-        return s;
-    if (tokens > uint64_t(INT32_MAX) / 256 / (query_heads + 2 * uint64_t(key_value_heads)))
-        return fail(ctx, MFH_OVERFLOW, "token count exceeds the kernel index range");
-    if (aliases(query_out, {query, key, value, query_weight, key_weight, rotation, tables,
-                            sequences, positions, key_pages, value_pages}) ||
-        aliases(key_pages, {query, key, value, query_weight, key_weight, rotation, tables,
-                            sequences, positions}) ||
-        aliases(value_pages, {query, key, value, query_weight, key_weight, rotation, tables,
-                              sequences, positions}))
-        return aliased(ctx);
-    DeviceGuard guard(ctx->device);
-    mark_written(query_out);
-    mark_written(key_pages);
-    mark_written(value_pages);
-    if (!tokens)
-        return MFH_OK;
-    p.query_out = dev_f32(query_out);
-    p.key_pages = key_pages->dev;
-    p.value_pages = value_pages->dev;
-    p.query = dev_f32(query);
-    p.key = dev_f32(key);
-    p.value = dev_f32(value);
-    p.query_weight = query_weight ? dev_f32(query_weight) : nullptr;
-    p.key_weight = key_weight ? dev_f32(key_weight) : nullptr;
-    p.rotation = dev_f32(rotation);
-    p.tables = dev_f32(tables);
-    p.sequences = sequences ? dev_f32(sequences) : nullptr;
-    p.positions = dev_f32(positions);
-    p.tokens = tokens;
-    p.rotation_rows = uint32_t(rotation->dims[0]);
-    p.rotary_dim = uint32_t(rotation->dims[1]);
-    p.sequence_count = uint32_t(tables->dims[0]);
-    p.max_pages = uint32_t(tables->dims[1]);
-    p.query_heads = query_heads;
-    p.interleaved = interleaved != 0;
-    p.epsilon = epsilon;
-    launch_paged_qk_norm_rope(ctx->stream, p);
-    return launched(ctx);
+    return enter(ctx, query_out, key_pages, value_pages, query, key, value, query_weight,
+                 key_weight, rotation, tables, sequences, positions, places, query_heads,
+                 key_value_heads, head_dim, interleaved, epsilon);
 }
 
 mfh_status mfh_paged_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,

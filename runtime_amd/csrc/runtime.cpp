@@ -881,16 +881,9 @@ void mfh_fence_free(mfh_fence *fence)
     delete fence;
 }
 
-mfh_status mfh_read_f32_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out)
+// A readback of `buf`, whose type the caller has checked.
+static mfh_status submit_readback(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out)
 {
-    if (!ctx || !out)
-        return MFH_INVALID_ARGUMENT;
-    *out = nullptr;
-    if (ctx->cancel_requested)
-        return fail(ctx, MFH_CANCELLED, "operation cancelled");
-    mfh_status s = check_f32(ctx, buf);
-    if (s)
-        return s;
     DeviceGuard guard(ctx->device);
     // The staging the completion owns until it is polled counts against the
     // total limit like device blocks do.  As for a device allocation, the
@@ -910,8 +903,10 @@ mfh_status mfh_read_f32_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **o
         return fail(ctx, MFH_RESOURCE_LIMIT, "host allocation failed");
     rb->ctx = ctx;
     rb->count = buf->elements;
+    rb->bytes = buf->bytes;
+    rb->narrow = buf->dtype == MFH_DTYPE_U8;
     if (rb->count) {
-        if (hipHostMalloc(reinterpret_cast<void **>(&rb->host), buf->bytes, hipHostMallocDefault) !=
+        if (hipHostMalloc(&rb->host, buf->bytes, hipHostMallocDefault) !=
             hipSuccess) {
             (void)hipGetLastError();
             delete rb;
@@ -941,6 +936,30 @@ mfh_status mfh_read_f32_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **o
     return MFH_OK;
 }
 
+mfh_status mfh_read_f32_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out)
+{
+    if (!ctx || !out)
+        return MFH_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (ctx->cancel_requested)
+        return fail(ctx, MFH_CANCELLED, "operation cancelled");
+    if (mfh_status s = check_f32(ctx, buf))
+        return s;
+    return submit_readback(ctx, buf, out);
+}
+
+mfh_status mfh_read_u8_async(mfh_ctx *ctx, const mfh_buf *buf, mfh_readback **out)
+{
+    if (!ctx || !out)
+        return MFH_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (ctx->cancel_requested)
+        return fail(ctx, MFH_CANCELLED, "operation cancelled");
+    if (mfh_status s = check_u8(ctx, buf))
+        return s;
+    return submit_readback(ctx, buf, out);
+}
+
 mfh_status mfh_readback_poll(mfh_readback *rb, int *ready, float *dst, size_t capacity,
                              size_t *count)
 {
@@ -965,13 +984,15 @@ mfh_status mfh_readback_poll(mfh_readback *rb, int *ready, float *dst, size_t ca
         return MFH_OK;
     *ready = 1;
     rb->consumed = true;
-    rb->ctx->pending_result_bytes -= rb->count * 4;
+    rb->ctx->pending_result_bytes -= rb->bytes;
     if (e != hipSuccess) {
         (void)hipGetLastError();
         return fail(rb->ctx, MFH_BACKEND_FAILURE, "device work failed before the readback");
     }
     size_t n = rb->count < capacity ? rb->count : capacity;
-    if (n && dst)
+    if (n && dst && rb->narrow)
+        std::copy_n(static_cast<const uint8_t *>(rb->host), n, dst);
+    else if (n && dst)
         std::memcpy(dst, rb->host, n * 4);
     if (count)
         *count = rb->count;
@@ -999,7 +1020,7 @@ void mfh_readback_free(mfh_readback *rb)
         if (rb->host)
             (void)hipHostFree(rb->host);
         if (!rb->consumed)
-            rb->ctx->pending_result_bytes -= rb->count * 4;
+            rb->ctx->pending_result_bytes -= rb->bytes;
         rb->ctx->live_readbacks.erase(rb);
     }
     delete rb;
