@@ -119,7 +119,14 @@ struct RunAttention {
     uint32_t value_dim = 0, max_pages = 0, query_heads = 0, group = 0, mask_bytes = 0;
     uint32_t longest = 0;  // places of a table row, below 2^24
     float scale = 0.0f;    // times log2 e
+    // Filled by run_attention_plan: blocks of the matrix-core kernel (0: the one of any
+    // width), and its workspace of run_attention_scratch_bytes.
+    uint32_t blocks = 0;
+    float *records = nullptr;
 };
+// Chooses the kernel and its split; false where the extents pass the index range.
+bool run_attention_plan(RunAttention &p, int cu_count);
+size_t run_attention_scratch_bytes(const RunAttention &p);
 void launch_run_attention(hipStream_t stream, const RunAttention &p);
 
 }  // namespace mfh

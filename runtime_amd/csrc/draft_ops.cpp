@@ -80,12 +80,18 @@ mfh_status attend(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
     if (aliases(output, {query, rotary_query, key_pages, value_pages, tables, starts, lengths,
                          mask}))
         return aliased(ctx);
-    if (tokens * p.query_heads > uint64_t(1) << 25)
-        return fail(ctx, MFH_OVERFLOW, "paged attention extent exceeds the kernel index range");
     const uint64_t longest = tables->dims[1] << p.shape.page_shift;
     p.longest = uint32_t(longest < kIndexLimit ? longest : kIndexLimit);
     p.max_pages = uint32_t(tables->dims[1]);
+    p.mask = mask ? static_cast<const uint8_t *>(mask->dev) : nullptr;
+    if (!run_attention_plan(p, ctx->cu_count))
+        return fail(ctx, MFH_OVERFLOW, "paged attention extent exceeds the kernel index range");
     DeviceGuard guard(ctx->device);
+    if (const size_t bytes = run_attention_scratch_bytes(p)) {
+        p.records = static_cast<float *>(paged_scratch(ctx, bytes));
+        if (!p.records)
+            return allocation_failed(ctx);
+    }
     mark_written(output);
     if (!tokens || !p.runs.sequences)
         return MFH_OK;
@@ -95,7 +101,6 @@ mfh_status attend(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
     p.key_pages = key_pages->dev;
     p.value_pages = value_pages->dev;
     p.tables = dev_f32(tables);
-    p.mask = mask ? static_cast<const uint8_t *>(mask->dev) : nullptr;
     launch_run_attention(ctx->stream, p);
     return launched(ctx);
 }
