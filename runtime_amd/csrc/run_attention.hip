@@ -130,7 +130,7 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 //
 // Query rows of a key/value head are (token, head of the group) pairs, counted through a run;
 // an item is (sequence, key/value head, 64 of its rows), a wave of a block has 16
-// of them.  The block walks the item's keys a tile at a time: all threads load a tile's rows
+// of them (of a latent cache two waves have the same 16).  The block walks the item's keys a tile at a time: all threads load a tile's rows
 // to registers (the next tile's while this one is worked on) and store them to LDS as
 // operands that the waves share.  Per tile, S^T = K Q^T leaves query row j in lane
 // column j (lane 16 q + j holds the scores of keys 16 c + 4 q + r in register r of
@@ -158,7 +158,6 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
-constexpr uint32_t kRows = 64;       // query rows of an item
 constexpr uint32_t kItemUnits = 2;
 constexpr uint32_t kLeastUnits = 4;  // of a block
 constexpr float kProbabilityShift = 15.0f;
@@ -171,11 +170,11 @@ struct Share {
 
 __host__ __device__ inline float *record_stats(const RunAttention &p)
 {
-    return p.records + 2 * uint64_t(p.blocks) * kRows * p.value_dim;
+    return p.records + 2 * uint64_t(p.blocks) * p.rows * p.value_dim;
 }
 __host__ __device__ inline Share *block_shares(const RunAttention &p)
 {
-    return reinterpret_cast<Share *>(record_stats(p) + 4 * uint64_t(p.blocks) * kRows);
+    return reinterpret_cast<Share *>(record_stats(p) + 4 * uint64_t(p.blocks) * p.rows);
 }
 
 // Inclusive scan over the wave's lanes by DPP moves; lane 63 ends with the sum.
@@ -219,11 +218,11 @@ __device__ __forceinline__ bool load_run(const RunAttention &p, uint32_t i, Run 
 }
 
 // Units of a sequence's items, SHIFT the logarithm of a tile's keys.  Where tokens attend
-// all before them, a later item has more keys: (64 / group) a row tile more, counted in
+// all before them, a later item has more keys: (rows / group) a row tile more, counted in
 // whole tiles, so that the sum has a closed form.
 template <int SHIFT>
 struct Units {
-    uint32_t group, base, step;  // step: tiles of a run's 64 tokens; 0: the same for all
+    uint32_t group, base, step;  // step: tiles that an item's rows are; 0: all items alike
     __device__ __forceinline__ Units(const RunAttention &p, const Run &run)
     {
         constexpr uint32_t KEYS = 1u << SHIFT;
@@ -235,7 +234,7 @@ struct Units {
         if (p.mask || run.count == 1) {
             base += (run.length + run.count + KEYS - 1) >> SHIFT;
         } else {
-            step = kRows / KEYS;
+            step = p.rows / KEYS;
             base += ((run.length + KEYS - 1) >> SHIFT) + step;
         }
     }
@@ -256,7 +255,7 @@ struct Units {
 };
 __device__ __forceinline__ uint32_t row_tiles(const RunAttention &p, const Run &run)
 {
-    return (run.count * p.group + kRows - 1) / kRows;
+    return (run.count * p.group + p.rows - 1) / p.rows;
 }
 
 // A block's place on the line of units: block b of n starts at floor(b total / n).
@@ -379,7 +378,7 @@ __device__ __forceinline__ bool next_part(const RunAttention &p, Line &line, Par
     part.keys = 0;
     if (run.length != UINT32_MAX) {
         // The item's last row is of this token.
-        const uint32_t token = (kRows * line.row_tile + kRows - 1) / p.group;
+        const uint32_t token = (p.rows * line.row_tile + p.rows - 1) / p.group;
         part.keys = run.length + (p.mask || token >= run.count ? run.count : token + 1);
     }
     const uint32_t tiles = (part.keys + (1u << SHIFT) - 1) >> SHIFT;
@@ -413,21 +412,21 @@ __device__ __forceinline__ bool next_part(const RunAttention &p, Line &line, Par
 
 // Chunks of a value row: as many 16-column tiles as one LDS read holds (16 bytes, then 8,
 // 4, 2).
-__host__ __device__ constexpr int chunk_tiles(int left)
+__host__ __device__ constexpr int chunk_tiles(int left, int most)
 {
-    int s = 8;
+    int s = most;
     while (s > left)
         s /= 2;
     return s;
 }
 // f(first tile, tiles) for each chunk of N tiles, both as constants.
-template <int N, int T = 0, typename F>
+template <int N, int MOST, int T = 0, typename F>
 __device__ __forceinline__ void for_chunks(F f)
 {
     if constexpr (T < N) {
-        constexpr int S = chunk_tiles(N - T);
+        constexpr int S = chunk_tiles(N - T, MOST);
         f(std::integral_constant<int, T>{}, std::integral_constant<int, S>{});
-        for_chunks<N, T + S>(f);
+        for_chunks<N, MOST, T + S>(f);
     }
 }
 
@@ -461,8 +460,8 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PAR
         if constexpr (HALF) {
             const v2h h = {_Float16(a), _Float16(b)};
             out[i] = __builtin_bit_cast(uint32_t, h);
-            a -= float(h[0]);
-            b -= float(h[1]);
+            a = __builtin_fmaf(float(h[0]), -1.0f, a);
+            b = __builtin_fmaf(float(h[1]), -1.0f, b);
         } else {
             out[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
             a -= __uint_as_float(out[i] << 16);
@@ -482,133 +481,179 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c)
                                                        __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
-// The products of a's parts (a cache's) with b's (a query's or a probability's), the
-// smallest first.
-template <bool HALF, int A, int B>
-__device__ __forceinline__ v4f products(const v4u (&a)[A], const v4u (&b)[B], v4f c)
-{
-    constexpr int most = HALF ? 1 : 2;  // the sum of the parts' numbers
-#pragma unroll
-    for (int sum = most; sum >= 0; --sum)
-#pragma unroll
-        for (int i = 0; i < A; ++i)
-            if (sum - i >= 0 && sum - i < B)
-                c = mfma<HALF>(a[i], b[sum - i], c);
-    return c;
-}
-
-// LDS rows of D 16-bit columns hold 16-byte chunks in an order of their own, by which 16
-// rows' equal chunks fall on all banks.
+// Elements between LDS rows of D 16-bit columns: 16 bytes more than the row, so that 16
+// rows' pieces of one column fall on all banks, at places that differ by constants (an
+// order of pieces by row in place of the padding took a register for each).
 template <int D>
-__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk)
+constexpr int kPitch = D + 8;
+
+// The value, which the compiler takes for a new one: what rarely run code forms from it is
+// formed there, not held in registers around the loop.
+__device__ __forceinline__ uint32_t formed_here(uint32_t v)
 {
-    constexpr uint32_t C = D / 8;
-    constexpr uint32_t G = C % 16 == 0 ? 16 : C % 8 == 0 ? 8 : C % 4 == 0 ? 4 : 2;
-    static_assert(C % G == 0, "whole groups of chunks");
-    return row * D + ((chunk ^ (row / (16 / G) & (G - 1))) * 8);
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
-// What a kernel of a width has in a tile, in LDS and on a CU.
-template <int DK, int DV, bool HALF, bool LATENT>
+// What a kernel of a width has in a tile, in LDS and on a CU.  A wave has GROUPS times 16
+// rows; SPLIT waves share them, each with a part of the key columns for the scores and of
+// the value columns for the output.
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
 struct Shape {
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int ROWS = 16 * GROUPS * WAVES / SPLIT;
     static constexpr int PARTS = HALF ? 1 : 3;          // of keys and values
     static constexpr int QUERY_PARTS = HALF ? 2 : 3;    // of queries and probabilities
-    static constexpr int SHIFT = DK <= (HALF ? 128 : 64) ? 6 : 5;
+    static constexpr int SHIFT = DK * GROUPS <= (HALF ? 128 : 64) ? 6 : 5;
     static constexpr int KEYS = 1 << SHIFT;
-    static constexpr int KEY_PLANE = KEYS * DK, VALUE_PLANE = LATENT ? 0 : KEYS * DV;
+    static constexpr int KEY_PLANE = KEYS * kPitch<DK>, VALUE_PLANE = LATENT ? 0 : KEY_PLANE;
     static constexpr int STAGE = PARTS * (KEY_PLANE + VALUE_PLANE);  // 16-bit elements
     static constexpr int STAGES = HALF ? 2 : 1;
-    static constexpr int RESIDENT = DK <= 128 ? 2 : 1;
+    static constexpr int RESIDENT = WAVES == 4 && DK <= 128 ? 2 : 1;
+    static constexpr int CHUNK = SPLIT > 1 ? 4 : 8;     // most tiles of a value chunk
 };
 
-template <int DK, int DV, bool HALF, bool LATENT>
-__global__ __launch_bounds__(kBlock, (Shape<DK, DV, HALF, LATENT>::RESIDENT))
+// 16-byte loads of a tile's rows of D columns, by wave: each load is of one run of eight
+// keys, which one page holds, so that its page is the wave's and its lanes' places in
+// the run never change.
+template <typename T, int D, int KEYS, int WAVES>
+struct Loads {
+    static constexpr int PIECE = 16 / sizeof(T);      // columns of a load
+    static constexpr int CHUNKS = 8 * D / PIECE;      // of eight keys
+    static constexpr int EACH = (CHUNKS + 63) / 64;   // loads of eight keys
+    static constexpr int ALL = KEYS / 8 * EACH;
+    static constexpr int MINE = (ALL + WAVES - 1) / WAVES;
+    __device__ __forceinline__ static uint32_t number(int i, uint32_t wave)
+    {
+        const uint32_t n = wave + i * WAVES;
+        return (i + 1) * WAVES > ALL && n >= uint32_t(ALL) ? ALL - 1 : n;
+    }
+    // The lane's chunk of the eight keys; past their end the last one again.
+    __device__ __forceinline__ static uint32_t chunk(uint32_t n, uint32_t lane)
+    {
+        const uint32_t c = n % EACH * 64 + lane;
+        return CHUNKS % 64 != 0 && c >= uint32_t(CHUNKS) ? CHUNKS - 1 : c;
+    }
+};
+
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
+__global__ __launch_bounds__(64 * WAVES, (Shape<DK, DV, HALF, LATENT, WAVES, SPLIT,
+                                                GROUPS>::RESIDENT * WAVES / 4))
 void run_attention_kernel(RunAttention p)
 {
-    using S = Shape<DK, DV, HALF, LATENT>;
+    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>;
     using T = typename std::conditional<HALF, _Float16, float>::type;
-    static_assert(DK % 16 == 0 && DV % 16 == 0, "widths of the matrix-core path");
+    static_assert(DK % (SPLIT > 1 ? 32 : 16) == 0 && DV % (16 * SPLIT) == 0,
+                  "widths of the matrix-core path");
     constexpr int KEYS = S::KEYS, SHIFT = S::SHIFT, PARTS = S::PARTS, QP = S::QUERY_PARTS;
+    constexpr uint32_t ROWS = S::ROWS;
     constexpr int NB = KEYS / 16;                  // key blocks of a tile
-    constexpr int U = (DK + 31) / 32;              // product depths of a key row
-    constexpr int N = DV / 16;                     // 16-column tiles of the output
-    constexpr int PIECE = 16 / sizeof(T);          // columns of a 16-byte load
-    constexpr int KC = DK / PIECE, VC = LATENT ? 0 : DV / PIECE;
-    constexpr int NK = (KEYS * KC + kBlock - 1) / kBlock;
-    constexpr int NV = (KEYS * VC + kBlock - 1) / kBlock;
+    constexpr int DEPTHS = (DK + 31) / 32;         // product depths of a key row
+    constexpr int U = (DEPTHS + SPLIT - 1) / SPLIT;  // of them a wave's
+    constexpr int N = DV / 16 / SPLIT;             // the wave's 16-column tiles of the output
+    using Load = Loads<T, DK, KEYS, WAVES>;        // values are as wide, or the keys
     __shared__ __attribute__((aligned(16))) uint16_t lds[S::STAGES * S::STAGE];
-    __shared__ unsigned long long flags[3];
+    __shared__ v4f partial[SPLIT > 1 ? WAVES * GROUPS * NB * 64 : 1];
+    __shared__ uint32_t flags[3][2];  // keys of a tile that are marked, by bit
 
     const uint32_t lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15;
-    const uint32_t wave = scalar(threadIdx.x >> 6);
+    const uint32_t wave = scalar(threadIdx.x >> 6), split = wave % SPLIT;
+    const uint32_t wave_row = 16 * GROUPS * (wave / SPLIT);  // the wave's first of the item's
     const uint32_t page_shift = p.shape.page_shift, in_page = p.shape.page_size() - 1;
+    // The lane's places in a load: bytes from its first key's row, and elements in LDS,
+    // which are held where they are few.
+    constexpr uint32_t PER_ROW = DK / Load::PIECE;
+    constexpr bool HELD = Load::MINE <= 5;
+    uint32_t load_at[Load::CHUNKS % 64 ? Load::MINE : 1], store_held[HELD ? Load::MINE : 1];
+    const auto place = [&](int i, uint32_t me) {
+        const uint32_t n = Load::number(i, wave), c = Load::chunk(n, me);
+        const uint32_t row = c / PER_ROW, piece = c - row * PER_ROW;
+        return (8 * (n / Load::EACH) + row) * kPitch<DK> + piece * Load::PIECE;
+    };
+    const auto store_at = [&](int i) {
+        return HELD ? store_held[HELD ? i : 0] : place(i, formed_here(lane));
+    };
+    load_at[0] = lane * 16;
+#pragma unroll
+    for (int i = 0; i < Load::MINE; ++i) {
+        if (Load::CHUNKS % 64)
+            load_at[i] = Load::chunk(Load::number(i, wave), lane) * 16;
+        if (HELD)
+            store_held[i] = place(i, lane);
+    }
     Line line;
     const bool any = find_line<SHIFT>(p, line);
     Share share = {};
     Part part;
     while (any && next_part<SHIFT>(p, line, part)) {
-        const uint32_t rows = part.run.count * p.group, row0 = kRows * part.row_tile;
-        const uint32_t row = row0 + 16 * wave + j;
-        const bool real = row < rows;
-        const uint32_t token = (real ? row : rows - 1) / p.group;  // of the run
-        const uint32_t head = part.kv_head * p.group + (real ? row : rows - 1) - token * p.group;
-        const uint64_t query_row = uint64_t(part.run.begin + token) * p.query_heads + head;
-        if (part.run.length == UINT32_MAX) {
-            if (part.opens && real)
-                for (uint32_t c = q; c < uint32_t(DV); c += 4)
-                    p.out[query_row * DV + c] = __builtin_nanf("");
-            continue;
+        const uint32_t rows = part.run.count * p.group, row0 = ROWS * part.row_tile;
+        const bool active = row0 + wave_row < rows;
+        bool real[GROUPS];
+        uint32_t token[GROUPS];      // of the run
+        uint64_t query_row[GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            uint32_t row = row0 + wave_row + 16 * g + j;
+            real[g] = row < rows;
+            row = real[g] ? row : rows - 1;
+            token[g] = row / p.group;
+            query_row[g] = uint64_t(part.run.begin + token[g]) * p.query_heads +
+                           part.kv_head * p.group + row - token[g] * p.group;
+            if (part.run.length == UINT32_MAX && part.opens && real[g])
+                for (uint32_t c = q + 4 * split; c < uint32_t(DV); c += 4 * SPLIT)
+                    p.out[query_row[g] * DV + c] = __builtin_nanf("");
         }
+        if (part.run.length == UINT32_MAX)
+            continue;
         if (!part.counts)
             continue;
         const float *table = p.tables + uint64_t(part.sequence) * p.max_pages;
         const uint32_t last_key = part.keys - 1, length = part.run.length;
-        const T *keys = static_cast<const T *>(p.key_pages);
-        const T *values = static_cast<const T *>(p.value_pages);
+        const uint64_t head_bytes =
+            (uint64_t(part.kv_head) << page_shift) * DK * sizeof(T);
+        const uint64_t page_bytes = p.shape.stride() * sizeof(T);
 
-        // A tile's page ids, lane r key r's; keys past the end are the last one.
-        const auto load_id = [&](uint32_t tile) {
-            const uint32_t key = tile * KEYS + (lane & (KEYS - 1));
-            return table[(key < last_key ? key : last_key) >> page_shift];
+        // The first key of a load, in the last eight with a key where it is past them.
+        const auto key_of = [&](uint32_t tile, int i) {
+            const uint32_t key = tile * KEYS + 8 * (Load::number(i, wave) / Load::EACH);
+            return key <= last_key ? key : last_key & ~7u;
         };
-        v4u key_reg[NK], value_reg[NV ? NV : 1];
-        uint64_t bad_pages = 0;
-        const auto load_tile = [&](uint32_t tile, float id) {
-            const bool ok = valid_index(id, p.shape.pages);
-            bad_pages = __ballot(!ok);
-            if (KEYS < 64)
-                bad_pages &= (uint64_t(1) << (KEYS & 63)) - 1;
-            const uint32_t page = ok ? uint32_t(id) : 0;
-            const auto at = [&](const T *pages, uint32_t key_row, uint32_t chunk, uint32_t width) {
-                const uint32_t key = tile * KEYS + key_row;
-                const uint32_t slot = (key < last_key ? key : last_key) & in_page;
-                const uint64_t base = uint64_t(uint32_t(__shfl(page, int(key_row), 64))) *
-                                          p.shape.stride() +
-                                      (uint64_t(part.kv_head) << page_shift) * width;
-                return reinterpret_cast<const v4u *>(pages + base + slot * width + chunk * PIECE);
-            };
+        // A tile's page ids, lane i the one of the wave's load i: a vector load, for a scalar
+        // one would be waited for with every LDS access.
+        float ids;
+        const auto load_ids = [&](uint32_t tile) {
+            const uint32_t i = lane < uint32_t(Load::MINE) ? lane : Load::MINE - 1;
+            ids = table[key_of(tile, int(i)) >> page_shift];
+        };
+        v4u key_reg[Load::MINE], value_reg[LATENT ? 1 : Load::MINE];
+        uint32_t bad = 0;  // loads of the tile whose page is none
+        const auto load_tile = [&](uint32_t tile) {
+            bad = 0;
 #pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                uint32_t n = threadIdx.x + i * kBlock;
-                if ((i + 1) * kBlock > KEYS * KC)
-                    n = n < uint32_t(KEYS * KC) ? n : KEYS * KC - 1;
-                key_reg[i] = __builtin_nontemporal_load(at(keys, n / KC, n % KC, DK));
+            for (int i = 0; i < Load::MINE; ++i) {
+                const float id = __uint_as_float(
+                    uint32_t(__builtin_amdgcn_readlane(__float_as_int(ids), i)));
+                const bool ok = valid_index(id, p.shape.pages);
+                bad |= ok ? 0 : 1u << i;
+                const uint32_t page = scalar(ok ? uint32_t(id) : 0);
+                uint64_t at = page * page_bytes + head_bytes +
+                              (key_of(tile, i) & in_page) * uint32_t(DK * sizeof(T));
+                if (Load::CHUNKS % 64 == 0)
+                    at += Load::number(i, wave) % Load::EACH * 1024;
+                const uint32_t lane_at = load_at[Load::CHUNKS % 64 ? i : 0];
+                key_reg[i] = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(
+                    static_cast<const char *>(p.key_pages) + at + lane_at));
+                if constexpr (!LATENT)
+                    value_reg[i] = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(
+                        static_cast<const char *>(p.value_pages) + at + lane_at));
             }
-            if constexpr (!LATENT)
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    uint32_t n = threadIdx.x + i * kBlock;
-                    if ((i + 1) * kBlock > KEYS * VC)
-                        n = n < uint32_t(KEYS * VC) ? n : KEYS * VC - 1;
-                    value_reg[i] = __builtin_nontemporal_load(at(values, n / VC, n % VC, DV));
-                }
         };
-        // 16 loaded bytes into the operand planes.  In a tile of the run, what is not finite
-        // becomes zero and its key is marked: only rows that attend it shall see it.
-        const auto store_piece = [&](v4u x, uint16_t *plane, int plane_size, uint32_t key_row,
-                                     uint32_t chunk, auto width, bool of_run, uint32_t turn) {
-            constexpr int D = width;
-            if (of_run) {
+        // 16 loaded bytes into the operand planes.  In a tile that not every row attends whole,
+        // what is not finite becomes zero and its key is marked: only rows that attend it
+        // shall see it.
+        const auto store_piece = [&](v4u x, uint16_t *to, int plane, uint32_t at, bool mixed,
+                                     uint32_t turn) {
+            if (mixed) {
                 bool odd = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -623,259 +668,356 @@ void run_attention_kernel(RunAttention p)
                         x[e] = all ? 0 : x[e];
                     }
                 }
-                if (odd)
-                    atomicOr(&flags[turn], 1ull << key_row);
+                if (odd) {
+                    const uint32_t key = formed_here(at) / kPitch<DK>;
+                    atomicOr(&flags[turn][key / 32], 1u << key % 32);
+                }
             }
             if constexpr (HALF) {
-                *reinterpret_cast<v4u *>(plane + swizzled<D>(key_row, chunk)) = x;
+                *reinterpret_cast<v4u *>(to) = x;
             } else {
                 uint32_t a[PARTS], b[PARTS];
                 split_pair<HALF>(__uint_as_float(x[0]), __uint_as_float(x[1]), a);
                 split_pair<HALF>(__uint_as_float(x[2]), __uint_as_float(x[3]), b);
-                uint16_t *to = plane + swizzled<D>(key_row, chunk / 2) + chunk % 2 * 4;
 #pragma unroll
                 for (int i = 0; i < PARTS; ++i)
-                    *reinterpret_cast<v2u *>(to + i * plane_size) = v2u{a[i], b[i]};
+                    *reinterpret_cast<v2u *>(to + i * plane) = v2u{a[i], b[i]};
             }
         };
-        const auto store_tile = [&](uint16_t *stage, bool of_run, uint32_t turn) {
+        const auto store_tile = [&](uint16_t *stage, bool mixed, uint32_t turn) {
 #pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                uint32_t n = threadIdx.x + i * kBlock;
-                if ((i + 1) * kBlock > KEYS * KC)
-                    n = n < uint32_t(KEYS * KC) ? n : KEYS * KC - 1;
-                store_piece(key_reg[i], stage, S::KEY_PLANE, n / KC, n % KC,
-                            std::integral_constant<int, DK>{}, of_run, turn);
+            for (int i = 0; i < Load::MINE; ++i) {
+                const uint32_t first = 8 * (Load::number(i, wave) / Load::EACH);
+                if (bad >> i & 1 && lane == 0)
+                    atomicOr(&flags[turn][first / 32], formed_here(0xff) << first % 32);
+                const uint32_t to = store_at(i);
+                store_piece(key_reg[i], stage + to, S::KEY_PLANE, to, mixed, turn);
+                if constexpr (!LATENT)
+                    store_piece(value_reg[i], stage + PARTS * S::KEY_PLANE + to, S::VALUE_PLANE,
+                                to, mixed, turn);
             }
-            if constexpr (!LATENT)
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    uint32_t n = threadIdx.x + i * kBlock;
-                    if ((i + 1) * kBlock > KEYS * VC)
-                        n = n < uint32_t(KEYS * VC) ? n : KEYS * VC - 1;
-                    store_piece(value_reg[i], stage + PARTS * S::KEY_PLANE, S::VALUE_PLANE,
-                                n / VC, n % VC, std::integral_constant<int, DV>{}, of_run, turn);
-                }
         };
 
-        float id = load_id(part.first);
-        // The wave's queries; rows past the run's are zero.
-        float qf[U][8];
+        load_ids(part.first);
+        // The wave's queries, in parts; rows past the run's are zero.
+        v4u query[GROUPS][U][QP];
+        float factor[GROUPS];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const uint32_t column = 32 * u + 8 * q + e;
-                const float *from;
-                if (LATENT && 32 * u >= DV)
-                    from = p.rotary_query + query_row * (DK - DV) + column - DV;
-                else
-                    from = p.query + query_row * DV + (column < uint32_t(DV) ? column : 0);
+        for (int g = 0; g < GROUPS; ++g) {
+            const float *at = p.query + query_row[g] * DV;
+            const auto load = [&](int u, int e) {
+                const uint32_t column = 32 * (split * U + u) + 8 * q + e;
+                const float *from = at + (column < uint32_t(DV) ? column : 0);
+                if (LATENT && column >= uint32_t(DV))
+                    from = p.rotary_query + query_row[g] * (DK - DV) +
+                           (column < uint32_t(DK) ? column - DV : 0);
                 const v4f piece = *reinterpret_cast<const v4f *>(from);
+                const bool mine = real[g] && column < uint32_t(DK);
+                return mine ? piece : v4f{0, 0, 0, 0};
+            };
+            factor[g] = p.scale;
+            int exponent = 0;
+            if (HALF) {
+                float most = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    qf[u][e + i] = real && column < uint32_t(DK) ? piece[i] : 0.0f;
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const v4f x = load(u, e);
+                        most = fmaxf(fmaxf(most, fmaxf(fabsf(x[0]), fabsf(x[1]))),
+                                     fmaxf(fabsf(x[2]), fabsf(x[3])));
+                    }
+                most = quad_max(most);
+                // 2^14 <= most 2^exponent < 2^15 (0 and infinities as they are; below
+                // 2^-86, where no score differs from 0, by 2^100, so that the factor stays
+                // normal).
+                if (most > 0.0f && most < __builtin_inff())
+                    exponent = 15 - (ilogbf(most) + 1);
+                exponent = exponent < 100 ? exponent : 100;
+                factor[g] = ldexpf(p.scale, -exponent);
+                // Read a second time rather than held: the registers are the tile's.
+                at += formed_here(0);
             }
-        if (part.first < part.last) {
-            load_tile(part.first, id);
-            id = load_id(part.first + 1 < part.last ? part.first + 1 : part.first);
-        }
-        float factor = p.scale;
-        int exponent = 0;
-        if (HALF) {
-            float most = 0.0f;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    most = fmaxf(most, fabsf(qf[u][e]));
-            most = quad_max(most);
-            // 2^14 <= most 2^exponent < 2^15 (0 and infinities as they are).
-            if (most > 0.0f && most < __builtin_inff())
-                exponent = 15 - (ilogbf(most) + 1);
-            factor = ldexpf(p.scale, -exponent);
+                for (int e = 0; e < 8; e += 4) {
+                    v4f x = load(u, e);
+#pragma unroll
+                    for (int i = 0; HALF && i < 4; ++i)
+                        x[i] = ldexpf(x[i], exponent);
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        uint32_t parts[QP];
+                        split_pair<HALF>(x[i], x[i + 1], parts);
+#pragma unroll
+                        for (int part = 0; part < QP; ++part)
+                            query[g][u][part][(e + i) / 2] = parts[part];
+                    }
+                }
         }
-        v4u query[U][QP];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float a = qf[u][2 * e], b = qf[u][2 * e + 1];
-                if (HALF)
-                    a = ldexpf(a, exponent), b = ldexpf(b, exponent);
-                uint32_t parts[QP];
-                split_pair<HALF>(a, b, parts);
-#pragma unroll
-                for (int i = 0; i < QP; ++i)
-                    query[u][i][e] = parts[i];
-            }
+        if (part.first < part.last) {
+            load_tile(part.first);
+            load_ids(part.first + 1 < part.last ? part.first + 1 : part.first);
+        }
 
-        v4f o[N];
+        v4f o[GROUPS][N];
+        float m[GROUPS], l[GROUPS];
+        bool poison[GROUPS];
 #pragma unroll
-        for (int t = 0; t < N; ++t)
-            o[t] = v4f{0, 0, 0, 0};
-        float m = -__builtin_inff(), l = 0.0f;
-        bool poison = false;
-        const uint8_t *mask = p.mask + uint64_t(part.run.begin + token) * p.mask_bytes;
+        for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+                o[g][t] = v4f{0, 0, 0, 0};
+            m[g] = -__builtin_inff();
+            l[g] = 0.0f;
+            poison[g] = false;
+        }
+        // Every row attends the keys before this one.
+        const uint32_t common = length + (p.mask ? 0 : row0 / p.group + 1);
         uint32_t turn = 0;
         __syncthreads();  // an earlier part's tiles and marks have been read
-        if (threadIdx.x < 3)
-            flags[threadIdx.x] = 0;
+        if (threadIdx.x < 6)
+            flags[threadIdx.x / 2][threadIdx.x % 2] = 0;
         __syncthreads();
 #pragma unroll 1
         for (uint32_t tile = part.first; tile < part.last; ++tile) {
             const uint32_t k0 = tile * KEYS;
-            const bool of_run = k0 + KEYS > length;
+            const bool mixed = k0 + KEYS > common;
             uint16_t *stage = lds + (S::STAGES == 2 && (tile & 1) ? S::STAGE : 0);
             if (S::STAGES == 1)
                 __syncthreads();  // the tile before has been read
-            store_tile(stage, of_run, turn);
-            uint64_t marks = bad_pages;
+            store_tile(stage, mixed, turn);
             if (tile + 1 < part.last) {
-                load_tile(tile + 1, id);
-                id = load_id(tile + 2 < part.last ? tile + 2 : tile + 1);
+                load_tile(tile + 1);
+                load_ids(tile + 2 < part.last ? tile + 2 : tile + 1);
             }
             __syncthreads();
-            if (of_run)
-                marks |= flags[turn];
+            const uint64_t marks = uint64_t(flags[turn][1]) << 32 | flags[turn][0];
             // The mark after the next one: no thread is past the next barrier.
             turn = turn == 2 ? 0 : turn + 1;
-            if (threadIdx.x == 0)
-                flags[turn == 2 ? 0 : turn + 1] = 0;
-            if (row0 + 16 * wave >= rows)
-                continue;
+            if (threadIdx.x < 2)
+                flags[turn == 2 ? 0 : turn + 1][threadIdx.x] = 0;
 
-            v4f s[NB];
+            v4f s[GROUPS][NB];
+            if (active) {
+                const uint32_t me = formed_here(lane);
+                const uint16_t *key_stage = stage + (me & 15) * kPitch<DK> + 8 * (me >> 4);
+                // f32 caches: the largest product apart from the others, whose sums it would
+                // round.
+                v4f rest[GROUPS][HALF ? 1 : NB];
 #pragma unroll
-            for (int c = 0; c < NB; ++c)
-                s[c] = v4f{0, 0, 0, 0};
+                for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                    for (int c = 0; c < NB; ++c)
+                        s[g][c] = rest[g][HALF ? 0 : c] = v4f{0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < NB; ++c) {
-                    uint32_t chunk = 4 * u + q;
+                for (int u = 0; u < U; ++u) {
                     // Past the row's end a lane reads columns that the query's zeros drop.
+                    uint32_t depth = split * U + u;
+                    if (DEPTHS % SPLIT != 0 && depth >= uint32_t(DEPTHS))
+                        depth = DEPTHS - 1;
+                    const uint16_t *from = key_stage + 32 * depth;
                     if (DK % 32 != 0 && u == U - 1 && q >= 2)
-                        chunk -= 2;
-                    v4u k[PARTS];
+                        from -= 16;
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i)
-                        k[i] = *reinterpret_cast<const v4u *>(stage + i * S::KEY_PLANE +
-                                                              swizzled<DK>(16 * c + j, chunk));
-                    s[c] = products<HALF>(k, query[u], s[c]);
-                }
-            float top = -__builtin_inff();
-            if (of_run || marks) {
-                const int first = int(k0) - int(length);  // the run's token at key 0
+                    for (int c = 0; c < NB; ++c)
 #pragma unroll
-                for (int c = 0; c < NB; ++c)
+                        for (int i = PARTS - 1; i >= 0; --i) {
+                            const v4u k = *reinterpret_cast<const v4u *>(
+                                from + 16 * c * kPitch<DK> + i * S::KEY_PLANE);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t at = 16 * c + 4 * q + r;
-                        const int i = first + int(at);
-                        bool seen = k0 + at <= last_key;
-                        if (p.mask) {
-                            if (i >= 0)
-                                seen = seen && uint32_t(i) < 8 * p.mask_bytes &&
-                                       (mask[uint32_t(i) >> 3] >> (i & 7) & 1);
-                        } else {
-                            seen = seen && i <= int(token);
+                            for (int b = (HALF ? 1 : 2) - i; b >= 0; --b)
+#pragma unroll
+                                for (int g = 0; g < GROUPS; ++g)
+                                    if (HALF || i + b == 0)
+                                        s[g][c] = mfma<HALF>(k, query[g][u][b], s[g][c]);
+                                    else
+                                        rest[g][HALF ? 0 : c] =
+                                            mfma<HALF>(k, query[g][u][b], rest[g][HALF ? 0 : c]);
                         }
-                        poison |= seen && (marks >> at & 1);
-                        s[c][r] = seen ? s[c][r] * factor : -__builtin_inff();
-                        top = fmaxf(top, s[c][r]);
+                }
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+                    for (int c = 0; c < NB; ++c) {
+                        if (!HALF)
+                            s[g][c] += rest[g][c];
+                        if (SPLIT > 1) {
+                            s[g][c] *= factor[g];
+                            partial[((wave * GROUPS + g) * NB + c) * 64 + lane] = s[g][c];
+                        }
                     }
-            } else {
+            }
+            if (SPLIT > 1) {
+                // The same sum, in the same order, in every wave of a row.
+                __syncthreads();
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+                    for (int c = 0; c < NB; ++c)
+#pragma unroll
+                        for (int w = 0; w < SPLIT; ++w) {
+                            const v4f x =
+                                partial[(((wave - split + w) * GROUPS + g) * NB + c) * 64 + lane];
+                            s[g][c] = w ? s[g][c] + x : x;
+                        }
+            }
+            if (!active)
+                continue;
+            const int first = int(k0) - int(length);  // the run's token at key 0
+            const int last = int(last_key - k0);
+            if (mixed) {
+                const uint32_t q4 = 4 * formed_here(q);
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    // Bit 4 c + r: whether the row attends key 16 c + 4 q + r.
+                    uint32_t seen = 0;
+                    if (p.mask) {
+                        const uint8_t *mask =
+                            p.mask + uint64_t(part.run.begin + token[g]) * p.mask_bytes;
+#pragma unroll
+                        for (int c = 0; c < NB; ++c)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int at = 16 * c + int(q4) + r, i = first + at;
+                                uint32_t bit = at <= last;
+                                if (i >= 0 && at <= last)
+                                    bit = uint32_t(i) < 8 * p.mask_bytes
+                                              ? mask[uint32_t(i) >> 3] >> (i & 7) & 1
+                                              : 0;
+                                seen |= bit << (4 * c + r);
+                            }
+                    } else {
+                        const int most = int(token[g]) - first;
+#pragma unroll
+                        for (int c = 0; c < NB; ++c)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                seen |= uint32_t(16 * c + int(q4) + r <= most) << (4 * c + r);
+                    }
+                    if (marks) {
+                        uint32_t mine = 0;
+#pragma unroll
+                        for (int c = 0; c < NB; ++c)
+                            mine |= uint32_t(marks >> (16 * c + q4) & 15) << (4 * c);
+                        poison[g] |= (seen & mine) != 0;
+                    }
+#pragma unroll
+                    for (int c = 0; c < NB; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            s[g][c][r] =
+                                seen >> (4 * c + r) & 1 ? s[g][c][r] : -__builtin_inff();
+                }
+            } else if (marks) {
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+                    poison[g] = true;
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const float times = SPLIT > 1 ? 1.0f : factor[g];
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        top = fmaxf(top, s[g][c][r]);
+                top = fmaxf(m[g], quad_max(top) * times);
+                // While every score is -infinity, nothing is added.
+                const float base = top == -__builtin_inff() ? 0.0f : top;
+                if (__any(top > m[g])) {
+                    const float rescale = __builtin_amdgcn_exp2f(m[g] - base);
+                    l[g] *= rescale;
+#pragma unroll
+                    for (int t = 0; t < N; ++t)
+                        o[g][t] *= rescale;
+                    m[g] = top;
+                }
+                const float line_at = HALF ? base - kProbabilityShift : base;
 #pragma unroll
                 for (int c = 0; c < NB; ++c)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        s[c][r] *= factor;
-                        top = fmaxf(top, s[c][r]);
+                        s[g][c][r] =
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][c][r], times, -line_at));
+                        l[g] += s[g][c][r];
                     }
             }
-            top = fmaxf(m, quad_max(top));
-            // While every score is -infinity, nothing is added.
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            if (__any(top > m)) {
-                const float rescale = __builtin_amdgcn_exp2f(m - base);
-                l *= rescale;
-#pragma unroll
-                for (int t = 0; t < N; ++t)
-                    o[t] *= rescale;
-                m = top;
-            }
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[c][r] =
-                        __builtin_amdgcn_exp2f(s[c][r] - (HALF ? base - kProbabilityShift : base));
-                    l += s[c][r];
-                }
-            const uint16_t *value_stage = LATENT ? stage : stage + PARTS * S::KEY_PLANE;
-            constexpr int VALUE_PLANE = LATENT ? S::KEY_PLANE : S::VALUE_PLANE;
+            const uint32_t me = formed_here(lane);
+            const uint16_t *value_stage = stage + (LATENT ? 0 : PARTS * S::KEY_PLANE) +
+                                          4 * (me >> 4) * kPitch<DK> + split * (DV / SPLIT);
+            const uint32_t column = me & 15;
 #pragma unroll
             for (int h = 0; h < NB / 2; ++h) {  // 32 keys, a product's depth
-                v4u prob[QP];
+                v4u prob[GROUPS][QP];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t parts[QP];
-                    split_pair<HALF>(s[2 * h + e / 2][2 * (e % 2)],
-                                     s[2 * h + e / 2][2 * (e % 2) + 1], parts);
+                for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-                    for (int i = 0; i < QP; ++i)
-                        prob[i][e] = parts[i];
-                }
-                for_chunks<N>([&](auto first_tile, auto tiles) {
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t parts[QP];
+                        split_pair<HALF>(s[g][2 * h + e / 2][2 * (e % 2)],
+                                         s[g][2 * h + e / 2][2 * (e % 2) + 1], parts);
+#pragma unroll
+                        for (int i = 0; i < QP; ++i)
+                            prob[g][i][e] = parts[i];
+                    }
+                for_chunks<N, S::CHUNK>([&](auto first_tile, auto tiles) {
                     constexpr int t0 = first_tile, n = tiles, W = (n + 1) / 2;
-                    uint32_t x[PARTS][8][W];
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i)
+                    for (int i = PARTS - 1; i >= 0; --i) {
+                        uint32_t x[8][W];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const uint32_t key = 32 * h + 16 * (e / 4) + 4 * q + e % 4;
-                            // Columns 16 t0 + n j .. + n - 1.
-                            const uint16_t *from = value_stage + i * VALUE_PLANE +
-                                                   swizzled<DK>(key, 2 * t0 + n * j / 8) +
-                                                   n * j % 8;
+                            // Columns 16 t0 + n j .. + n - 1 of the wave's, of the key
+                            // 32 h + 16 (e / 4) + 4 q + e % 4.
+                            const uint16_t *from =
+                                value_stage + i * S::KEY_PLANE +
+                                (32 * h + 16 * (e / 4) + e % 4) * kPitch<DK> + 16 * t0 +
+                                n * column;
                             if constexpr (n == 8) {
                                 const v4u piece = *reinterpret_cast<const v4u *>(from);
-                                x[i][e][0] = piece[0], x[i][e][1] = piece[1];
-                                x[i][e][2] = piece[2], x[i][e][3] = piece[3];
+                                x[e][0] = piece[0], x[e][1] = piece[1];
+                                x[e][2] = piece[2], x[e][3] = piece[3];
                             } else if constexpr (n == 4) {
                                 const v2u piece = *reinterpret_cast<const v2u *>(from);
-                                x[i][e][0] = piece[0], x[i][e][1] = piece[1];
+                                x[e][0] = piece[0], x[e][1] = piece[1];
                             } else if constexpr (n == 2) {
-                                x[i][e][0] = *reinterpret_cast<const uint32_t *>(from);
+                                x[e][0] = *reinterpret_cast<const uint32_t *>(from);
                             } else {
-                                x[i][e][0] = *from;
+                                x[e][0] = *from;
                             }
                         }
 #pragma unroll
-                    for (int t = 0; t < n; ++t) {
-                        v4u v[PARTS];
-#pragma unroll
-                        for (int i = 0; i < PARTS; ++i)
+                        for (int t = 0; t < n; ++t) {
+                            v4u v;
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                v[i][e] = __builtin_amdgcn_perm(
-                                    x[i][2 * e + 1][t / 2], x[i][2 * e][t / 2],
-                                    t % 2 ? 0x07060302u : 0x05040100u);
-                        o[t0 + t] = products<HALF>(v, prob, o[t0 + t]);
+                                v[e] = __builtin_amdgcn_perm(x[2 * e + 1][t / 2], x[2 * e][t / 2],
+                                                             t % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                            for (int b = (HALF ? 1 : 2) - i; b >= 0; --b)
+#pragma unroll
+                                for (int g = 0; g < GROUPS; ++g)
+                                    o[g][t0 + t] = mfma<HALF>(v, prob[g][b], o[g][t0 + t]);
+                        }
                     }
                 });
             }
         }
 
-        l = quad_sum(poison ? __builtin_nanf("") : l);
-        if (real) {
-            float *to = part.whole
-                            ? p.out + query_row * DV
-                            : p.records + (uint64_t(part.record) * kRows + 16 * wave + j) * DV;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const float total = quad_sum(poison[g] ? __builtin_nanf("") : l[g]);
+            if (!real[g])
+                continue;
+            const uint64_t record = uint64_t(part.record) * ROWS + wave_row + 16 * g + j;
+            float *to = (part.whole ? p.out + query_row[g] * DV : p.records + record * DV) +
+                        split * (DV / SPLIT);
             // Nothing attended: zeros.
-            const float scale = !part.whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            for_chunks<N>([&](auto first_tile, auto tiles) {
+            const float scale = !part.whole ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+            for_chunks<N, S::CHUNK>([&](auto first_tile, auto tiles) {
                 constexpr int t0 = first_tile, n = tiles;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -884,18 +1026,17 @@ void run_attention_kernel(RunAttention p)
 #pragma unroll
                         for (int t = 0; t < n; t += 4)
                             *reinterpret_cast<v4f *>(at + t) =
-                                v4f{o[t0 + t][r], o[t0 + t + 1][r], o[t0 + t + 2][r],
-                                    o[t0 + t + 3][r]} * scale;
+                                v4f{o[g][t0 + t][r], o[g][t0 + t + 1][r], o[g][t0 + t + 2][r],
+                                    o[g][t0 + t + 3][r]} * scale;
                     } else {
 #pragma unroll
                         for (int t = 0; t < n; ++t)
-                            at[t] = o[t0 + t][r] * scale;
+                            at[t] = o[g][t0 + t][r] * scale;
                     }
                 }
             });
-            if (!part.whole && q == 0)
-                reinterpret_cast<v2f *>(record_stats(p))[uint64_t(part.record) * kRows +
-                                                         16 * wave + j] = v2f{m, l};
+            if (!part.whole && q == 0 && split == 0)
+                reinterpret_cast<v2f *>(record_stats(p))[record] = v2f{m[g], total};
         }
         if (part.leads && !part.whole)
             share = {block_of(line, part.last_unit) - line.block + 1, part.record, part.run.begin,
@@ -912,14 +1053,14 @@ __global__ __launch_bounds__(kBlock) void run_attention_join_kernel(RunAttention
 {
     const Share share = block_shares(p)[blockIdx.x];
     const uint32_t in_tile = blockIdx.y * (kBlock / 64) + (threadIdx.x >> 6);
-    const uint32_t row = kRows * share.row_tile + in_tile;
+    const uint32_t row = p.rows * share.row_tile + in_tile;
     if (!share.count || row >= share.run * p.group)
         return;
     const uint32_t lane = threadIdx.x & 63, d = p.value_dim, pieces = d / 4;
     const uint32_t token = row / p.group, head = share.kv_head * p.group + row - token * p.group;
     float *out = p.out + (uint64_t(share.begin + token) * p.query_heads + head) * d;
     const auto record = [&](uint32_t i) {
-        return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * kRows + in_tile;
+        return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * p.rows + in_tile;
     };
     const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
     float most = -__builtin_inff();
@@ -966,45 +1107,67 @@ __global__ __launch_bounds__(kBlock) void run_attention_join_kernel(RunAttention
     }
 }
 
-// The kernel of a shape (null: none), the blocks of it that a CU holds, a tile's keys.
+// The kernel of a shape (null: none), its threads and rows of an item, the blocks of it that
+// a CU holds, a tile's keys.
 struct MatrixKernel {
     void (*run)(RunAttention) = nullptr;
-    int resident = 0, shift = 0;
+    int threads = 0, rows = 0, resident = 0, shift = 0;
 };
-template <int DK, int DV, bool LATENT>
-MatrixKernel matrix_kernel_of(bool half)
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
+MatrixKernel matrix_kernel_with()
+{
+    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>;
+    return {run_attention_kernel<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>, S::THREADS, S::ROWS,
+            S::RESIDENT, S::SHIFT};
+}
+// `many`: more rows than one item of the smaller kind has, on average over the sequences.
+template <int D>
+MatrixKernel matrix_kernel_of(bool half, bool many)
+{
+    constexpr bool WIDE = D > 128;
+    if (half)
+        return many && !WIDE ? matrix_kernel_with<D, D, true, false, 4, 1, WIDE ? 1 : 2>()
+                             : matrix_kernel_with<D, D, true, false, 4, 1, 1>();
+    // Three parts of a wide row need the registers of two waves.
+    constexpr int SPLIT = D < 128 ? 1 : 2;
+    return matrix_kernel_with<D, D, false, false, 4 * SPLIT, SPLIT, 1>();
+}
+template <int RANK, int ROPE>
+MatrixKernel latent_kernel_of(bool half, bool many)
 {
     if (half)
-        return {run_attention_kernel<DK, DV, true, LATENT>, Shape<DK, DV, true, LATENT>::RESIDENT,
-                Shape<DK, DV, true, LATENT>::SHIFT};
-    return {run_attention_kernel<DK, DV, false, LATENT>, Shape<DK, DV, false, LATENT>::RESIDENT,
-            Shape<DK, DV, false, LATENT>::SHIFT};
+        return many ? matrix_kernel_with<RANK + ROPE, RANK, true, true, 8, 2, 1>()
+                    : matrix_kernel_with<RANK + ROPE, RANK, true, true, 8, 4, 1>();
+    return matrix_kernel_with<RANK + ROPE, RANK, false, true, 8, 4, 1>();
 }
 MatrixKernel matrix_kernel(const RunAttention &p)
 {
     const bool half = p.shape.half;
     const uint32_t rope = p.shape.head_dim - p.value_dim;
+    const uint64_t rows = uint64_t(p.runs.tokens) * p.group;
     if (rope == 0) {
+        const bool many = rows > 64 * uint64_t(p.runs.sequences);
         switch (p.value_dim) {
-        case 32: return matrix_kernel_of<32, 32, false>(half);
-        case 64: return matrix_kernel_of<64, 64, false>(half);
-        case 80: return matrix_kernel_of<80, 80, false>(half);
-        case 96: return matrix_kernel_of<96, 96, false>(half);
-        case 112: return matrix_kernel_of<112, 112, false>(half);
-        case 128: return matrix_kernel_of<128, 128, false>(half);
-        case 160: return matrix_kernel_of<160, 160, false>(half);
-        case 192: return matrix_kernel_of<192, 192, false>(half);
-        case 256: return matrix_kernel_of<256, 256, false>(half);
+        case 32: return matrix_kernel_of<32>(half, many);
+        case 64: return matrix_kernel_of<64>(half, many);
+        case 80: return matrix_kernel_of<80>(half, many);
+        case 96: return matrix_kernel_of<96>(half, many);
+        case 112: return matrix_kernel_of<112>(half, many);
+        case 128: return matrix_kernel_of<128>(half, many);
+        case 160: return matrix_kernel_of<160>(half, many);
+        case 192: return matrix_kernel_of<192>(half, many);
+        case 256: return matrix_kernel_of<256>(half, many);
         default: return {};
         }
     }
+    const bool many = rows > 32 * uint64_t(p.runs.sequences);
     switch (p.value_dim * 1024 + rope) {
-    case 128 * 1024 + 32: return matrix_kernel_of<160, 128, true>(half);
-    case 128 * 1024 + 64: return matrix_kernel_of<192, 128, true>(half);
-    case 256 * 1024 + 32: return matrix_kernel_of<288, 256, true>(half);
-    case 256 * 1024 + 64: return matrix_kernel_of<320, 256, true>(half);
-    case 512 * 1024 + 32: return matrix_kernel_of<544, 512, true>(half);
-    case 512 * 1024 + 64: return matrix_kernel_of<576, 512, true>(half);
+    case 128 * 1024 + 32: return latent_kernel_of<128, 32>(half, many);
+    case 128 * 1024 + 64: return latent_kernel_of<128, 64>(half, many);
+    case 256 * 1024 + 32: return latent_kernel_of<256, 32>(half, many);
+    case 256 * 1024 + 64: return latent_kernel_of<256, 64>(half, many);
+    case 512 * 1024 + 32: return latent_kernel_of<512, 32>(half, many);
+    case 512 * 1024 + 64: return latent_kernel_of<512, 64>(half, many);
     default: return {};
     }
 }
@@ -1020,10 +1183,11 @@ bool run_attention_plan(RunAttention &p, int cu_count)
     const MatrixKernel kernel = matrix_kernel(p);
     if (!kernel.run || !rows || !p.runs.sequences)
         return true;
+    p.rows = kernel.rows;
     // Units stay in 32 bits.
-    const uint64_t items = (uint64_t(p.runs.tokens) * p.group / kRows + p.runs.sequences) *
+    const uint64_t items = (uint64_t(p.runs.tokens) * p.group / p.rows + p.runs.sequences) *
                            p.shape.kv_heads;
-    const uint64_t most = items * (kItemUnits + 4 + ((uint64_t(p.longest) + p.runs.tokens) >>
+    const uint64_t most = items * (kItemUnits + 6 + ((uint64_t(p.longest) + p.runs.tokens) >>
                                                      kernel.shift));
     if (most >= uint64_t(1) << 31)
         return false;
@@ -1035,15 +1199,16 @@ bool run_attention_plan(RunAttention &p, int cu_count)
 
 size_t run_attention_scratch_bytes(const RunAttention &p)
 {
-    return size_t(p.blocks) * (2 * size_t(kRows) * (p.value_dim + 2) * sizeof(float) +
+    return size_t(p.blocks) * (2 * size_t(p.rows) * (p.value_dim + 2) * sizeof(float) +
                                sizeof(Share));
 }
 
 void launch_run_attention(hipStream_t stream, const RunAttention &p)
 {
     if (p.blocks) {
-        matrix_kernel(p).run<<<p.blocks, kBlock, 0, stream>>>(p);
-        run_attention_join_kernel<<<dim3(p.blocks, kRows / (kBlock / 64)), kBlock, 0, stream>>>(p);
+        const MatrixKernel kernel = matrix_kernel(p);
+        kernel.run<<<p.blocks, kernel.threads, 0, stream>>>(p);
+        run_attention_join_kernel<<<dim3(p.blocks, p.rows / (kBlock / 64)), kBlock, 0, stream>>>(p);
         return;
     }
     const uint64_t blocks = uint64_t(p.runs.tokens) * p.query_heads;
