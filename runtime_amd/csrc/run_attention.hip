@@ -160,6 +160,7 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 constexpr int kBlock = 256;
 constexpr uint32_t kItemUnits = 2;
 constexpr uint32_t kLeastUnits = 4;  // of a block
+constexpr uint32_t kMostBlocks = 1024;
 constexpr float kProbabilityShift = 15.0f;
 
 // What a block's first unfinished item needs of the join.
@@ -699,6 +700,10 @@ void run_attention_kernel(RunAttention p)
         };
 
         load_ids(part.first);
+        if (part.first < part.last) {
+            load_tile(part.first);
+            load_ids(part.first + 1 < part.last ? part.first + 1 : part.first);
+        }
         // The wave's queries, in parts; rows past the run's are zero.
         v4u query[GROUPS][U][QP];
         float factor[GROUPS];
@@ -756,11 +761,6 @@ void run_attention_kernel(RunAttention p)
                     }
                 }
         }
-        if (part.first < part.last) {
-            load_tile(part.first);
-            load_ids(part.first + 1 < part.last ? part.first + 1 : part.first);
-        }
-
         v4f o[GROUPS][N];
         float m[GROUPS], l[GROUPS];
         bool poison[GROUPS];
@@ -1046,64 +1046,184 @@ void run_attention_kernel(RunAttention p)
         block_shares(p)[line.block] = share;
 }
 
-// A wave per row of a shared item: out = sum_i a_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over
-// the records, in their order.  Lanes are shares of the records, each of the row's
-// 4-column pieces.
+// A shared item's rows: out = sum_i a_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over its records,
+// in an order that their number fixes.  A thread has a 4-column piece of a row.  Up to
+// kFewRecords it reads all of them at once, with their statistics; of more, groups of
+// threads each take every so-many-th and add up in LDS.
+constexpr uint32_t kFewRecords = 8, kJoinRows = 16;
+
 __global__ __launch_bounds__(kBlock) void run_attention_join_kernel(RunAttention p)
 {
+    __shared__ float weights[kMostBlocks];
+    __shared__ v4f sums[kBlock];
     const Share share = block_shares(p)[blockIdx.x];
-    const uint32_t in_tile = blockIdx.y * (kBlock / 64) + (threadIdx.x >> 6);
-    const uint32_t row = p.rows * share.row_tile + in_tile;
-    if (!share.count || row >= share.run * p.group)
+    if (!share.count)
         return;
-    const uint32_t lane = threadIdx.x & 63, d = p.value_dim, pieces = d / 4;
-    const uint32_t token = row / p.group, head = share.kv_head * p.group + row - token * p.group;
-    float *out = p.out + (uint64_t(share.begin + token) * p.query_heads + head) * d;
-    const auto record = [&](uint32_t i) {
-        return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * p.rows + in_tile;
-    };
+    const uint32_t d = p.value_dim, pieces = d / 4, wide = kBlock / pieces;
+    const uint32_t piece = threadIdx.x % pieces, part = threadIdx.x / pieces;
+    const uint32_t row0 = p.rows * share.row_tile, all = share.run * p.group - row0;
+    const uint32_t rows = all < p.rows ? all : p.rows;
     const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
-    float most = -__builtin_inff();
-    for (uint32_t i = lane; i < share.count; i += 64)
-        most = fmaxf(most, stats[record(i)][0]);
+    const auto record = [&](uint32_t i, uint32_t row) {
+        return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * p.rows + row;
+    };
+    const auto piece_of = [&](uint64_t n) {
+        return *reinterpret_cast<const v4f *>(p.records + n * d + 4 * piece);
+    };
+    // A record without a key has no outputs.
+    const auto weighed = [](float w, v4f x) { return w != 0.0f ? x * w : v4f{0, 0, 0, 0}; };
+    const auto write = [&](uint32_t in_tile, uint32_t piece, v4f a, float total) {
+        const uint32_t row = row0 + in_tile, token = row / p.group;
+        const uint64_t at = uint64_t(share.begin + token) * p.query_heads +
+                            share.kv_head * p.group + row - token * p.group;
+        *reinterpret_cast<v4f *>(p.out + at * d + 4 * piece) =
+            a * (total == 0.0f ? 0.0f : 1.0f / total);
+    };
+    if (share.count <= kFewRecords) {
+        for (uint32_t row = blockIdx.y * wide + part; row < rows && part < wide;
+             row += kJoinRows * wide) {
+            v4f x[kFewRecords];
+            v2f stat[kFewRecords];
 #pragma unroll
-    for (int offset = 32; offset > 0; offset >>= 1)
-        most = fmaxf(most, __shfl_xor(most, offset, 64));
-    const float base = most == -__builtin_inff() ? 0.0f : most;
-    const uint32_t width = pieces < 64 ? pieces : 64, shares = 64 / width, mine = lane / width;
-    float total = 0.0f;
-    for (uint32_t column = 0; column < pieces; column += width) {
-        const uint32_t c = column + lane % width;
-        v4f a = {0, 0, 0, 0};
-        for (uint32_t group = 0; group < share.count; group += 64) {
-            const uint32_t left = share.count - group, count = left < 64 ? left : 64;
-            float weight = 0.0f;
-            if (lane < count) {
-                const v2f stat = stats[record(group + lane)];
-                weight = __builtin_amdgcn_exp2f(stat[0] - base);
-                if (column == 0)
-                    total += stat[1] * weight;
+            for (uint32_t i = 0; i < kFewRecords; ++i) {
+                const uint64_t n = record(i < share.count ? i : 0, row);
+                x[i] = piece_of(n);
+                stat[i] = stats[n];
             }
-            for (uint32_t i = 0; i < count; i += shares) {
-                const uint32_t n = i + mine;
-                const float w = __shfl(weight, int(n & 63), 64);
-                // A record without a key has no outputs.
-                if (n < count && mine < shares && c < pieces && w != 0.0f)
-                    a += w * *reinterpret_cast<const v4f *>(p.records + record(group + n) * d + 4 * c);
+            float most = -__builtin_inff(), total = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < kFewRecords; ++i)
+                most = fmaxf(most, stat[i][0]);
+            const float base = most == -__builtin_inff() ? 0.0f : most;
+            v4f a = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < kFewRecords; ++i) {
+                const float w =
+                    i < share.count ? __builtin_amdgcn_exp2f(stat[i][0] - base) : 0.0f;
+                if (i < share.count)
+                    total += stat[i][1] * w;
+                a += weighed(w, x[i]);
             }
+            write(row, piece, a, total);
         }
-        if (column == 0) {
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 63;
+    constexpr uint32_t HELD = 8;
+    if (pieces <= 64) {
+        // A wave per row, its lanes shares of the records.
+        const uint32_t shares = 64 / pieces, mine = lane / pieces, c = lane % pieces;
+        for (uint32_t row = blockIdx.y * (kBlock / 64) + threadIdx.x / 64; row < rows;
+             row += kJoinRows * (kBlock / 64)) {
+            v4f x[HELD];
+            const auto load = [&](uint32_t first) {
+#pragma unroll
+                for (uint32_t i = 0; i < HELD; ++i) {
+                    const uint32_t n = first + i * shares + mine;
+                    x[i] = *reinterpret_cast<const v4f *>(
+                        p.records + record(n < share.count ? n : share.count - 1, row) * d + 4 * c);
+                }
+            };
+            load(0);
+            float most = -__builtin_inff(), total = 0.0f, weight = 0.0f;
+            for (uint32_t i = lane; i < share.count; i += 64)
+                most = fmaxf(most, stats[record(i, row)][0]);
+#pragma unroll
+            for (int offset = 32; offset > 0; offset >>= 1)
+                most = fmaxf(most, __shfl_xor(most, offset, 64));
+            const float base = most == -__builtin_inff() ? 0.0f : most;
+            v4f a = {0, 0, 0, 0};
+            uint32_t group = share.count;  // of 64 weights, the lanes'
+            for (uint32_t first = 0; first < share.count; first += HELD * shares) {
+                v4f now[HELD];
+#pragma unroll
+                for (uint32_t i = 0; i < HELD; ++i)
+                    now[i] = x[i];
+                if (first + HELD * shares < share.count)
+                    load(first + HELD * shares);
+#pragma unroll
+                for (uint32_t i = 0; i < HELD; ++i) {
+                    // The records of one i are within 64 from a multiple of `shares`.
+                    const uint32_t at = first + i * shares;
+                    if (group == share.count || at + shares > group + 64) {
+                        group = at;
+                        const uint32_t n = at + lane;
+                        const v2f stat = stats[record(n < share.count ? n : share.count - 1, row)];
+                        weight = n < share.count ? __builtin_amdgcn_exp2f(stat[0] - base) : 0.0f;
+                    }
+                    const float w = __shfl(weight, int((at - group + mine) & 63), 64);
+                    a += weighed(mine < shares ? w : 0.0f, now[i]);
+                }
+            }
+            for (uint32_t i = lane; i < share.count; i += 64) {
+                const v2f stat = stats[record(i, row)];
+                total += stat[1] * __builtin_amdgcn_exp2f(stat[0] - base);
+            }
 #pragma unroll
             for (int offset = 32; offset > 0; offset >>= 1)
                 total += __shfl_xor(total, offset, 64);
-        }
-        v4f sum = a;
-        for (uint32_t s = 1; s < shares; ++s)
+            v4f sum = a;
+            for (uint32_t s = 1; s < shares; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sum[e] += __shfl(a[e], int((lane + s * width) & 63), 64);
-        if (mine == 0 && c < pieces)
-            *reinterpret_cast<v4f *>(out + 4 * c) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
+                for (int e = 0; e < 4; ++e)
+                    sum[e] += __shfl(a[e], int((lane + s * pieces) & 63), 64);
+            if (mine == 0)
+                write(row, c, sum, total);
+        }
+        return;
+    }
+    for (uint32_t row = blockIdx.y; row < rows; row += kJoinRows) {
+        v4f x[HELD];
+        const auto load = [&](uint32_t first) {
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) {
+                const uint32_t n = first + i * wide + part;
+                x[i] = piece_of(record(n < share.count ? n : share.count - 1, row));
+            }
+        };
+        load(0);
+        // Every wave forms the sum, the first one's weights are shared.
+        float most = -__builtin_inff(), total = 0.0f;
+        for (uint32_t i = lane; i < share.count; i += 64)
+            most = fmaxf(most, stats[record(i, row)][0]);
+#pragma unroll
+        for (int offset = 32; offset > 0; offset >>= 1)
+            most = fmaxf(most, __shfl_xor(most, offset, 64));
+        const float base = most == -__builtin_inff() ? 0.0f : most;
+        __syncthreads();  // the row before has been read
+        for (uint32_t i = lane; i < share.count; i += 64) {
+            const v2f stat = stats[record(i, row)];
+            const float w = __builtin_amdgcn_exp2f(stat[0] - base);
+            total += stat[1] * w;
+            if (threadIdx.x < 64)
+                weights[i] = w;
+        }
+#pragma unroll
+        for (int offset = 32; offset > 0; offset >>= 1)
+            total += __shfl_xor(total, offset, 64);
+        __syncthreads();
+        v4f a = {0, 0, 0, 0};
+        for (uint32_t first = 0; first < share.count; first += HELD * wide) {
+            v4f now[HELD];
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i)
+                now[i] = x[i];
+            if (first + HELD * wide < share.count)
+                load(first + HELD * wide);
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) {
+                const uint32_t n = first + i * wide + part;
+                const float w = n < share.count && part < wide ? weights[n] : 0.0f;
+                a += weighed(w, now[i]);
+            }
+        }
+        sums[threadIdx.x] = a;
+        __syncthreads();
+        if (part == 0) {
+            for (uint32_t w = 1; w < wide; ++w)
+                a += sums[w * pieces + piece];
+            write(row, piece, a, total);
+        }
     }
 }
 
@@ -1194,6 +1314,7 @@ bool run_attention_plan(RunAttention &p, int cu_count)
     const uint64_t wanted = (most + kLeastUnits - 1) / kLeastUnits;
     const uint64_t resident = uint64_t(cu_count) * kernel.resident;
     p.blocks = uint32_t(wanted < resident ? wanted : resident);
+    p.blocks = p.blocks < kMostBlocks ? p.blocks : kMostBlocks;
     return true;
 }
 
@@ -1208,7 +1329,7 @@ void launch_run_attention(hipStream_t stream, const RunAttention &p)
     if (p.blocks) {
         const MatrixKernel kernel = matrix_kernel(p);
         kernel.run<<<p.blocks, kernel.threads, 0, stream>>>(p);
-        run_attention_join_kernel<<<dim3(p.blocks, p.rows / (kBlock / 64)), kBlock, 0, stream>>>(p);
+        run_attention_join_kernel<<<dim3(p.blocks, kJoinRows), kBlock, 0, stream>>>(p);
         return;
     }
     const uint64_t blocks = uint64_t(p.runs.tokens) * p.query_heads;
