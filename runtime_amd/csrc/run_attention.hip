@@ -6,6 +6,7 @@
 // of the run that its mask names.
 #include <type_traits>
 
+#include "digits.hpp"
 #include "draft.hpp"
 #include "kernels.hpp"
 
@@ -507,10 +508,16 @@ struct Shape {
     static constexpr int QUERY_PARTS = HALF ? 2 : 3;    // of queries and probabilities
     static constexpr int SHIFT = DK * GROUPS <= (HALF ? 128 : 64) ? 6 : 5;
     static constexpr int KEYS = 1 << SHIFT;
-    static constexpr int KEY_PLANE = KEYS * kPitch<DK>, VALUE_PLANE = LATENT ? 0 : KEY_PLANE;
+    // Copied to LDS without passing through registers: rows as they are, of which eight
+    // are whole copies of a wave.
+    static constexpr bool COPIED = HALF && DK % 64 == 0;
+    static constexpr int PITCH = COPIED ? DK : kPitch<DK>;
+    static constexpr int KEY_PLANE = KEYS * PITCH, VALUE_PLANE = LATENT ? 0 : KEY_PLANE;
     static constexpr int STAGE = PARTS * (KEY_PLANE + VALUE_PLANE);  // 16-bit elements
-    static constexpr int STAGES = HALF ? 2 : 1;
     static constexpr int RESIDENT = WAVES == 4 && DK <= 128 ? 2 : 1;
+    // Of a CU's 160 KB of LDS, beside the scores that waves exchange.
+    static constexpr int ROOM = (SPLIT > 1 ? 61440 : 73728) / RESIDENT / STAGE;
+    static constexpr int STAGES = !HALF ? 1 : !COPIED || ROOM < 2 ? 2 : ROOM < 4 ? ROOM : 4;
     static constexpr int CHUNK = SPLIT > 1 ? 4 : 8;     // most tiles of a value chunk
 };
 
@@ -537,6 +544,30 @@ struct Loads {
     }
 };
 
+// Copied rows hold their 16-byte chunks in an order of their own, chunk c at c ^ turn(row) of
+// its group of G, by which 16 rows' equal chunks fall on all banks.
+template <int D>
+struct Turned {
+    static constexpr uint32_t G = D / 8 % 16 == 0 ? 16 : 8;
+    __device__ __forceinline__ static uint32_t turn(uint32_t row)
+    {
+        return row / (16 / G) & (G - 1);
+    }
+    __device__ __forceinline__ static uint32_t place(uint32_t row, uint32_t chunk)
+    {
+        return (chunk & ~(G - 1)) + ((chunk ^ turn(row)) & (G - 1));
+    }
+};
+
+// Waits until at most `count` of the wave's loads and copies are on their way.
+template <int COUNT>
+__device__ __forceinline__ void wait_loads()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (COUNT & 15) | (COUNT >> 4) << 14);
+}
+
+constexpr uint32_t kPagesHeld = 512;  // of runs of eight keys, in LDS
+
 template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
 __global__ __launch_bounds__(64 * WAVES, (Shape<DK, DV, HALF, LATENT, WAVES, SPLIT,
                                                 GROUPS>::RESIDENT * WAVES / 4))
@@ -556,6 +587,10 @@ void run_attention_kernel(RunAttention p)
     __shared__ __attribute__((aligned(16))) uint16_t lds[S::STAGES * S::STAGE];
     __shared__ v4f partial[SPLIT > 1 ? WAVES * GROUPS * NB * 64 : 1];
     __shared__ uint32_t flags[3][2];  // keys of a tile that are marked, by bit
+    __shared__ uint32_t pages_held[S::COPIED ? kPagesHeld : 1];
+    constexpr bool COPIED = S::COPIED;
+    constexpr int STAGES = S::STAGES, PITCH = S::PITCH, THREADS = S::THREADS;
+    using Order = Turned<DK>;
 
     const uint32_t lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15;
     const uint32_t wave = scalar(threadIdx.x >> 6), split = wave % SPLIT;
@@ -564,12 +599,12 @@ void run_attention_kernel(RunAttention p)
     // The lane's places in a load: bytes from its first key's row, and elements in LDS,
     // which are held where they are few.
     constexpr uint32_t PER_ROW = DK / Load::PIECE;
-    constexpr bool HELD = Load::MINE <= 5;
-    uint32_t load_at[Load::CHUNKS % 64 ? Load::MINE : 1], store_held[HELD ? Load::MINE : 1];
+    constexpr bool HELD = Load::MINE <= 5 && !COPIED, OWN_AT = COPIED || Load::CHUNKS % 64 != 0;
+    uint32_t load_at[OWN_AT ? Load::MINE : 1], store_held[HELD ? Load::MINE : 1];
     const auto place = [&](int i, uint32_t me) {
         const uint32_t n = Load::number(i, wave), c = Load::chunk(n, me);
         const uint32_t row = c / PER_ROW, piece = c - row * PER_ROW;
-        return (8 * (n / Load::EACH) + row) * kPitch<DK> + piece * Load::PIECE;
+        return (8 * (n / Load::EACH) + row) * PITCH + piece * Load::PIECE;
     };
     const auto store_at = [&](int i) {
         return HELD ? store_held[HELD ? i : 0] : place(i, formed_here(lane));
@@ -577,11 +612,20 @@ void run_attention_kernel(RunAttention p)
     load_at[0] = lane * 16;
 #pragma unroll
     for (int i = 0; i < Load::MINE; ++i) {
-        if (Load::CHUNKS % 64)
-            load_at[i] = Load::chunk(Load::number(i, wave), lane) * 16;
+        const uint32_t n = Load::number(i, wave), c = Load::chunk(n, lane);
+        if (COPIED) {
+            // What belongs to the chunk of LDS that the lane writes.
+            const uint32_t row = c / PER_ROW;
+            load_at[i] = (row * PER_ROW +
+                          Order::place(8 * (n / Load::EACH) + row, c - row * PER_ROW)) * 16;
+        } else if (OWN_AT) {
+            load_at[i] = c * 16;
+        }
         if (HELD)
             store_held[i] = place(i, lane);
     }
+    const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) uint16_t *)&lds[0]));
     Line line;
     const bool any = find_line<SHIFT>(p, line);
     Share share = {};
@@ -641,7 +685,7 @@ void run_attention_kernel(RunAttention p)
                               (key_of(tile, i) & in_page) * uint32_t(DK * sizeof(T));
                 if (Load::CHUNKS % 64 == 0)
                     at += Load::number(i, wave) % Load::EACH * 1024;
-                const uint32_t lane_at = load_at[Load::CHUNKS % 64 ? i : 0];
+                const uint32_t lane_at = load_at[OWN_AT ? i : 0];
                 key_reg[i] = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(
                     static_cast<const char *>(p.key_pages) + at + lane_at));
                 if constexpr (!LATENT)
@@ -670,7 +714,7 @@ void run_attention_kernel(RunAttention p)
                     }
                 }
                 if (odd) {
-                    const uint32_t key = formed_here(at) / kPitch<DK>;
+                    const uint32_t key = formed_here(at) / PITCH;
                     atomicOr(&flags[turn][key / 32], 1u << key % 32);
                 }
             }
@@ -683,6 +727,56 @@ void run_attention_kernel(RunAttention p)
 #pragma unroll
                 for (int i = 0; i < PARTS; ++i)
                     *reinterpret_cast<v2u *>(to + i * plane) = v2u{a[i], b[i]};
+            }
+        };
+        // The pages of the kPagesHeld / 2 runs of eight keys from one on, UINT32_MAX for none.
+        const auto hold_pages = [&](uint32_t first) {
+            for (uint32_t i = threadIdx.x; i < kPagesHeld / 2; i += THREADS) {
+                const uint32_t key = 8 * (first + i);
+                const float id = table[(key < last_key ? key : last_key) >> page_shift];
+                pages_held[(first + i) % kPagesHeld] =
+                    valid_index(id, p.shape.pages) ? uint32_t(id) : UINT32_MAX;
+            }
+        };
+        const auto starts_pages = [&](uint32_t tile) {
+            return tile * (KEYS / 8) % (kPagesHeld / 2) == 0;
+        };
+        // Starts the copies of a tile, the same number in every wave and tile.
+        constexpr int COPIES = Load::MINE * (LATENT ? 1 : 2);
+        const auto copy_tile = [&](uint32_t tile) {
+            const uint32_t stage = lds_at + tile % STAGES * (2 * S::STAGE);
+#pragma unroll
+            for (int i = 0; i < Load::MINE; ++i) {
+                const uint32_t n = Load::number(i, wave), eight = n / Load::EACH;
+                const uint32_t held =
+                    scalar(pages_held[(tile * (KEYS / 8) + eight) % kPagesHeld]);
+                const uint64_t at = (held == UINT32_MAX ? 0 : held) * page_bytes + head_bytes +
+                                    (key_of(tile, i) & in_page) * uint32_t(DK * sizeof(T));
+                const uint32_t to = stage + n * 1024;
+                copy_to_lds(static_cast<const uint8_t *>(p.key_pages) + at, load_at[OWN_AT ? i : 0],
+                            to);
+                if constexpr (!LATENT)
+                    copy_to_lds(static_cast<const uint8_t *>(p.value_pages) + at,
+                                load_at[OWN_AT ? i : 0], to + 2 * S::KEY_PLANE);
+            }
+        };
+        // In a copied tile, as store_piece does in a loaded one.
+        const auto check_tile = [&](uint16_t *stage, uint32_t turn) {
+            for (uint32_t n = threadIdx.x; n < uint32_t(S::STAGE / 8); n += THREADS) {
+                v4u x = *reinterpret_cast<v4u *>(stage + 8 * n);
+                bool odd = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool low = (x[e] & 0x7c00u) == 0x7c00u;
+                    const bool high = (x[e] & 0x7c000000u) == 0x7c000000u;
+                    odd |= low || high;
+                    x[e] &= (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u);
+                }
+                if (odd) {
+                    const uint32_t key = n / (PITCH / 8) % KEYS;
+                    *reinterpret_cast<v4u *>(stage + 8 * n) = x;
+                    atomicOr(&flags[turn][key / 32], 1u << key % 32);
+                }
             }
         };
         const auto store_tile = [&](uint16_t *stage, bool mixed, uint32_t turn) {
@@ -699,10 +793,25 @@ void run_attention_kernel(RunAttention p)
             }
         };
 
-        load_ids(part.first);
-        if (part.first < part.last) {
-            load_tile(part.first);
-            load_ids(part.first + 1 < part.last ? part.first + 1 : part.first);
+        if constexpr (COPIED) {
+            __syncthreads();  // an earlier part's tiles and pages have been read
+            hold_pages(part.first * (KEYS / 8) / (kPagesHeld / 2) * (kPagesHeld / 2));
+            __syncthreads();
+#pragma unroll
+            for (int ahead = 0; ahead < STAGES - 1; ++ahead)
+                if (part.first + ahead < part.last) {
+                    if (ahead && starts_pages(part.first + ahead)) {
+                        hold_pages((part.first + ahead) * (KEYS / 8));
+                        __syncthreads();
+                    }
+                    copy_tile(part.first + ahead);
+                }
+        } else {
+            load_ids(part.first);
+            if (part.first < part.last) {
+                load_tile(part.first);
+                load_ids(part.first + 1 < part.last ? part.first + 1 : part.first);
+            }
         }
         // The wave's queries, in parts; rows past the run's are zero.
         v4u query[GROUPS][U][QP];
@@ -784,25 +893,63 @@ void run_attention_kernel(RunAttention p)
         for (uint32_t tile = part.first; tile < part.last; ++tile) {
             const uint32_t k0 = tile * KEYS;
             const bool mixed = k0 + KEYS > common;
-            uint16_t *stage = lds + (S::STAGES == 2 && (tile & 1) ? S::STAGE : 0);
-            if (S::STAGES == 1)
-                __syncthreads();  // the tile before has been read
-            store_tile(stage, mixed, turn);
-            if (tile + 1 < part.last) {
-                load_tile(tile + 1);
-                load_ids(tile + 2 < part.last ? tile + 2 : tile + 1);
+            uint16_t *stage = lds + tile % STAGES * S::STAGE;
+            uint64_t marks = 0;
+            if constexpr (COPIED) {
+                // This tile's copies have ended, those of the ones behind it may not have.
+                const uint32_t behind = part.last - 1 - tile;
+                if (STAGES >= 4 && behind >= 2)
+                    wait_loads<2 * COPIES>();
+                else if (STAGES >= 3 && behind >= 1)
+                    wait_loads<COPIES>();
+                else
+                    wait_loads<0>();
+                const uint32_t next = tile + STAGES - 1;
+                if (next < part.last && starts_pages(next))
+                    hold_pages(next * (KEYS / 8));
+                __syncthreads();
+                if (next < part.last)
+                    copy_tile(next);
+                uint32_t none = uint32_t(__ballot(
+                    lane < KEYS / 8 &&
+                    pages_held[(tile * (KEYS / 8) + lane % (KEYS / 8)) % kPagesHeld] ==
+                        UINT32_MAX));
+                if (mixed) {
+                    check_tile(stage, turn);
+                    __syncthreads();
+                    marks = uint64_t(flags[turn][1]) << 32 | flags[turn][0];
+                    turn ^= 1;
+                    if (threadIdx.x < 2)
+                        flags[turn][threadIdx.x] = 0;
+                }
+                for (; none; none &= none - 1)
+                    marks |= 0xffull << 8 * __builtin_ctz(none);
+            } else {
+                if (STAGES == 1)
+                    __syncthreads();  // the tile before has been read
+                store_tile(stage, mixed, turn);
+                if (tile + 1 < part.last) {
+                    load_tile(tile + 1);
+                    load_ids(tile + 2 < part.last ? tile + 2 : tile + 1);
+                }
+                __syncthreads();
+                marks = uint64_t(flags[turn][1]) << 32 | flags[turn][0];
+                // The mark after the next one: no thread is past the next barrier.
+                turn = turn == 2 ? 0 : turn + 1;
+                if (threadIdx.x < 2)
+                    flags[turn == 2 ? 0 : turn + 1][threadIdx.x] = 0;
             }
-            __syncthreads();
-            const uint64_t marks = uint64_t(flags[turn][1]) << 32 | flags[turn][0];
-            // The mark after the next one: no thread is past the next barrier.
-            turn = turn == 2 ? 0 : turn + 1;
-            if (threadIdx.x < 2)
-                flags[turn == 2 ? 0 : turn + 1][threadIdx.x] = 0;
 
             v4f s[GROUPS][NB];
             if (active) {
-                const uint32_t me = formed_here(lane);
-                const uint16_t *key_stage = stage + (me & 15) * kPitch<DK> + 8 * (me >> 4);
+                const uint32_t me = SPLIT > 1 ? formed_here(lane) : lane;
+                // Copied rows: where depth v of a group of chunks lies.
+                constexpr uint32_t PLACES = COPIED ? Order::G / 4 : 1;
+                uint32_t key_lane[PLACES];
+#pragma unroll
+                for (uint32_t v = 0; v < PLACES; ++v)
+                    key_lane[v] = (me & 15) * PITCH +
+                                  8 * (COPIED ? Order::place(me & 15, 4 * v + (me >> 4)) : me >> 4);
                 // f32 caches: the largest product apart from the others, whose sums it would
                 // round.
                 v4f rest[GROUPS][HALF ? 1 : NB];
@@ -817,7 +964,15 @@ void run_attention_kernel(RunAttention p)
                     uint32_t depth = split * U + u;
                     if (DEPTHS % SPLIT != 0 && depth >= uint32_t(DEPTHS))
                         depth = DEPTHS - 1;
-                    const uint16_t *from = key_stage + 32 * depth;
+                    const uint16_t *from = stage;
+                    static_assert(!COPIED || SPLIT == 1 || PLACES == 2, "depths of split rows");
+                    if constexpr (COPIED && SPLIT == 1)
+                        from += key_lane[u % PLACES] + u / PLACES * (32 * PLACES);
+                    else if constexpr (COPIED)
+                        from += (depth % 2 ? key_lane[PLACES - 1] : key_lane[0]) +
+                                depth / PLACES * (32 * PLACES);
+                    else
+                        from += key_lane[0] + 32 * depth;
                     if (DK % 32 != 0 && u == U - 1 && q >= 2)
                         from -= 16;
 #pragma unroll
@@ -825,7 +980,7 @@ void run_attention_kernel(RunAttention p)
 #pragma unroll
                         for (int i = PARTS - 1; i >= 0; --i) {
                             const v4u k = *reinterpret_cast<const v4u *>(
-                                from + 16 * c * kPitch<DK> + i * S::KEY_PLANE);
+                                from + 16 * c * PITCH + i * S::KEY_PLANE);
 #pragma unroll
                             for (int b = (HALF ? 1 : 2) - i; b >= 0; --b)
 #pragma unroll
@@ -945,10 +1100,8 @@ void run_attention_kernel(RunAttention p)
                         l[g] += s[g][c][r];
                     }
             }
-            const uint32_t me = formed_here(lane);
-            const uint16_t *value_stage = stage + (LATENT ? 0 : PARTS * S::KEY_PLANE) +
-                                          4 * (me >> 4) * kPitch<DK> + split * (DV / SPLIT);
-            const uint32_t column = me & 15;
+            const uint32_t me = SPLIT > 1 ? formed_here(lane) : lane;
+            const uint16_t *value_stage = stage + (LATENT ? 0 : PARTS * S::KEY_PLANE);
 #pragma unroll
             for (int h = 0; h < NB / 2; ++h) {  // 32 keys, a product's depth
                 v4u prob[GROUPS][QP];
@@ -968,14 +1121,24 @@ void run_attention_kernel(RunAttention p)
 #pragma unroll
                     for (int i = PARTS - 1; i >= 0; --i) {
                         uint32_t x[8][W];
+                        // Columns 16 t0 + n j .. + n - 1 of the wave's, of the key 32 h + 16
+                        // (e / 4) + 4 q + e % 4; copied rows have 2 or 4 orders among them.
+                        constexpr uint32_t ORDERS = !COPIED ? 1 : Order::G == 16 ? 4 : 2;
+                        static_assert(!COPIED || 2 * t0 % Order::G == 0, "whole groups of chunks");
+                        uint32_t value_lane[ORDERS];
+#pragma unroll
+                        for (uint32_t v = 0; v < ORDERS; ++v) {
+                            const uint32_t row = 4 * (me >> 4) + v * (4 / ORDERS);
+                            const uint32_t column = split * (DV / SPLIT) + n * (me & 15);
+                            value_lane[v] =
+                                4 * (me >> 4) * PITCH +
+                                (COPIED ? 8 * Order::place(row, column / 8) + column % 8 : column);
+                        }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            // Columns 16 t0 + n j .. + n - 1 of the wave's, of the key
-                            // 32 h + 16 (e / 4) + 4 q + e % 4.
-                            const uint16_t *from =
-                                value_stage + i * S::KEY_PLANE +
-                                (32 * h + 16 * (e / 4) + e % 4) * kPitch<DK> + 16 * t0 +
-                                n * column;
+                            const uint16_t *from = value_stage + i * S::KEY_PLANE +
+                                                   (32 * h + 16 * (e / 4) + e % 4) * PITCH +
+                                                   16 * t0 + value_lane[e % 4 * ORDERS / 4];
                             if constexpr (n == 8) {
                                 const v4u piece = *reinterpret_cast<const v4u *>(from);
                                 x[e][0] = piece[0], x[e][1] = piece[1];
