@@ -159,8 +159,14 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
-constexpr uint32_t kItemUnits = 2;
-constexpr uint32_t kLeastUnits = 4;  // of a block
+#ifndef LEAST
+#define LEAST 4
+#endif
+#ifndef ITEM
+#define ITEM 2
+#endif
+constexpr uint32_t kItemUnits = ITEM;
+constexpr uint32_t kLeastUnits = LEAST;  // of a block
 constexpr uint32_t kMostBlocks = 1024;
 constexpr float kProbabilityShift = 15.0f;
 
@@ -460,10 +466,15 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PAR
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
         if constexpr (HALF) {
-            const v2h h = {_Float16(a), _Float16(b)};
-            out[i] = __builtin_bit_cast(uint32_t, h);
-            a = __builtin_fmaf(float(h[0]), -1.0f, a);
-            b = __builtin_fmaf(float(h[1]), -1.0f, b);
+            out[i] = __builtin_bit_cast(uint32_t, v2h{_Float16(a), _Float16(b)});
+            if (i + 1 < PARTS) {
+                // What is left, from the packed halves as they are: a - half in one
+                // instruction.
+                asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
+                    : "+v"(a) : "v"(out[i]));
+                asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                    : "+v"(b) : "v"(out[i]));
+            }
         } else {
             out[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
             a -= __uint_as_float(out[i] << 16);
@@ -829,47 +840,40 @@ void run_attention_kernel(RunAttention p)
                 const bool mine = real[g] && column < uint32_t(DK);
                 return mine ? piece : v4f{0, 0, 0, 0};
             };
+            v4f x[2 * U];
+#pragma unroll
+            for (int i = 0; i < 2 * U; ++i)
+                x[i] = load(i / 2, 4 * (i % 2));
             factor[g] = p.scale;
             int exponent = 0;
             if (HALF) {
                 float most = 0.0f;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        const v4f x = load(u, e);
-                        most = fmaxf(fmaxf(most, fmaxf(fabsf(x[0]), fabsf(x[1]))),
-                                     fmaxf(fabsf(x[2]), fabsf(x[3])));
-                    }
+                for (int i = 0; i < 2 * U; ++i)
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(x[i][0]), fabsf(x[i][1]))),
+                                 fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
                 most = quad_max(most);
                 // 2^14 <= most 2^exponent < 2^15 (0 and infinities as they are; below
                 // 2^-86, where no score differs from 0, by 2^100, so that the factor stays
                 // normal).
                 if (most > 0.0f && most < __builtin_inff())
-                    exponent = 15 - (ilogbf(most) + 1);
+                    exponent = 15 - __builtin_amdgcn_frexp_expf(most);
                 exponent = exponent < 100 ? exponent : 100;
                 factor[g] = ldexpf(p.scale, -exponent);
-                // Read a second time rather than held: the registers are the tile's.
-                at += formed_here(0);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int i = 0; i < 2 * U; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    v4f x = load(u, e);
+                for (int e = 0; e < 4; e += 2) {
+                    uint32_t parts[QP];
+                    split_pair<HALF>(HALF ? ldexpf(x[i][e], exponent) : x[i][e],
+                                     HALF ? ldexpf(x[i][e + 1], exponent) : x[i][e + 1], parts);
 #pragma unroll
-                    for (int i = 0; HALF && i < 4; ++i)
-                        x[i] = ldexpf(x[i], exponent);
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        uint32_t parts[QP];
-                        split_pair<HALF>(x[i], x[i + 1], parts);
-#pragma unroll
-                        for (int part = 0; part < QP; ++part)
-                            query[g][u][part][(e + i) / 2] = parts[part];
-                    }
+                    for (int part = 0; part < QP; ++part)
+                        query[g][i / 2][part][2 * (i % 2) + e / 2] = parts[part];
                 }
         }
+
         v4f o[GROUPS][N];
         float m[GROUPS], l[GROUPS];
         bool poison[GROUPS];
@@ -1031,25 +1035,25 @@ void run_attention_kernel(RunAttention p)
                     if (p.mask) {
                         const uint8_t *mask =
                             p.mask + uint64_t(part.run.begin + token[g]) * p.mask_bytes;
-#pragma unroll
-                        for (int c = 0; c < NB; ++c)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int at = 16 * c + int(q4) + r, i = first + at;
-                                uint32_t bit = at <= last;
-                                if (i >= 0 && at <= last)
-                                    bit = uint32_t(i) < 8 * p.mask_bytes
-                                              ? mask[uint32_t(i) >> 3] >> (i & 7) & 1
-                                              : 0;
-                                seen |= bit << (4 * c + r);
-                            }
+#pragma unroll 1
+                        for (int n = 0; n < 4 * NB; ++n) {
+                            const int at = 16 * (n / 4) + int(q4) + n % 4, i = first + at;
+                            uint32_t bit = at <= last;
+                            if (i >= 0 && at <= last)
+                                bit = uint32_t(i) < 8 * p.mask_bytes
+                                          ? mask[uint32_t(i) >> 3] >> (i & 7) & 1
+                                          : 0;
+                            seen |= bit << n;
+                        }
                     } else {
                         const int most = int(token[g]) - first;
+                        // Of each four keys, the first most + 1 - (their first) ones.
 #pragma unroll
-                        for (int c = 0; c < NB; ++c)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                seen |= uint32_t(16 * c + int(q4) + r <= most) << (4 * c + r);
+                        for (int c = 0; c < NB; ++c) {
+                            int n = most + 1 - 16 * c - int(q4);
+                            n = n < 0 ? 0 : n > 4 ? 4 : n;
+                            seen |= ((1u << n) - 1) << (4 * c);
+                        }
                     }
                     if (marks) {
                         uint32_t mine = 0;
@@ -1209,183 +1213,195 @@ void run_attention_kernel(RunAttention p)
         block_shares(p)[line.block] = share;
 }
 
-// A shared item's rows: out = sum_i a_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over its records,
-// in an order that their number fixes.  A thread has a 4-column piece of a row.  Up to
-// kFewRecords it reads all of them at once, with their statistics; of more, groups of
-// threads each take every so-many-th and add up in LDS.
-constexpr uint32_t kFewRecords = 8, kJoinRows = 16;
+// The shared items' rows: out = sum_i a_i 2^(m_i - M) / sum_i l_i 2^(m_i - M) over the
+// records, in an order that their number fixes.  Every block reads how many rows each block
+// of the first launch has left to join and takes every so-many-th task of them.  A lane has a
+// 4-column piece; up to kFewRecords records a wave takes as many rows as its lanes hold
+// and reads all of a row's records at once, of more a block takes one row (and 256
+// columns), its lanes' shares every so-many-th record.
+constexpr uint32_t kFewRecords = 8, kJoinHeld = 8, kJoinsPerCu = 4;
 
 __global__ __launch_bounds__(kBlock) void run_attention_join_kernel(RunAttention p)
 {
-    __shared__ float weights[kMostBlocks];
+    __shared__ uint32_t ends[kMostBlocks];  // of the tasks of each block's share
+    __shared__ uint32_t wave_sums[kBlock / 64];
     __shared__ v4f sums[kBlock];
-    const Share share = block_shares(p)[blockIdx.x];
-    if (!share.count)
-        return;
-    const uint32_t d = p.value_dim, pieces = d / 4, wide = kBlock / pieces;
-    const uint32_t piece = threadIdx.x % pieces, part = threadIdx.x / pieces;
-    const uint32_t row0 = p.rows * share.row_tile, all = share.run * p.group - row0;
-    const uint32_t rows = all < p.rows ? all : p.rows;
+    __shared__ float weights[kMostBlocks];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t d = p.value_dim, pieces = d / 4, width = pieces < 64 ? pieces : 64;
+    const uint32_t columns = (pieces + 63) / 64, shares = 64 / width;
+    const uint32_t mine = lane / width, c = lane % width;
+    const Share *all = block_shares(p);
+    const auto rows_of = [&](const Share &s) {
+        const uint32_t left = s.run * p.group - p.rows * s.row_tile;
+        return left < p.rows ? left : p.rows;
+    };
+    // Units that a wave takes at once: their records together are kFewRecords.
+    const auto rows_at_once = [](uint32_t count) { return count <= 2 ? 4 : count <= 4 ? 2 : 1; };
+    // Tasks, four blocks' shares a thread.
+    uint32_t upto[kMostBlocks / kBlock], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostBlocks / kBlock; ++i) {
+        const uint32_t b = threadIdx.x * (kMostBlocks / kBlock) + i;
+        if (b < p.blocks) {
+            const Share s = all[b];
+            const uint32_t units = rows_of(s) * columns;
+            const uint32_t each = (kBlock / 64) * shares * rows_at_once(s.count);
+            sum += !s.count ? 0 : s.count > kFewRecords ? units : (units + each - 1) / each;
+        }
+        upto[i] = sum;
+    }
+    const uint32_t scan = lanes_scan(sum);
+    if (lane == 63)
+        wave_sums[wave] = scan;
+    __syncthreads();
+    uint32_t before = scan - sum, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kBlock / 64; ++w) {
+        before += w < wave ? wave_sums[w] : 0;
+        total += wave_sums[w];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kMostBlocks / kBlock; ++i)
+        ends[threadIdx.x * (kMostBlocks / kBlock) + i] = before + upto[i];
+    __syncthreads();
     const v2f *stats = reinterpret_cast<const v2f *>(record_stats(p));
-    const auto record = [&](uint32_t i, uint32_t row) {
-        return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * p.rows + row;
-    };
-    const auto piece_of = [&](uint64_t n) {
-        return *reinterpret_cast<const v4f *>(p.records + n * d + 4 * piece);
-    };
-    // A record without a key has no outputs.
-    const auto weighed = [](float w, v4f x) { return w != 0.0f ? x * w : v4f{0, 0, 0, 0}; };
-    const auto write = [&](uint32_t in_tile, uint32_t piece, v4f a, float total) {
-        const uint32_t row = row0 + in_tile, token = row / p.group;
-        const uint64_t at = uint64_t(share.begin + token) * p.query_heads +
-                            share.kv_head * p.group + row - token * p.group;
-        *reinterpret_cast<v4f *>(p.out + at * d + 4 * piece) =
-            a * (total == 0.0f ? 0.0f : 1.0f / total);
-    };
-    if (share.count <= kFewRecords) {
-        for (uint32_t row = blockIdx.y * wide + part; row < rows && part < wide;
-             row += kJoinRows * wide) {
-            v4f x[kFewRecords];
-            v2f stat[kFewRecords];
+#pragma unroll 1
+    for (uint32_t task = blockIdx.x; task < total; task += gridDim.x) {
+        // The first block whose tasks end behind this one.
+        uint32_t b = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kFewRecords; ++i) {
-                const uint64_t n = record(i < share.count ? i : 0, row);
-                x[i] = piece_of(n);
-                stat[i] = stats[n];
-            }
-            float most = -__builtin_inff(), total = 0.0f;
+        for (uint32_t step = kMostBlocks / 2; step; step /= 2)
+            if (ends[b + step - 1] <= task)
+                b += step;
+        Share share = all[b];
+        share = {scalar(share.count), scalar(share.record), scalar(share.begin), scalar(share.run),
+                 scalar(share.kv_head), scalar(share.row_tile)};
+        const uint32_t number = scalar(task - (b ? ends[b - 1] : 0));
+        const uint32_t units = rows_of(share) * columns;
+        const auto record = [&](uint32_t i, uint32_t in_tile) {
+            return uint64_t(i ? share.record / 2 * 2 + 2 * i : share.record) * p.rows + in_tile;
+        };
+        const auto piece_at = [&](uint64_t n, uint32_t piece) {
+            return *reinterpret_cast<const v4f *>(p.records + n * d + 4 * piece);
+        };
+        // A record without a key has no outputs.
+        const auto weighed = [](float w, v4f y) { return w != 0.0f ? y * w : v4f{0, 0, 0, 0}; };
+        const auto write = [&](uint32_t in_tile, uint32_t piece, v4f a, float sum_l) {
+            const uint32_t row = p.rows * share.row_tile + in_tile, token = row / p.group;
+            const uint64_t at = uint64_t(share.begin + token) * p.query_heads +
+                                share.kv_head * p.group + row - token * p.group;
+            *reinterpret_cast<v4f *>(p.out + at * d + 4 * piece) =
+                a * (sum_l == 0.0f ? 0.0f : 1.0f / sum_l);
+        };
+        // Up to RECORDS of them, kFewRecords / RECORDS units a wave.
+        const auto join_few = [&](auto records) {
+            constexpr uint32_t RECORDS = records, UNITS = kFewRecords / RECORDS;
+            v4f x[UNITS][RECORDS];
+            v2f stat[UNITS][RECORDS];
+            uint32_t in_tile[UNITS], piece[UNITS];
+            bool real[UNITS];
 #pragma unroll
-            for (uint32_t i = 0; i < kFewRecords; ++i)
-                most = fmaxf(most, stat[i][0]);
-            const float base = most == -__builtin_inff() ? 0.0f : most;
-            v4f a = {0, 0, 0, 0};
+            for (uint32_t u = 0; u < UNITS; ++u) {
+                const uint32_t unit =
+                    ((number * UNITS + u) * (kBlock / 64) + wave) * shares + mine;
+                real[u] = unit < units && mine < shares;
+                in_tile[u] = (real[u] ? unit : 0) / columns;
+                piece[u] = ((real[u] ? unit : 0) - in_tile[u] * columns) * 64 + c;
 #pragma unroll
-            for (uint32_t i = 0; i < kFewRecords; ++i) {
-                const float w =
-                    i < share.count ? __builtin_amdgcn_exp2f(stat[i][0] - base) : 0.0f;
-                if (i < share.count)
-                    total += stat[i][1] * w;
-                a += weighed(w, x[i]);
-            }
-            write(row, piece, a, total);
-        }
-        return;
-    }
-    const uint32_t lane = threadIdx.x & 63;
-    constexpr uint32_t HELD = 8;
-    if (pieces <= 64) {
-        // A wave per row, its lanes shares of the records.
-        const uint32_t shares = 64 / pieces, mine = lane / pieces, c = lane % pieces;
-        for (uint32_t row = blockIdx.y * (kBlock / 64) + threadIdx.x / 64; row < rows;
-             row += kJoinRows * (kBlock / 64)) {
-            v4f x[HELD];
-            const auto load = [&](uint32_t first) {
-#pragma unroll
-                for (uint32_t i = 0; i < HELD; ++i) {
-                    const uint32_t n = first + i * shares + mine;
-                    x[i] = *reinterpret_cast<const v4f *>(
-                        p.records + record(n < share.count ? n : share.count - 1, row) * d + 4 * c);
-                }
-            };
-            load(0);
-            float most = -__builtin_inff(), total = 0.0f, weight = 0.0f;
-            for (uint32_t i = lane; i < share.count; i += 64)
-                most = fmaxf(most, stats[record(i, row)][0]);
-#pragma unroll
-            for (int offset = 32; offset > 0; offset >>= 1)
-                most = fmaxf(most, __shfl_xor(most, offset, 64));
-            const float base = most == -__builtin_inff() ? 0.0f : most;
-            v4f a = {0, 0, 0, 0};
-            uint32_t group = share.count;  // of 64 weights, the lanes'
-            for (uint32_t first = 0; first < share.count; first += HELD * shares) {
-                v4f now[HELD];
-#pragma unroll
-                for (uint32_t i = 0; i < HELD; ++i)
-                    now[i] = x[i];
-                if (first + HELD * shares < share.count)
-                    load(first + HELD * shares);
-#pragma unroll
-                for (uint32_t i = 0; i < HELD; ++i) {
-                    // The records of one i are within 64 from a multiple of `shares`.
-                    const uint32_t at = first + i * shares;
-                    if (group == share.count || at + shares > group + 64) {
-                        group = at;
-                        const uint32_t n = at + lane;
-                        const v2f stat = stats[record(n < share.count ? n : share.count - 1, row)];
-                        weight = n < share.count ? __builtin_amdgcn_exp2f(stat[0] - base) : 0.0f;
-                    }
-                    const float w = __shfl(weight, int((at - group + mine) & 63), 64);
-                    a += weighed(mine < shares ? w : 0.0f, now[i]);
+                for (uint32_t i = 0; i < RECORDS; ++i) {
+                    const uint64_t n = record(i < share.count ? i : 0, in_tile[u]);
+                    x[u][i] = piece_at(n, piece[u]);
+                    stat[u][i] = stats[n];
                 }
             }
-            for (uint32_t i = lane; i < share.count; i += 64) {
-                const v2f stat = stats[record(i, row)];
-                total += stat[1] * __builtin_amdgcn_exp2f(stat[0] - base);
-            }
 #pragma unroll
-            for (int offset = 32; offset > 0; offset >>= 1)
-                total += __shfl_xor(total, offset, 64);
-            v4f sum = a;
-            for (uint32_t s = 1; s < shares; ++s)
+            for (uint32_t u = 0; u < UNITS; ++u) {
+                float most = -__builtin_inff(), sum_l = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sum[e] += __shfl(a[e], int((lane + s * pieces) & 63), 64);
-            if (mine == 0)
-                write(row, c, sum, total);
-        }
-        return;
-    }
-    for (uint32_t row = blockIdx.y; row < rows; row += kJoinRows) {
-        v4f x[HELD];
-        const auto load = [&](uint32_t first) {
+                for (uint32_t i = 0; i < RECORDS; ++i)
+                    most = fmaxf(most, stat[u][i][0]);
+                const float base = most == -__builtin_inff() ? 0.0f : most;
+                v4f a = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i) {
-                const uint32_t n = first + i * wide + part;
-                x[i] = piece_of(record(n < share.count ? n : share.count - 1, row));
+                for (uint32_t i = 0; i < RECORDS; ++i) {
+                    const float w =
+                        i < share.count ? __builtin_amdgcn_exp2f(stat[u][i][0] - base) : 0.0f;
+                    sum_l += i < share.count ? stat[u][i][1] * w : 0.0f;
+                    a += weighed(w, x[u][i]);
+                }
+                if (real[u])
+                    write(in_tile[u], piece[u], a, sum_l);
             }
         };
-        load(0);
-        // Every wave forms the sum, the first one's weights are shared.
-        float most = -__builtin_inff(), total = 0.0f;
+        if (share.count <= 2) {
+            join_few(std::integral_constant<uint32_t, 2>{});
+            continue;
+        }
+        if (share.count <= 4) {
+            join_few(std::integral_constant<uint32_t, 4>{});
+            continue;
+        }
+        if (share.count <= kFewRecords) {
+            join_few(std::integral_constant<uint32_t, 8>{});
+            continue;
+        }
+        const uint32_t in_tile = number / columns, piece = (number - in_tile * columns) * 64 + c;
+        // The lane's records, `by` apart from its first one.
+        const uint32_t first = wave * shares + (mine < shares ? mine : 0);
+        const uint32_t by = (kBlock / 64) * shares;
+        v4f x[kJoinHeld];
+        const auto load = [&](uint32_t from) {
+#pragma unroll
+            for (uint32_t i = 0; i < kJoinHeld; ++i) {
+                const uint32_t n = from + i * by;
+                x[i] = piece_at(record(n < share.count ? n : share.count - 1, in_tile), piece);
+            }
+        };
+        load(first);
+        // Each wave forms the row's maximum and sum, the first one's weights are shared.
+        float most = -__builtin_inff(), sum_l = 0.0f;
         for (uint32_t i = lane; i < share.count; i += 64)
-            most = fmaxf(most, stats[record(i, row)][0]);
+            most = fmaxf(most, stats[record(i, in_tile)][0]);
 #pragma unroll
         for (int offset = 32; offset > 0; offset >>= 1)
             most = fmaxf(most, __shfl_xor(most, offset, 64));
         const float base = most == -__builtin_inff() ? 0.0f : most;
-        __syncthreads();  // the row before has been read
+        __syncthreads();  // the task before has been read
         for (uint32_t i = lane; i < share.count; i += 64) {
-            const v2f stat = stats[record(i, row)];
+            const v2f stat = stats[record(i, in_tile)];
             const float w = __builtin_amdgcn_exp2f(stat[0] - base);
-            total += stat[1] * w;
-            if (threadIdx.x < 64)
+            sum_l += stat[1] * w;
+            if (wave == 0)
                 weights[i] = w;
         }
 #pragma unroll
         for (int offset = 32; offset > 0; offset >>= 1)
-            total += __shfl_xor(total, offset, 64);
+            sum_l += __shfl_xor(sum_l, offset, 64);
         __syncthreads();
         v4f a = {0, 0, 0, 0};
-        for (uint32_t first = 0; first < share.count; first += HELD * wide) {
-            v4f now[HELD];
+#pragma unroll 1
+        for (uint32_t n0 = 0; n0 < share.count; n0 += kJoinHeld * by) {
+            v4f now[kJoinHeld];
 #pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i)
+            for (uint32_t i = 0; i < kJoinHeld; ++i)
                 now[i] = x[i];
-            if (first + HELD * wide < share.count)
-                load(first + HELD * wide);
+            if (n0 + kJoinHeld * by < share.count)
+                load(first + n0 + kJoinHeld * by);
 #pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i) {
-                const uint32_t n = first + i * wide + part;
-                const float w = n < share.count && part < wide ? weights[n] : 0.0f;
-                a += weighed(w, now[i]);
+            for (uint32_t i = 0; i < kJoinHeld; ++i) {
+                const uint32_t n = first + n0 + i * by;
+                a += weighed(n < share.count && mine < shares ? weights[n] : 0.0f, now[i]);
             }
         }
         sums[threadIdx.x] = a;
         __syncthreads();
-        if (part == 0) {
-            for (uint32_t w = 1; w < wide; ++w)
-                a += sums[w * pieces + piece];
-            write(row, piece, a, total);
+        if (threadIdx.x < width && piece < pieces) {
+            a = v4f{0, 0, 0, 0};
+            for (uint32_t w = 0; w < kBlock / 64; ++w)
+                for (uint32_t s = 0; s < shares; ++s)
+                    a += sums[64 * w + s * width + c];
+            write(in_tile, piece, a, sum_l);
         }
     }
 }
@@ -1478,6 +1494,7 @@ bool run_attention_plan(RunAttention &p, int cu_count)
     const uint64_t resident = uint64_t(cu_count) * kernel.resident;
     p.blocks = uint32_t(wanted < resident ? wanted : resident);
     p.blocks = p.blocks < kMostBlocks ? p.blocks : kMostBlocks;
+    p.joins = uint32_t(cu_count) * kJoinsPerCu;
     return true;
 }
 
@@ -1492,7 +1509,7 @@ void launch_run_attention(hipStream_t stream, const RunAttention &p)
     if (p.blocks) {
         const MatrixKernel kernel = matrix_kernel(p);
         kernel.run<<<p.blocks, kernel.threads, 0, stream>>>(p);
-        run_attention_join_kernel<<<dim3(p.blocks, kJoinRows), kBlock, 0, stream>>>(p);
+        run_attention_join_kernel<<<p.joins, kBlock, 0, stream>>>(p);
         return;
     }
     const uint64_t blocks = uint64_t(p.runs.tokens) * p.query_heads;
