@@ -159,14 +159,8 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
-#ifndef LEAST
-#define LEAST 4
-#endif
-#ifndef ITEM
-#define ITEM 2
-#endif
-constexpr uint32_t kItemUnits = ITEM;
-constexpr uint32_t kLeastUnits = LEAST;  // of a block
+constexpr uint32_t kItemUnits = 5;
+constexpr uint32_t kLeastUnits = 1;  // of a block
 constexpr uint32_t kMostBlocks = 1024;
 constexpr float kProbabilityShift = 15.0f;
 
@@ -577,7 +571,7 @@ __device__ __forceinline__ void wait_loads()
     __builtin_amdgcn_s_waitcnt(0x0f70 | (COUNT & 15) | (COUNT >> 4) << 14);
 }
 
-constexpr uint32_t kPagesHeld = 512;  // of runs of eight keys, in LDS
+constexpr uint32_t kHeld = 512;  // places of runs of eight keys, in LDS
 
 template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
 __global__ __launch_bounds__(64 * WAVES, (Shape<DK, DV, HALF, LATENT, WAVES, SPLIT,
@@ -598,7 +592,8 @@ void run_attention_kernel(RunAttention p)
     __shared__ __attribute__((aligned(16))) uint16_t lds[S::STAGES * S::STAGE];
     __shared__ v4f partial[SPLIT > 1 ? WAVES * GROUPS * NB * 64 : 1];
     __shared__ uint32_t flags[3][2];  // keys of a tile that are marked, by bit
-    __shared__ uint32_t pages_held[S::COPIED ? kPagesHeld : 1];
+    __shared__ uint2 held[S::COPIED ? kHeld : 1];  // bytes from the cache's first; bit 63: no page
+    __shared__ uint32_t any_bad;
     constexpr bool COPIED = S::COPIED;
     constexpr int STAGES = S::STAGES, PITCH = S::PITCH, THREADS = S::THREADS;
     using Order = Turned<DK>;
@@ -740,29 +735,37 @@ void run_attention_kernel(RunAttention p)
                     *reinterpret_cast<v2u *>(to + i * plane) = v2u{a[i], b[i]};
             }
         };
-        // The pages of the kPagesHeld / 2 runs of eight keys from one on, UINT32_MAX for none.
-        const auto hold_pages = [&](uint32_t first) {
-            for (uint32_t i = threadIdx.x; i < kPagesHeld / 2; i += THREADS) {
+        // Where the kHeld / 2 runs of eight keys from one on lie.
+        const auto hold_places = [&](uint32_t first) {
+            for (uint32_t i = threadIdx.x; i < kHeld / 2; i += THREADS) {
                 const uint32_t key = 8 * (first + i);
-                const float id = table[(key < last_key ? key : last_key) >> page_shift];
-                pages_held[(first + i) % kPagesHeld] =
-                    valid_index(id, p.shape.pages) ? uint32_t(id) : UINT32_MAX;
+                const uint32_t at = key <= last_key ? key : last_key & ~7u;
+                const float id = table[at >> page_shift];
+                const bool ok = valid_index(id, p.shape.pages);
+                const uint64_t bytes = (ok ? uint32_t(id) : 0) * page_bytes + head_bytes +
+                                       (at & in_page) * uint32_t(DK * sizeof(T));
+                held[(first + i) % kHeld] =
+                    uint2{uint32_t(bytes), uint32_t(bytes >> 32) | (ok ? 0 : 1u << 31)};
+                if (!ok)
+                    any_bad = 1;
             }
         };
-        const auto starts_pages = [&](uint32_t tile) {
-            return tile * (KEYS / 8) % (kPagesHeld / 2) == 0;
+        const auto starts_places = [&](uint32_t tile) {
+            return tile * (KEYS / 8) % (kHeld / 2) == 0;
         };
         // Starts the copies of a tile, the same number in every wave and tile.
         constexpr int COPIES = Load::MINE * (LATENT ? 1 : 2);
-        const auto copy_tile = [&](uint32_t tile) {
-            const uint32_t stage = lds_at + tile % STAGES * (2 * S::STAGE);
+        const auto copy_tile = [&](uint32_t tile, uint32_t slot) {
+            const uint32_t stage = lds_at + slot * (2 * S::STAGE);
+            uint2 place[Load::MINE];
+#pragma unroll
+            for (int i = 0; i < Load::MINE; ++i)
+                place[i] = held[(tile * (KEYS / 8) + Load::number(i, wave) / Load::EACH) % kHeld];
 #pragma unroll
             for (int i = 0; i < Load::MINE; ++i) {
-                const uint32_t n = Load::number(i, wave), eight = n / Load::EACH;
-                const uint32_t held =
-                    scalar(pages_held[(tile * (KEYS / 8) + eight) % kPagesHeld]);
-                const uint64_t at = (held == UINT32_MAX ? 0 : held) * page_bytes + head_bytes +
-                                    (key_of(tile, i) & in_page) * uint32_t(DK * sizeof(T));
+                const uint32_t n = Load::number(i, wave);
+                const uint64_t at =
+                    uint64_t(scalar(place[i].y) & 0x7fffffffu) << 32 | scalar(place[i].x);
                 const uint32_t to = stage + n * 1024;
                 copy_to_lds(static_cast<const uint8_t *>(p.key_pages) + at, load_at[OWN_AT ? i : 0],
                             to);
@@ -805,17 +808,20 @@ void run_attention_kernel(RunAttention p)
         };
 
         if constexpr (COPIED) {
-            __syncthreads();  // an earlier part's tiles and pages have been read
-            hold_pages(part.first * (KEYS / 8) / (kPagesHeld / 2) * (kPagesHeld / 2));
+            __syncthreads();  // an earlier part's tiles and places have been read
+            if (threadIdx.x == 0)
+                any_bad = 0;
+            __syncthreads();
+            hold_places(part.first * (KEYS / 8) / (kHeld / 2) * (kHeld / 2));
             __syncthreads();
 #pragma unroll
             for (int ahead = 0; ahead < STAGES - 1; ++ahead)
                 if (part.first + ahead < part.last) {
-                    if (ahead && starts_pages(part.first + ahead)) {
-                        hold_pages((part.first + ahead) * (KEYS / 8));
+                    if (ahead && starts_places(part.first + ahead)) {
+                        hold_places((part.first + ahead) * (KEYS / 8));
                         __syncthreads();
                     }
-                    copy_tile(part.first + ahead);
+                    copy_tile(part.first + ahead, ahead);
                 }
         } else {
             load_ids(part.first);
@@ -888,7 +894,7 @@ void run_attention_kernel(RunAttention p)
         }
         // Every row attends the keys before this one.
         const uint32_t common = length + (p.mask ? 0 : row0 / p.group + 1);
-        uint32_t turn = 0;
+        uint32_t turn = 0, slot = 0;
         __syncthreads();  // an earlier part's tiles and marks have been read
         if (threadIdx.x < 6)
             flags[threadIdx.x / 2][threadIdx.x % 2] = 0;
@@ -897,8 +903,12 @@ void run_attention_kernel(RunAttention p)
         for (uint32_t tile = part.first; tile < part.last; ++tile) {
             const uint32_t k0 = tile * KEYS;
             const bool mixed = k0 + KEYS > common;
-            uint16_t *stage = lds + tile % STAGES * S::STAGE;
+            uint16_t *stage = lds + slot * S::STAGE;
+            // The tile before's, free once every wave is here.
+            const uint32_t slot_behind = slot ? slot - 1 : STAGES - 1;
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
             uint64_t marks = 0;
+            const uint32_t next = tile + STAGES - 1;
             if constexpr (COPIED) {
                 // This tile's copies have ended, those of the ones behind it may not have.
                 const uint32_t behind = part.last - 1 - tile;
@@ -908,26 +918,24 @@ void run_attention_kernel(RunAttention p)
                     wait_loads<COPIES>();
                 else
                     wait_loads<0>();
-                const uint32_t next = tile + STAGES - 1;
-                if (next < part.last && starts_pages(next))
-                    hold_pages(next * (KEYS / 8));
+                if (next < part.last && starts_places(next))
+                    hold_places(next * (KEYS / 8));
                 __syncthreads();
-                if (next < part.last)
-                    copy_tile(next);
-                uint32_t none = uint32_t(__ballot(
-                    lane < KEYS / 8 &&
-                    pages_held[(tile * (KEYS / 8) + lane % (KEYS / 8)) % kPagesHeld] ==
-                        UINT32_MAX));
+                if (any_bad) {
+                    const uint32_t place = tile * (KEYS / 8) + lane % (KEYS / 8);
+                    uint32_t none = uint32_t(
+                        __ballot(lane < KEYS / 8 && held[place % kHeld].y >> 31));
+                    for (; none; none &= none - 1)
+                        marks |= 0xffull << 8 * __builtin_ctz(none);
+                }
                 if (mixed) {
                     check_tile(stage, turn);
                     __syncthreads();
-                    marks = uint64_t(flags[turn][1]) << 32 | flags[turn][0];
+                    marks |= uint64_t(flags[turn][1]) << 32 | flags[turn][0];
                     turn ^= 1;
                     if (threadIdx.x < 2)
                         flags[turn][threadIdx.x] = 0;
                 }
-                for (; none; none &= none - 1)
-                    marks |= 0xffull << 8 * __builtin_ctz(none);
             } else {
                 if (STAGES == 1)
                     __syncthreads();  // the tile before has been read
@@ -947,13 +955,16 @@ void run_attention_kernel(RunAttention p)
             v4f s[GROUPS][NB];
             if (active) {
                 const uint32_t me = SPLIT > 1 ? formed_here(lane) : lane;
-                // Copied rows: where depth v of a group of chunks lies.
+                // Copied rows: where the wave's depths v, v + PLACES, ... lie in their groups of
+                // chunks.
                 constexpr uint32_t PLACES = COPIED ? Order::G / 4 : 1;
                 uint32_t key_lane[PLACES];
 #pragma unroll
-                for (uint32_t v = 0; v < PLACES; ++v)
-                    key_lane[v] = (me & 15) * PITCH +
-                                  8 * (COPIED ? Order::place(me & 15, 4 * v + (me >> 4)) : me >> 4);
+                for (uint32_t v = 0; v < PLACES; ++v) {
+                    const uint32_t chunk = 4 * ((split * U + v) % PLACES) + (me >> 4);
+                    key_lane[v] =
+                        (me & 15) * PITCH + 8 * (COPIED ? Order::place(me & 15, chunk) : me >> 4);
+                }
                 // f32 caches: the largest product apart from the others, whose sums it would
                 // round.
                 v4f rest[GROUPS][HALF ? 1 : NB];
@@ -962,40 +973,50 @@ void run_attention_kernel(RunAttention p)
 #pragma unroll
                     for (int c = 0; c < NB; ++c)
                         s[g][c] = rest[g][HALF ? 0 : c] = v4f{0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    // Past the row's end a lane reads columns that the query's zeros drop.
+                // Reads are in the order (depth, key block, part), the smallest part first.
+                constexpr int READS = U * NB * PARTS, AHEAD = READS < 6 ? READS : 6;
+                const auto read = [&](int n) {
+                    const int u = n / (NB * PARTS), c = n / PARTS % NB;
+                    const int i = PARTS - 1 - n % PARTS;
                     uint32_t depth = split * U + u;
                     if (DEPTHS % SPLIT != 0 && depth >= uint32_t(DEPTHS))
-                        depth = DEPTHS - 1;
+                        depth = DEPTHS - 1;  // its queries are zero
                     const uint16_t *from = stage;
-                    static_assert(!COPIED || SPLIT == 1 || PLACES == 2, "depths of split rows");
-                    if constexpr (COPIED && SPLIT == 1)
-                        from += key_lane[u % PLACES] + u / PLACES * (32 * PLACES);
-                    else if constexpr (COPIED)
-                        from += (depth % 2 ? key_lane[PLACES - 1] : key_lane[0]) +
-                                depth / PLACES * (32 * PLACES);
-                    else
-                        from += key_lane[0] + 32 * depth;
+                    from += key_lane[u % PLACES] + depth / PLACES * (32 * PLACES);
+                    // Past the row's end a lane reads columns that the query's zeros drop.
                     if (DK % 32 != 0 && u == U - 1 && q >= 2)
                         from -= 16;
+                    return *reinterpret_cast<const v4u *>(from + 16 * c * PITCH +
+                                                          i * S::KEY_PLANE);
+                };
+                // Each is issued some products ahead of its own, where the compiler would
+                // place it right before them and wait.
+                v4u ahead[AHEAD];
 #pragma unroll
-                    for (int c = 0; c < NB; ++c)
+                for (int n = 0; n < AHEAD; ++n)
+                    ahead[n] = read(n);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int i = PARTS - 1; i >= 0; --i) {
-                            const v4u k = *reinterpret_cast<const v4u *>(
-                                from + 16 * c * PITCH + i * S::KEY_PLANE);
+                for (int n = 0; n < READS; ++n) {
+                    const int u = n / (NB * PARTS), c = n / PARTS % NB;
+                    const int i = PARTS - 1 - n % PARTS;
+                    const v4u k = ahead[n % AHEAD];
 #pragma unroll
-                            for (int b = (HALF ? 1 : 2) - i; b >= 0; --b)
+                    for (int b = (HALF ? 1 : 2) - i; b >= 0; --b)
 #pragma unroll
-                                for (int g = 0; g < GROUPS; ++g)
-                                    if (HALF || i + b == 0)
-                                        s[g][c] = mfma<HALF>(k, query[g][u][b], s[g][c]);
-                                    else
-                                        rest[g][HALF ? 0 : c] =
-                                            mfma<HALF>(k, query[g][u][b], rest[g][HALF ? 0 : c]);
-                        }
+                        for (int g = 0; g < GROUPS; ++g)
+                            if (HALF || i + b == 0)
+                                s[g][c] = mfma<HALF>(k, query[g][u][b], s[g][c]);
+                            else
+                                rest[g][HALF ? 0 : c] =
+                                    mfma<HALF>(k, query[g][u][b], rest[g][HALF ? 0 : c]);
+                    if (n + AHEAD < READS)
+                        ahead[n % AHEAD] = read(n + AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if constexpr (COPIED)
+                    if (next < part.last)
+                        copy_tile(next, slot_behind);  // beside the products
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
@@ -1007,6 +1028,9 @@ void run_attention_kernel(RunAttention p)
                             partial[((wave * GROUPS + g) * NB + c) * 64 + lane] = s[g][c];
                         }
                     }
+            } else if constexpr (COPIED) {
+                if (next < part.last)
+                    copy_tile(next, slot_behind);
             }
             if (SPLIT > 1) {
                 // The same sum, in the same order, in every wave of a row.
