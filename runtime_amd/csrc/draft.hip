@@ -10,30 +10,46 @@ constexpr int kBlock = 256;
 
 // ---- layout ----------------------------------------------------------------
 
-// Block s lays out the run of sequence s, block `sequences` marks the tokens in no run.
-// A token's ancestors have falling numbers, so one walk writes its mask from the last
-// word to the first.
+// Block s lays out the run of sequence s, block `sequences` marks the tokens in no run.  Runs
+// of up to 64 tokens are a wave's lanes, which form their ancestors in six steps: after k of
+// them a lane knows 2^k generations, and where the next one is.  Of longer runs a thread walks
+// from a token up; ancestors have falling numbers, so one walk writes the mask from its
+// last byte to its first.  Bound by the launch and three dependent reads: 16 tokens 4.6
+// us, 96 sequences of 8 to 64 (3.6 ancestors a token on average) the same; the walks and
+// bytes of a thread each took 13.0.
 constexpr uint32_t kLayoutParents = 4096;  // of a run, held in LDS
 
 __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
 {
     __shared__ float held[kLayoutParents];
-    const uint32_t s = blockIdx.x;
+    const uint32_t s = blockIdx.x, lane = threadIdx.x & 63;
+    const auto put = [&](uint32_t t, float sequence, float position, float place) {
+        p.sequences[t] = sequence;
+        p.positions[t] = position;
+        p.places[t] = place;
+    };
     const auto unset = [&](uint32_t t) {
-        p.sequences[t] = p.positions[t] = p.places[t] = -1.0f;
+        put(t, -1.0f, -1.0f, -1.0f);
         for (uint32_t b = 0; b < p.mask_bytes; ++b)
             p.mask[uint64_t(t) * p.mask_bytes + b] = 0;
     };
     if (s == p.runs.sequences) {
         // The list's first and last valid entry.
         uint32_t first = p.runs.tokens, last = p.runs.tokens;
-        for (uint32_t i = 0; i < p.runs.sequences; ++i) {
+        for (uint32_t base = 0; base < p.runs.sequences; base += 64) {
             RunBounds b;
-            if (!valid_bounds(p.runs, i, b))
+            const uint32_t i = base + lane;
+            const bool mine = i < p.runs.sequences;
+            const bool ok = mine && valid_bounds(p.runs, i, b);
+            const uint64_t wrong = __ballot(mine && !ok);
+            const uint64_t good = wrong ? (wrong & -wrong) - 1 : __ballot(ok);
+            if (good) {
+                if (base == 0)
+                    first = __shfl(b.begin, 0, 64);
+                last = __shfl(b.end, 63 - __builtin_clzll(good), 64);
+            }
+            if (wrong)
                 break;
-            if (i == 0)
-                first = b.begin;
-            last = b.end;
         }
         for (uint32_t t = threadIdx.x; t < p.runs.tokens; t += kBlock)
             if (t < first || t >= last)
@@ -44,6 +60,43 @@ __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
     const uint32_t n = run.end - run.begin;
     const float length = p.runs.lengths[s];
     const bool fits = valid_length(length, n, 1u << 24);
+    if (n <= 64) {
+        if (threadIdx.x >= 64 || !n)
+            return;
+        const uint32_t t = run.begin + (lane < n ? lane : n - 1);
+        int parent = int(lane) - 1;
+        bool good = lane < n;
+        if (p.parents) {
+            const float v = p.parents[t];
+            good = good && (v == -1.0f || valid_index(v, lane));
+            parent = good ? int(v) : -1;
+        }
+        // A token past the mask's last bit has no place.
+        good = good && (!p.mask || lane < 8ull * p.mask_bytes);
+        uint64_t seen = 1ull << lane;
+#pragma unroll
+        for (int step = 0; step < 6; ++step) {
+            const int from = parent < 0 ? int(lane) : parent;
+            const uint32_t low = __shfl(uint32_t(seen), from, 64);
+            const uint32_t high = __shfl(uint32_t(seen >> 32), from, 64);
+            const int far = __shfl(parent, from, 64);
+            const bool sound = __shfl(int(good), from, 64);
+            seen |= uint64_t(high) << 32 | low;
+            good = good && sound;
+            parent = parent < 0 ? parent : far;
+        }
+        if (lane >= n)
+            return;
+        if (!good || !fits) {
+            unset(t);
+            return;
+        }
+        put(t, float(s), length + float(__popcll(seen) - 1), length + float(lane));
+        uint8_t *row = p.mask + uint64_t(t) * p.mask_bytes;
+        for (uint32_t b = 0; b < p.mask_bytes; ++b)
+            row[b] = b < 8 ? uint8_t(seen >> 8 * b) : 0;
+        return;
+    }
     if (p.parents) {
         for (uint32_t i = threadIdx.x; i < n && i < kLayoutParents; i += kBlock)
             held[i] = p.parents[run.begin + i];
@@ -60,15 +113,16 @@ __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
         const uint32_t t = run.begin + i;
         uint32_t depth = 0;
         int at = int(i);
-        while ((at = parent_of(uint32_t(at))) >= 0)
-            ++depth;
+        if (p.parents)
+            while ((at = parent_of(uint32_t(at))) >= 0)
+                ++depth;
+        else
+            depth = i, at = -1;
         if (at == -2 || !fits || (p.mask && i >= 8ull * p.mask_bytes)) {
             unset(t);
             continue;
         }
-        p.sequences[t] = float(s);
-        p.positions[t] = length + float(depth);
-        p.places[t] = length + float(i);
+        put(t, float(s), length + float(depth), length + float(i));
         uint8_t *row = p.mask + uint64_t(t) * p.mask_bytes;
         at = int(i);
         for (int b = int(p.mask_bytes) - 1; b >= 0; --b) {
@@ -194,14 +248,25 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
 
 // ---- new tokens into latent caches --------------------------------------------
 
-// Block t takes token t: the sum of its latent's squares over the block, then latent,
-// key and queries, each pair of columns by a thread.
+// Block t takes token t: queries and key by V columns (and the V that they turn with) a
+// thread, the latent's squares summed over the block, then the latent.  V is 4 where the
+// widths allow, as it does everywhere but for odd ones.  Bound by the bytes: 4099 tokens of
+// 32 heads, rank 512 and rope 64 (82 MB).
+template <int V>
 __global__ __launch_bounds__(kBlock) void latent_append_kernel(LatentAppend p)
 {
+    typedef float piece __attribute__((ext_vector_type(V)));
+    typedef _Float16 half_piece __attribute__((ext_vector_type(V)));
     __shared__ float sums[kBlock / 64];
     const uint64_t t = blockIdx.x;
-    const float nan = __builtin_nanf("");
     const uint32_t pairs = p.rope / 2, width = p.rank + p.rope;
+    const uint32_t turns = pairs / V;  // of a head, V pairs each
+    const auto load = [](const float *at) { return *reinterpret_cast<const piece *>(at); };
+    // The first of a thread's loads go out before anything that they do not need.
+    const float *latent = p.latent + t * p.rank;
+    piece first = {};
+    if (threadIdx.x * V < p.rank)
+        first = load(latent + threadIdx.x * V);
     const float position = p.positions[t];
     const float place = p.places ? p.places[t] : position;
     const float sequence = p.sequences ? p.sequences[t] : float(t);
@@ -221,21 +286,65 @@ __global__ __launch_bounds__(kBlock) void latent_append_kernel(LatentAppend p)
     }
     if (!good) {
         for (uint32_t c = threadIdx.x; c < p.query_heads * p.rope; c += kBlock)
-            p.query_out[t * p.query_heads * p.rope + c] = nan;
+            p.query_out[t * p.query_heads * p.rope + c] = __builtin_nanf("");
         return;
     }
-    const auto store = [&](uint32_t c, float v) {
-        if (p.shape.half)
-            static_cast<_Float16 *>(p.pages)[row + c] = to_half(v);
-        else
-            static_cast<float *>(p.pages)[row + c] = v;
+    const auto store = [&](uint32_t c, piece v) {
+        if (p.shape.half) {
+            half_piece h;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                h[e] = to_half(v[e]);
+            *reinterpret_cast<half_piece *>(static_cast<_Float16 *>(p.pages) + row + c) = h;
+        } else {
+            *reinterpret_cast<piece *>(static_cast<float *>(p.pages) + row + c) = v;
+        }
     };
-    const float *latent = p.latent + t * p.rank;
+    const float *turn = p.rotation + uint64_t(uint32_t(position)) * p.rope;
+    // V pairs of a head: the V columns from `at` on and those behind them (interleaved), or
+    // half a head further.
+    const auto turned = [&](const float *in, uint32_t c, auto put) {
+        const piece cosine = load(turn + c), sine = load(turn + pairs + c);
+        const uint32_t low = p.interleaved ? 2 * c : c, high = p.interleaved ? low + V : pairs + c;
+        const piece x = load(in + low), y = load(in + high);
+        piece a = x, b = y;
+        if (p.interleaved) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                a[e] = 2 * e < V ? x[2 * e % V] : y[2 * e % V];
+                b[e] = 2 * e + 1 < V ? x[(2 * e + 1) % V] : y[(2 * e + 1) % V];
+            }
+        }
+        const piece u = a * cosine - b * sine, v = b * cosine + a * sine;
+        piece to_low = u, to_high = v;
+        if (p.interleaved) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                to_low[e] = e % 2 ? v[e / 2] : u[e / 2];
+                to_high[e] = (V + e) % 2 ? v[(V + e) / 2] : u[(V + e) / 2];
+            }
+        }
+        put(low, to_low);
+        put(high, to_high);
+    };
+    for (uint32_t i = threadIdx.x; i < p.query_heads * turns; i += kBlock) {
+        const uint32_t head = i / turns;
+        const uint64_t base = (t * p.query_heads + head) * p.rope;
+        turned(p.query + base, (i - head * turns) * V, [&](uint32_t at, piece v) {
+            *reinterpret_cast<piece *>(p.query_out + base + at) = v;
+        });
+    }
+    for (uint32_t c = threadIdx.x; c < turns; c += kBlock)
+        turned(p.key + t * p.rope, c * V, [&](uint32_t at, piece v) { store(p.rank + at, v); });
     float reciprocal = 1.0f;
     if (p.weight) {
         float squares = 0.0f;
-        for (uint32_t c = threadIdx.x; c < p.rank; c += kBlock)
-            squares += latent[c] * latent[c];
+        for (uint32_t c = threadIdx.x * V; c < p.rank; c += kBlock * V) {
+            const piece x = c < kBlock * V ? first : load(latent + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                squares += x[e] * x[e];
+        }
 #pragma unroll
         for (int offset = 32; offset > 0; offset >>= 1)
             squares += __shfl_xor(squares, offset, 64);
@@ -248,23 +357,9 @@ __global__ __launch_bounds__(kBlock) void latent_append_kernel(LatentAppend p)
             squares += sums[w];
         reciprocal = 1.0f / sqrtf(squares / float(p.rank) + p.epsilon);
     }
-    for (uint32_t c = threadIdx.x; c < p.rank; c += kBlock)
-        store(c, p.weight ? latent[c] * reciprocal * p.weight[c] : latent[c]);
-    const float *turn = p.rotation + uint64_t(uint32_t(position)) * p.rope;
-    const auto turned = [&](const float *in, uint32_t c, auto put) {
-        const uint32_t first = p.interleaved ? 2 * c : c;
-        const uint32_t second = p.interleaved ? 2 * c + 1 : pairs + c;
-        const float a = in[first], b = in[second], cosine = turn[c], sine = turn[pairs + c];
-        put(first, a * cosine - b * sine);
-        put(second, b * cosine + a * sine);
-    };
-    for (uint32_t c = threadIdx.x; c < pairs; c += kBlock)
-        turned(p.key + t * p.rope, c, [&](uint32_t at, float v) { store(p.rank + at, v); });
-    for (uint32_t i = threadIdx.x; i < p.query_heads * pairs; i += kBlock) {
-        const uint32_t head = i / pairs;
-        const uint64_t base = (t * p.query_heads + head) * p.rope;
-        turned(p.query + base, i - head * pairs,
-               [&](uint32_t at, float v) { p.query_out[base + at] = v; });
+    for (uint32_t c = threadIdx.x * V; c < p.rank; c += kBlock * V) {
+        const piece x = c < kBlock * V ? first : load(latent + c);
+        store(c, p.weight ? x * reciprocal * load(p.weight + c) : x);
     }
 }
 
@@ -295,8 +390,12 @@ void launch_settle(hipStream_t stream, const Settle &p)
 
 void launch_latent_append(hipStream_t stream, const LatentAppend &p)
 {
-    if (p.tokens)
-        latent_append_kernel<<<p.tokens, kBlock, 0, stream>>>(p);
+    if (!p.tokens)
+        return;
+    if (p.rank % 4 == 0 && p.rope % 8 == 0)
+        latent_append_kernel<4><<<p.tokens, kBlock, 0, stream>>>(p);
+    else
+        latent_append_kernel<1><<<p.tokens, kBlock, 0, stream>>>(p);
 }
 
 }  // namespace mfh
