@@ -140,8 +140,9 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 // key rows.
 //
 // Binary16 caches: keys and values are operands as they are, queries (scaled by a power of
-// two to below 2^15) and probabilities (times 2^15) two binary16 parts each, which are
-// within 2^-24 of the value.  f32 caches: all four are three bfloat16 parts, which hold 24
+// two to below 2^15) and probabilities (times 2^12, up to 2^15) two binary16 parts each, which
+// are within 2^-24 of the value; what is cut off of a probability is below 2^-36 of the
+// largest.  f32 caches: all four are three bfloat16 parts, which hold 24
 // bits, and six of the nine products are formed (the others are below 2^-26).
 //
 // The work is a line of units (a tile of keys; items in order, kItemUnits besides for each),
@@ -162,7 +163,9 @@ constexpr int kBlock = 256;
 constexpr uint32_t kItemUnits = 5;
 constexpr uint32_t kLeastUnits = 1;  // of a block
 constexpr uint32_t kMostBlocks = 1024;
-constexpr float kProbabilityShift = 15.0f;
+// A row's maximum is followed once it has risen by kSlack (powers of two), which the
+// probabilities are below then; binary16 ones are times 2^kProbabilityShift.
+constexpr float kSlack = 3.0f, kProbabilityShift = 12.0f;
 
 // What a block's first unfinished item needs of the join.
 struct Share {
@@ -464,10 +467,11 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PAR
             if (i + 1 < PARTS) {
                 // What is left, from the packed halves as they are: a - half in one
                 // instruction.
-                asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
-                    : "+v"(a) : "v"(out[i]));
-                asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-                    : "+v"(b) : "v"(out[i]));
+                const float x = a, y = b;
+                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
+                    : "=v"(a) : "v"(out[i]), "v"(x));
+                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                    : "=v"(b) : "v"(out[i]), "v"(y));
             }
         } else {
             out[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
@@ -1108,9 +1112,8 @@ void run_attention_kernel(RunAttention p)
                     for (int r = 0; r < 4; ++r)
                         top = fmaxf(top, s[g][c][r]);
                 top = fmaxf(m[g], quad_max(top) * times);
-                // While every score is -infinity, nothing is added.
-                const float base = top == -__builtin_inff() ? 0.0f : top;
-                if (__any(top > m[g])) {
+                if (__any(top > m[g] + kSlack)) {
+                    const float base = top == -__builtin_inff() ? 0.0f : top;
                     const float rescale = __builtin_amdgcn_exp2f(m[g] - base);
                     l[g] *= rescale;
 #pragma unroll
@@ -1118,6 +1121,8 @@ void run_attention_kernel(RunAttention p)
                         o[g][t] *= rescale;
                     m[g] = top;
                 }
+                // While every score is -infinity, nothing is added.
+                const float base = m[g] == -__builtin_inff() ? 0.0f : m[g];
                 const float line_at = HALF ? base - kProbabilityShift : base;
 #pragma unroll
                 for (int c = 0; c < NB; ++c)
