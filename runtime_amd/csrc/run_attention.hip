@@ -223,37 +223,38 @@ __device__ __forceinline__ bool load_run(const RunAttention &p, uint32_t i, Run 
 }
 
 // Units of a sequence's items, SHIFT the logarithm of a tile's keys.  Where tokens attend
-// all before them, a later item has more keys: (rows / group) a row tile more, counted in
-// whole tiles, so that the sum has a closed form.
+// all before them, a later item has more keys: `step` tiles more after every `every` items,
+// in whole numbers, so that the sum has a closed form.
 template <int SHIFT>
 struct Units {
-    uint32_t group, base, step;  // step: tiles that an item's rows are; 0: all items alike
+    uint32_t base, step, every;  // step 0: all items alike
     __device__ __forceinline__ Units(const RunAttention &p, const Run &run)
     {
         constexpr uint32_t KEYS = 1u << SHIFT;
-        group = p.group;
-        step = 0;
         base = kItemUnits;
+        step = 0;
+        every = 1;
         if (run.length == UINT32_MAX)
             return;
         if (p.mask || run.count == 1) {
             base += (run.length + run.count + KEYS - 1) >> SHIFT;
         } else {
-            step = p.rows / KEYS;
+            step = p.rows < KEYS ? 1 : p.rows / KEYS;
+            every = p.rows < KEYS ? KEYS / p.rows * p.group : p.group;
             base += ((run.length + KEYS - 1) >> SHIFT) + step;
         }
     }
     __device__ __forceinline__ uint32_t of(uint32_t tile) const
     {
-        return base + (step ? tile / group * step : 0);
+        return base + (step ? tile / every * step : 0);
     }
     // Of the first `tiles` items.
     __device__ __forceinline__ uint32_t upto(uint32_t tiles) const
     {
         uint32_t sum = tiles * base;
         if (step) {
-            const uint32_t whole = tiles / group, left = tiles - whole * group;
-            sum += step * (group * (whole * (whole - 1) / 2) + whole * left);
+            const uint32_t whole = tiles / every, left = tiles - whole * every;
+            sum += step * (every * (whole * (whole - 1) / 2) + whole * left);
         }
         return sum;
     }
@@ -609,7 +610,7 @@ void run_attention_kernel(RunAttention p)
     // The lane's places in a load: bytes from its first key's row, and elements in LDS,
     // which are held where they are few.
     constexpr uint32_t PER_ROW = DK / Load::PIECE;
-    constexpr bool HELD = Load::MINE <= 5 && !COPIED, OWN_AT = COPIED || Load::CHUNKS % 64 != 0;
+    constexpr bool HELD = Load::MINE <= 5 && DK != 256 && !COPIED, OWN_AT = COPIED || Load::CHUNKS % 64 != 0;
     uint32_t load_at[OWN_AT ? Load::MINE : 1], store_held[HELD ? Load::MINE : 1];
     const auto place = [&](int i, uint32_t me) {
         const uint32_t n = Load::number(i, wave), c = Load::chunk(n, me);
@@ -978,7 +979,8 @@ void run_attention_kernel(RunAttention p)
                     for (int c = 0; c < NB; ++c)
                         s[g][c] = rest[g][HALF ? 0 : c] = v4f{0, 0, 0, 0};
                 // Reads are in the order (depth, key block, part), the smallest part first.
-                constexpr int READS = U * NB * PARTS, AHEAD = READS < 6 ? READS : 6;
+                constexpr int READS = U * NB * PARTS, MOST = HALF ? 6 : 3;
+                constexpr int AHEAD = READS < MOST ? READS : MOST;
                 const auto read = [&](int n) {
                     const int u = n / (NB * PARTS), c = n / PARTS % NB;
                     const int i = PARTS - 1 - n % PARTS;
@@ -1452,21 +1454,24 @@ MatrixKernel matrix_kernel_with()
 template <int D>
 MatrixKernel matrix_kernel_of(bool half, bool many)
 {
-    constexpr bool WIDE = D > 128;
     if (half)
-        return many && !WIDE ? matrix_kernel_with<D, D, true, false, 4, 1, WIDE ? 1 : 2>()
-                             : matrix_kernel_with<D, D, true, false, 4, 1, 1>();
+        return many ? matrix_kernel_with<D, D, true, false, 4, 1, (D <= 128 ? 2 : 1)>()
+                    : matrix_kernel_with<D, D, true, false, 4, 1, 1>();
     // Three parts of a wide row need the registers of two waves.
     constexpr int SPLIT = D < 128 ? 1 : 2;
     return matrix_kernel_with<D, D, false, false, 4 * SPLIT, SPLIT, 1>();
 }
 template <int RANK, int ROPE>
-MatrixKernel latent_kernel_of(bool half, bool many)
+MatrixKernel latent_kernel_of(bool half, uint64_t rows, uint64_t sequences)
 {
+    constexpr int DK = RANK + ROPE;
     if (half)
-        return many ? matrix_kernel_with<RANK + ROPE, RANK, true, true, 8, 2, 1>()
-                    : matrix_kernel_with<RANK + ROPE, RANK, true, true, 8, 4, 1>();
-    return matrix_kernel_with<RANK + ROPE, RANK, false, true, 8, 4, 1>();
+        return rows > 32 * sequences ? matrix_kernel_with<DK, RANK, true, true, 8, 2, 1>()
+                                     : matrix_kernel_with<DK, RANK, true, true, 8, 4, 1>();
+    if constexpr (RANK == 512)
+        if (rows <= 16 * sequences)
+            return matrix_kernel_with<DK, RANK, false, true, 8, 8, 1>();
+    return matrix_kernel_with<DK, RANK, false, true, 8, 4, 1>();
 }
 MatrixKernel matrix_kernel(const RunAttention &p)
 {
@@ -1488,14 +1493,14 @@ MatrixKernel matrix_kernel(const RunAttention &p)
         default: return {};
         }
     }
-    const bool many = rows > 32 * uint64_t(p.runs.sequences);
+    const uint64_t sequences = p.runs.sequences;
     switch (p.value_dim * 1024 + rope) {
-    case 128 * 1024 + 32: return latent_kernel_of<128, 32>(half, many);
-    case 128 * 1024 + 64: return latent_kernel_of<128, 64>(half, many);
-    case 256 * 1024 + 32: return latent_kernel_of<256, 32>(half, many);
-    case 256 * 1024 + 64: return latent_kernel_of<256, 64>(half, many);
-    case 512 * 1024 + 32: return latent_kernel_of<512, 32>(half, many);
-    case 512 * 1024 + 64: return latent_kernel_of<512, 64>(half, many);
+    case 128 * 1024 + 32: return latent_kernel_of<128, 32>(half, rows, sequences);
+    case 128 * 1024 + 64: return latent_kernel_of<128, 64>(half, rows, sequences);
+    case 256 * 1024 + 32: return latent_kernel_of<256, 32>(half, rows, sequences);
+    case 256 * 1024 + 64: return latent_kernel_of<256, 64>(half, rows, sequences);
+    case 512 * 1024 + 32: return latent_kernel_of<512, 32>(half, rows, sequences);
+    case 512 * 1024 + 64: return latent_kernel_of<512, 64>(half, rows, sequences);
     default: return {};
     }
 }

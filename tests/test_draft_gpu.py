@@ -265,7 +265,8 @@ def check(got, want, bound, untouched):
 
 SHAPES = {"one": [(0, 1)], "first": [(0, 40)], "single": [(1, 1), (33, 1), (64, 1), (500, 1)],
           "mixed": [(0, 3), (5, 1), (16, 0), (31, 17), (64, 8), (100, 33), (0, 0), (129, 2)],
-          "long": [(4090, 9)], "wide": [(70, 130)], "many": [(3, 2)] * 70 + [(90, 5)]}
+          "long": [(4090, 9)], "wide": [(70, 130)], "many": [(3, 2)] * 70 + [(90, 5)],
+          "few": [(0, 2), (0, 0), (7, 0), (40, 3), (5, 0), (0, 1), (3, 0), (0, 0)]}
 
 
 def run_tree(backend, batch, query, keys, values, heads, kv_heads, dim):
@@ -286,8 +287,6 @@ def run_tree(backend, batch, query, keys, values, heads, kv_heads, dim):
 @pytest.mark.parametrize("kind", ["chain", "tree", "bits"])
 @pytest.mark.parametrize("which", list(SHAPES))
 def test_attention_of_runs(backend, which, kind, heads, kv_heads, dim, size, half):
-    if dim > 256 and which in ("long", "wide", "many"):
-        pytest.skip("the plain widths cover it")
     say("tree", which, kind, heads, kv_heads, dim, size, half)
     batch = Batch(dim * 31 + size + half, SHAPES[which], kind, size, 1, 2)
     keys, values = (random_pages(batch.rng, batch.pages, kv_heads, size, dim, half)
@@ -473,12 +472,11 @@ def run_latent(backend, batch, latent_query, rotary_query, pages, heads, scale):
     (16, 512, 64, 16), (5, 512, 32, 64), (128, 512, 64, 8), (20, 256, 64, 16), (64, 256, 32, 8),
     (3, 128, 64, 128), (33, 128, 32, 16), (4, 96, 32, 16), (7, 30, 6, 8), (1, 1, 2, 8),
     (2, 960, 64, 8), (6, 64, 0, 16)])
-@pytest.mark.parametrize("kind", ["chain", "tree", "bits", "none"])
-@pytest.mark.parametrize("which", ["one", "single", "mixed", "long", "wide"])
+@pytest.mark.parametrize("which,kind", [("one", "none"), ("single", "none")] + [
+    (which, kind) for which in ("one", "single", "mixed", "long", "wide", "few")
+    for kind in ("chain", "tree", "bits")])
 def test_latent_attention(backend, which, kind, heads, rank, rope, size, half):
     shapes = SHAPES[which]
-    if kind == "none" and which not in ("one", "single"):
-        pytest.skip("one token each")
     if heads * sum(n for _, n in shapes) > 5000:
         shapes = [(a, min(n, 40)) for a, n in shapes]
     say("latent", which, kind, heads, rank, rope, size, half)
@@ -728,3 +726,362 @@ def test_settling_of_bad_sequences(backend):
     assert emitted[4, 2:].tolist() == [-1, -1]
     assert counts[5] == 0 and last[5] == -1 and np.all(emitted[5] == -1)
     assert np.array_equal(backend.read(cache), old)
+
+
+# ---- together ---------------------------------------------------------------------------------
+
+def captured(backend, call):
+    """The call as a graph: (replay, end)."""
+    hip, stream = hiptime.hip(), ctypes.c_void_p(backend.stream())
+    graph, program = ctypes.c_void_p(), ctypes.c_void_p()
+    hiptime.check(hip.hipStreamBeginCapture(stream, 0), "begin capture")
+    try:
+        call()
+    finally:
+        hiptime.check(hip.hipStreamEndCapture(stream, ctypes.byref(graph)), "end capture")
+    hiptime.check(hip.hipGraphInstantiate(ctypes.byref(program), graph, None, None,
+                                          ctypes.c_size_t(0)), "instantiate")
+
+    def replay():
+        hiptime.check(hip.hipGraphLaunch(program, stream), "launch")
+
+    def end():
+        hiptime.check(hip.hipGraphExecDestroy(program), "destroy")
+        hiptime.check(hip.hipGraphDestroy(graph), "destroy")
+
+    return replay, end
+
+
+class Model:
+    """A layer of keys and values and one of latents over a vocabulary of projections; its
+    choice of the next token is the largest of its logits."""
+
+    heads, kv_heads, dim, rank, rope, vocab, size, sequences, columns = 4, 2, 64, 128, 32, 97, 8, 3, 6
+    most = 64  # places of a sequence
+
+    def __init__(self, backend, half, seed=3):
+        rng = np.random.default_rng(seed)
+        self.b = backend
+        shape = {"q": self.heads * self.dim, "k": self.kv_heads * self.dim,
+                 "v": self.kv_heads * self.dim, "lq": self.heads * self.rank,
+                 "lr": self.heads * self.rope, "c": self.rank, "r": self.rope}
+        self.by_token = {n: upload(backend, rng.standard_normal((self.vocab, w)).astype(np.float32))
+                         for n, w in shape.items()}
+        self.heads_out = {n: upload(backend, rng.standard_normal((self.vocab, w)).astype(np.float32))
+                          for n, w in (("q", shape["q"]), ("lq", shape["lq"]))}
+        self.weight = f32(backend, 1 + 0.1 * rng.standard_normal(self.rank))
+        self.turn, self.latent_turn = (backend.allocate_f32((self.most, w))
+                                       for w in (self.dim, self.rope))
+        backend.rotation_table(self.turn, 1.0e4)
+        backend.rotation_table(self.latent_turn, 1.0e4)
+        pages = self.sequences * self.most // self.size
+        self.table = f32(backend, rng.permutation(pages).reshape(self.sequences, -1))
+        self.caches = [backend.alloc_pages(pages, self.kv_heads, self.size, self.dim, half)
+                       for _ in range(2)]
+        self.caches.append(backend.alloc_pages(pages, 1, self.size, self.rank + self.rope, half))
+
+    def buffers(self, tokens):
+        a = self.b.allocate_f32
+        got = {n: a((tokens, w.shape[1])) for n, w in self.by_token.items()}
+        got |= {n: a((tokens, self.by_token[of].shape[1]))
+                for n, of in (("q'", "q"), ("lr'", "lr"), ("o", "q"), ("lo", "lq"))}
+        got |= {n: a((tokens, self.vocab)) for n in ("first", "second", "logits")}
+        return got | {n: a((tokens,)) for n in ("sequence", "position", "place", "choice")}
+
+    def run(self, w, tokens, starts, parents, lengths, mask):
+        """The choices after every token, whose keys, values and latents enter the caches."""
+        b = self.b
+        b.draft_layout(w["sequence"], w["position"], w["place"], mask, starts, parents, lengths)
+        for n in self.by_token:
+            b.gather_rows(w[n], self.by_token[n], tokens)
+        b.paged_qk_norm_rope_at(w["q'"], *self.caches[:2], w["q"], w["k"], w["v"], None, None,
+                                self.turn, self.table, w["sequence"], w["position"], w["place"],
+                                PagedRopeSpec(self.heads, self.kv_heads, self.dim), EPSILON)
+        b.paged_latent_append(w["lr'"], self.caches[2], w["lr"], w["c"], w["r"], self.weight,
+                              self.latent_turn, self.table, w["sequence"], w["position"],
+                              w["place"], self.heads, True, EPSILON)
+        b.paged_tree_gqa(w["o"], w["q'"], *self.caches[:2], self.table, starts, lengths, mask,
+                         GqaSpec(self.heads, self.kv_heads, self.dim))
+        b.paged_latent_attention(w["lo"], w["lq"], w["lr'"], self.caches[2], self.table, starts,
+                                 lengths, mask, self.heads, 0.08)
+        b.linear(w["first"], w["o"], self.heads_out["q"])
+        b.linear(w["second"], w["lo"], self.heads_out["lq"])
+        b.add(w["logits"], w["first"], w["second"])
+        b.argmax(w["choice"], w["logits"])
+
+
+def plain_decode(backend, half, prompts, steps):
+    """Token by token, each sequence's run of one."""
+    model = Model(backend, half)
+    lengths, last, said = np.zeros(3, np.float32), None, [[] for _ in prompts]
+    for at in range(max(map(len, prompts)) + steps):
+        tokens = np.array([p[at] if at < len(p) else s[-1] for p, s in zip(prompts, said)],
+                          np.float32)
+        w = model.buffers(3)
+        model.run(w, f32(backend, tokens), f32(backend, [0, 1, 2, 3]), None,
+                  f32(backend, lengths), None)
+        last = backend.read(w["choice"])
+        for i, p in enumerate(prompts):
+            if at >= len(p) - 1:
+                said[i].append(int(last[i]))
+        lengths += 1
+    return said
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_drafted_decoding_says_what_plain_decoding_says(backend, half, graph):
+    """Prompts in one run, then trees whose branches hold some of the true tokens: the
+    emitted tokens are those of decoding one at a time.  Largest logits stand apart by far
+    more than the order of sums moves them."""
+    rng = np.random.default_rng(17)
+    prompts = [list(rng.integers(0, 97, n)) for n in (9, 1, 4)]
+    truth = plain_decode(backend, half, prompts, 32)
+    model, b = Model(backend, half), backend
+    runs = [len(p) for p in prompts]
+    w = model.buffers(sum(runs) + 2)  # two padded tokens
+    tokens = f32(b, sum(prompts, []) + [5, 6])
+    model.run(w, tokens, f32(b, starts_of(runs)), None, f32(b, [0, 0, 0]), None)
+    choice = b.read(w["choice"])
+    said = [[int(choice[int(e) - 1])] for e in starts_of(runs)[1:]]
+    assert [s[0] for s in said] == [t[0] for t in truth]
+    lengths, n = f32(b, runs), 8
+    # Slots for runs of up to n tokens; the graph is captured once.
+    slot = {"tokens": b.allocate_f32((3 * n,)), "parents": b.allocate_f32((3 * n,)),
+            "starts": b.allocate_f32((4,)), "lengths": b.allocate_f32((3,)),
+            "mask": upload(b, np.zeros((3 * n, 1), np.uint8)),
+            "emitted": b.allocate_f32((3, model.columns)), "counts": b.allocate_f32((3,)),
+            "next": b.allocate_f32((3,)), "grown": b.allocate_f32((3,))}
+    w = model.buffers(3 * n)
+
+    def step():
+        model.run(w, slot["tokens"], slot["starts"], slot["parents"], slot["lengths"], slot["mask"])
+        b.settle_drafts(slot["emitted"], slot["counts"], slot["next"], model.caches,
+                        slot["tokens"], w["choice"], slot["starts"], slot["parents"],
+                        slot["lengths"], model.table)
+        b.add(slot["grown"], slot["lengths"], slot["counts"])
+
+    b.copy(slot["lengths"], lengths)
+    b.copy(slot["starts"], f32(b, [0, 0, 0, 0]))
+    step()  # of no runs: the workspace
+    assert np.all(b.read(slot["counts"]) == 0) and np.all(b.read(slot["next"]) == -1)
+    replay, end = captured(b, step) if graph else (step, lambda: None)
+    accepted = 0
+    for turn in range(4):
+        drafted, parents, sizes = [], [], [8, 5, 7] if turn % 2 else [3, 8, 1]
+        for s, t, size in zip(said, truth, sizes):
+            tree = random_tree(rng, size)
+            tree[1:] = np.maximum(tree[1:], 0)
+            depth = ancestors(tree).sum(axis=1) - 1
+            at = len(s) - 1
+            # The true token of a place on some branches, others elsewhere.
+            drafted += [s[-1] if i == 0 else t[at + d] if rng.random() < 0.7
+                        else (t[at + d] + 1) % 97 for i, d in enumerate(depth)]
+            parents += list(tree)
+        pad = 3 * n - len(drafted)
+        b.copy(slot["tokens"], f32(b, drafted + [0] * pad))
+        b.copy(slot["parents"], f32(b, parents + [-1] * pad))
+        b.copy(slot["starts"], f32(b, starts_of(sizes)))
+        replay()
+        emitted, counts = b.read(slot["emitted"]), b.read(slot["counts"]).astype(int)
+        last, grown = b.read(slot["next"]), b.read(slot["grown"])
+        for i in range(3):
+            assert 1 <= counts[i] <= model.columns
+            said[i] += [int(v) for v in emitted[i, :counts[i]]]
+            assert last[i] == said[i][-1] and np.all(emitted[i, counts[i]:] == -1)
+            assert said[i] == truth[i][:len(said[i])], (turn, i)
+            accepted += counts[i] - 1
+        b.copy(slot["lengths"], f32(b, grown))
+        assert np.all(grown == [len(p) + len(s) - 1 for p, s in zip(prompts, said)])
+    end()
+    assert accepted > 3
+
+
+def test_two_contexts_at_once():
+    """Calls of two contexts, queued without waiting, equal each one's alone."""
+    worlds = []
+    for seed, shapes in ((1, [(900, 12), (33, 4)]), (2, [(2000, 7)])):
+        backend = HipBackend(0)
+        batch = Batch(seed, shapes, "tree", 16)
+        keys, values = (random_pages(batch.rng, batch.pages, 2, 16, 64, True) for _ in range(2))
+        query = batch.rng.standard_normal((batch.tokens, 512)).astype(np.float32)
+        args = (upload(backend, query), upload(backend, keys), upload(backend, values),
+                *batch.args(backend), GqaSpec(8, 2, 64))
+        alone = backend.allocate_f32(query.shape)
+        backend.paged_tree_gqa(alone, *args)
+        worlds.append((backend, args, backend.read(alone),
+                       [backend.allocate_f32(query.shape) for _ in range(20)]))
+    for i in range(20):
+        for backend, args, _, outs in worlds:
+            backend.paged_tree_gqa(outs[i], *args)
+    for backend, _, want, outs in worlds:
+        assert all(np.array_equal(backend.read(out), want) for out in outs)
+        backend.close()
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("rank,rope", [(512, 64), (512, 32), (130, 32)])
+def test_latents_past_32_bits(backend, rank, rope, half):
+    """Pages whose elements, or bytes, lie past 2^32, entered, settled and attended."""
+    pages, size = 2000, 4096
+    assert 1990 * size * (rank + rope) > (2 ** 32 if rank == 512 else 2 ** 30)
+    rng = np.random.default_rng(5)
+    cache = backend.alloc_pages(pages, 1, size, rank + rope, half)
+    table = f32(backend, [[1999], [1990]])
+    latent, key, query = (rng.standard_normal((4, w)).astype(np.float32) for w in (rank, rope, rope))
+    out = backend.allocate_f32((4, rope))
+    turn = backend.allocate_f32((8, rope))
+    backend.rotation_table(turn, 1.0e4)
+    backend.paged_latent_append(out, cache, upload(backend, query), upload(backend, latent),
+                                upload(backend, key), None, turn, table,
+                                f32(backend, [0, 0, 0, 1]), f32(backend, [0, 1, 1, 0]),
+                                f32(backend, [0, 1, 2, 0]), 1, False, EPSILON)
+    emitted, counts, last = (backend.allocate_f32(s) for s in ((2, 4), (2,), (2,)))
+    # The second child is accepted and moves to place 1.
+    backend.settle_drafts(emitted, counts, last, [cache], f32(backend, [1, 2, 3, 1]),
+                          f32(backend, [3, 9, 8, 7]), f32(backend, [0, 3, 4]),
+                          f32(backend, [-1, 0, 0, -1]), f32(backend, [0, 0]), table)
+    assert backend.read(counts).tolist() == [2, 1] and backend.read(last).tolist() == [8, 7]
+    # A query that meets one row alone: the others' scores are far below.
+    result = backend.allocate_f32((2, rank))
+    want = latent.astype(np.float16).astype(np.float32) if half else latent
+    big = np.stack([want[2], want[3]]) * 40
+    backend.paged_latent_attention(result, upload(backend, big), backend.allocate_f32((2, rope)),
+                                   cache, table, None, f32(backend, [1, 0]), None, 1, 1.0)
+    assert np.all(np.abs(backend.read(result) - want[2:]) <= 4 * F32 * np.abs(want[2:]))
+    del cache
+
+
+# ---- refusals -----------------------------------------------------------------------------------
+
+def refused(variant, call, *args):
+    with pytest.raises(ExecutorError) as error:
+        call(*args)
+    assert error.value.variant == variant, error.value
+
+
+def changed(arguments, **of):
+    return [of.get(name, value) for name, value in arguments.items()]
+
+
+def test_layout_refusals(backend):
+    a = backend.allocate_f32
+    good = dict(sequences=a((6,)), positions=a((6,)), places=a((6,)),
+                mask=upload(backend, np.zeros((6, 1), np.uint8)), starts=a((3,)), parents=a((6,)),
+                lengths=a((2,)))
+    call = backend.draft_layout
+    call(*good.values())
+    call(*changed(good, parents=None, mask=None))
+    for name, other, variant in (
+            ("positions", a((5,)), "InvalidShape"), ("places", a((6, 1)), "InvalidShape"),
+            ("starts", a((2,)), "InvalidShape"), ("parents", a((7,)), "InvalidShape"),
+            ("lengths", a((2, 1)), "InvalidShape"), ("mask", a((6, 1)), "InvalidDType"),
+            ("mask", upload(backend, np.zeros((6, 0), np.uint8)), "InvalidShape"),
+            ("mask", upload(backend, np.zeros((5, 1), np.uint8)), "InvalidShape"),
+            ("places", good["positions"], "InvalidArgument"),
+            ("sequences", good["parents"], "InvalidArgument"),
+            ("sequences", good["mask"], "InvalidDType")):
+        refused(variant, call, *changed(good, **{name: other}))
+
+
+def test_attention_refusals(backend):
+    a = backend.allocate_f32
+    pages = lambda *shape: backend.alloc_pages(*shape)  # noqa: E731
+    good = dict(output=a((6, 256)), query=a((6, 256)), key_pages=pages(3, 2, 8, 64),
+                value_pages=pages(3, 2, 8, 64), tables=a((2, 4)), starts=a((3,)), lengths=a((2,)),
+                mask=upload(backend, np.zeros((6, 1), np.uint8)), spec=GqaSpec(4, 2, 64))
+    call = backend.paged_tree_gqa
+    call(*good.values())
+    for name, other, variant in (
+            ("output", a((6, 255)), "InvalidShape"), ("query", a((6, 128)), "InvalidShape"),
+            ("output", good["query"], "InvalidArgument"), ("tables", a((3, 4)), "InvalidShape"),
+            ("starts", a((4,)), "InvalidShape"), ("starts", None, "InvalidShape"),
+            ("lengths", a((3,)), "InvalidShape"), ("value_pages", good["key_pages"], "InvalidArgument"),
+            ("value_pages", pages(3, 2, 8, 32), "InvalidShape"),
+            ("mask", a((6, 1)), "InvalidDType"),
+            ("mask", upload(backend, np.zeros((5, 1), np.uint8)), "InvalidShape"),
+            ("spec", GqaSpec(3, 2, 64), "InvalidShape"), ("spec", GqaSpec(4, 2, 32), "InvalidShape")):
+        refused(variant, call, *changed(good, **{name: other}))
+    refused("Unsupported", call, a((2, 1025)), a((2, 1025)), pages(1, 1, 8, 1025),
+            pages(1, 1, 8, 1025), a((2, 1)), None, a((2,)), None, GqaSpec(1, 1, 1025))
+    good = dict(output=a((6, 4 * 128)), latent_query=a((6, 4 * 128)), rotary_query=a((6, 4 * 32)),
+                pages=pages(3, 1, 8, 160), tables=a((2, 4)), starts=a((3,)), lengths=a((2,)),
+                mask=None, heads=4, scale=0.1)
+    call = backend.paged_latent_attention
+    call(*good.values())
+    for name, other, variant in (
+            ("output", a((6, 4 * 160)), "InvalidShape"), ("rotary_query", a((6, 100)), "InvalidShape"),
+            ("rotary_query", a((5, 128)), "InvalidShape"), ("pages", pages(3, 2, 8, 160), "InvalidShape"),
+            ("pages", pages(3, 1, 8, 192), "InvalidShape"), ("heads", 3, "InvalidShape"),
+            ("heads", 0, "InvalidArgument"), ("scale", 0.0, "InvalidArgument"),
+            ("scale", NAN, "InvalidArgument"), ("output", good["latent_query"], "InvalidArgument"),
+            ("starts", None, "InvalidShape")):
+        refused(variant, call, *changed(good, **{name: other}))
+
+
+def test_entry_refusals(backend):
+    a = backend.allocate_f32
+    good = dict(query_out=a((2, 64)), pages=backend.alloc_pages(3, 1, 8, 48), query=a((2, 64)),
+                latent=a((2, 32)), key=a((2, 16)), weight=a((32,)), rotation=a((5, 16)),
+                tables=a((2, 2)), sequences=a((2,)), positions=a((2,)), places=a((2,)), heads=4,
+                interleaved=False, epsilon=EPSILON)
+    call = backend.paged_latent_append
+    call(*good.values())
+    call(*changed(good, sequences=None, places=None, weight=None))
+    for name, other, variant in (
+            ("query_out", a((2, 32)), "InvalidShape"), ("query", a((2, 60)), "InvalidShape"),
+            ("latent", a((2, 31)), "InvalidShape"), ("latent", a((2, 49)), "InvalidShape"),
+            ("key", a((2, 15)), "InvalidShape"), ("key", a((3, 16)), "InvalidShape"),
+            ("weight", a((16,)), "InvalidShape"), ("rotation", a((5, 14)), "InvalidShape"),
+            ("tables", a((2,)), "InvalidShape"), ("sequences", a((3,)), "InvalidShape"),
+            ("places", a((3,)), "InvalidShape"), ("positions", a((1,)), "InvalidShape"),
+            ("heads", 0, "InvalidArgument"), ("epsilon", 0.0, "InvalidArgument"),
+            ("pages", backend.alloc_pages(3, 2, 8, 48), "InvalidShape"),
+            ("query_out", good["query"], "InvalidArgument")):
+        refused(variant, call, *changed(good, **{name: other}))
+    pages = [backend.alloc_pages(2, 1, 8, 16) for _ in range(2)]
+    call = lambda places: backend.paged_qk_norm_rope_at(  # noqa: E731
+        a((2, 16)), *pages, a((2, 16)), a((2, 16)), a((2, 16)), None, None, a((4, 16)), a((2, 1)),
+        None, a((2,)), places, PagedRopeSpec(1, 1, 16), EPSILON)
+    call(f32(backend, [0, 1]))
+    refused("InvalidShape", call, a((3,)))
+    refused("InvalidDType", call, upload(backend, np.zeros(2, np.uint8)))
+
+
+def test_settling_refusals(backend):
+    a = backend.allocate_f32
+    pages = backend.alloc_pages(3, 2, 8, 4)
+    good = dict(emitted=a((2, 4)), counts=a((2,)), next=a((2,)), pages=[pages], tokens=a((6,)),
+                choices=a((6,)), starts=a((3,)), parents=a((6,)), lengths=a((2,)), tables=a((2, 1)))
+    call = backend.settle_drafts
+    call(*good.values())
+    for name, other, variant in (
+            ("emitted", a((3, 4)), "InvalidShape"), ("emitted", a((2, 0)), "InvalidShape"),
+            ("emitted", a((2, 1025)), "Unsupported"), ("counts", a((3,)), "InvalidShape"),
+            ("next", a((1,)), "InvalidShape"), ("choices", a((5,)), "InvalidShape"),
+            ("starts", a((2,)), "InvalidShape"), ("parents", a((5,)), "InvalidShape"),
+            ("tables", a((3, 1)), "InvalidShape"), ("pages", [pages, pages], "InvalidArgument"),
+            ("pages", [pages, backend.alloc_pages(3, 2, 16, 4)], "InvalidShape"),
+            ("pages", [a((3, 4))], "InvalidShape"), ("next", good["counts"], "InvalidArgument"),
+            ("counts", good["lengths"], "InvalidArgument")):
+        refused(variant, call, *changed(good, **{name: other}))
+
+
+def test_u8_readbacks(backend):
+    values = np.arange(300, dtype=np.uint8).reshape(30, 10)
+    buffer = upload(backend, values)
+    assert np.array_equal(backend.read_u8(buffer), values)
+    with pytest.raises(ExecutorError) as error:
+        backend.read(buffer)
+    assert error.value.variant == "InvalidDType"
+    with pytest.raises(ExecutorError) as error:
+        backend.read_u8(backend.allocate_f32((3,)))
+    assert error.value.variant == "InvalidDType"
+    limited = HipBackend(0, limits=Limits(max_total_bytes=64 << 20))
+    small = limited.upload_u8_classified((1000,), values.reshape(-1)[:300].repeat(4)[:1000], SCRATCH)
+    readback = limited.read_u8_async(small)
+    assert limited.resource_report().pending_operation_bytes == 1000
+    while readback.poll_step() is None:
+        pass
+    assert limited.resource_report().pending_operation_bytes == 0
+    limited.close()
