@@ -514,8 +514,10 @@ mfh_status mfh_draft_layout(mfh_ctx *ctx, mfh_buf *sequences, mfh_buf *positions
  * of a sequence whose length is no whole number, or that passes the table's row or
  * 2^24 with its run, and one that attends a key whose page id is bad, give NaN
  * rows.  What a token does not attend does not reach its row, whatever it holds (NaN
- * included); what it attends is expected to be finite.  head_dim <= 1024; 32, 64, 80, 96,
- * 112, 128, 160, 192 and 256 run on matrix cores, others many times slower. */
+ * included); what it attends is expected to be finite, and with f32 caches queries, keys
+ * and values are below 3.39e38 (larger ones give NaN) and, for the precision of f32, zero
+ * or above 2^-100.  head_dim <= 1024; 32, 64, 80, 96, 112, 128, 160, 192 and 256 run on
+ * matrix cores, others many times slower. */
 mfh_status mfh_paged_tree_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                               const mfh_buf *key_pages, const mfh_buf *value_pages,
                               const mfh_buf *tables, const mfh_buf *starts,

@@ -719,7 +719,8 @@ void run_attention_kernel(RunAttention p)
                         odd |= low || high;
                         x[e] &= (low ? 0xffff0000u : ~0u) & (high ? 0xffffu : ~0u);
                     } else {
-                        const bool all = (x[e] & 0x7f800000u) == 0x7f800000u;
+                        // The largest finite ones too: their first part would be infinite.
+                        const bool all = (x[e] & 0x7fffffffu) >= 0x7f7f8000u;
                         odd |= all;
                         x[e] = all ? 0 : x[e];
                     }

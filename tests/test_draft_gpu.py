@@ -411,6 +411,22 @@ def test_values_that_are_not_finite_reach_those_that_attend_them(backend, kind, 
     assert np.all(np.abs(got[~reached] - want[~reached]) <= bound[~reached])
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128, 20])
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_the_largest_finite_values_stay_with_those_that_attend_them(backend, kind, dim):
+    batch = Batch(dim + 8, [(37, 50)], kind, 16)
+    keys, values = (random_pages(batch.rng, batch.pages, 2, 16, dim, False) for _ in range(2))
+    query = batch.rng.standard_normal((50, 8 * dim)).astype(np.float32)
+    want, bound = batch.attend(query.reshape(-1, 8, dim), keys, values, 1 / math.sqrt(dim))
+    for token, pages in ((21, keys), (30, values)):
+        place = 37 + token
+        pages[int(batch.table[0, place // 16]), 1, place % 16] = np.finfo(np.float32).max
+    got = run_tree(backend, batch, query, keys, values, 8, 2, dim).reshape(want.shape)
+    reached = np.zeros((50, 8), bool)
+    reached[:, 4:] = batch.seen[0][:, [21, 30]].any(axis=1)[:, None]
+    assert np.all(np.abs(got[~reached] - want[~reached]) <= bound[~reached])
+
+
 @pytest.mark.parametrize("count", [1, 3, 64, 65, 255, 256, 257, 300])
 @pytest.mark.parametrize("dim", [64, 20])
 def test_any_count_of_runs(backend, count, dim):
