@@ -482,8 +482,8 @@ mfh_status mfh_paged_qk_norm_rope_at(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *
  * Runs: several new tokens of each sequence in one call.  The run of sequence s is
  * tokens starts[s] .. starts[s + 1] - 1 of the batch (`starts` F32 [sequences + 1]),
  * possibly none; its token i is cached at place lengths[s] + i, behind the
- * lengths[s] tokens that the sequence holds without it.  The first entry of
- * `starts` that is no whole number, falls below the one before it or passes the
+ * lengths[s] tokens that the sequence holds without it.  There are up to 65536
+ * sequences.  The first entry of `starts` that is no whole number, falls below the one before it or passes the
  * batch ends the list: sequences from there on have no run.  Rows of the batch
  * that are in no run (behind the last one, or padding before the first) are
  * left as they were by the attention calls.

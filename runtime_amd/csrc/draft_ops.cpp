@@ -15,6 +15,8 @@ namespace {
 
 // Blocks of 256 threads that a launch may have in one direction.
 constexpr uint64_t kMostBlocks = uint64_t(INT32_MAX) / 256;
+// Runs of a batch: blocks look through the list of starts up to their own.
+constexpr uint64_t kMostRuns = 65536;
 
 // The runs of a batch of `tokens`; `starts` may be null where `one_each`.
 mfh_status check_runs(mfh_ctx *ctx, const mfh_buf *starts, const mfh_buf *lengths,
@@ -34,7 +36,7 @@ mfh_status check_runs(mfh_ctx *ctx, const mfh_buf *starts, const mfh_buf *length
                                  "starts must be one per sequence and one"))) {
         return s;
     }
-    if (tokens > kMostBlocks || sequences > kMostBlocks)
+    if (tokens > kMostBlocks || sequences > kMostBlocks || (starts && sequences > kMostRuns))
         return fail(ctx, MFH_OVERFLOW, "token or sequence count exceeds the kernel index range");
     out->starts = starts ? dev_f32(starts) : nullptr;
     out->lengths = dev_f32(lengths);

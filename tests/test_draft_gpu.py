@@ -1000,6 +1000,37 @@ def test_layout_refusals(backend):
         refused(variant, call, *changed(good, **{name: other}))
 
 
+def test_runs_beyond_the_longest_list(backend):
+    a = backend.allocate_f32
+    most = 65536
+    for count in (most, most + 1):
+        layout = [a((1,)), a((1,)), a((1,)), None, a((count + 1,)), None, a((count,))]
+        attention = [a((1, 64)), a((1, 64)), backend.alloc_pages(1, 1, 8, 64),
+                     backend.alloc_pages(1, 1, 8, 64), a((count, 1)), a((count + 1,)),
+                     a((count,)), None, GqaSpec(1, 1, 64)]
+        settle = [a((count, 1)), a((count,)), a((count,)), [], a((1,)), a((1,)), a((count + 1,)),
+                  None, a((count,)), a((count, 1))]
+        for call, arguments in ((backend.draft_layout, layout), (backend.paged_tree_gqa, attention),
+                                (backend.settle_drafts, settle)):
+            if count > most:
+                refused("Overflow", call, *arguments)
+            else:
+                call(*arguments)
+    backend.synchronize()
+
+
+def test_many_sequences(backend):
+    # The last of the longest list's runs has all three tokens.
+    most = 65536
+    starts = np.zeros(most + 1, np.float32)
+    starts[-1] = 3
+    outputs = [backend.allocate_f32((3,)) for _ in range(3)]
+    backend.draft_layout(*outputs, None, f32(backend, starts), None,
+                         f32(backend, np.full(most, 5, np.float32)))
+    got = [backend.read(o) for o in outputs]
+    assert np.array_equal(got, [[most - 1] * 3, [5, 6, 7], [5, 6, 7]])
+
+
 def test_attention_refusals(backend):
     a = backend.allocate_f32
     pages = lambda *shape: backend.alloc_pages(*shape)  # noqa: E731
