@@ -1,4 +1,5 @@
-// Device code shared by the digit GEMMs (gemm_mx.hip, gemm_i8.hip).
+// Device code shared by the digit GEMMs (gemm_mx.hip, gemm_i8.hip); copy_to_lds also serves
+// attention of runs (run_attention.hip).
 //
 // Number range.  The kernels' sums are true magnitudes in f32, which serves
 // ordinary values.  Where a row's 128-group is so small that a factor of its

@@ -16,7 +16,10 @@ namespace {
 // ---- any width -----------------------------------------------------------------
 
 // A wave per (token, query head): 64 keys at a time, a lane forms one key's score, then the
-// lanes are columns of the values.
+// lanes are columns of the values.  Every token and head reads the cache for itself, a
+// lane a row of its own: bound by the latency of scattered reads.  The cases given below
+// take 37 to 300 times as long (one tree 749 us, 48 trees 14.6 ms); it is for widths that
+// have no kernel there.
 __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention p)
 {
     extern __shared__ float lds[];
@@ -129,27 +132,47 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 
 // ---- matrix cores ---------------------------------------------------------------
 //
-// Query rows of a key/value head are (token, head of the group) pairs, counted through a run;
-// an item is (sequence, key/value head, 64 of its rows), a wave of a block has 16
-// of them (of a latent cache two waves have the same 16).  The block walks the item's keys a tile at a time: all threads load a tile's rows
-// to registers (the next tile's while this one is worked on) and store them to LDS as
-// operands that the waves share.  Per tile, S^T = K Q^T leaves query row j in lane
-// column j (lane 16 q + j holds the scores of keys 16 c + 4 q + r in register r of
-// block c), the softmax follows online in the row's four lanes, and O^T += V^T P^T takes
-// those registers as its second operand; its first is put together from pieces of eight
-// key rows.
+// Query rows of a key/value head are (token, head of the group) pairs, counted through a run.
+// An item is (sequence, key/value head, a tile of its rows); a block walks the item's keys a
+// tile at a time, which all its waves share in LDS, a wave having 16 or 32 of the rows, or
+// (SPLIT waves to the same 16) a part of the key columns for the scores and of the value
+// columns for the output: one wave cannot hold queries and outputs 512 wide.  Per tile,
+// S^T = K Q^T leaves query row j in lane column j (lane 16 q + j holds the scores of keys
+// 16 c + 4 q + r in register r of block c), the softmax follows online in the row's four
+// lanes, and O^T += V^T P^T takes those registers as its second operand, so that
+// probabilities never pass through LDS; its first is put together from pieces of eight key
+// rows.
 //
 // Binary16 caches: keys and values are operands as they are, queries (scaled by a power of
 // two to below 2^15) and probabilities (times 2^12, up to 2^15) two binary16 parts each, which
 // are within 2^-24 of the value; what is cut off of a probability is below 2^-36 of the
 // largest.  f32 caches: all four are three bfloat16 parts, which hold 24
-// bits, and six of the nine products are formed (the others are below 2^-26).
+// bits, and six of the nine products are formed (the others are below 2^-26).  Six
+// products of 16 bits take 6/16 of the cycles of one of f32.
+//
+// Tiles of binary16 whose rows are whole groups of 64 columns are copied straight to LDS,
+// two to four stages ahead of the products: no registers, no instructions to store them, the
+// page ids of 256 runs of eight keys looked up at once.  Others pass through registers: f32
+// for its parts, other widths for their padding.
 //
 // The work is a line of units (a tile of keys; items in order, kItemUnits besides for each),
 // which every block adds up itself, for starts and lengths live on the device, and takes
 // an equal run of.  A block that holds all tiles of an item writes its rows; the others
 // store records (maximum, sum, unnormalised output) that a second launch joins in block
 // order, so that results do not depend on timing.
+//
+// What bounds it, in us of a call (the time of its bytes at a copy's 4.7 TB/s, or of its
+// products at the 1083 TFLOP/s of a large one):
+// - few rows over long caches, the cache's reads: 48 trees of 4 to 32 tokens over 17 to 8191
+//   keys, 32 / 8 heads of 128, binary16, 90 (63); 64 tokens of 16 heads over 100 to
+//   8191 latents of 512 + 64 49 (30);
+// - prompts, the issue of vector and matrix instructions, which share a SIMD's slot: 2048
+//   tokens over 2048, 32 / 8 heads of 64, 139 to 160 (95 with both parts of queries and
+//   probabilities), 37.0 M instructions of waves, 6.4 M of them products; 1024 over 1024
+//   latents, 32 heads, 305 to 330 (202);
+// - single sequences, what a launch and its dependent reads (starts, page ids, a tile, the
+//   join's shares and records) cost: 16 tokens over 2047 keys of 64, f32, 20, the
+//   smallest call (a tree over 127 keys) 14.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -160,11 +183,17 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
+// An item's queries, records and rows cost about five tiles (48 trees as above: 112 us at 2,
+// 100 at 4, 92 at 6, 100 at 8).
 constexpr uint32_t kItemUnits = 5;
-constexpr uint32_t kLeastUnits = 1;  // of a block
+// Units of a block: of more than one, a short call leaves CUs empty (one tree as above 20
+// us at 1, 28 at 4).
+constexpr uint32_t kLeastUnits = 1;
 constexpr uint32_t kMostBlocks = 1024;
 // A row's maximum is followed once it has risen by kSlack (powers of two), which the
-// probabilities are below then; binary16 ones are times 2^kProbabilityShift.
+// probabilities are below then; binary16 ones are times 2^kProbabilityShift.  Most tiles
+// then leave the outputs as they are (the prompts above 161 and 333 us; with every rise
+// followed 163 and 344).
 constexpr float kSlack = 3.0f, kProbabilityShift = 12.0f;
 
 // What a block's first unfinished item needs of the join.
@@ -493,9 +522,9 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c)
                                                        __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
-// Elements between LDS rows of D 16-bit columns: 16 bytes more than the row, so that 16
-// rows' pieces of one column fall on all banks, at places that differ by constants (an
-// order of pieces by row in place of the padding took a register for each).
+// Elements between LDS rows that pass through registers, of D 16-bit columns: 16 bytes more
+// than the row, so that 16 rows' pieces of one column fall on all banks, at places that
+// differ by constants.
 template <int D>
 constexpr int kPitch = D + 8;
 
@@ -524,6 +553,7 @@ struct Shape {
     static constexpr int PITCH = COPIED ? DK : kPitch<DK>;
     static constexpr int KEY_PLANE = KEYS * PITCH, VALUE_PLANE = LATENT ? 0 : KEY_PLANE;
     static constexpr int STAGE = PARTS * (KEY_PLANE + VALUE_PLANE);  // 16-bit elements
+    // Blocks on a CU: two waves to a SIMD either way, one where a wave needs all registers.
     static constexpr int RESIDENT = WAVES == 4 && DK <= 128 ? 2 : 1;
     // Of a CU's 160 KB of LDS, beside the scores that waves exchange.
     static constexpr int ROOM = (SPLIT > 1 ? 61440 : 73728) / RESIDENT / STAGE;
@@ -1250,7 +1280,9 @@ void run_attention_kernel(RunAttention p)
 // of the first launch has left to join and takes every so-many-th task of them.  A lane has a
 // 4-column piece; up to kFewRecords records a wave takes as many rows as its lanes hold
 // and reads all of a row's records at once, of more a block takes one row (and 256
-// columns), its lanes' shares every so-many-th record.
+// columns), its lanes' shares every so-many-th record.  Bound by dependent reads (shares,
+// then statistics and records): 5 us for one tree, 12 and 18 for the two prompts above,
+// whose records it reads once.
 constexpr uint32_t kFewRecords = 8, kJoinHeld = 8, kJoinsPerCu = 4;
 
 __global__ __launch_bounds__(kBlock) void run_attention_join_kernel(RunAttention p)
@@ -1452,16 +1484,24 @@ MatrixKernel matrix_kernel_with()
             S::RESIDENT, S::SHIFT};
 }
 // `many`: more rows than one item of the smaller kind has, on average over the sequences.
+// Then a wave has 32 of them, for which each operand read from LDS serves two products: the
+// prompt above 160 us against 180, 48 sequences of 24 tokens over 2047 (96 rows) 169 against
+// 193; of 16 tokens (64 rows) 147 against 126, of 8 118 against 105.
 template <int D>
 MatrixKernel matrix_kernel_of(bool half, bool many)
 {
     if (half)
         return many ? matrix_kernel_with<D, D, true, false, 4, 1, (D <= 128 ? 2 : 1)>()
                     : matrix_kernel_with<D, D, true, false, 4, 1, 1>();
-    // Three parts of a wide row need the registers of two waves.
+    // Three parts of a wide row need the registers of two waves (one wave spilled them).
     constexpr int SPLIT = D < 128 ? 1 : 2;
     return matrix_kernel_with<D, D, false, false, 4 * SPLIT, SPLIT, 1>();
 }
+// The fewer rows an item has, the more of a row's columns are a wave's own: items of 64
+// rows (two waves to a row), of 32 (four) and of 16 (eight, whose operand reads no other
+// wave shares).  Binary16, 64 sequences over 2047 latents of 512 + 64: of 32 rows 62 us in
+// items of 64, 60 of 32; of 64 rows 83 and 98; the prompt above 328 and 452.  f32, the same
+// of 16 rows: 121 in items of 16, 141 of 32; of 32 rows 202 and 167.
 template <int RANK, int ROPE>
 MatrixKernel latent_kernel_of(bool half, uint64_t rows, uint64_t sequences)
 {
