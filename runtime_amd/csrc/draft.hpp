@@ -120,8 +120,9 @@ struct RunAttention {
     uint32_t longest = 0;  // places of a table row, below 2^24
     float scale = 0.0f;    // times log2 e
     // Filled by run_attention_plan: blocks of the matrix-core kernel (0: the one of any
-    // width) and of the join, query rows of an item; its workspace of run_attention_scratch_bytes.
-    uint32_t blocks = 0, rows = 0, joins = 0;
+    // width) and of the join, query rows of an item, units besides its tiles; its workspace
+    // of run_attention_scratch_bytes.
+    uint32_t blocks = 0, rows = 0, joins = 0, item_units = 0;
     float *records = nullptr;
 };
 // Chooses the kernel and its split; false where the extents pass the index range.

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 // page ids of 256 runs of eight keys looked up at once.  Others pass through registers: f32
 // for its parts, other widths for their padding.
 //
-// The work is a line of units (a tile of keys; items in order, kItemUnits besides for each),
+// The work is a line of units (a tile of keys; items in order, item_units besides for each),
 // which every block adds up itself, for starts and lengths live on the device, and takes
 // an equal run of.  A block that holds all tiles of an item writes its rows; the others
 // store records (maximum, sum, unnormalised output) that a second launch joins in block
@@ -184,8 +184,9 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
 // An item's queries, records and rows cost about five tiles (48 trees as above: 112 us at 2,
-// 100 at 4, 92 at 6, 100 at 8).
-constexpr uint32_t kItemUnits = 5;
+// 100 at 4, 92 at 6, 100 at 8); where a CU has three blocks, of tiles of 32 keys, eight
+// (104 us at 3, 98 at 5, 90 at 8 and 12).
+constexpr uint32_t kItemUnits = 5, kItemUnitsOfThree = 8;
 // Units of a block: of more than one, a short call leaves CUs empty (one tree as above 20
 // us at 1, 28 at 4).
 constexpr uint32_t kLeastUnits = 1;
@@ -260,7 +261,7 @@ struct Units {
     __device__ __forceinline__ Units(const RunAttention &p, const Run &run)
     {
         constexpr uint32_t KEYS = 1u << SHIFT;
-        base = kItemUnits;
+        base = p.item_units;
         step = 0;
         every = 1;
         if (run.length == UINT32_MAX)
@@ -419,14 +420,14 @@ __device__ __forceinline__ bool next_part(const RunAttention &p, Line &line, Par
     const uint32_t tiles = (part.keys + (1u << SHIFT) - 1) >> SHIFT;
     // The item's last units may be more or fewer than its tiles.
     const auto tile_at = [&](uint32_t unit) {
-        const uint32_t t = unit > kItemUnits ? unit - kItemUnits : 0;
+        const uint32_t t = unit > p.item_units ? unit - p.item_units : 0;
         return unit == units || t > tiles ? tiles : t;
     };
     part.first = tile_at(from);
     part.last = tile_at(to);
-    part.leads = from <= kItemUnits;
+    part.leads = from <= p.item_units;
     part.opens = from == 0;
-    part.counts = to > kItemUnits;
+    part.counts = to > p.item_units;
     part.whole = part.leads && to == units;
     part.record = 2 * line.block + (line.at == line.start ? 0 : 1);
     part.last_unit = line.at - from + units - 1;
@@ -539,13 +540,13 @@ __device__ __forceinline__ uint32_t formed_here(uint32_t v)
 // What a kernel of a width has in a tile, in LDS and on a CU.  A wave has GROUPS times 16
 // rows; SPLIT waves share them, each with a part of the key columns for the scores and of
 // the value columns for the output.
-template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS, int RESIDENT>
 struct Shape {
     static constexpr int THREADS = 64 * WAVES;
     static constexpr int ROWS = 16 * GROUPS * WAVES / SPLIT;
     static constexpr int PARTS = HALF ? 1 : 3;          // of keys and values
     static constexpr int QUERY_PARTS = HALF ? 2 : 3;    // of queries and probabilities
-    static constexpr int SHIFT = DK * GROUPS <= (HALF ? 128 : 64) ? 6 : 5;
+    static constexpr int SHIFT = RESIDENT < 3 && DK * GROUPS <= (HALF ? 128 : 64) ? 6 : 5;
     static constexpr int KEYS = 1 << SHIFT;
     // Copied to LDS without passing through registers: rows as they are, of which eight
     // are whole copies of a wave.
@@ -553,8 +554,6 @@ struct Shape {
     static constexpr int PITCH = COPIED ? DK : kPitch<DK>;
     static constexpr int KEY_PLANE = KEYS * PITCH, VALUE_PLANE = LATENT ? 0 : KEY_PLANE;
     static constexpr int STAGE = PARTS * (KEY_PLANE + VALUE_PLANE);  // 16-bit elements
-    // Blocks on a CU: two waves to a SIMD either way, one where a wave needs all registers.
-    static constexpr int RESIDENT = WAVES == 4 && DK <= 128 ? 2 : 1;
     // Of a CU's 160 KB of LDS, beside the scores that waves exchange.
     static constexpr int ROOM = (SPLIT > 1 ? 61440 : 73728) / RESIDENT / STAGE;
     static constexpr int STAGES = !HALF ? 1 : !COPIED || ROOM < 2 ? 2 : ROOM < 4 ? ROOM : 4;
@@ -608,12 +607,11 @@ __device__ __forceinline__ void wait_loads()
 
 constexpr uint32_t kHeld = 512;  // places of runs of eight keys, in LDS
 
-template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
-__global__ __launch_bounds__(64 * WAVES, (Shape<DK, DV, HALF, LATENT, WAVES, SPLIT,
-                                                GROUPS>::RESIDENT * WAVES / 4))
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS, int RESIDENT>
+__global__ __launch_bounds__(64 * WAVES, (RESIDENT * WAVES / 4))
 void run_attention_kernel(RunAttention p)
 {
-    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>;
+    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS, RESIDENT>;
     using T = typename std::conditional<HALF, _Float16, float>::type;
     static_assert(DK % (SPLIT > 1 ? 32 : 16) == 0 && DV % (16 * SPLIT) == 0,
                   "widths of the matrix-core path");
@@ -1476,26 +1474,39 @@ struct MatrixKernel {
     void (*run)(RunAttention) = nullptr;
     int threads = 0, rows = 0, resident = 0, shift = 0;
 };
-template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS>
+template <int DK, int DV, bool HALF, bool LATENT, int WAVES, int SPLIT, int GROUPS, int RESIDENT>
 MatrixKernel matrix_kernel_with()
 {
-    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>;
-    return {run_attention_kernel<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS>, S::THREADS, S::ROWS,
-            S::RESIDENT, S::SHIFT};
+    using S = Shape<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS, RESIDENT>;
+    return {run_attention_kernel<DK, DV, HALF, LATENT, WAVES, SPLIT, GROUPS, RESIDENT>, S::THREADS,
+            S::ROWS, RESIDENT, S::SHIFT};
 }
-// `many`: more rows than one item of the smaller kind has, on average over the sequences.
-// Then a wave has 32 of them, for which each operand read from LDS serves two products: the
-// prompt above 160 us against 180, 48 sequences of 24 tokens over 2047 (96 rows) 169 against
-// 193; of 16 tokens (64 rows) 147 against 126, of 8 118 against 105.
+// Blocks on a CU: two waves to a SIMD, one where a wave needs all registers, three as below.
+//
+// `many`: more rows than one item has, on average over the sequences.  Up to 112 wide a wave
+// then has 32 of them, for which each operand read from LDS serves two products: the
+// prompt above 160 us against 180, and of heads 128 wide 48 sequences of 24 tokens over 2047
+// (96 rows) 169 against 193, of 16 tokens (64 rows) 147 against 126.  Of 128 columns that
+// is all registers of two waves and some spilled; three waves of 16 rows, with tiles of 32
+// keys, take 158 there, and 172 against 189 of 32 tokens, but with few rows, where loads
+// and the start count, longer than two with tiles of 64: 16 tokens over 2047 31 us against 23,
+// 48 x 4 over 17 to 8191 62 against 59.
 template <int D>
 MatrixKernel matrix_kernel_of(bool half, bool many)
 {
-    if (half)
-        return many ? matrix_kernel_with<D, D, true, false, 4, 1, (D <= 128 ? 2 : 1)>()
-                    : matrix_kernel_with<D, D, true, false, 4, 1, 1>();
+    constexpr int RESIDENT = D <= 128 ? 2 : 1;
+    if (half) {
+        if constexpr (D <= 128)
+            if (many)
+                return matrix_kernel_with<D, D, true, false, 4, 1, (D < 128 ? 2 : 1),
+                                          (D < 128 ? 2 : 3)>();
+        return matrix_kernel_with<D, D, true, false, 4, 1, 1, RESIDENT>();
+    }
     // Three parts of a wide row need the registers of two waves (one wave spilled them).
-    constexpr int SPLIT = D < 128 ? 1 : 2;
-    return matrix_kernel_with<D, D, false, false, 4 * SPLIT, SPLIT, 1>();
+    if constexpr (D < 128)
+        return matrix_kernel_with<D, D, false, false, 4, 1, 1, RESIDENT>();
+    else
+        return matrix_kernel_with<D, D, false, false, 8, 2, 1, 1>();
 }
 // The fewer rows an item has, the more of a row's columns are a wave's own: items of 64
 // rows (two waves to a row), of 32 (four) and of 16 (eight, whose operand reads no other
@@ -1507,12 +1518,12 @@ MatrixKernel latent_kernel_of(bool half, uint64_t rows, uint64_t sequences)
 {
     constexpr int DK = RANK + ROPE;
     if (half)
-        return rows > 32 * sequences ? matrix_kernel_with<DK, RANK, true, true, 8, 2, 1>()
-                                     : matrix_kernel_with<DK, RANK, true, true, 8, 4, 1>();
+        return rows > 32 * sequences ? matrix_kernel_with<DK, RANK, true, true, 8, 2, 1, 1>()
+                                     : matrix_kernel_with<DK, RANK, true, true, 8, 4, 1, 1>();
     if constexpr (RANK == 512)
         if (rows <= 16 * sequences)
-            return matrix_kernel_with<DK, RANK, false, true, 8, 8, 1>();
-    return matrix_kernel_with<DK, RANK, false, true, 8, 4, 1>();
+            return matrix_kernel_with<DK, RANK, false, true, 8, 8, 1, 1>();
+    return matrix_kernel_with<DK, RANK, false, true, 8, 4, 1, 1>();
 }
 MatrixKernel matrix_kernel(const RunAttention &p)
 {
@@ -1558,10 +1569,11 @@ bool run_attention_plan(RunAttention &p, int cu_count)
     if (!kernel.run || !rows || !p.runs.sequences)
         return true;
     p.rows = kernel.rows;
+    p.item_units = kernel.resident == 3 ? kItemUnitsOfThree : kItemUnits;
     // Units stay in 32 bits.
     const uint64_t items = (uint64_t(p.runs.tokens) * p.group / p.rows + p.runs.sequences) *
                            p.shape.kv_heads;
-    const uint64_t most = items * (kItemUnits + 6 + ((uint64_t(p.longest) + p.runs.tokens) >>
+    const uint64_t most = items * (p.item_units + 6 + ((uint64_t(p.longest) + p.runs.tokens) >>
                                                      kernel.shift));
     if (most >= uint64_t(1) << 31)
         return false;
