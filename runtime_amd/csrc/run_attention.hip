@@ -1493,7 +1493,7 @@ MatrixKernel matrix_kernel_with()
 // prompt above 160 us against 180, and of heads 128 wide 48 sequences of 24 tokens over 2047
 // (96 rows) 169 against 193, of 16 tokens (64 rows) 147 against 126.  Of 128 columns that
 // is all registers of two waves and some spilled; three waves of 16 rows, with tiles of 32
-// keys, take 158 there, and 172 against 189 of 32 tokens, but with few rows, where loads
+// keys, take 158 there, and 168 against 189 of 32 tokens, but with few rows, where loads
 // and the start count, longer than two with tiles of 64: 16 tokens over 2047 31 us against 23,
 // 48 x 4 over 17 to 8191 62 against 59.
 template <int D>
