@@ -570,13 +570,23 @@ mfh_status mfh_paged_latent_attention(mfh_ctx *ctx, mfh_buf *output,
  * token of its next run (-1 without a run).  In each of the page buffers (of any heads,
  * widths and formats, one page size; all layers' keys, values or latents) the path's rows are
  * moved to places lengths[s], lengths[s] + 1, ...; what lies behind them is as before
- * or a moved row.  A sequence whose length is bad, or whose path has a place without a
- * page, is left as it is, with NaN for its three outputs.  columns <= 1024. */
+ * or a moved row.  A sequence with a run that is left as it is, with NaN for its three
+ * outputs: its length is bad, its first token's parent is not -1, or its path has a place
+ * without a page.  All tokens of a run count as stored; where the layout may refuse some
+ * (those past a mask's last bit), mfh_settle_drafts_at is told.  columns <= 1024. */
 mfh_status mfh_settle_drafts(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mfh_buf *next,
                              mfh_buf *const *pages, size_t buffers, const mfh_buf *tokens,
                              const mfh_buf *choices, const mfh_buf *starts,
                              const mfh_buf *parents, const mfh_buf *lengths,
                              const mfh_buf *tables);
+/* The same with the `places` of mfh_draft_layout: a token whose place is not lengths[s] + its
+ * number (-1: it was not stored) is not accepted, and a run whose first token is one is a
+ * bad one, as above. */
+mfh_status mfh_settle_drafts_at(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mfh_buf *next,
+                                mfh_buf *const *pages, size_t buffers, const mfh_buf *tokens,
+                                const mfh_buf *choices, const mfh_buf *starts,
+                                const mfh_buf *parents, const mfh_buf *places,
+                                const mfh_buf *lengths, const mfh_buf *tables);
 
 /* Copy page from_pages[i] of sources[b] to page to_pages[i] of destinations[b],
  * for every i < count and b < buffers (a model's key and value pages of all

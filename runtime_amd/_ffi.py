@@ -145,6 +145,7 @@ SIGNATURES = {
     "mfh_paged_latent_append": (S, [P] * 12 + [ctypes.c_uint32, ctypes.c_int, ctypes.c_float]),
     "mfh_paged_latent_attention": (S, [P] * 9 + [ctypes.c_uint32, ctypes.c_float]),
     "mfh_settle_drafts": (S, [P] * 4 + [PP, SZ] + [P] * 6),
+    "mfh_settle_drafts_at": (S, [P] * 4 + [PP, SZ] + [P] * 7),
     "mfh_copy_pages": (S, [P, PP, PP, SZ, P, P, SZ]),
     "mfh_sample_rows": (S, [P] * 6),
     # LFM2 token pass (minifield_lfm2.h)

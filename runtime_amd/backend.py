@@ -530,12 +530,16 @@ class HipBackend:
 
     def settle_drafts(self, emitted: Buffer, counts: Buffer, next: Buffer,
                       pages: Sequence[Buffer], tokens: Buffer, choices: Buffer, starts: Buffer,
-                      parents: Buffer | None, lengths: Buffer, tables: Buffer) -> None:
+                      parents: Buffer | None, lengths: Buffer, tables: Buffer,
+                      places: Buffer | None = None) -> None:
         handles = (ctypes.c_void_p * max(1, len(pages)))(*[b.handle for b in pages])
-        self._check(_ffi.lib().mfh_settle_drafts(
-            self._ctx, emitted.handle, counts.handle, next.handle, handles, len(pages),
-            tokens.handle, choices.handle, starts.handle, _h(parents), lengths.handle,
-            tables.handle))
+        given = (self._ctx, emitted.handle, counts.handle, next.handle, handles, len(pages),
+                 tokens.handle, choices.handle, starts.handle, _h(parents))
+        if places is None:
+            self._check(_ffi.lib().mfh_settle_drafts(*given, lengths.handle, tables.handle))
+        else:
+            self._check(_ffi.lib().mfh_settle_drafts_at(*given, places.handle, lengths.handle,
+                                                        tables.handle))
 
     def copy_pages(self, destinations: Sequence[Buffer], sources: Sequence[Buffer], from_pages,
                    to_pages) -> None:

@@ -180,7 +180,11 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
     const RunBounds run = run_of(p.runs, s);
     const uint32_t n = run.end - run.begin;
     const float length = p.runs.lengths[s];
-    const bool fits = n && valid_length(length, n, 1u << 24);
+    // The layout refuses a run whose first token follows another.
+    const float root = n && p.parents ? p.parents[run.begin] : -1.0f;
+    const float first = n && p.places ? p.places[run.begin] : length;
+    const bool fits =
+        n && valid_length(length, n, 1u << 24) && root == -1.0f && first == length;
     uint32_t count = 0;
     if (threadIdx.x == 0)
         bad = 0;
@@ -199,8 +203,10 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
             for (uint32_t base = at + 1; base < n; base += 64) {
                 const uint32_t i = base + lane, t = run.begin + (i < n ? i : n - 1);
                 const float parent = p.parents ? p.parents[t] : float(int(i) - 1);
-                const uint64_t found =
-                    __ballot(i < n && parent == float(at) && p.drafted[t] == choice);
+                // A token without a place was not stored.
+                const float own = length + float(i), place = p.places ? p.places[t] : own;
+                const uint64_t found = __ballot(i < n && parent == float(at) &&
+                                                p.drafted[t] == choice && place == own);
                 if (found) {
                     child = base + uint32_t(__builtin_ctzll(found));
                     break;

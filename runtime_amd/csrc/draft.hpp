@@ -76,7 +76,7 @@ void launch_draft_layout(hipStream_t stream, const DraftLayout &p);
 constexpr uint32_t kSettleBuffers = 64, kSettleColumns = 1024;
 struct Settle {
     Runs runs;
-    const float *parents = nullptr;  // [tokens], may be null
+    const float *parents = nullptr, *places = nullptr;   // [tokens], may be null
     const float *drafted = nullptr, *choices = nullptr;  // [tokens]
     const float *tables = nullptr;   // [sequences, max_pages]
     float *emitted = nullptr;        // [sequences, columns], null past the first launch

@@ -107,6 +107,100 @@ mfh_status attend(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
     return launched(ctx);
 }
 
+// Settling; `parents` and `places` may be null.
+mfh_status settle(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mfh_buf *next,
+                  mfh_buf *const *pages, size_t buffers, const mfh_buf *tokens,
+                  const mfh_buf *choices, const mfh_buf *starts, const mfh_buf *parents,
+                  const mfh_buf *places, const mfh_buf *lengths, const mfh_buf *tables)
+{
+    if (!ctx)
+        return MFH_INVALID_ARGUMENT;
+    mfh_status s = check_operation(ctx, MFH_OP_COPY);
+    if (!s)
+        s = check_f32(ctx, tokens);
+    if (s)
+        return s;
+    if (tokens->rank != 1)
+        return fail(ctx, MFH_INVALID_SHAPE, "drafted tokens must be one per token");
+    Settle p;
+    if ((s = check_runs(ctx, starts, lengths, tokens->dims[0], false, &p.runs)) ||
+        (s = check_vector(ctx, choices, tokens->dims[0], "choices must be one per token")) ||
+        (parents && (s = check_vector(ctx, parents, tokens->dims[0],
+                                      "parents must be one per token"))) ||
+        (places && (s = check_vector(ctx, places, tokens->dims[0],
+                                     "places must be one per token"))) ||
+        (s = check_tables(ctx, tables)) || (s = check_f32(ctx, emitted)) ||
+        (s = check_vector(ctx, counts, p.runs.sequences, "counts must be one per sequence")) ||
+        (s = check_vector(ctx, next, p.runs.sequences, "next tokens must be one per sequence")))
+        return s;
+    if (tables->dims[0] != p.runs.sequences)
+        return fail(ctx, MFH_INVALID_SHAPE, "page tables must have a row per sequence");
+    if (emitted->rank != 2 || emitted->dims[0] != p.runs.sequences || emitted->dims[1] == 0)
+        return fail(ctx, MFH_INVALID_SHAPE, "emitted tokens must be [sequences, columns]");
+    if (emitted->dims[1] > kSettleColumns)
+        return fail(ctx, MFH_UNSUPPORTED, "accepted paths are at most 1024 tokens long");
+    if (buffers && !pages)
+        return fail(ctx, MFH_INVALID_ARGUMENT, "page buffer list is null");
+    PageShape first;
+    for (size_t i = 0; i < buffers; ++i) {
+        PageShape shape;
+        if ((s = page_shape(ctx, pages[i], &shape)))
+            return s;
+        if (i == 0)
+            first = shape;
+        if (shape.page_shift != first.page_shift)
+            return fail(ctx, MFH_INVALID_SHAPE, "page buffers differ in page size");
+        // A path's pages are in every buffer.
+        first.pages = shape.pages < first.pages ? shape.pages : first.pages;
+        if (uint64_t(shape.kv_heads) * shape.head_dim > uint64_t(UINT16_MAX) * 256)
+            return fail(ctx, MFH_OVERFLOW, "page extent exceeds the kernel index range");
+        if (aliases(pages[i], {emitted, counts, next, tokens, choices, starts, parents, places,
+                               lengths, tables}))
+            return aliased(ctx);
+        for (size_t j = 0; j < i; ++j)
+            if (pages[j]->dev == pages[i]->dev)
+                return fail(ctx, MFH_INVALID_ARGUMENT, "a page buffer is listed twice");
+    }
+    if (aliases(emitted, {counts, next, tokens, choices, starts, parents, places, lengths, tables}) ||
+        aliases(counts, {next, tokens, choices, starts, parents, places, lengths, tables}) ||
+        aliases(next, {tokens, choices, starts, parents, places, lengths, tables}))
+        return aliased(ctx);
+    DeviceGuard guard(ctx->device);
+    for (mfh_buf *out : {emitted, counts, next})
+        mark_written(out);
+    for (size_t i = 0; i < buffers; ++i)
+        mark_written(pages[i]);
+    if (!p.runs.sequences)
+        return MFH_OK;
+    p.parents = parents ? dev_f32(parents) : nullptr;
+    p.places = places ? dev_f32(places) : nullptr;
+    p.drafted = dev_f32(tokens);
+    p.choices = dev_f32(choices);
+    p.tables = dev_f32(tables);
+    p.emitted = dev_f32(emitted);
+    p.counts = dev_f32(counts);
+    p.next = dev_f32(next);
+    p.max_pages = uint32_t(tables->dims[1]);
+    p.columns = uint32_t(emitted->dims[1]);
+    p.pages = first.pages;
+    p.page_shift = first.page_shift;
+    p.path_pages = buffers != 0;
+    size_t done = 0;
+    do {
+        p.buffers = uint32_t(buffers - done < kSettleBuffers ? buffers - done : kSettleBuffers);
+        for (uint32_t i = 0; i < p.buffers; ++i) {
+            const mfh_buf *b = pages[done + i];
+            p.buffer[i] = b->dev;
+            p.heads[i] = uint32_t(b->dims[1]);
+            p.row_bytes[i] = uint32_t(b->dims[3] * (b->dtype == MFH_DTYPE_U8 ? 1 : 4));
+        }
+        launch_settle(ctx->stream, p);
+        p.emitted = nullptr;
+        done += p.buffers;
+    } while (done < buffers);
+    return launched(ctx);
+}
+
 // Scores are formed times log2 e: the kernels take powers of two.
 constexpr double kLog2E = 1.4426950408889634;
 
@@ -320,89 +414,22 @@ mfh_status mfh_settle_drafts(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mf
                              const mfh_buf *parents, const mfh_buf *lengths,
                              const mfh_buf *tables)
 {
+    return settle(ctx, emitted, counts, next, pages, buffers, tokens, choices, starts, parents,
+                  nullptr, lengths, tables);
+}
+
+mfh_status mfh_settle_drafts_at(mfh_ctx *ctx, mfh_buf *emitted, mfh_buf *counts, mfh_buf *next,
+                                mfh_buf *const *pages, size_t buffers, const mfh_buf *tokens,
+                                const mfh_buf *choices, const mfh_buf *starts,
+                                const mfh_buf *parents, const mfh_buf *places,
+                                const mfh_buf *lengths, const mfh_buf *tables)
+{
     if (!ctx)
         return MFH_INVALID_ARGUMENT;
-    mfh_status s = check_operation(ctx, MFH_OP_COPY);
-    if (!s)
-        s = check_f32(ctx, tokens);
-    if (s)
+    if (mfh_status s = check_f32(ctx, places))
         return s;
-    if (tokens->rank != 1)
-        return fail(ctx, MFH_INVALID_SHAPE, "drafted tokens must be one per token");
-    Settle p;
-    if ((s = check_runs(ctx, starts, lengths, tokens->dims[0], false, &p.runs)) ||
-        (s = check_vector(ctx, choices, tokens->dims[0], "choices must be one per token")) ||
-        (parents && (s = check_vector(ctx, parents, tokens->dims[0],
-                                      "parents must be one per token"))) ||
-        (s = check_tables(ctx, tables)) || (s = check_f32(ctx, emitted)) ||
-        (s = check_vector(ctx, counts, p.runs.sequences, "counts must be one per sequence")) ||
-        (s = check_vector(ctx, next, p.runs.sequences, "next tokens must be one per sequence")))
-        return s;
-    if (tables->dims[0] != p.runs.sequences)
-        return fail(ctx, MFH_INVALID_SHAPE, "page tables must have a row per sequence");
-    if (emitted->rank != 2 || emitted->dims[0] != p.runs.sequences || emitted->dims[1] == 0)
-        return fail(ctx, MFH_INVALID_SHAPE, "emitted tokens must be [sequences, columns]");
-    if (emitted->dims[1] > kSettleColumns)
-        return fail(ctx, MFH_UNSUPPORTED, "accepted paths are at most 1024 tokens long");
-    if (buffers && !pages)
-        return fail(ctx, MFH_INVALID_ARGUMENT, "page buffer list is null");
-    PageShape first;
-    for (size_t i = 0; i < buffers; ++i) {
-        PageShape shape;
-        if ((s = page_shape(ctx, pages[i], &shape)))
-            return s;
-        if (i == 0)
-            first = shape;
-        if (shape.page_shift != first.page_shift)
-            return fail(ctx, MFH_INVALID_SHAPE, "page buffers differ in page size");
-        // A path's pages are in every buffer.
-        first.pages = shape.pages < first.pages ? shape.pages : first.pages;
-        if (uint64_t(shape.kv_heads) * shape.head_dim > uint64_t(UINT16_MAX) * 256)
-            return fail(ctx, MFH_OVERFLOW, "page extent exceeds the kernel index range");
-        if (aliases(pages[i], {emitted, counts, next, tokens, choices, starts, parents, lengths,
-                               tables}))
-            return aliased(ctx);
-        for (size_t j = 0; j < i; ++j)
-            if (pages[j]->dev == pages[i]->dev)
-                return fail(ctx, MFH_INVALID_ARGUMENT, "a page buffer is listed twice");
-    }
-    if (aliases(emitted, {counts, next, tokens, choices, starts, parents, lengths, tables}) ||
-        aliases(counts, {next, tokens, choices, starts, parents, lengths, tables}) ||
-        aliases(next, {tokens, choices, starts, parents, lengths, tables}))
-        return aliased(ctx);
-    DeviceGuard guard(ctx->device);
-    for (mfh_buf *out : {emitted, counts, next})
-        mark_written(out);
-    for (size_t i = 0; i < buffers; ++i)
-        mark_written(pages[i]);
-    if (!p.runs.sequences)
-        return MFH_OK;
-    p.parents = parents ? dev_f32(parents) : nullptr;
-    p.drafted = dev_f32(tokens);
-    p.choices = dev_f32(choices);
-    p.tables = dev_f32(tables);
-    p.emitted = dev_f32(emitted);
-    p.counts = dev_f32(counts);
-    p.next = dev_f32(next);
-    p.max_pages = uint32_t(tables->dims[1]);
-    p.columns = uint32_t(emitted->dims[1]);
-    p.pages = first.pages;
-    p.page_shift = first.page_shift;
-    p.path_pages = buffers != 0;
-    size_t done = 0;
-    do {
-        p.buffers = uint32_t(buffers - done < kSettleBuffers ? buffers - done : kSettleBuffers);
-        for (uint32_t i = 0; i < p.buffers; ++i) {
-            const mfh_buf *b = pages[done + i];
-            p.buffer[i] = b->dev;
-            p.heads[i] = uint32_t(b->dims[1]);
-            p.row_bytes[i] = uint32_t(b->dims[3] * (b->dtype == MFH_DTYPE_U8 ? 1 : 4));
-        }
-        launch_settle(ctx->stream, p);
-        p.emitted = nullptr;
-        done += p.buffers;
-    } while (done < buffers);
-    return launched(ctx);
+    return settle(ctx, emitted, counts, next, pages, buffers, tokens, choices, starts, parents,
+                  places, lengths, tables);
 }
 
 }  // extern "C"

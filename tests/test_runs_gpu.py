@@ -1,0 +1,103 @@
+"""Runs of tokens on the GPU, where the helpers of the drafted trees' tests serve: settling of
+runs that the layout refuses, against plain implementations in 64 bits.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_draft_gpu import (NAN, f32, random_pages, read_pages, refused, run_layout, settled,
+                            starts_of, tables_for, upload)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- settling ------------------------------------------------------------------------------
+
+def settle_at(backend, starts, parents, tokens, choices, lengths, table, columns, caches, places):
+    n = len(lengths)
+    outs = [upload(backend, np.full(shape, 9.0, np.float32)) for shape in ((n, columns), (n,), (n,))]
+    backend.settle_drafts(*outs, caches, f32(backend, tokens), f32(backend, choices),
+                          f32(backend, starts), None if parents is None else f32(backend, parents),
+                          f32(backend, lengths), upload(backend, table),
+                          places=None if places is None else f32(backend, places))
+    return [backend.read(o) for o in outs]
+
+
+@pytest.mark.parametrize("given", [False, True], ids=["alone", "places"])
+def test_settling_of_runs_whose_first_token_follows_another(backend, given):
+    """The layout refuses them, so nothing was stored for them: no token is accepted."""
+    rng = np.random.default_rng(4)
+    firsts = [NAN, 0, 5, -2, -0.5, -1]
+    starts, lengths = starts_of([4] * 6), [3, 0, 9, 2, 5, 7]
+    tokens = np.arange(24, dtype=np.float32) % 4
+    choices = np.roll(tokens, -1)
+    parents = np.tile(np.array([0, 0, 0, 2], np.float32), 6)  # the first child never drafted
+    parents[::4] = firsts
+    choices[::4] = 2  # the second child, which moves
+    pages, table = tables_for(rng, [16] * 6, 8)
+    old = random_pages(rng, pages, 2, 8, 5, False)
+    cache = upload(backend, old)
+    (_, _, places), _ = run_layout(backend, starts, parents, lengths, 24, 1)
+    assert np.array_equal(places, [-1] * 20 + [7, 8, 9, 10])
+    emitted, counts, last = settle_at(backend, starts, parents, tokens, choices, lengths, table, 4,
+                                      [cache], places if given else None)
+    for got in (emitted[:5], counts[:5], last[:5]):
+        assert np.all(np.isnan(got))
+    want = settled(starts[5:], parents, tokens, choices, lengths[5:], table[5:], 8, 4, [old])
+    for got, w in zip((emitted, counts, last), want):
+        assert np.array_equal(got[5], w[0])
+    assert counts[5] == 3
+    assert np.array_equal(backend.read(cache), old)
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["chain", "tree"])
+def test_settling_stops_where_tokens_have_no_place(backend, tree):
+    """Tokens past the mask's last bit were not stored: the path ends before them."""
+    rng = np.random.default_rng(5)
+    runs, lengths = [12, 100, 3, 9], [4, 30, 0, 11]
+    starts = starts_of(runs)
+    # In the tree odd tokens are one branch, even ones another, which is accepted.
+    parents = np.concatenate([np.maximum(np.arange(n) - 2, -1) if tree else np.arange(n) - 1
+                              for n in runs])
+    if tree:
+        parents[starts[:-1].astype(int) + 1] = 0
+    tokens = np.concatenate([np.arange(n) for n in runs])
+    choices = tokens + (2 if tree else 1)
+    pages, table = tables_for(rng, [160] * 4, 16)
+    old = random_pages(rng, pages, 1, 16, 6, True)
+    cache = upload(backend, old)
+    (_, _, places), _ = run_layout(backend, starts, parents, lengths, sum(runs), 1)
+    got = settle_at(backend, starts, parents if tree else None, tokens, choices, lengths, table, 64,
+                    [cache], places)
+    # As of runs of the tokens that have one.
+    short = [min(n, 8) for n in runs]
+    keep = np.concatenate([int(a) + np.arange(n) for a, n in zip(starts, short)])
+    want = settled(starts_of(short), parents[keep], tokens[keep], choices[keep], lengths, table, 16,
+                   64, [old])
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w)
+    assert got[1].tolist() == ([4, 4, 2, 4] if tree else [8, 8, 3, 8])
+    assert np.array_equal(read_pages(backend, cache), old.astype(np.float32))
+    # Places that are not the tokens' own are none; without the first one the sequence is bad.
+    places[3] += 1
+    places[12], places[113] = -1, NAN
+    got = settle_at(backend, starts, parents if tree else None, tokens, choices, lengths, table, 64,
+                    [cache], places)
+    assert np.array_equal(got[1], [4, NAN, 2, 4] if tree else [3, NAN, 1, 8], equal_nan=True)
+
+
+def test_settling_refusals_of_places(backend):
+    a = backend.allocate_f32
+    pages = backend.alloc_pages(3, 2, 8, 4)
+    good = [a((2, 4)), a((2,)), a((2,)), [pages], a((6,)), a((6,)), a((3,)), a((6,)), a((2,)),
+            a((2, 1))]
+    backend.settle_drafts(*good, places=a((6,)))
+    for places, variant in ((a((5,)), "InvalidShape"), (a((6, 1)), "InvalidShape"),
+                            (good[0], "InvalidShape"), (pages, "InvalidShape"),
+                            (upload(backend, np.zeros(6, np.uint8)), "InvalidDType")):
+        refused(variant, backend.settle_drafts, *good, places)
+    # Outputs of as many sequences as tokens.
+    good = [a((2, 4)), a((2,)), a((2,)), [], a((2,)), a((2,)), a((3,)), None, a((2,)), a((2, 1))]
+    for places in good[1:3]:
+        refused("InvalidArgument", backend.settle_drafts, *good, places)
