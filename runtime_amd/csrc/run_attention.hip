@@ -899,12 +899,13 @@ void run_attention_kernel(RunAttention p)
                                  fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
                 most = quad_max(most);
                 // 2^14 <= most 2^exponent < 2^15 (0 and infinities as they are; below
-                // 2^-86, where no score differs from 0, by 2^100, so that the factor stays
-                // normal).
+                // 2^-86, where no score of an ordinary scale differs from 0, by 2^100).
                 if (most > 0.0f && most < __builtin_inff())
                     exponent = 15 - __builtin_amdgcn_frexp_expf(most);
                 exponent = exponent < 100 ? exponent : 100;
-                factor[g] = ldexpf(p.scale, -exponent);
+                // Never 0, which a masked score of -infinity would meet: scores are below
+                // 2^42, and times the least normal factor as good as 0.
+                factor[g] = fmaxf(ldexpf(p.scale, -exponent), 0x1p-126f);
             }
 #pragma unroll
             for (int i = 0; i < 2 * U; ++i)

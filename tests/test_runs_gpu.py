@@ -1,15 +1,36 @@
 """Runs of tokens on the GPU, where the helpers of the drafted trees' tests serve: settling of
-runs that the layout refuses, against plain implementations in 64 bits.
+runs that the layout refuses, and attention at the ends of its ranges, against plain
+implementations in 64 bits.
 """
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
-from test_draft_gpu import (NAN, f32, random_pages, read_pages, refused, run_layout, settled,
-                            starts_of, tables_for, upload)
+from test_draft_gpu import (NAN, Batch, check, f32, random_pages, read_pages, refused, run_latent,
+                            run_layout, say, settled, starts_of, tables_for, upload)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- scales of latents ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("rank,rope", [(64, 0), (128, 0), (256, 0), (128, 64), (512, 64), (30, 6)])
+@pytest.mark.parametrize("scale,size", [(1e-20, 1e-27), (1e-44, 1.0), (1e-30, 1e30)])
+def test_scales_and_queries_whose_product_vanishes(backend, scale, size, rank, rope, half):
+    """Scores of about 0: each row is the mean of the values that it attends."""
+    say("scale", scale, size, rank, rope, half)
+    batch = Batch(rank + half, [(70, 9), (0, 5)], "tree", 16)
+    pages = random_pages(batch.rng, batch.pages, 1, 16, rank + rope, half)
+    batch.spoil(pages)
+    latent, rotary = ((size * batch.rng.standard_normal((14, 4 * w))).astype(np.float32)
+                      for w in (rank, rope))
+    scale = float(np.float32(scale))
+    got = run_latent(backend, batch, latent, rotary, pages, 4, scale)
+    query = np.concatenate([x.reshape(14, 4, -1 if x.size else 0) for x in (latent, rotary)], axis=2)
+    want, bound = batch.attend(query, pages, pages[..., :rank], scale)
+    check(got.reshape(want.shape), want, bound, 7.0)
 
 
 # ---- settling ------------------------------------------------------------------------------
