@@ -551,7 +551,8 @@ mfh_status mfh_paged_latent_append(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *pa
  * query_heads * rope], rotated), scores are its products with the cached rows times
  * `scale`, and its output [tokens, query_heads * rank] is their softmax times the cached
  * latents.  Runs, masks, lengths, bad ids and the workspace as in mfh_paged_tree_gqa.
- * rank + rope <= 1024; ranks 128, 256 and 512 with rope 32 or 64 run on matrix cores,
+ * `scale` is positive and below 2.35e38 (larger ones pass f32 in the powers of two that the
+ * kernels form).  rank + rope <= 1024; ranks 128, 256 and 512 with rope 32 or 64 run on matrix cores,
  * others many times slower. */
 mfh_status mfh_paged_latent_attention(mfh_ctx *ctx, mfh_buf *output,
                                       const mfh_buf *latent_query, const mfh_buf *rotary_query,

@@ -303,8 +303,10 @@ mfh_status mfh_paged_latent_attention(mfh_ctx *ctx, mfh_buf *output,
         return fail(ctx, MFH_INVALID_SHAPE, "latent pages must have one head");
     if (query_heads == 0 || query_heads > UINT16_MAX)
         return fail(ctx, MFH_INVALID_ARGUMENT, "query head count must be in [1, 65535]");
-    if (!positive(scale))
-        return fail(ctx, MFH_INVALID_ARGUMENT, "attention scale must be finite and positive");
+    p.scale = float(kLog2E * double(scale));
+    if (!positive(scale) || !positive(p.scale))
+        return fail(ctx, MFH_INVALID_ARGUMENT,
+                    "attention scale must be positive and below 2.35e38");
     if (latent_query->rank != 2 || rotary_query->rank != 2 ||
         latent_query->dims[0] != rotary_query->dims[0] ||
         latent_query->dims[1] % query_heads != 0 || rotary_query->dims[1] % query_heads != 0)
@@ -315,7 +317,6 @@ mfh_status mfh_paged_latent_attention(mfh_ctx *ctx, mfh_buf *output,
         return fail(ctx, MFH_INVALID_SHAPE, "latent page width differs from rank + rope");
     p.value_dim = uint32_t(rank);
     p.query_heads = p.group = query_heads;
-    p.scale = float(kLog2E * double(scale));
     return attend(ctx, output, latent_query, rotary_query, pages, pages, tables, starts, lengths,
                   mask, p);
 }

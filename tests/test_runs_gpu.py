@@ -33,6 +33,17 @@ def test_scales_and_queries_whose_product_vanishes(backend, scale, size, rank, r
     check(got.reshape(want.shape), want, bound, 7.0)
 
 
+def test_scales_beyond_f32(backend):
+    """Scores are formed times log2 e: scales that pass f32 with it are refused."""
+    a, pages = backend.allocate_f32, backend.alloc_pages(1, 1, 8, 64)
+    given = [a((1, 64)), a((1, 64)), a((1, 0)), pages, a((1, 1)), None, a((1,)), None, 1]
+    for scale in (2.35e38, 1e-45):
+        backend.paged_latent_attention(*given, scale)
+        assert np.all(backend.read(given[0]) == 0)  # one key of zeros
+    for scale in (2.36e38, 3.4e38, np.inf, -1.0):
+        refused("InvalidArgument", backend.paged_latent_attention, *given, scale)
+
+
 # ---- settling ------------------------------------------------------------------------------
 
 def settle_at(backend, starts, parents, tokens, choices, lengths, table, columns, caches, places):
