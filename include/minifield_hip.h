@@ -482,9 +482,9 @@ mfh_status mfh_paged_qk_norm_rope_at(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *
  * Runs: several new tokens of each sequence in one call.  The run of sequence s is
  * tokens starts[s] .. starts[s + 1] - 1 of the batch (`starts` F32 [sequences + 1]),
  * possibly none; its token i is cached at place lengths[s] + i, behind the
- * lengths[s] tokens that the sequence holds without it.  There are up to 65536
- * sequences.  The first entry of `starts` that is no whole number, falls below the one before it or passes the
- * batch ends the list: sequences from there on have no run.  Rows of the batch
+ * lengths[s] tokens that the sequence holds without it.  A list of starts has up to 65536
+ * runs (MFH_OVERFLOW beyond).  Its first entry that is no whole number, falls below the one
+ * before it or passes the batch ends it: sequences from there on have no run.  Rows of the batch
  * that are in no run (behind the last one, or padding before the first) are
  * left as they were by the attention calls.
  * Trees: parents[t] (F32 [tokens]) is the token of the same run that token t follows, as
@@ -509,14 +509,17 @@ mfh_status mfh_draft_layout(mfh_ctx *ctx, mfh_buf *sequences, mfh_buf *positions
  * keys and values are in the cache already: token t attends all lengths[s] cached
  * tokens before the run and, of the run, those that its mask row names (`mask` null:
  * itself and all before it, as in a prompt).  `starts` null: one token for each row
- * of `tables`.  Queries [tokens, query_heads * head_dim], otherwise as
+ * of `tables`, of any number (mfh_paged_gqa of lengths + 1 gives the same, faster where it
+ * has a matrix-core kernel).  Queries [tokens, query_heads * head_dim], otherwise as
  * mfh_paged_gqa, its workspace included.  A token that attends nothing gives zeros; one
  * of a sequence whose length is no whole number, or that passes the table's row or
  * 2^24 with its run, and one that attends a key whose page id is bad, give NaN
  * rows.  What a token does not attend does not reach its row, whatever it holds (NaN
  * included); what it attends is expected to be finite, and with f32 caches queries, keys
  * and values are below 3.39e38 (larger ones give NaN) and, for the precision of f32, zero
- * or above 2^-100.  head_dim <= 1024; 32, 64, 80, 96, 112, 128, 160, 192 and 256 run on
+ * or above 2^-100.  tokens * query_heads <= 2^25, and (sequences + tokens * query_heads /
+ * key_value_heads / 16) * key_value_heads * (places of a table's row / 32 + 14) below 2^31:
+ * of larger calls some are refused (MFH_OVERFLOW).  head_dim <= 1024; 32, 64, 80, 96, 112, 128, 160, 192 and 256 run on
  * matrix cores, others many times slower. */
 mfh_status mfh_paged_tree_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                               const mfh_buf *key_pages, const mfh_buf *value_pages,

@@ -15,7 +15,8 @@ namespace {
 
 // Blocks of 256 threads that a launch may have in one direction.
 constexpr uint64_t kMostBlocks = uint64_t(INT32_MAX) / 256;
-// Runs of a batch: blocks look through the list of starts up to their own.
+// Runs of a batch with a list of starts: layout's and settling's blocks look through it up to
+// their own.
 constexpr uint64_t kMostRuns = 65536;
 
 // The runs of a batch of `tokens`; `starts` may be null where `one_each`.

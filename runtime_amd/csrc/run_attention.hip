@@ -1576,11 +1576,11 @@ bool run_attention_plan(RunAttention &p, int cu_count)
         return true;
     p.rows = kernel.rows;
     p.item_units = kernel.resident == 3 ? kItemUnitsOfThree : kItemUnits;
-    // Units stay in 32 bits.
+    // Units stay in 32 bits.  A run that passes its table's row has no tiles; past the others'
+    // keys an item has up to six units for what is rounded up.
     const uint64_t items = (uint64_t(p.runs.tokens) * p.group / p.rows + p.runs.sequences) *
                            p.shape.kv_heads;
-    const uint64_t most = items * (p.item_units + 6 + ((uint64_t(p.longest) + p.runs.tokens) >>
-                                                     kernel.shift));
+    const uint64_t most = items * (p.item_units + 6 + (p.longest >> kernel.shift));
     if (most >= uint64_t(1) << 31)
         return false;
     const uint64_t wanted = (most + kLeastUnits - 1) / kLeastUnits;

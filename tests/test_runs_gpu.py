@@ -4,13 +4,77 @@ implementations in 64 bits.
 """
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 
-from test_draft_gpu import (NAN, Batch, check, f32, random_pages, read_pages, refused, run_latent,
-                            run_layout, say, settled, starts_of, tables_for, upload)
+from runtime_amd.backend import GqaSpec
+from test_draft_gpu import (F32, NAN, Batch, check, f32, random_pages, read_pages, refused,
+                            run_latent, run_layout, say, settled, starts_of, tables_for, upload)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- long lists --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [32, 20])
+@pytest.mark.parametrize("count", [65536, 65537, 400000])
+def test_many_sequences_of_a_token_each(backend, count, dim):
+    """Without starts there is no list to look through, and no limit to it."""
+    say("many", count, dim)
+    rng = np.random.default_rng(count + dim)
+    keys, values = (random_pages(rng, 97, 1, 8, dim, False) for _ in range(2))
+    table = rng.integers(0, 97, (count, 1)).astype(np.float32)
+    lengths = rng.integers(0, 8, count).astype(np.float32)
+    lengths[[0, count // 2, -1]] = 8, NAN, 7
+    query = rng.standard_normal((count, dim)).astype(np.float32)
+    out = backend.allocate_f32((count, dim))
+    backend.paged_tree_gqa(out, upload(backend, query), upload(backend, keys),
+                           upload(backend, values), upload(backend, table), None,
+                           upload(backend, lengths), None, GqaSpec(1, 1, dim))
+    got = backend.read(out)
+    bad = np.isnan(lengths) | (lengths == 8)  # a ninth token has no page
+    assert np.all(np.isnan(got[bad])) and bad.sum() == 2
+    for first in range(0, count, 40000):
+        rows = slice(first, first + 40000)
+        page = table[rows, 0].astype(int)
+        key, value = (x[page, 0].astype(np.float64) for x in (keys, values))
+        seen = np.arange(8) <= np.nan_to_num(lengths[rows])[:, None]
+        terms = key * query[rows, None] / math.sqrt(dim)
+        score = np.where(seen, terms.sum(axis=2), -np.inf)
+        p = np.exp(score - score.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        want = (p[..., None] * value).sum(axis=1)
+        # As Batch.attend bounds it, of one tile.
+        size = np.where(seen, np.abs(terms).sum(axis=2), 0).max(axis=1)[:, None]
+        relative = 2 * (dim + 8) * F32 * size + 97 * F32
+        bound = relative * (p[..., None] * np.abs(value)).sum(axis=1) + 2.0 ** -37
+        good = ~bad[rows]
+        assert np.all(np.abs(got[rows] - want)[good] <= bound[good])
+
+
+def test_extents_of_runs_past_the_index_range(backend):
+    a = backend.allocate_f32
+    # Rows: 2^25 at most.
+    pages = [backend.alloc_pages(1, 1, 8, 1) for _ in range(2)]
+    for tokens in (512, 513):
+        given = [a((tokens, 65535)), a((tokens, 65535)), *pages, a((tokens, 1)), None, a((tokens,)),
+                 None, GqaSpec(65535, 1, 1)]
+        if tokens == 512:
+            backend.paged_tree_gqa(*given)
+        else:
+            refused("Overflow", backend.paged_tree_gqa, *given)
+    # Units: 64 heads of 2^24 places a row are 2^24 for each sequence, and some more.
+    pages = [backend.alloc_pages(1, 64, 4096, 64) for _ in range(2)]
+    for sequences in (126, 127):
+        given = [a((sequences, 4096)), a((sequences, 4096)), *pages, a((sequences, 4096)), None,
+                 a((sequences,)), None, GqaSpec(64, 64, 64)]
+        if sequences == 126:
+            backend.paged_tree_gqa(*given)
+            assert np.all(backend.read(given[0]) == 0)
+        else:
+            refused("Overflow", backend.paged_tree_gqa, *given)
 
 
 # ---- scales of latents ------------------------------------------------------------------------
