@@ -12,15 +12,35 @@ constexpr int kBlock = 256;
 
 // Block s lays out the run of sequence s, block `sequences` marks the tokens in no run.  Runs
 // of up to 64 tokens are a wave's lanes, which form their ancestors in six steps: after k of
-// them a lane knows 2^k generations, and where the next one is.  Of longer runs a thread walks
-// from a token up; ancestors have falling numbers, so one walk writes the mask from its
-// last byte to its first.  Bound by the launch and three dependent reads: 16 tokens 4.6
-// us, 96 sequences of 8 to 64 the same; the walks and bytes of a thread each took 13.0.
-constexpr uint32_t kLayoutParents = 4096;  // of a run, held in LDS
+// them a lane knows 2^k generations, and where the next one is.  Longer runs go 64 tokens at
+// a time, whose ancestors before them are those of one earlier token: its depth and its
+// mask row are read back.  Bound by the launch and three dependent reads: 16 tokens 4.5
+// us, 96 sequences of 8 to 64 the same.  Of longer runs by the steps of 64, which follow one
+// another: 2048 tokens 26 us, 295 with their 512 KB of masks, 8192 97.
+
+// The lane's ancestors among the wave's 64 tokens and itself; `good` where it and they are.
+// `parent`: a lower lane, or -1.
+__device__ __forceinline__ uint64_t lane_ancestors(uint32_t lane, int parent, bool &good)
+{
+    uint64_t seen = 1ull << lane;
+#pragma unroll
+    for (int step = 0; step < 6; ++step) {
+        const int from = parent < 0 ? int(lane) : parent;
+        const uint32_t low = __shfl(uint32_t(seen), from, 64);
+        const uint32_t high = __shfl(uint32_t(seen >> 32), from, 64);
+        const int far = __shfl(parent, from, 64);
+        const bool sound = __shfl(int(good), from, 64);
+        seen |= uint64_t(high) << 32 | low;
+        good = good && sound;
+        parent = parent < 0 ? parent : far;
+    }
+    return seen;
+}
 
 __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
 {
-    __shared__ float held[kLayoutParents];
+    __shared__ uint64_t seen_of[64];  // of a long run's 64 tokens
+    __shared__ int root_of[64];
     const uint32_t s = blockIdx.x, lane = threadIdx.x & 63;
     const auto put = [&](uint32_t t, float sequence, float position, float place) {
         p.sequences[t] = sequence;
@@ -72,18 +92,7 @@ __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
         }
         // A token past the mask's last bit has no place.
         good = good && (!p.mask || lane < 8ull * p.mask_bytes);
-        uint64_t seen = 1ull << lane;
-#pragma unroll
-        for (int step = 0; step < 6; ++step) {
-            const int from = parent < 0 ? int(lane) : parent;
-            const uint32_t low = __shfl(uint32_t(seen), from, 64);
-            const uint32_t high = __shfl(uint32_t(seen >> 32), from, 64);
-            const int far = __shfl(parent, from, 64);
-            const bool sound = __shfl(int(good), from, 64);
-            seen |= uint64_t(high) << 32 | low;
-            good = good && sound;
-            parent = parent < 0 ? parent : far;
-        }
+        const uint64_t seen = lane_ancestors(lane, parent, good);
         if (lane >= n)
             return;
         if (!good || !fits) {
@@ -96,40 +105,58 @@ __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
             row[b] = b < 8 ? uint8_t(seen >> 8 * b) : 0;
         return;
     }
-    if (p.parents) {
-        for (uint32_t i = threadIdx.x; i < n && i < kLayoutParents; i += kBlock)
-            held[i] = p.parents[run.begin + i];
-        __syncthreads();
+    const auto barred = [&](uint32_t i) { return !fits || (p.mask && i >= 8ull * p.mask_bytes); };
+    if (!p.parents) {
+        for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
+            const uint32_t t = run.begin + i;
+            if (barred(i)) {
+                unset(t);
+                continue;
+            }
+            put(t, float(s), length + float(i), length + float(i));
+            uint8_t *row = p.mask + uint64_t(t) * p.mask_bytes;
+            for (uint32_t b = 0; b < p.mask_bytes; ++b) {
+                const int left = int(i) + 1 - 8 * int(b);
+                row[b] = left >= 8 ? 0xff : left <= 0 ? 0 : uint8_t((1u << left) - 1);
+            }
+        }
+        return;
     }
-    // -2: a bad one.
-    const auto parent_of = [&](uint32_t i) {
-        if (!p.parents)
-            return int(i) - 1;
-        const float v = i < kLayoutParents ? held[i] : p.parents[run.begin + i];
-        return v == -1.0f ? -1 : valid_index(v, i) ? int(v) : -2;
-    };
-    for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
-        const uint32_t t = run.begin + i;
-        uint32_t depth = 0;
-        int at = int(i);
-        if (p.parents)
-            while ((at = parent_of(uint32_t(at))) >= 0)
-                ++depth;
-        else
-            depth = i, at = -1;
-        if (at == -2 || !fits || (p.mask && i >= 8ull * p.mask_bytes)) {
-            unset(t);
-            continue;
+    for (uint32_t base = 0; base < n; base += 64) {
+        if (threadIdx.x < 64) {
+            const uint32_t i = base + lane, t = run.begin + (i < n ? i : n - 1);
+            const float v = p.parents[t];
+            bool good = i < n && !barred(i) && (v == -1.0f || valid_index(v, i));
+            const int parent = good ? int(v) : -1;
+            const bool inside = parent >= int(base);
+            const uint64_t seen = lane_ancestors(lane, inside ? parent - int(base) : -1, good);
+            // What the first of them follows, of an earlier 64.
+            const int root = __shfl(inside ? -1 : parent, __builtin_ctzll(seen), 64);
+            const float before = root < 0 ? length - 1.0f : p.positions[run.begin + root];
+            good = good && (root < 0 || before >= 0.0f);
+            if (i < n) {
+                if (good)
+                    put(t, float(s), before + float(__popcll(seen)), length + float(i));
+                else
+                    put(t, -1.0f, -1.0f, -1.0f);
+            }
+            seen_of[lane] = good ? seen : 0;
+            root_of[lane] = good ? root : -1;
         }
-        put(t, float(s), length + float(depth), length + float(i));
-        uint8_t *row = p.mask + uint64_t(t) * p.mask_bytes;
-        at = int(i);
-        for (int b = int(p.mask_bytes) - 1; b >= 0; --b) {
-            uint32_t bits = 0;
-            for (; at >= 8 * b; at = parent_of(uint32_t(at)))
-                bits |= 1u << (at & 7);
-            row[b] = uint8_t(bits);
+        __syncthreads();
+        // A wave a row; rows before this 64 are whole, and their bytes are.
+        for (uint32_t r = threadIdx.x >> 6; p.mask && r < 64 && base + r < n; r += kBlock / 64) {
+            const uint64_t seen = seen_of[r];
+            const uint8_t *from = p.mask + uint64_t(run.begin + root_of[r]) * p.mask_bytes;
+            uint8_t *row = p.mask + uint64_t(run.begin + base + r) * p.mask_bytes;
+            for (uint32_t b = lane; b < p.mask_bytes; b += 64) {
+                const uint32_t in = b - base / 8;  // of the 64 tokens' bytes
+                row[b] = b < base / 8 ? (root_of[r] < 0 ? 0 : from[b])
+                         : in < 8     ? uint8_t(seen >> 8 * in)
+                                      : 0;
+            }
         }
+        __syncthreads();  // rows, positions and what the waves share
     }
 }
 

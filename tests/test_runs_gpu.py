@@ -1,6 +1,6 @@
-"""Runs of tokens on the GPU, where the helpers of the drafted trees' tests serve: settling of
-runs that the layout refuses, and attention at the ends of its ranges, against plain
-implementations in 64 bits.
+"""Runs of tokens on the GPU, where the helpers of the drafted trees' tests serve: layout of
+long runs, settling of runs that the layout refuses, and attention at the ends of its ranges,
+against plain implementations in 64 bits.
 """
 from __future__ import annotations
 
@@ -75,6 +75,74 @@ def test_extents_of_runs_past_the_index_range(backend):
             assert np.all(backend.read(given[0]) == 0)
         else:
             refused("Overflow", backend.paged_tree_gqa, *given)
+
+
+# ---- layout of long runs ------------------------------------------------------------------------
+
+def laid_out(parents, length, bytes_):
+    """(positions, places, bad) of one run, by one pass over it; mask rows where bytes_ > 0."""
+    n = len(parents)
+    depth, rows = np.full(n, -1), np.zeros((n, bytes_), np.uint8)
+    for i, parent in enumerate(parents):
+        if bytes_ and i >= 8 * bytes_:
+            continue
+        if parent == -1:
+            depth[i] = 0
+        elif 0 <= parent < i and parent == int(parent) and depth[int(parent)] >= 0:
+            depth[i] = depth[int(parent)] + 1
+            rows[i] = rows[int(parent)]
+        else:
+            continue
+        if bytes_:
+            rows[i, i // 8] |= 1 << i % 8
+    good = depth >= 0
+    return (np.where(good, length + depth, -1), np.where(good, length + np.arange(n), -1), good, rows)
+
+
+@pytest.mark.parametrize("runs,bytes_", [
+    ([65], 9), ([64, 66, 127, 128, 129], 17), ([1000], 125), ([700, 3, 2048], 200), ([500], 0),
+    ([300], 1)])
+@pytest.mark.parametrize("kind", ["chain", "tree", "star", "far", "bad"])
+def test_layout_of_long_runs(backend, kind, runs, bytes_):
+    say("layout", kind, runs, bytes_)
+    rng = np.random.default_rng(sum(runs) + bytes_)
+    parents = []
+    for n in runs:
+        i = np.arange(n)
+        each = {"chain": i - 1, "star": np.where(i, 0, -1), "far": np.floor(rng.random(n) * i),
+                }.get(kind, i - 1 - np.floor(rng.random(n) * np.minimum(i, 9))).astype(np.float32)
+        each[0] = -1
+        if kind == "bad":
+            each[rng.integers(0, n, 2)] = NAN, 0.5
+            each[rng.integers(1, n, 3)] = n, -2, -1
+        parents.append(each)
+    lengths, starts = rng.integers(0, 9000, len(runs)), starts_of(runs, 1)
+    tokens = int(starts[-1]) + 1
+    flat = np.concatenate([[0], *parents, [0]])
+    got, mask = run_layout(backend, starts, flat, lengths, tokens, bytes_)
+    for s, n in enumerate(runs):
+        at = slice(int(starts[s]), int(starts[s]) + n)
+        positions, places, good, rows = laid_out(parents[s], lengths[s], bytes_)
+        assert np.array_equal(got[0][at], np.where(good, s, -1))
+        assert np.array_equal(got[1][at], positions)
+        assert np.array_equal(got[2][at], places)
+        assert mask is None or np.array_equal(mask[at], rows)
+    assert all(out[0] == out[-1] == -1 for out in got)
+
+
+def test_layout_of_the_longest_runs(backend):
+    """Time grows as the run, not as its square: a chain of 300000 takes some 4 ms."""
+    n = 300000
+    rng = np.random.default_rng(1)
+    i = np.arange(n)
+    for parents in (i - 1, np.where(i, i - 1 - np.floor(rng.random(n) * np.minimum(i, 99)), -1)):
+        say("layout", parents[-1])
+        got, _ = run_layout(backend, [0, n], parents, [5], n, 0)
+        positions, places, _, _ = laid_out(parents, 5, 0)
+        assert np.array_equal(got, [np.zeros(n), positions, places])
+    # A length that leaves no places.
+    got, _ = run_layout(backend, [0, n], i - 1, [2 ** 24 - n + 1], n, 0)
+    assert np.all(np.array(got) == -1)
 
 
 # ---- scales of latents ------------------------------------------------------------------------
