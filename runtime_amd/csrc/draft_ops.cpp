@@ -16,7 +16,8 @@ namespace {
 // Blocks of 256 threads that a launch may have in one direction.
 constexpr uint64_t kMostBlocks = uint64_t(INT32_MAX) / 256;
 // Runs of a batch with a list of starts: layout's and settling's blocks look through it up to
-// their own.
+// their own, settling's once for each buffer (1024 runs of two 9 us and 10 with a buffer, 52
+// with 16; 65536 3.8 ms, 3.7 and 58).
 constexpr uint64_t kMostRuns = 65536;
 
 // The runs of a batch of `tokens`; `starts` may be null where `one_each`.

@@ -18,6 +18,26 @@ pytestmark = pytest.mark.gpu
 
 # ---- long lists --------------------------------------------------------------------------------
 
+def attended_page(query, keys, values, page, count):
+    """(outputs, bound) in 64 bits of tokens that attend the first `count` places of a page each."""
+    want, bound = np.empty(query.shape), np.empty(query.shape)
+    dim = query.shape[1]
+    for first in range(0, len(query), 40000):
+        rows = slice(first, first + 40000)
+        key, value = (x[page[rows], 0].astype(np.float64) for x in (keys, values))
+        seen = np.arange(8) < count[rows, None]
+        terms = key * query[rows, None] / math.sqrt(dim)
+        score = np.where(seen, terms.sum(axis=2), -np.inf)
+        p = np.exp(score - score.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        want[rows] = (p[..., None] * value).sum(axis=1)
+        # As Batch.attend bounds it, of one tile.
+        size = np.where(seen, np.abs(terms).sum(axis=2), 0).max(axis=1)[:, None]
+        relative = 2 * (dim + 8) * F32 * size + 97 * F32
+        bound[rows] = relative * (p[..., None] * np.abs(value)).sum(axis=1) + 2.0 ** -37
+    return want, bound
+
+
 @pytest.mark.parametrize("dim", [32, 20])
 @pytest.mark.parametrize("count", [65536, 65537, 400000])
 def test_many_sequences_of_a_token_each(backend, count, dim):
@@ -36,22 +56,43 @@ def test_many_sequences_of_a_token_each(backend, count, dim):
     got = backend.read(out)
     bad = np.isnan(lengths) | (lengths == 8)  # a ninth token has no page
     assert np.all(np.isnan(got[bad])) and bad.sum() == 2
-    for first in range(0, count, 40000):
-        rows = slice(first, first + 40000)
-        page = table[rows, 0].astype(int)
-        key, value = (x[page, 0].astype(np.float64) for x in (keys, values))
-        seen = np.arange(8) <= np.nan_to_num(lengths[rows])[:, None]
-        terms = key * query[rows, None] / math.sqrt(dim)
-        score = np.where(seen, terms.sum(axis=2), -np.inf)
-        p = np.exp(score - score.max(axis=1, keepdims=True))
-        p /= p.sum(axis=1, keepdims=True)
-        want = (p[..., None] * value).sum(axis=1)
-        # As Batch.attend bounds it, of one tile.
-        size = np.where(seen, np.abs(terms).sum(axis=2), 0).max(axis=1)[:, None]
-        relative = 2 * (dim + 8) * F32 * size + 97 * F32
-        bound = relative * (p[..., None] * np.abs(value)).sum(axis=1) + 2.0 ** -37
-        good = ~bad[rows]
-        assert np.all(np.abs(got[rows] - want)[good] <= bound[good])
+    want, bound = attended_page(query, keys, values, table[:, 0].astype(int),
+                                np.where(bad, 1, lengths + 1))
+    assert np.all(np.abs(got - want)[~bad] <= bound[~bad])
+
+
+@pytest.mark.parametrize("dim", [32, 20])
+def test_the_longest_list_of_starts(backend, dim):
+    """65536 runs of no, one and two tokens: attended, and settled."""
+    say("starts", dim)
+    count, rng = 65536, np.random.default_rng(dim)
+    runs = rng.integers(0, 3, count)
+    starts = starts_of(runs, 3)
+    sequence = np.repeat(np.arange(count), runs)
+    tokens, number = 3 + len(sequence) + 2, np.arange(len(sequence)) + 3 - starts[sequence]
+    lengths = rng.integers(0, 7, count).astype(np.float32)
+    # Each sequence has a page of its own, which settling changes.
+    keys, values = (random_pages(rng, count, 1, 8, dim, False) for _ in range(2))
+    table = rng.permutation(count).astype(np.float32)[:, None]
+    query = rng.standard_normal((tokens, dim)).astype(np.float32)
+    out = upload(backend, np.full(query.shape, 7.0, np.float32))
+    caches = [upload(backend, keys), upload(backend, values)]
+    given = [upload(backend, table), f32(backend, starts), upload(backend, lengths)]
+    backend.paged_tree_gqa(out, upload(backend, query), *caches, *given, None, GqaSpec(1, 1, dim))
+    got = backend.read(out)
+    mine = slice(3, 3 + len(sequence))
+    want, bound = attended_page(query[mine], keys, values, table[sequence, 0].astype(int),
+                                lengths[sequence] + number + 1)
+    assert np.all(np.abs(got[mine] - want) <= bound)
+    assert np.all(got[:3] == 7) and np.all(got[-2:] == 7)
+    drafted, choices = rng.integers(0, 2, (2, tokens)).astype(np.float32)
+    got = settle_at(backend, starts, None, drafted, choices, lengths, table, 2, caches, None)
+    want = settled(starts, None, drafted, choices, lengths.astype(int), table, 8, 2, [keys, values])
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w)
+    assert set(want[1]) == {0, 1, 2}
+    for buffer, array in zip(caches, (keys, values)):
+        assert np.array_equal(backend.read(buffer), array)
 
 
 def test_extents_of_runs_past_the_index_range(backend):
