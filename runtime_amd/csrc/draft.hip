@@ -207,11 +207,7 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
     const RunBounds run = run_of(p.runs, s);
     const uint32_t n = run.end - run.begin;
     const float length = p.runs.lengths[s];
-    // The layout refuses a run whose first token follows another.
-    const float root = n && p.parents ? p.parents[run.begin] : -1.0f;
-    const float first = n && p.places ? p.places[run.begin] : length;
-    const bool fits =
-        n && valid_length(length, n, 1u << 24) && root == -1.0f && first == length;
+    const bool fits = n && valid_length(length, n, 1u << 24);
     uint32_t count = 0;
     if (threadIdx.x == 0)
         bad = 0;
@@ -230,10 +226,11 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
             for (uint32_t base = at + 1; base < n; base += 64) {
                 const uint32_t i = base + lane, t = run.begin + (i < n ? i : n - 1);
                 const float parent = p.parents ? p.parents[t] : float(int(i) - 1);
+                bool next = i < n && parent == float(at) && p.drafted[t] == choice;
                 // A token without a place was not stored.
-                const float own = length + float(i), place = p.places ? p.places[t] : own;
-                const uint64_t found = __ballot(i < n && parent == float(at) &&
-                                                p.drafted[t] == choice && place == own);
+                if (p.places)
+                    next = next && p.places[t] == length + float(i);
+                const uint64_t found = __ballot(next);
                 if (found) {
                     child = base + uint32_t(__builtin_ctzll(found));
                     break;
@@ -255,6 +252,11 @@ __global__ __launch_bounds__(kBlock) void settle_kernel(Settle p)
         }
         return (uint64_t(uint32_t(id)) << p.page_shift) + (place & ((1u << p.page_shift) - 1));
     };
+    // The layout refuses a run whose first token follows another.
+    if (threadIdx.x == kBlock - 1 && fits &&
+        ((p.parents && p.parents[run.begin] != -1.0f) ||
+         (p.places && p.places[run.begin] != length)))
+        bad = 1;
     for (uint32_t k = threadIdx.x; p.path_pages && k < count; k += kBlock) {
         const uint32_t base = uint32_t(length);
         rows[kSettleColumns + k] = row_of(base + k);

@@ -903,9 +903,11 @@ void run_attention_kernel(RunAttention p)
                 if (most > 0.0f && most < __builtin_inff())
                     exponent = 15 - __builtin_amdgcn_frexp_expf(most);
                 exponent = exponent < 100 ? exponent : 100;
-                // Never 0, which a masked score of -infinity would meet: scores are below
-                // 2^42, and times the least normal factor as good as 0.
-                factor[g] = fmaxf(ldexpf(p.scale, -exponent), 0x1p-126f);
+                factor[g] = ldexpf(p.scale, -exponent);
+                // Not 0 where a masked score of -infinity meets it: scores are below 2^42, and
+                // times the least normal factor as good as 0.
+                if (SPLIT == 1)
+                    factor[g] = fmaxf(factor[g], 0x1p-126f);
             }
 #pragma unroll
             for (int i = 0; i < 2 * U; ++i)
