@@ -484,8 +484,8 @@ mfh_status mfh_paged_qk_norm_rope_at(mfh_ctx *ctx, mfh_buf *query_out, mfh_buf *
  * possibly none; its token i is cached at place lengths[s] + i, behind the
  * lengths[s] tokens that the sequence holds without it.  A list of starts has up to 65536
  * runs (MFH_OVERFLOW beyond).  Its first entry that is no whole number, falls below the one
- * before it or passes the batch ends it: sequences from there on have no run.  Rows of the batch
- * that are in no run (behind the last one, or padding before the first) are
+ * before it or passes the batch ends it: sequences from there on have no run.  Rows of the
+ * batch that are in no run (behind the last one, or padding before the first) are
  * left as they were by the attention calls.
  * Trees: parents[t] (F32 [tokens]) is the token of the same run that token t follows, as
  * its number in the run, below t's own; -1 for one that follows the cached tokens
@@ -519,8 +519,8 @@ mfh_status mfh_draft_layout(mfh_ctx *ctx, mfh_buf *sequences, mfh_buf *positions
  * and values are below 3.39e38 (larger ones give NaN) and, for the precision of f32, zero
  * or above 2^-100.  tokens * query_heads <= 2^25, and (sequences + tokens * query_heads /
  * key_value_heads / 16) * key_value_heads * (places of a table's row / 32 + 14) below 2^31:
- * of larger calls some are refused (MFH_OVERFLOW).  head_dim <= 1024; 32, 64, 80, 96, 112, 128, 160, 192 and 256 run on
- * matrix cores, others many times slower. */
+ * of larger calls some are refused (MFH_OVERFLOW).  head_dim <= 1024; 32, 64, 80, 96, 112,
+ * 128, 160, 192 and 256 run on matrix cores, others many times slower. */
 mfh_status mfh_paged_tree_gqa(mfh_ctx *ctx, mfh_buf *output, const mfh_buf *query,
                               const mfh_buf *key_pages, const mfh_buf *value_pages,
                               const mfh_buf *tables, const mfh_buf *starts,

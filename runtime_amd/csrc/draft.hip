@@ -166,8 +166,8 @@ __global__ __launch_bounds__(kBlock) void draft_layout_kernel(DraftLayout p)
 // in buffer b: a thread has one unit (16, 4 or 2 bytes of a head's row) of every
 // row and moves them in the path's order, whose sources never lie before its targets.
 // Bound by dependent reads: the lists, a search of the run per accepted token, page ids,
-// the rows.  12 buffers of 8 heads of 64: one run of 16 tokens, f32, 7.5 us a call, 96 of 4
-// to 32, binary16, 8.6.  Each block walks for itself: a launch between the walk and the
+// the rows.  12 buffers of 8 heads of 64: one run of 16 tokens, f32, 7.8 us a call, 96 of 4
+// to 32, binary16, 8.7 to 9.9 (two cards).  Each block walks for itself: a launch between the walk and the
 // moves would add its own latency.
 template <typename T>
 __device__ __forceinline__ void move_rows(const Settle &p, uint32_t b, const uint64_t *from,

@@ -144,9 +144,10 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 // rows.
 //
 // Binary16 caches: keys and values are operands as they are, queries (scaled by a power of
-// two to below 2^15) and probabilities (times 2^12, up to 2^15) two binary16 parts each, which
-// are within 2^-24 of the value; what is cut off of a probability is below 2^-36 of the
-// largest.  f32 caches: all four are three bfloat16 parts, which hold 24
+// two to below 2^15) and probabilities (times 2^12, up to 2^15) two binary16 parts each.  They
+// are within 2^-23 of the value from 2^-2 on and within 2^-25 of smaller ones (a second part
+// below 2^-14 has fewer bits), which is 2^-39 of a row's largest query column and 2^-37 of its
+// largest probability, or less.  f32 caches: all four are three bfloat16 parts, which hold 24
 // bits, and six of the nine products are formed (the others are below 2^-26).  Six
 // products of 16 bits take 6/16 of the cycles of one of f32.
 //
@@ -166,13 +167,16 @@ __global__ __launch_bounds__(64) void run_attention_general_kernel(RunAttention 
 // - few rows over long caches, the cache's reads: 48 trees of 4 to 32 tokens over 17 to 8191
 //   keys, 32 / 8 heads of 128, binary16, 90 (63); 64 tokens of 16 heads over 100 to
 //   8191 latents of 512 + 64 49 (30);
-// - prompts, the issue of vector and matrix instructions, which share a SIMD's slot: 2048
-//   tokens over 2048, 32 / 8 heads of 64, 139 to 160 (95 with both parts of queries and
-//   probabilities), 37.0 M instructions of waves, 6.4 M of them products; 1024 over 1024
-//   latents, 32 heads, 305 to 330 (202);
-// - single sequences, what a launch and its dependent reads (starts, page ids, a tile, the
-//   join's shares and records) cost: 16 tokens over 2047 keys of 64, f32, 20, the
-//   smallest call (a tree over 127 keys) 14.
+// - prompts, products and the vector instructions between them, in turn: 2048 tokens over 2048,
+//   32 / 8 heads of 64, 138 to 160 (95 with both parts of queries and probabilities); of
+//   the SIMDs' 256 M cycles matrix cores are busy in 102 M, and the 30.7 M other vector
+//   instructions take about 123 M; 1024 over 1024 latents, 32 heads, 300 to 345 (202);
+// - f32 caches, six products for one and the parts of every tile: the prompt above 435 (278), 48
+//   trees as above 262 (121);
+// - single sequences, the chain of a launch's dependent reads (starts, page ids, queries, a
+//   tile) and the join's: 16 tokens over 2047 keys of 64, f32, 20, the smallest call (a
+//   tree over 127 keys) 14.  One token over the same keys takes 17 here and 11 in the
+//   kernel for single tokens, whose chain is shorter.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -183,9 +187,11 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 256;
-// An item's queries, records and rows cost about five tiles (48 trees as above: 112 us at 2,
-// 100 at 4, 92 at 6, 100 at 8); where a CU has three blocks, of tiles of 32 keys, eight
-// (104 us at 3, 98 at 5, 90 at 8 and 12).
+// An item's queries, records and rows cost about five tiles: 48 trees as above take 99 us at 4,
+// 95 at 5, 92 at 6, 48 x 8 tokens over 2047 keys 101, 104 and 105, the prompt of heads of 64
+// 144, 144 and 147, trees over f32 caches 257, 259 and 266.  Where a CU has three blocks, of
+// tiles of 32 keys, eight (48 x 32 tokens over 2047 keys 160 us at 6, 157 to 165 at 8, 161
+// at 10).
 constexpr uint32_t kItemUnits = 5, kItemUnitsOfThree = 8;
 // Units of a block: of more than one, a short call leaves CUs empty (one tree as above 20
 // us at 1, 28 at 4).
@@ -1491,7 +1497,11 @@ MatrixKernel matrix_kernel_with()
 }
 // Blocks on a CU: two waves to a SIMD, one where a wave needs all registers, three as below.
 //
-// `many`: more rows than one item has, on average over the sequences.  Up to 112 wide a wave
+// `many`: more rows than one item has, on average over the sequences, for the starts live on the
+// device.  Batches of a prompt and single tokens take what the two take apart, or less: 256
+// tokens, and 47 of one over 2047 keys, 32 / 8 heads, binary16, of 64 columns 21 and 44 us,
+// together 49, of 128 26 and 87, together 94; with 1024 over 1024 58 and 44, together 106, and 82
+// and 87, together 131.  Up to 112 wide a wave
 // then has 32 of them, for which each operand read from LDS serves two products: the
 // prompt above 160 us against 180, and of heads 128 wide 48 sequences of 24 tokens over 2047
 // (96 rows) 169 against 193, of 16 tokens (64 rows) 147 against 126.  Of 128 columns that
@@ -1510,7 +1520,8 @@ MatrixKernel matrix_kernel_of(bool half, bool many)
                                           (D < 128 ? 2 : 3)>();
         return matrix_kernel_with<D, D, true, false, 4, 1, 1, RESIDENT>();
     }
-    // Three parts of a wide row need the registers of two waves (one wave spilled them).
+    // Three parts of a wide row need the registers of two waves; of 256 columns these spill 28
+    // still (48 trees over 17 to 4095 keys, 16 / 4 heads, 164 us, its bytes' time 70).
     if constexpr (D < 128)
         return matrix_kernel_with<D, D, false, false, 4, 1, 1, RESIDENT>();
     else
@@ -1520,7 +1531,11 @@ MatrixKernel matrix_kernel_of(bool half, bool many)
 // rows (two waves to a row), of 32 (four) and of 16 (eight, whose operand reads no other
 // wave shares).  Binary16, 64 sequences over 2047 latents of 512 + 64: of 32 rows 62 us in
 // items of 64, 60 of 32; of 64 rows 83 and 98; the prompt above 328 and 452.  f32, the same
-// of 16 rows: 121 in items of 16, 141 of 32; of 32 rows 202 and 167.
+// of 16 rows: 121 in items of 16, 141 of 32; of 32 rows 202 and 167.  Of rank 512 the f32
+// kernel for items of 32 rows spills registers (62, with 32 rotated columns 65), and so
+// does the binary16 one for 64 rows and 32 rotated columns (33).  64 and 128 rows to a
+// sequence, 64 sequences over 2047: binary16 88 and 138 us (36 and 67 of bytes or products),
+// f32 266 and 436 (98 and 197).
 template <int RANK, int ROPE>
 MatrixKernel latent_kernel_of(bool half, uint64_t rows, uint64_t sequences)
 {
