@@ -10,8 +10,9 @@ import numpy as np
 import pytest
 
 from runtime_amd.backend import GqaSpec
-from test_draft_gpu import (F32, NAN, Batch, check, f32, random_pages, read_pages, refused,
-                            run_latent, run_layout, say, settled, starts_of, tables_for, upload)
+from test_draft_gpu import (F32, NAN, Batch, Model, captured, check, f32, plain_decode, random_pages,
+                            read_pages, refused, run_latent, run_layout, say, settled, starts_of,
+                            tables_for, upload)
 
 pytestmark = pytest.mark.gpu
 
@@ -306,3 +307,45 @@ def test_settling_refusals_of_places(backend):
     good = [a((2, 4)), a((2,)), a((2,)), [], a((2,)), a((2,)), a((3,)), None, a((2,)), a((2, 1))]
     for places in good[1:3]:
         refused("InvalidArgument", backend.settle_drafts, *good, places)
+
+
+# ---- together -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+def test_drafts_longer_than_the_mask(backend, graph):
+    """Drafts of 12 tokens, all of them true, where the mask has eight bits: eight are accepted a
+    step, and decoding goes on as one token at a time does."""
+    prompts = [[5, 80, 3], [11], [40, 41]]
+    truth = plain_decode(backend, True, prompts, 30)
+    model, b, n = Model(backend, True), backend, 12
+    said = [[t[0]] for t in truth]
+    w = model.buffers(6)
+    model.run(w, f32(b, sum(prompts, [])), f32(b, starts_of([3, 1, 2])), None, f32(b, [0, 0, 0]), None)
+    w = model.buffers(3 * n)
+    tokens, starts, lengths = f32(b, np.zeros(3 * n)), f32(b, np.zeros(4)), f32(b, [3, 1, 2])
+    mask = upload(b, np.zeros((3 * n, 1), np.uint8))
+    parents = f32(b, np.tile(np.arange(n) - 1, 3))
+    emitted, counts, last = b.allocate_f32((3, 16)), b.allocate_f32((3,)), b.allocate_f32((3,))
+    grown = b.allocate_f32((3,))
+
+    def step():
+        model.run(w, tokens, starts, parents, lengths, mask)
+        b.settle_drafts(emitted, counts, last, model.caches, tokens, w["choice"], starts, parents,
+                        lengths, model.table, places=w["place"])
+        b.add(grown, lengths, counts)
+
+    step()  # of no runs: the workspace
+    replay, end = captured(b, step) if graph else (step, lambda: None)
+    b.copy(starts, f32(b, starts_of([n] * 3)))
+    for _ in range(3):
+        b.copy(tokens, f32(b, np.concatenate([t[len(x) - 1:len(x) - 1 + n]
+                                              for t, x in zip(truth, said)])))
+        replay()
+        got, count = b.read(emitted), b.read(counts)
+        assert count.tolist() == [8, 8, 8]
+        for i in range(3):
+            said[i] += [int(v) for v in got[i, :8]]
+            assert said[i] == truth[i][:len(said[i])]
+        b.copy(lengths, grown)
+    end()
+    assert [len(x) for x in said] == [25] * 3
